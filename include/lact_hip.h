@@ -249,6 +249,73 @@ int lact_window_attention_backward(int32_t B, int32_t L, int32_t H, int32_t D, i
                                    int64_t v_bs, const void* out, const float* lse, const void* dout, int32_t do_ld,
                                    int64_t do_bs, float* delta, void* dq, void* dk, void* dv, void* stream);
 
+/* ---- Token mixers beside the operation (no counterpart in the reference) -----------------------------------------------
+ *
+ * Softmax attention of a sequence with itself, act_dtype bf16 or fp32, D = 64 or 128, H a multiple of HK (query heads h * H / HK ...
+ * share key head h).  Query i sees key j of its own document when j > i - window and (j <= i or j lies in the document's prefix);
+ *   s_ij = f(scale q_i . k_j) - slopes[h] |i - j|,  f(x) = score_cap tanh(x / score_cap), or x where score_cap is 0;
+ *   out_i = sum_j softmax_j(s_ij) v_j,  0 where i sees nothing (tokens in no document).
+ * What a masked place holds, infinities and NaN among it, does not reach a row that does not see it.
+ * q, dout: [B, L, H, D], k, v: [B, L, HK, D]: token stride *_ld and batch stride *_bs in elements, rows 16-byte aligned, heads contiguous
+ * inside a token; window >= L: none.  n_documents 0: one document of L tokens without a prefix; else documents [B, n_documents + 1] (null with
+ * n_documents 1: one of L tokens), where document n covers the tokens [documents[n], documents[n + 1]) (not falling; device memory, so not checked: bounds outside the sequence are cut
+ * to it), and prefixes [B, n_documents] or null.  slopes: [H] fp32 or null, without a gradient.
+ * out, dq, dk, dv contiguous; lse, delta: [B, H, L] fp32; ranges: lact_attention_ranges_bytes bytes (0 without documents), written by the
+ * forward, read by the backward. */
+typedef struct lact_attention_desc {
+  int32_t act_dtype, B, L, H, HK, D, window, n_documents;
+  float scale, score_cap;
+  int32_t q_ld, k_ld, v_ld, do_ld;
+  int64_t q_bs, k_bs, v_bs, do_bs;
+  const float* slopes;
+  const int32_t* documents;
+  const int32_t* prefixes;
+} lact_attention_desc_t;
+size_t lact_attention_ranges_bytes(const lact_attention_desc_t* desc);
+int lact_masked_attention_forward(const lact_attention_desc_t* desc, const void* q, const void* k, const void* v, void* out, float* lse,
+                                  void* ranges, void* stream);
+int lact_masked_attention_backward(const lact_attention_desc_t* desc, const void* q, const void* k, const void* v, const void* out,
+                                   const float* lse, const void* ranges, const void* dout, float* delta, void* dq, void* dk, void* dv,
+                                   void* stream);
+
+/* The same for one new token of every sequence: q, out [B, H, D]; k, v: caches [B, N, HK, D] with token (*_ld), batch (*_bs) and head (*_hs)
+ * strides in elements, rows 16-byte aligned; lengths [B] int32 in device memory: the first lengths[b] entries are the sequence, the last of them
+ * the new token, whose query sees the last `window` of them (cut to 0 .. N; 0: output 0).  Entries past the length are not read.
+ * workspace: lact_attention_step_workspace_bytes bytes. */
+typedef struct lact_attention_step_desc {
+  int32_t act_dtype, B, N, H, HK, D, window;
+  float scale, score_cap;
+  int64_t q_bs, k_ld, k_bs, k_hs, v_ld, v_bs, v_hs;
+  const float* slopes;
+} lact_attention_step_desc_t;
+size_t lact_attention_step_workspace_bytes(const lact_attention_step_desc_t* desc);
+int lact_attention_step(const lact_attention_step_desc_t* desc, const void* q, const void* k, const void* v, const int32_t* lengths, void* out,
+                        void* workspace, void* stream);
+
+/* Linear attention with a decay: S_t = e^(g_t) S_(t-1) + k_t v_t^T, out_t = scale S_t^T q_t; dk, dv = 64 or 128.
+ * q, k: [b, l, h, dk], v, dout: [b, l, h, dv] as above; g: fp32 log decays, contiguous [b, l, h] (decay_per_token) or [h]; -infinity (anything
+ * below -200) forgets the state.  state: [b, h, dk, dv] fp32 in front of the first token, null: zero; last (nullable): behind the last one.
+ * states: states_bytes bytes kept from the forward for the backward (may be 0); scratch: scratch_bytes bytes, the backward's own.
+ * Backward: dlast nullable; dg (nullable, shape of g) and dstate (nullable) fp32; with dlast and dg it reads `last`. */
+typedef struct lact_linear_desc {
+  int32_t act_dtype, b, l, h, dk, dv, decay_per_token;
+  float scale;
+  int32_t q_ld, k_ld, v_ld, do_ld;
+  int64_t q_bs, k_bs, v_bs, do_bs;
+} lact_linear_desc_t;
+int lact_linear_attention_sizes(const lact_linear_desc_t* desc, size_t* states_bytes, size_t* scratch_bytes);
+int lact_linear_attention_forward(const lact_linear_desc_t* desc, const void* q, const void* k, const void* v, const float* g,
+                                  const float* state, void* out, float* last, void* states, void* stream);
+int lact_linear_attention_backward(const lact_linear_desc_t* desc, const void* q, const void* k, const void* v, const float* g,
+                                   const float* state, const float* last, const void* states, const void* dout, const float* dlast, void* dq,
+                                   void* dk, void* dv, float* dg, float* dstate, void* scratch, void* stream);
+
+/* One token of it: q, k [b, h, dk], v [b, h, dv] with batch strides *_bs (heads contiguous), g [b, h] or [h]; state and state_out [b, h, dk, dv]
+ * fp32, the same memory or apart; out [b, h, dv]. */
+int lact_linear_attention_step(int32_t act_dtype, int32_t b, int32_t h, int32_t dk, int32_t dv, int32_t decay_per_token, float scale,
+                               const void* q, int64_t q_bs, const void* k, int64_t k_bs, const void* v, int64_t v_bs, const float* g,
+                               const float* state, float* state_out, void* out, void* stream);
+
 /* Execution options (process-wide; no counterpart in the reference, where PyTorch enqueues the whole layer on one
  * stream as separate kernels).  The switches are on by default and change no result bit.
  *   LACT_OPT_STREAM_OVERLAP: the apply steps of a program do not depend on the update chain that runs beside

@@ -34,6 +34,22 @@ class Desc(Structure):
     ]
 
 
+class AttentionDesc(Structure):
+    _fields_ = ([(n, c_int32) for n in ("act_dtype", "B", "L", "H", "HK", "D", "window", "n_documents")] + [("scale", c_float), ("score_cap", c_float)] +
+                [(n, c_int32) for n in ("q_ld", "k_ld", "v_ld", "do_ld")] + [(n, c_int64) for n in ("q_bs", "k_bs", "v_bs", "do_bs")] +
+                [(n, c_void_p) for n in ("slopes", "documents", "prefixes")])
+
+
+class AttentionStepDesc(Structure):
+    _fields_ = ([(n, c_int32) for n in ("act_dtype", "B", "N", "H", "HK", "D", "window")] + [("scale", c_float), ("score_cap", c_float)] +
+                [(n, c_int64) for n in ("q_bs", "k_ld", "k_bs", "k_hs", "v_ld", "v_bs", "v_hs")] + [("slopes", c_void_p)])
+
+
+class LinearDesc(Structure):
+    _fields_ = ([(n, c_int32) for n in ("act_dtype", "b", "l", "h", "dk", "dv", "decay_per_token")] + [("scale", c_float)] +
+                [(n, c_int32) for n in ("q_ld", "k_ld", "v_ld", "do_ld")] + [(n, c_int64) for n in ("q_bs", "k_bs", "v_bs", "do_bs")])
+
+
 OPT_STREAM_OVERLAP, OPT_FUSED_NEWTON_SCHULZ, OPT_NS_BARRIER_SPIN_LIMIT, OPT_PERSISTENT_TILES, OPT_KEEP_PREACTIVATIONS = 0, 1, 2, 3, 4
 EXPORTS = ("lact_last_error", "lact_version", "lact_query_sizes", "lact_forward", "lact_forward_from_state", "lact_backward",
            "lact_forward_shared_weights", "lact_backward_shared_weights",
@@ -44,7 +60,10 @@ EXPORTS = ("lact_last_error", "lact_version", "lact_query_sizes", "lact_forward"
            "lact_weight_grad", "lact_weight_grad_workspace_bytes", "lact_layer_sum_rows", "lact_layer_pre_forward", "lact_layer_pre_backward", "lact_layer_lr_forward",
            "lact_layer_lr_backward", "lact_layer_post_forward", "lact_layer_post_dw_rows", "lact_layer_post_backward",
            "lact_window_attention_forward", "lact_window_attention_backward", "lact_layer_pre_attn_forward",
-           "lact_layer_pre_attn_part_rows", "lact_layer_pre_attn_backward", "lact_layer_post_add_forward")
+           "lact_layer_pre_attn_part_rows", "lact_layer_pre_attn_backward", "lact_layer_post_add_forward",
+           "lact_attention_ranges_bytes", "lact_masked_attention_forward", "lact_masked_attention_backward", "lact_attention_step_workspace_bytes",
+           "lact_attention_step", "lact_linear_attention_sizes", "lact_linear_attention_forward", "lact_linear_attention_backward",
+           "lact_linear_attention_step")
 
 HOST_PATH = os.path.join(HERE, "lib", "_lact_host.so")
 
@@ -125,6 +144,20 @@ def lib():
     L.lact_layer_pre_attn_backward.argtypes = [i32] * 6 + [vp] * 13
     for fn in ("lact_layer_post_add_forward", "lact_layer_pre_attn_forward", "lact_layer_pre_attn_part_rows", "lact_layer_pre_attn_backward", "lact_window_attention_forward", "lact_window_attention_backward", "lact_layer_pre_forward", "lact_layer_pre_backward", "lact_layer_lr_forward", "lact_layer_lr_backward",
                "lact_layer_post_forward", "lact_layer_post_dw_rows", "lact_layer_post_backward"):
+        getattr(L, fn).restype = c_int32
+    L.lact_attention_ranges_bytes.argtypes = [POINTER(AttentionDesc)]
+    L.lact_attention_ranges_bytes.restype = c_size_t
+    L.lact_masked_attention_forward.argtypes = [POINTER(AttentionDesc)] + [vp] * 7
+    L.lact_masked_attention_backward.argtypes = [POINTER(AttentionDesc)] + [vp] * 12
+    L.lact_attention_step_workspace_bytes.argtypes = [POINTER(AttentionStepDesc)]
+    L.lact_attention_step_workspace_bytes.restype = c_size_t
+    L.lact_attention_step.argtypes = [POINTER(AttentionStepDesc)] + [vp] * 7
+    L.lact_linear_attention_sizes.argtypes = [POINTER(LinearDesc), POINTER(c_size_t), POINTER(c_size_t)]
+    L.lact_linear_attention_forward.argtypes = [POINTER(LinearDesc)] + [vp] * 9
+    L.lact_linear_attention_backward.argtypes = [POINTER(LinearDesc)] + [vp] * 16
+    L.lact_linear_attention_step.argtypes = [i32] * 6 + [f32, vp, c_int64, vp, c_int64, vp, c_int64] + [vp] * 5
+    for fn in ("lact_masked_attention_forward", "lact_masked_attention_backward", "lact_attention_step", "lact_linear_attention_sizes",
+               "lact_linear_attention_forward", "lact_linear_attention_backward", "lact_linear_attention_step"):
         getattr(L, fn).restype = c_int32
     L.lact_profile_enable.argtypes = [c_int32]
     L.lact_profile_enable.restype = c_int32

@@ -6,14 +6,14 @@ import sys
 import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRC = os.path.join(HERE, "csrc", "lact_api.hip")
+SOURCES = [os.path.join(HERE, "csrc", f) for f in ("lact_api.hip", "mixers_api.hip")]
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "liblact_hip.so")
 HOST_SRC = os.path.join(HERE, "csrc", "torch_host.cpp")
 HOST_LIB = os.path.join(LIB_DIR, "_lact_host.so")
 
 FLAGS = [
-    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     # packed-fp32 VALU forms are kept out of the generated code
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     # A multiply and an add fuse only where one source expression writes them together.  HIP's default ("fast") also
@@ -47,25 +47,31 @@ def _host_commands():
 def build(verbose: bool = True) -> str:
     os.makedirs(LIB_DIR, exist_ok=True)
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    compile_, link = _host_commands()
-    cmds = [[hipcc] + FLAGS + [SRC, "-o", LIB], compile_]
+    host_compile, host_link = _host_commands()
+    objs = [os.path.join(LIB_DIR, os.path.basename(src).replace(".hip", ".o")) for src in SOURCES]
+    compiles = [[hipcc] + FLAGS + ["-c", src, "-o", obj] for src, obj in zip(SOURCES, objs)] + [host_compile]
+    links = [[hipcc, "--offload-arch=gfx950", "-shared", "-fPIC"] + objs + ["-o", LIB], host_link]
     if verbose:
-        for cmd in cmds:
+        for cmd in compiles + links:
             print(" ".join(cmd), flush=True)
-    # the device library and the host module compile side by side
-    procs = [subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for cmd in cmds]
-    outs = [p.communicate()[0] for p in procs]
-    if all(p.returncode == 0 for p in procs):
-        res = subprocess.run(link, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-        procs.append(res)
-        outs.append(res.stdout)
-    for cmd, p, text in zip(cmds + [link], procs, outs):
+
+    def report(cmd, code, text):
         text = "\n".join(l for l in text.splitlines() if "packed-fp32-ops" not in l)
-        if p.returncode != 0:
+        if code != 0:
             raise RuntimeError(f"{cmd[0]} failed:\n" + text)
         if verbose and text.strip():
             print(text)
-    os.remove(os.path.join(LIB_DIR, "torch_host.o"))
+
+    # the units of the device library and the host module compile side by side
+    procs = [subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True) for cmd in compiles]
+    outs = [p.communicate()[0] for p in procs]
+    for cmd, p, text in zip(compiles, procs, outs):
+        report(cmd, p.returncode, text)
+    for cmd in links:
+        res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        report(cmd, res.returncode, res.stdout)
+    for obj in objs + [os.path.join(LIB_DIR, "torch_host.o")]:
+        os.remove(obj)
     return LIB
 
 

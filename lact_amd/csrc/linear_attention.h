@@ -1,0 +1,655 @@
+// Linear attention with a decay, bf16 and fp32, key and value sizes 64 and 128:
+//
+//   S_t = e^(g_t) S_(t-1) + k_t v_t^T,   o_t = scale S_t^T q_t
+//
+// q, k: [B, L, H, DK], v: [B, L, H, DV] with token and batch strides, heads next to each other; g: log decays, fp32, [B, L, H] or one per
+// head; S: [B, H, DK, DV] fp32.
+//
+// In chunks of 64 tokens, with G the sum of g from the chunk's start to a token, itself included:
+//
+//   o_i = scale (sum_(j <= i) e^(G_i - G_j) (q_i . k_j) v_j + e^(G_i) S^T q_i),   S <- e^(G_last) S + sum_j e^(G_last - G_j) k_j v_j^T
+//
+// Only differences of later and earlier sums are exponentiated, so no decay overflows; the sums are formed in fp64 and kept in two floats.
+// The gradients are the same recurrence with other operands: of q with (dout, v, k) and the transposed state; of k with (v, dout, q) and of v with (k, q, dout)
+// backwards in time from the gradient of the last state.  One kernel, k_lin_walk, is all four.
+//
+// A block walks the chunks of a segment of one head; a wave owns a quarter of the state's columns, in accumulators, from where they are
+// packed as the next product's operand where they lie (an accumulator's rows are k slots there; which row of the state an accumulator row
+// holds is chosen so that the queries' operand is 8 neighbours).  Segments start from states that k_lin_segments and k_lin_scan form first, where heads
+// and batch alone do not fill the chip.
+//
+// The state is held, and added to, in fp32: what is added is a product of bf16 inputs with a weight, which goes into the matrix product
+// as three bf16 parts (24 bits).  Probabilities and, where only rounded outputs depend on it, the state as an operand are rounded to bf16.
+//
+// A gradient of the decays adds what crosses a token: dg_s = sum_(i >= s > j) M_ij + ..., M_ij = e^(G_i - G_j) (q_i . k_j)(dout_i . v_j) scale.
+// Rows and columns of M are summed from the same products (they cancel outside the crossing), the state's shares likewise, and the sum over a
+// segment starts from <dS, S> at its end.
+#pragma once
+#include "masked_attention.h"
+
+namespace lact {
+
+constexpr int LIN_CHUNK = 64;
+constexpr float LIN_MIN_LOG = -200.f;      // e^-200 is 0 in fp32: a log decay of -infinity forgets everything, and its sums stay finite
+
+struct LinDecay {
+  const float* g;         // [B, L, H] or [H]
+  int per_token;
+  __device__ __forceinline__ float at(int b, int t, int h, int L, int H) const {
+    if (t >= L) return 0.f;
+    const float x = per_token ? g[((size_t)b * L + t) * H + h] : g[h];
+    return x < LIN_MIN_LOG ? LIN_MIN_LOG : x;
+  }
+};
+
+template <typename T>
+struct LinRows {          // [B, L, H, D]
+  const T* p;
+  int ld;
+  long long bs;
+};
+
+template <typename T>
+struct LinParams {
+  int B, L, H, segments, seg_chunks;     // chunks of a segment
+  LinRows<T> x, y, z, w;                 // out_i = sum_j (x_i . y_j) z_j + x_i S, S += y_j z_j^T; w: see k_lin_walk
+  LinDecay decay;
+  float pair_scale, state_scale, source_scale;
+  T* out;                                // [B, L, H, DZ]
+  const float* states;                   // [segments][B * H][DX * DZ] (or transposed): where each segment starts, null: from zero
+  const float* state0;                   // [B * H][..]: the same for a single segment
+  int transposed;                        // the states in memory are [DZ][DX]
+  float* last;                           // [B * H][..]: state behind the walk's last chunk, nullable
+  float* dots;                           // [B, L, H] fp32, for the gradient of the decays
+  UDiv by_heads;                         // H
+};
+
+// ---- operands of 16x16 products with 32 k slots: lane l holds row (or column) l & 15, slots 8 * (l >> 4) + j
+__device__ __forceinline__ f32x4 mma16(const bf16x8& a, const bf16x8& b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma16(const f32x8& a, const f32x8& b, f32x4 c) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ void lin_zero(f32x4& v) { v = f32x4{0.f, 0.f, 0.f, 0.f}; }
+
+__device__ __forceinline__ bf16x8 lin_pack(const float (&v)[8], uint16_t) {
+  return __builtin_bit_cast(bf16x8, make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])));
+}
+__device__ __forceinline__ f32x8 lin_pack(const float (&v)[8], float) { return f32x8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}; }
+// Eight floats as PARTS operands whose sum they are, largest first; fp32 needs one.
+template <typename T, int PARTS>
+__device__ __forceinline__ void lin_split(float (&v)[8], typename AttnType<T>::Frag (&f)[PARTS]) {
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    f[p] = lin_pack(v, T());
+    if (p + 1 < PARTS)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] -= (float)f[p][i];
+  }
+}
+template <typename T> constexpr int lin_parts() { return sizeof(T) == 2 ? 3 : 1; }
+
+// Reads of a 64 x D tile laid out as MaskTile.
+template <typename T, int D> struct LinFrag {
+  using S = MaskTile<T, D>;
+  using Frag = typename AttnType<T>::Frag;
+  // rows [16 * rt, +16), columns 32 * u + 8 * (l >> 4) + j
+  __device__ static __forceinline__ Frag rows(const char* tile, int rt, int u) {
+    const int l = threadIdx.x & 63, r = rt * 16 + (l & 15), c = l >> 4;
+    const char* p = tile + r * S::ROWB;
+    if constexpr (sizeof(T) == 2) {
+      return __builtin_bit_cast(Frag, *reinterpret_cast<const uint4*>(p + (((4 * u + c) ^ S::key(r)) << 4)));
+    } else {
+      const float4 a = *reinterpret_cast<const float4*>(p + (((8 * u + 2 * c) ^ S::key(r)) << 4));
+      const float4 b = *reinterpret_cast<const float4*>(p + (((8 * u + 2 * c + 1) ^ S::key(r)) << 4));
+      return Frag{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    }
+  }
+  // Transposed: lane l holds column `col(l & 15)`, slot j tile row 32 * v + 8 * (l >> 4) + j.  col(i) = c0 + cs * (i >> 2) + (i & 3).
+  template <int CS>
+  __device__ static __forceinline__ Frag cols(const char* tile, int c0, int v) {
+    const int l = threadIdx.x & 63, c = l >> 4;
+    if constexpr (sizeof(T) == 2) {
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      typedef short s16x8 __attribute__((ext_vector_type(8)));
+      // inside 16 lanes, lane i receives element i & 3 of the 8 bytes that lanes 4 j + (i >> 2) address, j = 0 .. 3
+      const int r = 32 * v + 8 * c + ((l >> 2) & 3), col = c0 + CS * (l & 3);
+      const uint32_t in = (col & 7) * 2;
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + r * S::ROWB + (((col >> 3) ^ S::key(r)) << 4) + in));
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + (r + 4) * S::ROWB + (((col >> 3) ^ S::key(r + 4)) << 4) + in));
+      const s16x8 x = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      return __builtin_bit_cast(Frag, x);
+    } else {
+      const int col = c0 + CS * ((l & 15) >> 2) + (l & 3);
+      Frag x;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = 32 * v + 8 * c + j;
+        x[j] = *reinterpret_cast<const float*>(tile + r * S::ROWB + (((col >> 2) ^ S::key(r)) << 4) + (col & 3) * 4);
+      }
+      return x;
+    }
+  }
+  __device__ static __forceinline__ const char* at(const char* tile, int r, int col) {
+    constexpr int E = 16 / (int)sizeof(T);
+    return tile + r * S::ROWB + (((col / E) ^ S::key(r)) << 4) + (col % E) * (int)sizeof(T);
+  }
+};
+
+// What the tokens of a chunk weigh, in LDS of a wave's own: sums of log2 decays in two floats, weight of the state in an output, weight of a token
+// in the state.
+struct LinWeights {
+  float4* w;
+  float whole;       // decay of the state over the chunk
+  template <bool REV>
+  __device__ __forceinline__ void form(float4* lds, float g, bool valid, float state_scale, float source_scale) {
+    w = lds;
+    double s = (double)g * 1.4426950408889634;
+    const int l = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double u = __shfl_up(s, o, 64);
+      if (l >= o) s += u;
+    }
+    const double end = __shfl(s, 63, 64);
+    const float hi = (float)s, lo = (float)(s - (double)hi);
+    const float to = __builtin_amdgcn_exp2f((float)s), from = __builtin_amdgcn_exp2f((float)(end - s));
+    whole = __builtin_amdgcn_exp2f((float)end);
+    w[l] = make_float4(hi, lo, (REV ? from : to) * state_scale, valid ? (REV ? to : from) * source_scale : 0.f);
+    wave_lds_fence();
+  }
+  // 2^(later - earlier)
+  __device__ static __forceinline__ float between(const float4& later, const float4& earlier) {
+    return __builtin_amdgcn_exp2f((later.x - earlier.x) + (later.y - earlier.y));
+  }
+};
+
+template <typename T, int DX, int DZ, bool GATE>
+struct LinShape {
+  static constexpr int X = MaskTile<T, DX>::BYTES, Z = MaskTile<T, DZ>::BYTES;
+  static constexpr int STAGE = 2 * X + (GATE ? 2 : 1) * Z;                // x, y, z (, w)
+  static constexpr int BUFFERS = sizeof(T) == 2 ? 2 : 1;
+  static constexpr int PAIRS = MaskTile<T, 64>::BYTES;
+  static constexpr int WEIGHTS = 4 * 64 * 16;
+  static constexpr int SUMS = GATE ? 4 * 64 * 4 * 2 : 0;                  // per wave: what its columns, and its pairs, add to the dots
+  static constexpr int LDS = BUFFERS * STAGE + PAIRS + WEIGHTS + SUMS;
+  static_assert(LDS <= 160 * 1024, "LDS");
+};
+
+template <typename T, int DX, int DZ>
+struct LinState {        // columns [wave * DZ / 4, + DZ / 4): accumulator a, row 4 c + r holds state row 32 (a / 2) + 8 c + 4 (a % 2) + r
+  static constexpr int NT = DZ / 64, AT = DX / 16;
+  f32x4 s[AT][NT];
+  __device__ static __forceinline__ int row(int a) { return 32 * (a >> 1) + 8 * ((threadIdx.x & 63) >> 4) + 4 * (a & 1); }
+  __device__ static __forceinline__ int col(int wave, int nt) { return wave * (DZ / 4) + nt * 16 + (threadIdx.x & 15); }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int a = 0; a < AT; ++a)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) lin_zero(s[a][n]);
+  }
+  __device__ __forceinline__ void load(const float* m, bool transposed, int wave) {
+#pragma unroll
+    for (int a = 0; a < AT; ++a)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (transposed) {
+          const float4 v = *reinterpret_cast<const float4*>(m + (size_t)col(wave, n) * DX + row(a));
+          s[a][n] = f32x4{v.x, v.y, v.z, v.w};
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) s[a][n][r] = m[(size_t)(row(a) + r) * DZ + col(wave, n)];
+        }
+      }
+  }
+  __device__ __forceinline__ void store(float* m, bool transposed, int wave) const {
+#pragma unroll
+    for (int a = 0; a < AT; ++a)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (transposed) {
+          *reinterpret_cast<float4*>(m + (size_t)col(wave, n) * DX + row(a)) = make_float4(s[a][n][0], s[a][n][1], s[a][n][2], s[a][n][3]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) m[(size_t)(row(a) + r) * DZ + col(wave, n)] = s[a][n][r];
+        }
+      }
+  }
+  // decays by `whole` and adds y^T (weight z); zf: the wave's columns of z
+  template <typename Frag>
+  __device__ __forceinline__ void update(const char* y, const Frag (&zf)[2][NT], const LinWeights& lw) {
+    constexpr int PARTS = lin_parts<T>();
+#pragma unroll
+    for (int a = 0; a < AT; ++a)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) s[a][n] *= lw.whole;
+    const int c = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      Frag zw[NT][PARTS];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = (float)zf[v][n][j] * lw.w[32 * v + 8 * c + j].w;
+        lin_split<T, PARTS>(x, zw[n]);
+      }
+#pragma unroll
+      for (int a = 0; a < AT; ++a) {
+        const Frag yf = LinFrag<T, DX>::template cols<8>(y, 32 * (a >> 1) + 4 * (a & 1), v);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int p = 0; p < PARTS; ++p) s[a][n] = mma16(yf, zw[n][p], s[a][n]);
+      }
+    }
+  }
+};
+
+// A chunk's rows of one operand, 64 from token t on; rows past the end repeat the last one.
+template <typename T, int D>
+__device__ __forceinline__ void lin_copy(const LinRows<T>& m, int b, int h, int t, int L, uint32_t lds, int wave) {
+  using S = MaskTile<T, D>;
+  const T* from = uniform(m.p + b * m.bs + (long long)t * m.ld + (long long)h * D);
+#pragma unroll
+  for (int i = 0; i < S::G / 4; ++i) {
+    const int c = (wave + i * 4) * 64 + (threadIdx.x & 63), r = c / S::G, slot = c % S::G;
+    dma16<false>(from, (uint32_t)min(r, L - 1 - t) * (uint32_t)m.ld * (uint32_t)sizeof(T) + (uint32_t)((slot ^ S::key(r)) << 4), lds + (wave + i * 4) * 1024);
+  }
+}
+
+// The walk over a segment.  REV: from its end to its beginning, sources are the later tokens.
+// GATE: also dots[t], for the gradient of the decays.  Forwards (x, y, z, w = dout, v, k, q): row sum minus column sum of M at t, and the state's share in
+// q_t . dq_t; backwards (x, y, z, w = k, q, dout, v): the state's share in v_t . dv_t.
+template <typename T, int DX, int DZ, bool REV, bool GATE>
+__global__ __launch_bounds__(256, 1) void k_lin_walk(const LinParams<T> p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  using Sh = LinShape<T, DX, DZ, GATE>;
+  using St = LinState<T, DX, DZ>;
+  using Frag = typename AttnType<T>::Frag;
+  using FX = LinFrag<T, DX>;
+  using FZ = LinFrag<T, DZ>;
+  using FP = LinFrag<T, 64>;
+  constexpr int NT = St::NT, UX = DX / 32, UZ = DZ / 32, SP = GATE ? lin_parts<T>() : 1;
+  prefetch_args<sizeof(p)>();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane >> 4, li = lane & 15;
+  const int seg = blockIdx.x % p.segments, bh = blockIdx.x / p.segments, b = p.by_heads.div(bh), h = bh - b * p.H;
+  const int L = p.L, chunks = (L + 63) / 64, first = seg * p.seg_chunks, n = min(p.seg_chunks, chunks - first);
+  char* pairs = smem + Sh::BUFFERS * Sh::STAGE;
+  float4* weights = reinterpret_cast<float4*>(pairs + Sh::PAIRS) + wave * 64;
+  float* sums = reinterpret_cast<float*>(pairs + Sh::PAIRS + Sh::WEIGHTS);
+  const uint32_t lds0 = lds_addr(smem);
+  auto token = [&](int i) { return (first + (REV ? n - 1 - i : i)) * 64; };
+  auto issue = [&](int i) LACT_INLINE_LAMBDA {
+    const int t = token(i);
+    const uint32_t to = lds0 + i % Sh::BUFFERS * Sh::STAGE;
+    lin_copy<T, DX>(p.x, b, h, t, L, to, wave);
+    lin_copy<T, DX>(p.y, b, h, t, L, to + Sh::X, wave);
+    lin_copy<T, DZ>(p.z, b, h, t, L, to + 2 * Sh::X, wave);
+    if (GATE) lin_copy<T, DZ>(p.w, b, h, t, L, to + 2 * Sh::X + Sh::Z, wave);
+  };
+  St st;
+  const float* start = p.states ? p.states + ((size_t)seg * p.B * p.H + bh) * (DX * DZ) : p.state0 ? p.state0 + (size_t)bh * (DX * DZ) : nullptr;
+  if (start) st.load(start, p.transposed, wave);
+  else st.zero();
+  const bool final = p.last && seg == (REV ? 0 : p.segments - 1);
+  float g_next = p.decay.at(b, token(0) + lane, h, L, p.H);
+  issue(0);
+  for (int i = 0; i < n; ++i) {
+    const int t0 = token(i);
+    const float g = g_next;
+    if (i + 1 < n) g_next = p.decay.at(b, token(i + 1) + lane, h, L, p.H);
+    if (Sh::BUFFERS == 1 || i == 0) wait_vmcnt<0>();
+    __syncthreads();      // the chunk is there, and every wave is through with the one before
+    if (Sh::BUFFERS == 2 && i + 1 < n) issue(i + 1);
+    const char* x = smem + i % Sh::BUFFERS * Sh::STAGE;
+    const char* y = x + Sh::X;
+    const char* z = y + Sh::X;
+    const char* w = z + Sh::Z;
+    LinWeights lw;
+    lw.form<REV>(weights, g, t0 + lane < L, p.state_scale, p.source_scale);
+    // Pairs of outputs [16 wave, +16) with their sources, [output][source] in LDS
+    {
+      const float4 mine = lw.w[16 * wave + li];
+      float rowsum = 0.f;
+#pragma unroll
+      for (int jt = 0; jt < 4; ++jt) {
+        const bool none = REV ? jt < wave : jt > wave;
+        if (none && (jt >> 1) != (wave >> 1)) continue;      // no product reads it
+        float v[4] = {0.f, 0.f, 0.f, 0.f}, m[4] = {0.f, 0.f, 0.f, 0.f};
+        if (!none) {
+          f32x4 acc, other;
+          lin_zero(acc);
+          lin_zero(other);
+#pragma unroll
+          for (int u = 0; u < UX; ++u) acc = mma16(FX::rows(y, jt, u), FX::rows(x, wave, u), acc);
+          if constexpr (GATE && !REV)
+#pragma unroll
+            for (int u = 0; u < UZ; ++u) other = mma16(FZ::rows(z, jt, u), FZ::rows(w, wave, u), other);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int j = 16 * jt + 4 * c + r, o = 16 * wave + li;
+            const float4 theirs = lw.w[j];
+            const float e = REV ? LinWeights::between(theirs, mine) : LinWeights::between(mine, theirs);
+            const bool on = (REV ? j >= o : j <= o) && t0 + max(j, o) < L;
+            v[r] = on ? acc[r] * e * p.pair_scale : 0.f;
+            if constexpr (GATE && !REV) {
+              m[r] = on && j != o ? v[r] * other[r] : 0.f;
+              rowsum += m[r];
+            }
+          }
+        }
+        Elem<T>::store4(reinterpret_cast<T*>(const_cast<char*>(FP::at(pairs, 16 * wave + li, 16 * jt + 4 * c))), v[0], v[1], v[2], v[3]);
+        if constexpr (GATE && !REV) {      // columns of M over the wave's outputs
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int s = 1; s < 16; s <<= 1) m[r] += __shfl_xor(m[r], s, 64);
+            if (li == 0) sums[256 + wave * 64 + 16 * jt + 4 * c + r] = m[r];
+          }
+        }
+      }
+      if constexpr (GATE && !REV) {
+        rowsum += __shfl_xor(rowsum, 16, 64);
+        rowsum += __shfl_xor(rowsum, 32, 64);
+        // (tiles that were passed over hold nothing)
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt)
+          if (jt > wave && (jt >> 1) != (wave >> 1) && li == 0)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sums[256 + wave * 64 + 16 * jt + 4 * c + r] = 0.f;
+        wave_lds_fence();
+        if (lane < 16) sums[256 + wave * 64 + 16 * wave + li] -= rowsum;
+      }
+    }
+    // The state's share: columns of the output are tokens
+    f32x4 o[4][NT];
+#pragma unroll
+    for (int it = 0; it < 4; ++it)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) lin_zero(o[it][nt]);
+#pragma unroll
+    for (int u = 0; u < UX; ++u) {
+      Frag sf[NT][SP];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = st.s[2 * u + (j >> 2)][nt][j & 3];
+        lin_split<T, SP>(v, sf[nt]);
+      }
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const Frag xf = FX::rows(x, it, u);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int q = 0; q < SP; ++q) o[it][nt] = mma16(sf[nt][q], xf, o[it][nt]);
+      }
+    }
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const float e = lw.w[16 * it + li].z;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) o[it][nt] *= e;
+      if constexpr (GATE) {
+        float d = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float v[4];
+          Elem<T>::load4(reinterpret_cast<const T*>(FZ::at(w, 16 * it + li, wave * (DZ / 4) + nt * 16 + 4 * c)), v);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) d = fmaf(v[r], o[it][nt][r], d);
+        }
+        d += __shfl_xor(d, 16, 64);
+        d += __shfl_xor(d, 32, 64);
+        if (lane < 16) sums[wave * 64 + 16 * it + li] = d;
+      }
+    }
+    Frag zf[2][NT];
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) zf[v][nt] = FZ::template cols<4>(z, wave * (DZ / 4) + nt * 16, v);
+    __syncthreads();      // the pairs of all waves
+    if constexpr (GATE)
+      if (wave == 0 && t0 + lane < L) {
+        float d = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) d += sums[k * 64 + lane];
+        if constexpr (!REV)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) d -= sums[256 + k * 64 + lane];
+        p.dots[((size_t)b * L + t0 + lane) * p.H + h] = d;
+      }
+    // A value that is not finite must not reach the outputs that do not see its token (0 * inf): those chunks are summed term by term.
+    if (__any(any_unfinite(zf[0]) || any_unfinite(zf[1]))) {
+      for (int j = 0; j < 64; ++j) {
+        if (t0 + j >= L) break;
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const int out = 16 * it + li;
+          const float pr = Elem<T>::load(reinterpret_cast<const T*>(FP::at(pairs, out, j)));
+          const bool sees = REV ? j >= out : j <= out;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float zv = Elem<T>::load(reinterpret_cast<const T*>(FZ::at(z, j, wave * (DZ / 4) + nt * 16 + 4 * c + r)));
+              o[it][nt][r] = sees ? fmaf(pr, zv, o[it][nt][r]) : o[it][nt][r];
+            }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          if (REV ? v < (it >> 1) : v > (it >> 1)) continue;
+          const Frag pf = FP::rows(pairs, it, v);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) o[it][nt] = mma16(zf[v][nt], pf, o[it][nt]);
+        }
+    }
+    if (Sh::BUFFERS == 2) wait_vmcnt<0>();      // for the next chunk, here and not behind the stores
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const int t = t0 + 16 * it + li;
+      if (t < L)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          Elem<T>::store4(p.out + (((size_t)b * L + t) * p.H + h) * DZ + wave * (DZ / 4) + nt * 16 + 4 * c, o[it][nt][0], o[it][nt][1], o[it][nt][2], o[it][nt][3]);
+    }
+    if (i + 1 < n || final) st.update(y, zf, lw);
+    if (Sh::BUFFERS == 1 && i + 1 < n) {
+      __syncthreads();
+      issue(i + 1);
+    }
+  }
+  if (final) st.store(p.last + (size_t)bh * (DX * DZ), p.transposed, wave);
+}
+
+// What the tokens of a segment add to the state, into entry `seg + 1` (REV: `seg - 1`) of states, and the segment's sum of log2 decays.
+template <typename T, int DX, int DZ, bool REV>
+__global__ __launch_bounds__(256, 1) void k_lin_segments(const LinParams<T> p, float* states, float* sums) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  using St = LinState<T, DX, DZ>;
+  using Frag = typename AttnType<T>::Frag;
+  constexpr int NT = St::NT, STAGE = MaskTile<T, DX>::BYTES + MaskTile<T, DZ>::BYTES;
+  prefetch_args<sizeof(p)>();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int count = p.segments - 1, seg = blockIdx.x % count + (REV ? 1 : 0), bh = blockIdx.x / count, b = p.by_heads.div(bh), h = bh - b * p.H;
+  const int L = p.L, chunks = (L + 63) / 64, first = seg * p.seg_chunks, n = min(p.seg_chunks, chunks - first);
+  float4* weights = reinterpret_cast<float4*>(smem + 2 * STAGE) + wave * 64;
+  const uint32_t lds0 = lds_addr(smem);
+  auto token = [&](int i) { return (first + (REV ? n - 1 - i : i)) * 64; };
+  auto issue = [&](int i) LACT_INLINE_LAMBDA {
+    const uint32_t to = lds0 + i % 2 * STAGE;
+    lin_copy<T, DX>(p.y, b, h, token(i), L, to, wave);
+    lin_copy<T, DZ>(p.z, b, h, token(i), L, to + MaskTile<T, DX>::BYTES, wave);
+  };
+  St st;
+  st.zero();
+  double total = 0.0;
+  float g_next = p.decay.at(b, token(0) + lane, h, L, p.H);
+  issue(0);
+  for (int i = 0; i < n; ++i) {
+    const int t0 = token(i);
+    const float g = g_next;
+    if (i + 1 < n) g_next = p.decay.at(b, token(i + 1) + lane, h, L, p.H);
+    wait_vmcnt<0>();
+    __syncthreads();
+    if (i + 1 < n) issue(i + 1);
+    const char* y = smem + i % 2 * STAGE;
+    const char* z = y + MaskTile<T, DX>::BYTES;
+    LinWeights lw;
+    lw.form<REV>(weights, g, t0 + lane < L, p.state_scale, p.source_scale);
+    Frag zf[2][NT];
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) zf[v][nt] = LinFrag<T, DZ>::template cols<4>(z, wave * (DZ / 4) + nt * 16, v);
+    st.update(y, zf, lw);
+    total += (double)lw.w[63].x + (double)lw.w[63].y;
+  }
+  st.store(states + ((size_t)(seg + (REV ? -1 : 1)) * p.B * p.H + bh) * (DX * DZ), p.transposed, wave);
+  if (threadIdx.x == 0) sums[(size_t)seg * p.B * p.H + bh] = (float)total;
+}
+
+// entry[s + 1] += 2^sums[s] entry[s] from entry[0] = initial on, or (reverse) entry[s - 1] += 2^sums[s] entry[s] from the last on; a
+// thread has four elements of one matrix.
+__global__ __launch_bounds__(256) void k_lin_scan(int segments, long long matrices, int elems, int reverse, const float* initial, const float* sums, float* states) {
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4, n = matrices * elems;
+  if (i >= n) return;
+  const long long m = i / elems;
+  float4 s = initial ? *reinterpret_cast<const float4*>(initial + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < segments; ++k) {
+    const int e = reverse ? segments - 1 - k : k;
+    float4* at = reinterpret_cast<float4*>(states + (size_t)e * n + i);
+    if (k > 0) {
+      const float f = __builtin_amdgcn_exp2f(sums[(size_t)(reverse ? e + 1 : e - 1) * matrices + m]);
+      const float4 a = *at;
+      s = make_float4(fmaf(f, s.x, a.x), fmaf(f, s.y, a.y), fmaf(f, s.z, a.z), fmaf(f, s.w, a.w));
+    }
+    *at = s;
+  }
+}
+
+// <gradient of the state, state> at the end of every segment: states [segments][n], the state in front of each; ends, the gradients behind each;
+// last: the state behind the last one (null: its gradient is zero).
+__global__ __launch_bounds__(256) void k_lin_crossing(int segments, long long matrices, int elems, const float* states, const float* ends, const float* last,
+                                                      const float* dlast, float* out) {
+  __shared__ float red[16];
+  const int seg = blockIdx.x % segments;
+  const long long m = blockIdx.x / segments, n = matrices * elems;
+  const bool end = seg == segments - 1;
+  const float* a = end ? (last ? last + m * elems : nullptr) : states + (size_t)(seg + 1) * n + m * elems;
+  const float* d = end ? (dlast ? dlast + m * elems : nullptr) : ends + (size_t)seg * n + m * elems;
+  float s = 0.f;
+  if (a && d)
+    for (int i = threadIdx.x * 4; i < elems; i += 1024) {
+      const float4 u = *reinterpret_cast<const float4*>(a + i), v = *reinterpret_cast<const float4*>(d + i);
+      s += u.x * v.x + u.y * v.y + u.z * v.z + u.w * v.w;
+    }
+  s = block_sum(s, red);
+  if (threadIdx.x == 0) out[blockIdx.x] = s;      // [matrix][segment]
+}
+
+// dg_t = crossing at the segment's end + sum over the segment's tokens from t on of (dq's dots - dv's); per_head: their sums over a segment instead,
+// into part [segment][B * H].  0 where the decay forgets everything.  One wave per segment and head.
+__global__ __launch_bounds__(64) void k_lin_decay_grad(int B, int L, int H, int segments, int seg_tokens, const float* up, const float* down, const float* crossing,
+                                                       LinDecay decay, float* dg, double* part) {
+  const int seg = blockIdx.x % segments, bh = blockIdx.x / segments, b = bh / H, h = bh - b * H, lane = threadIdx.x;
+  const int first = seg * seg_tokens, end = min(L, first + seg_tokens);
+  double run = crossing[blockIdx.x], sum = 0.0;
+  for (int t0 = first + (end - first - 1) / 64 * 64; t0 >= first; t0 -= 64) {
+    const int t = t0 + 63 - lane;                   // lane 0 holds the latest
+    const size_t at = ((size_t)b * L + t) * H + h;
+    double v = t < end ? (double)up[at] - (double)down[at] : 0.0;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double u = __shfl_up(v, o, 64);
+      if (lane >= o) v += u;
+    }
+    v += run;
+    run = __shfl(v, 63, 64);
+    if (t < end) {
+      if (decay.at(b, t, h, L, H) <= LIN_MIN_LOG) v = 0.0;
+      if (decay.per_token) dg[at] = (float)v;
+      else sum += v;
+    }
+  }
+  if (!decay.per_token) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) part[(size_t)seg * B * H + bh] = sum;
+  }
+}
+// One wave per head: the sum of part [rows][H].
+__global__ __launch_bounds__(64) void k_lin_decay_sum(int rows, int H, const double* part, float* dg) {
+  double s = 0.0;
+  for (int r = threadIdx.x; r < rows; r += 64) s += part[(size_t)r * H + blockIdx.x];
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (threadIdx.x == 0) dg[blockIdx.x] = (float)s;
+}
+
+// ---- one token: S' = e^g S + k v^T, o = scale S'^T q.  Bound by the state's way in and out.  A block has 32 columns of one head's state: 8 lanes of four columns,
+// 32 rows at a time.
+template <typename T>
+struct LinStepParams {
+  int H, DK, DV, per_token;            // g: [B, H] or [H]
+  const T* q; const T* k; const T* v;  // [B, H, D], batch strides
+  long long bsq, bsk, bsv;
+  const float* g;
+  const float* state;
+  float* state_out;                    // may be `state`
+  float scale;
+  T* out;                              // [B, H, DV]
+};
+template <typename T>
+__global__ __launch_bounds__(256) void k_lin_step(const LinStepParams<T> p) {
+  __shared__ float4 red[4][8];
+  const int parts = p.DV / 32, bh = blockIdx.x / parts, col = (blockIdx.x - bh * parts) * 32 + (threadIdx.x & 7) * 4, b = bh / p.H, h = bh - b * p.H;
+  const int row = threadIdx.x >> 3;
+  const float decay = __expf(p.g[p.per_token ? bh : h]);
+  const T* q = p.q + b * p.bsq + h * p.DK;
+  const T* k = p.k + b * p.bsk + h * p.DK;
+  float v[4];
+  Elem<T>::load4(p.v + b * p.bsv + h * p.DV + col, v);
+  const float* s = p.state + (size_t)bh * p.DK * p.DV + col;
+  float* s_out = p.state_out + (size_t)bh * p.DK * p.DV + col;
+  float4 x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (row + 32 * i < p.DK) x[i] = *reinterpret_cast<const float4*>(s + (size_t)(row + 32 * i) * p.DV);
+  float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = row + 32 * i;
+    if (r >= p.DK) break;
+    const float kr = Elem<T>::load(k + r), qr = Elem<T>::load(q + r);
+    const float4 y = make_float4(fmaf(decay, x[i].x, kr * v[0]), fmaf(decay, x[i].y, kr * v[1]), fmaf(decay, x[i].z, kr * v[2]), fmaf(decay, x[i].w, kr * v[3]));
+    *reinterpret_cast<float4*>(s_out + (size_t)r * p.DV) = y;
+    o[0] = fmaf(qr, y.x, o[0]); o[1] = fmaf(qr, y.y, o[1]); o[2] = fmaf(qr, y.z, o[2]); o[3] = fmaf(qr, y.w, o[3]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int m = 8; m < 64; m <<= 1) o[i] += __shfl_xor(o[i], m, 64);
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) < 8) red[wave][threadIdx.x & 7] = make_float4(o[0], o[1], o[2], o[3]);
+  __syncthreads();
+  if (threadIdx.x < 8) {
+    float4 a = red[0][threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+      const float4 u = red[w][threadIdx.x];
+      a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+    }
+    Elem<T>::store4(p.out + (size_t)bh * p.DV + col, a.x * p.scale, a.y * p.scale, a.z * p.scale, a.w * p.scale);
+  }
+}
+
+}  // namespace lact

@@ -1,0 +1,791 @@
+// Softmax attention of a sequence with itself under a mask of intervals, bf16 and fp32, head sizes 64 and 128, forward and backward:
+//
+//   s_ij = f(q_i . k_j / sqrt(D)) - slope_h |i - j|,   f(x) = cap tanh(x / cap) or x,   o_i = sum_j softmax_j(s_ij) v_j
+//
+// over the keys j in [lo_i, hi_i).  Every mask here is such an interval: a causal window (i - window < j <= i), packed documents (both
+// ends cut at the document's) and prefixes (hi_i reaches the end of the prefix).  For a key the queries that see it are an interval too.
+// k_attn_ranges writes both where there are documents; a causal window needs no memory for them.  A row that sees nothing has output 0.
+//
+// q: [B, L, H, D], k, v: [B, L, HK, D] with strides; a head's D elements are contiguous and heads follow each other; H is a multiple of
+// HK, and query heads h * H / HK ... share key head h.  out: [B, L, H, D] contiguous.  lse: [B, H, L] fp32, log2 of the row's sum of 2^s.
+//
+// One wave owns 32 rows (queries in the forward and in dq, keys in dk/dv) as the columns of 32x32 matrix products, so that a lane holds
+// one row and the softmax needs no exchange but where the row's maximum is moved; it walks the 64-row tiles of the other side that its
+// intervals touch, which travel through a ring of asynchronous global -> LDS copies shared by the block.  The scores feed the next
+// product as they lie: k slots 0..3 / 4..7 of lane half h stand for rows 4h + i / 8 + 4h + i of 16, on both operands.  fp32 runs the same
+// code: eight 32x32x2 products for one 32x32x16.
+//
+// A masked place weighs exactly nothing, whatever lies there: scores, probabilities and their gradients are selected, not multiplied,
+// and where a tile is masked for some row, values that are not finite are taken out of the product's other operand (0 * inf is NaN) and given
+// back as NaN to the rows that see them.
+#pragma once
+#include "gemm_dma.h"
+#include "window_attention.h"
+
+namespace lact {
+
+template <typename T>
+struct MaskedAttnParams {
+  int B, L, H, HK, group, window;    // group = H / HK; window >= L: none
+  const T* q; const T* k; const T* v;
+  int ldq, ldk, ldv;                 // elements between tokens
+  long long bsq, bsk, bsv;           // elements between batch entries
+  const int2* rows;                  // [B, L]: the keys that a query sees, null: those of the causal window
+  const int2* cols;                  // [B, L]: the queries that see a key
+  const float* slopes;               // [H] or null
+  float scale, cap;                  // cap 0: none
+  T* out;                            // [B, L, H, D]
+  float* lse;                        // [B, H, L]
+  // backward
+  const T* dout; int lddo; long long bsdo;
+  const T* o;
+  float* delta;                      // [B, H, L]: sum_d dout * out, written by dq, read by dk/dv
+  T* dq; T* dk; T* dv;               // contiguous
+  UDiv by_heads, by_kv;              // B * (blocks' heads), B * HK
+  __device__ __forceinline__ void locate(int& x, int& z) const {
+    x = by_heads.div(blockIdx.x);
+    z = blockIdx.x - x * (int)by_heads.d;
+  }
+  // Query heads that share a key head lie B * HK blocks apart: on one die, whose L2 then holds their keys, where that is a multiple of eight.
+  __device__ __forceinline__ void query_head(int z, int& b, int& h, int& hk) const {
+    const int g = by_kv.div(z), e = z - g * (int)by_kv.d;
+    b = e / HK;
+    hk = e - b * HK;
+    h = hk * group + g;
+  }
+  __device__ __forceinline__ int2 row_range(int b, int i) const {      // empty: {INT_MAX, 0}
+    if (i >= L) return make_int2(0x7fffffff, 0);
+    if (rows) {
+      const int2 r = rows[(size_t)b * L + i];
+      return r.x < r.y ? r : make_int2(0x7fffffff, 0);
+    }
+    return make_int2(max(0, i - window + 1), i + 1);
+  }
+  __device__ __forceinline__ int2 col_range(int b, int j) const {
+    if (j >= L) return make_int2(0x7fffffff, 0);
+    if (cols) {
+      const int2 r = cols[(size_t)b * L + j];
+      return r.x < r.y ? r : make_int2(0x7fffffff, 0);
+    }
+    return make_int2(j, window >= L ? L : min(L, j + window));
+  }
+};
+
+// Intervals from the documents' bounds [B, n + 1] (null: one document) and the lengths of their prefixes [B, n] (null: none).  Whatever the bounds hold, the
+// intervals lie inside [0, L).
+__global__ void k_attn_ranges(int B, int L, int n, int window, const int* __restrict__ bounds, const int* __restrict__ prefixes, int2* rows, int2* cols) {
+  const int b = blockIdx.y, t = blockIdx.x * blockDim.x + threadIdx.x;
+  if (t >= L) return;
+  int lo = 1, start = 0, end = L;
+  if (bounds) {
+    const int* bd = bounds + (size_t)b * (n + 1);
+    lo = 0;
+    for (int hi = n + 1; lo < hi;) {      // the first bound past t
+      const int m = (lo + hi) >> 1;
+      if (bd[m] <= t) lo = m + 1;
+      else hi = m;
+    }
+    start = lo > 0 ? bd[lo - 1] : 0;
+    end = lo <= n ? bd[lo] : 0;
+  }
+  int2 r = make_int2(0, 0), c = make_int2(0, 0);
+  if (lo > 0 && lo <= n) {
+    const int s = min(max(start, 0), L), e = min(max(end, 0), L);
+    if (s <= t && t < e) {
+      const int p = s + (prefixes ? min(max(prefixes[(size_t)b * n + lo - 1], 0), e - s) : 0);
+      r = make_int2(max(s, t - window + 1), max(t + 1, p));
+      c = make_int2(t < p ? s : t, window >= L ? e : min(e, t + window));
+    }
+  }
+  rows[(size_t)b * L + t] = r;
+  cols[(size_t)b * L + t] = c;
+}
+
+// ---- what depends on the element type ---------------------------------------------------------------
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+template <typename T> struct AttnType;
+template <> struct AttnType<uint16_t> { using Frag = bf16x8; };
+template <> struct AttnType<float> { using Frag = f32x8; };
+
+__device__ __forceinline__ f32x16 mma32(const f32x8& a, const f32x8& b, f32x16 c) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) c = mma32(a[i], b[i], c);
+  return c;
+}
+
+template <typename T, int D>
+struct MaskTile {       // 64 x D, the 16-byte granule g of row r at slot g ^ key(r): 16 rows of one granule fall into different banks
+  static constexpr int ROWB = D * (int)sizeof(T), G = ROWB / 16, BYTES = 64 * ROWB;
+  __device__ static __forceinline__ int key(int r) {
+    if constexpr (sizeof(T) == 2) return AttnTile<D>::key(r);
+    else return r & 15;
+  }
+};
+
+template <typename T, int D, int NW>
+struct MaskCopy {
+  using S = MaskTile<T, D>;
+  static constexpr int NC = S::G / NW;      // copies of a wave and tile
+  static_assert(S::G % NW == 0, "copies must split evenly over the waves");
+  uint32_t voff[NC], vlast[NC];
+  const T* base;
+  int step, last;
+  // the 64-row tiles [0, n) from row `first` on of a head whose rows end at L
+  __device__ __forceinline__ void init(int wave, const T* head, int ld, int first, int n, int L) {
+    base = uniform(head + (size_t)first * ld);
+    step = 64 * ld; last = n - 1;
+    const int rows = L - 1 - (first + last * 64);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (wave + i * NW) * 64 + (threadIdx.x & 63), row = c / S::G, slot = c % S::G;
+      const uint32_t col = (uint32_t)(slot ^ S::key(row)) * 16;
+      voff[i] = (uint32_t)row * ld * sizeof(T) + col;
+      vlast[i] = (uint32_t)min(row, rows) * ld * sizeof(T) + col;      // rows past the end repeat the last one
+    }
+  }
+  __device__ __forceinline__ void issue(int t, const T* from, uint32_t lds, int wave) const {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) dma16<false>(from + (long long)t * step, t == last ? vlast[i] : voff[i], lds + (wave + i * NW) * 1024);
+  }
+};
+
+template <typename T, int D> struct MaskFrag;
+template <int D> struct MaskFrag<uint16_t, D> : AttnFrag<D> {};
+template <int D>
+struct MaskFrag<float, D> {
+  using S = MaskTile<float, D>;
+  uint32_t row_base, row_key, col_off[8];
+  __device__ __forceinline__ void init() {
+    const int l = threadIdx.x & 63, h = l >> 5;
+    row_base = (l & 31) * S::ROWB;
+    row_key = (l & 15) << 4;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = (j < 4 ? 0 : 4) + 4 * h + j;      // tile row of slot j: 4h + j, 8 + 4h + j - 4
+      col_off[j] = r * S::ROWB + (((((l & 31) >> 2) ^ r) << 4) | ((l & 3) << 2));
+    }
+  }
+  __device__ __forceinline__ f32x8 rows(const char* tile, int rt, int ks) const {
+    const uint32_t g = (uint32_t)(ks * 4 + 2 * ((threadIdx.x & 63) >> 5)) << 4;
+    const char* p = tile + rt * 32 * S::ROWB + row_base;
+    const float4 a = *reinterpret_cast<const float4*>(p + (g ^ row_key)), b = *reinterpret_cast<const float4*>(p + ((g + 16) ^ row_key));
+    return f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  }
+  __device__ __forceinline__ f32x8 cols(const char* tile, int dt, int st) const {
+    f32x8 v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      v[j] = *reinterpret_cast<const float*>(tile + st * 16 * S::ROWB + (dt >> 1) * 256 + (col_off[j] ^ (uint32_t)((dt & 1) << 7)));
+    return v;
+  }
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void mask_own_rows(typename AttnType<T>::Frag (&f)[D / 16], const T* base, int ld, int row, int L) {
+  if constexpr (sizeof(T) == 2) {
+    attn_own_rows<D>(f, base, ld, row, L);
+  } else {
+    const T* p = base + (size_t)min(row, L - 1) * ld + 8 * ((threadIdx.x & 63) >> 5);
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      const float4 a = *reinterpret_cast<const float4*>(p + s * 16), b = *reinterpret_cast<const float4*>(p + s * 16 + 4);
+      f[s] = f32x8{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    }
+  }
+}
+// See attn_arrived: what was loaded is there behind this, so that no wait for it lies in the loop.
+template <int N>
+__device__ __forceinline__ void mask_arrived(bf16x8 (&f)[N]) { attn_arrived(f); }
+template <int N>
+__device__ __forceinline__ void mask_arrived(f32x8 (&f)[N]) {
+#pragma unroll
+  for (int s = 0; s < N; ++s) asm volatile("" : "+v"(f[s]));
+}
+
+// Eight of a lane's accumulators as an operand.  bf16: probabilities and their gradients are rounded to 8 bits for the product, whose
+// sum stays in fp32.
+template <typename T>
+__device__ __forceinline__ typename AttnType<T>::Frag mask_pack(const f32x16& s, int st) {
+  if constexpr (sizeof(T) == 2) return attn_pack(s, st);
+  else return f32x8{s[8 * st], s[8 * st + 1], s[8 * st + 2], s[8 * st + 3], s[8 * st + 4], s[8 * st + 5], s[8 * st + 6], s[8 * st + 7]};
+}
+
+// Whether an operand holds something that is not finite; bit j of the result: slot j does.
+__device__ __forceinline__ uint32_t unfinite(const bf16x8& f) {
+  const uint4 u = __builtin_bit_cast(uint4, f);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m |= ((w[i] & 0x7f80u) == 0x7f80u ? 1u << (2 * i) : 0u) | ((w[i] & 0x7f800000u) == 0x7f800000u ? 2u << (2 * i) : 0u);
+  return m;
+}
+__device__ __forceinline__ uint32_t unfinite(const f32x8& f) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m |= (__float_as_uint(f[i]) & 0x7f800000u) == 0x7f800000u ? 1u << i : 0u;
+  return m;
+}
+template <int N>
+__device__ __forceinline__ bool any_unfinite(const bf16x8 (&f)[N]) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int s = 0; s < N; ++s) {
+    const uint4 u = __builtin_bit_cast(uint4, f[s]);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+  }
+  return m[0] >= 0x7f80 || m[1] >= 0x7f80;
+}
+template <int N>
+__device__ __forceinline__ bool any_unfinite(const f32x8 (&f)[N]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int s = 0; s < N; ++s)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[s][i]) & 0x7fffffffu);
+  return m >= 0x7f800000u;
+}
+__device__ __forceinline__ void drop(bf16x8& f, uint32_t bad) {
+  uint4 u = __builtin_bit_cast(uint4, f);
+  uint32_t* w = &u.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] &= (bad >> (2 * i) & 1 ? 0u : 0xffffu) | (bad >> (2 * i) & 2 ? 0u : 0xffff0000u);
+  f = __builtin_bit_cast(bf16x8, u);
+}
+__device__ __forceinline__ void drop(f32x8& f, uint32_t bad) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = bad >> i & 1 ? 0.f : f[i];
+}
+// Takes what is not finite out of the operands of 16 tile rows; bit j of the result: the row of this lane's slot j held such a value
+// in any column.
+template <typename F, int N>
+__device__ __forceinline__ uint32_t make_finite(F (&f)[N]) {
+  uint32_t bad = 0, rows = 0;
+#pragma unroll
+  for (int s = 0; s < N; ++s) {
+    const uint32_t m = unfinite(f[s]);
+    drop(f[s], m);
+    bad |= m;
+  }
+  const int half = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint64_t who = __ballot(bad >> j & 1);
+    rows |= (uint32_t)(who >> (32 * half)) ? 1u << j : 0u;
+  }
+  return rows;
+}
+
+// tanh in fp32.  Small x: Lambert's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + x^2 / (7 + x^2 / 9)))), relative error below 1e-8
+// up to 0.8; 1 - 2 / (1 + e^2x) there loses the bits that x has below 1.
+__device__ __forceinline__ float tanh_f32(float x) {
+  const float a = fabsf(x), y = a * a;
+  const float near = a * fmaf(y, fmaf(y, 1.f, 105.f), 945.f) / fmaf(y, fmaf(y, 15.f, 420.f), 945.f);
+  const float far = 1.f - 2.f / (1.f + __builtin_amdgcn_exp2f(a * (2.f * ATTN_LOG2E)));
+  return copysignf(a < 0.8f ? near : far, x);
+}
+
+// Scores as they come out of the product -> what 2^ is taken of, times `unit` (see below)
+template <typename T>
+struct Scores {
+  float c;          // log2(e) / sqrt(D) without a cap: the scores then keep it out until they meet the maximum
+  float k1, k2;     // with a cap: 2 log2(e) scale / cap, cap log2(e)
+  float slope;      // times log2(e)
+  bool cap, bias;
+  __device__ __forceinline__ void init(float scale, float cap_, const float* slopes, int h) {
+    cap = cap_ > 0.f; bias = slopes != nullptr;
+    k1 = sizeof(T) == 2 ? 2.f * ATTN_LOG2E * scale / cap_ : scale / cap_;
+    k2 = cap_ * ATTN_LOG2E;
+    slope = bias ? slopes[h] * ATTN_LOG2E : 0.f;
+    c = scale * ATTN_LOG2E;
+  }
+  // what is left to multiply by behind apply()
+  __device__ __forceinline__ float unit() const { return cap || bias ? 1.f : c; }
+  __device__ __forceinline__ float bent(float s) const {      // tanh of the score over the cap
+    if constexpr (sizeof(T) == 2) return fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * k1)), -2.f, 1.f);   // to 2^-23
+    else return tanh_f32(s * k1);
+  }
+  // `first`: the place of the lane's element 0 minus the place of its own row
+  __device__ __forceinline__ void apply(f32x16& s, int first) const {
+    if (cap) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[j] = bent(s[j]) * k2;
+    } else if (bias) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[j] *= c;
+    }
+    lower(s, first);
+  }
+  // the same, and the gradients dp (of what the softmax weighs) times the derivative of the cap
+  __device__ __forceinline__ void apply(f32x16& s, f32x16& dp, int first) const {
+    if (cap) {
+      f32x16 t;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) t[j] = bent(s[j]);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[j] = t[j] * k2;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) dp[j] *= fmaf(-t[j], t[j], 1.f);
+    } else if (bias) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[j] *= c;
+    }
+    lower(s, first);
+  }
+  __device__ __forceinline__ void lower(f32x16& s, int first) const {
+    if (!bias) return;
+    const float f = (float)first;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s[j] = fmaf(fabsf(f + (float)(8 * (j / 4) + j % 4)), -slope, s[j]);
+  }
+};
+
+template <typename T, int D> constexpr int mask_ring() { return sizeof(T) == 2 ? 3 : 2; }      // 64-row tiles of both operands in LDS
+template <typename T, int D, int NW>
+constexpr int mask_lds_bytes(bool stats) {
+  constexpr int R = mask_ring<T, D>();
+  return cmax(R * 2 * MaskTile<T, D>::BYTES + (stats ? R * 512 : 0), NW * 32 * (D + 16 / (int)sizeof(T)) * (int)sizeof(T));
+}
+
+// Walks the tiles [0, n): issue(t) starts the copies of tile t, COPIES of a wave, RING - 1 tiles ahead; body(t) uses it.
+template <int COPIES, int RING, typename Issue, typename Body>
+__device__ __forceinline__ void mask_walk(int n, Issue issue, Body body) {
+#pragma unroll
+  for (int t = 0; t < RING - 1; ++t)
+    if (t < n) issue(t);
+  for (int t = 0; t < n; ++t) {
+    if (RING == 3 && t + 1 < n) wait_vmcnt<COPIES>();
+    else wait_vmcnt<0>();
+    __syncthreads();      // tile t is there for every wave, and all are through with t - 1, whose place the next one takes
+    if (t + RING - 1 < n) issue(t + RING - 1);
+    body(t);
+  }
+}
+
+// A wave's [D][32] accumulator (rows = D, columns = its own rows), times `f`, to 32 rows of a tensor with rows ld apart.
+template <typename T, int D>
+__device__ __forceinline__ void mask_store_rows(char* lds, const f32x16 (&acc)[D / 32], float f, T* out, size_t ld, int row0, int L) {
+  constexpr int E = 16 / (int)sizeof(T), LD = D + E, LPR = D / E;
+  const int l = threadIdx.x & 63;
+  T* t = reinterpret_cast<T*>(lds);
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      Elem<T>::store4(t + (l & 31) * LD + dt * 32 + 8 * g + 4 * (l >> 5), acc[dt][4 * g] * f, acc[dt][4 * g + 1] * f, acc[dt][4 * g + 2] * f, acc[dt][4 * g + 3] * f);
+  wave_lds_fence();
+#pragma unroll
+  for (int i = 0; i < 32 * LPR / 64; ++i) {
+    const int id = i * 64 + l, r = id / LPR, c = (id % LPR) * E;
+    const uint4 u = *reinterpret_cast<const uint4*>(t + r * LD + c);
+    if (row0 + r < L) *reinterpret_cast<uint4*>(out + (size_t)(row0 + r) * ld + c) = u;
+  }
+  wave_lds_fence();
+}
+
+// Intervals of the rows [row0, row0 + 32 N) that a wave sees as one: union (x, y), and for its own 32 the largest lower and least upper end.
+__device__ __forceinline__ int wave_min(int v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ int wave_max(int v) { return -wave_min(-v); }
+
+struct WaveReach {
+  int lo, hi;          // union over the wave's rows
+  int full_lo, full_hi;  // what every one of them sees
+  __device__ __forceinline__ void init(int2 own) {
+    lo = wave_min(own.x); hi = wave_max(own.y);
+    full_lo = wave_max(own.x); full_hi = wave_min(own.y);
+  }
+  __device__ __forceinline__ bool sees(int a, int n) const { return a < hi && a + n > lo; }
+  __device__ __forceinline__ bool masked(int a, int n) const { return a < full_lo || a + n > full_hi; }
+};
+
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_fwd(const MaskedAttnParams<T> p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  using S = MaskTile<T, D>;
+  using Copy = MaskCopy<T, D, NW>;
+  using Frag = typename AttnType<T>::Frag;
+  constexpr int STAGE = 2 * S::BYTES, RING = mask_ring<T, D>();
+  prefetch_args<sizeof(p)>();
+  int bx, z, b, h, hk;
+  p.locate(bx, z);
+  bx = (p.L - 1) / (32 * NW) - bx;      // the longest rows of a causal mask first
+  p.query_head(z, b, h, hk);
+  const int L = p.L;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int blk0 = bx * 32 * NW, row0 = blk0 + wave * 32, row = row0 + (lane & 31);
+  Frag qf[D / 16];
+  mask_own_rows<T, D>(qf, p.q + b * p.bsq + h * D, p.ldq, row, L);
+  const int2 own = p.row_range(b, row);
+  WaveReach reach;
+  reach.init(own);
+  int first = 0x7fffffff, last = 0;
+#pragma unroll
+  for (int i = 0; i < NW / 2; ++i) {
+    const int2 r = p.row_range(b, blk0 + i * 64 + lane);
+    first = min(first, r.x); last = max(last, r.y);
+  }
+  first = wave_min(first); last = wave_max(last);
+  Scores<T> sc;
+  sc.init(p.scale, p.cap, p.slopes, h);
+  MaskFrag<T, D> fr;
+  fr.init();
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+  const float c = sc.unit();
+  float mc = -1e30f, sum = 0.f;        // running row maximum (of what 2^ is taken of) and this lane's share of the row sum
+  first = min(first, L) / 64 * 64;
+  const int tiles = last > first ? (last - first + 63) / 64 : 0;
+  Copy ck, cv;
+  ck.init(wave, p.k + b * p.bsk + hk * D, p.ldk, first, tiles, L);
+  cv.init(wave, p.v + b * p.bsv + hk * D, p.ldv, first, tiles, L);
+  const uint32_t lds0 = lds_addr(smem);
+  auto larger = [](float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_inff()); };
+  mask_arrived(qf);
+  mask_walk<2 * Copy::NC, RING>(tiles,
+    [&](int t) LACT_INLINE_LAMBDA {
+      const uint32_t slot = lds0 + t % RING * STAGE;
+      ck.issue(t, ck.base, slot, wave);
+      cv.issue(t, cv.base, slot + S::BYTES, wave);
+    },
+    [&](int t) LACT_INLINE_LAMBDA {
+      const int k0 = first + t * 64;
+      if (!reach.sees(k0, 64)) return;
+      const char* kt = smem + t % RING * STAGE;
+      const char* vt = kt + S::BYTES;
+      f32x16 s[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[i][j] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s[i] = mma32(fr.rows(kt, i, ks), qf[ks], s[i]);
+      const int at = k0 + 4 * (lane >> 5);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) sc.apply(s[i], at + 32 * i - row);
+      const bool masked = reach.masked(k0, 64);
+      if (masked) {
+        const int lo = own.x - at, hi = own.y - at;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int key = i * 32 + 8 * (j / 4) + j % 4;
+            s[i][j] = (key >= lo && key < hi) ? s[i][j] : -__builtin_inff();
+          }
+      }
+      float mx = larger(s[0][0], s[1][0]);
+#pragma unroll
+      for (int j = 1; j < 16; ++j) mx = larger(mx, larger(s[0][j], s[1][j]));
+      mx *= c;
+      // The maximum only has to keep exp2 in range: it follows the row when it is exceeded by more than 2^8 (its own row only: what a row
+      // gives does not depend on the others).
+      if (__any(mx > mc + 8.f)) {
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float nm = mx > mc + 8.f ? mx : mc, f = __builtin_amdgcn_exp2f(mc - nm);
+        mc = nm;
+        sum *= f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[i][j] *= f;
+      }
+      float part[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          s[i][j] = __builtin_amdgcn_exp2f(fmaf(s[i][j], c, -mc));
+          part[i] += s[i][j];
+        }
+      sum += part[0] + part[1];
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        const Frag pf = mask_pack<T>(s[st >> 1], st & 1);
+        Frag vb[D / 32];
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) vb[dt] = fr.cols(vt, dt, st);
+        if (masked && __any(any_unfinite(vb))) {
+          const uint32_t bad = make_finite(vb);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int key = at + 16 * st + (j < 4 ? j : 4 + j);
+            if ((bad >> j & 1) && key >= own.x && key < own.y) sum = __builtin_nanf("");
+          }
+        }
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) o[dt] = mma32(vb[dt], pf, o[dt]);
+      }
+    });
+  sum += __shfl_xor(sum, 32, 64);
+  const bool empty = own.x >= own.y;
+  if (lane < 32 && row < L) p.lse[(size_t)(b * p.H + h) * L + row] = empty ? 0.f : mc + __builtin_amdgcn_logf(sum);   // v_log_f32 is base 2
+  __syncthreads();
+  mask_store_rows<T, D>(smem + wave * 32 * (D + 16 / sizeof(T)) * sizeof(T), o, empty ? 0.f : 1.f / sum, p.out + ((size_t)b * L * p.H + h) * D, (size_t)p.H * D, row0, L);
+}
+
+// dq = scale * sum_keys ds k with ds = p (dp - delta) f', and delta itself.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dq(const MaskedAttnParams<T> p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  using S = MaskTile<T, D>;
+  using Copy = MaskCopy<T, D, NW>;
+  using Frag = typename AttnType<T>::Frag;
+  constexpr int STAGE = 2 * S::BYTES, RING = mask_ring<T, D>();
+  prefetch_args<sizeof(p)>();
+  int bx, z, b, h, hk;
+  p.locate(bx, z);
+  bx = (p.L - 1) / (32 * NW) - bx;
+  p.query_head(z, b, h, hk);
+  const int L = p.L;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int blk0 = bx * 32 * NW, row0 = blk0 + wave * 32, row = row0 + (lane & 31);
+  Frag qf[D / 16], gf[D / 16];
+  mask_own_rows<T, D>(gf, p.dout + b * p.bsdo + h * D, p.lddo, row, L);
+  float delta = 0.f;
+  {
+    Frag of[D / 16];
+    mask_own_rows<T, D>(of, p.o + ((size_t)b * L * p.H + h) * D, p.H * D, row, L);
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) delta += (float)gf[s][i] * (float)of[s][i];
+    delta += __shfl_xor(delta, 32, 64);
+  }
+  const size_t stat = (size_t)(b * p.H + h) * L;
+  if (lane < 32 && row < L) p.delta[stat + row] = delta;
+  mask_own_rows<T, D>(qf, p.q + b * p.bsq + h * D, p.ldq, row, L);
+  float lse = p.lse[stat + min(row, L - 1)];
+  const int2 own = p.row_range(b, row);
+  WaveReach reach;
+  reach.init(own);
+  int first = 0x7fffffff, last = 0;
+#pragma unroll
+  for (int i = 0; i < NW / 2; ++i) {
+    const int2 r = p.row_range(b, blk0 + i * 64 + lane);
+    first = min(first, r.x); last = max(last, r.y);
+  }
+  first = wave_min(first); last = wave_max(last);
+  Scores<T> sc;
+  sc.init(p.scale, p.cap, p.slopes, h);
+  MaskFrag<T, D> fr;
+  fr.init();
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+  const float c = sc.unit();
+  first = min(first, L) / 64 * 64;
+  const int tiles = last > first ? (last - first + 63) / 64 : 0;
+  Copy ck, cv;
+  ck.init(wave, p.k + b * p.bsk + hk * D, p.ldk, first, tiles, L);
+  cv.init(wave, p.v + b * p.bsv + hk * D, p.ldv, first, tiles, L);
+  const uint32_t lds0 = lds_addr(smem);
+  mask_arrived(qf);
+  mask_arrived(gf);
+  asm volatile("" : "+v"(lse), "+v"(delta));
+  mask_walk<2 * Copy::NC, RING>(tiles,
+    [&](int t) LACT_INLINE_LAMBDA {
+      const uint32_t slot = lds0 + t % RING * STAGE;
+      ck.issue(t, ck.base, slot, wave);
+      cv.issue(t, cv.base, slot + S::BYTES, wave);
+    },
+    [&](int t) LACT_INLINE_LAMBDA {
+      const char* kt = smem + t % RING * STAGE;
+      const char* vt = kt + S::BYTES;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int k0 = first + t * 64 + 32 * i;
+        if (!reach.sees(k0, 32)) continue;
+        f32x16 s, dp;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = dp[j] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          s = mma32(fr.rows(kt, i, ks), qf[ks], s);
+          dp = mma32(fr.rows(vt, i, ks), gf[ks], dp);
+        }
+        const int at = k0 + 4 * (lane >> 5);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) dp[j] -= delta;
+        sc.apply(s, dp, at - row);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], c, -lse)) * dp[j];
+        const bool masked = reach.masked(k0, 32);
+        if (masked) {
+          const int lo = own.x - at, hi = own.y - at;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int key = 8 * (j / 4) + j % 4;
+            s[j] = (key >= lo && key < hi) ? s[j] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const Frag pf = mask_pack<T>(s, st);
+          Frag kb[D / 32];
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt) kb[dt] = fr.cols(kt, dt, 2 * i + st);
+          // (a row that sees such a key has a gradient of its score that is not finite)
+          if (masked && __any(any_unfinite(kb))) make_finite(kb);
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt) o[dt] = mma32(kb[dt], pf, o[dt]);
+        }
+      }
+    });
+  __syncthreads();
+  mask_store_rows<T, D>(smem + wave * 32 * (D + 16 / sizeof(T)) * sizeof(T), o, p.scale, p.dq + ((size_t)b * L * p.H + h) * D, (size_t)p.H * D, row0, L);
+}
+
+// dv = sum_queries p dout, dk = scale * sum_queries ds q, over the queries of all heads that share the key head: a wave owns 32 keys and
+// walks the queries that see them, head after head.
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dkv(const MaskedAttnParams<T> p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  using S = MaskTile<T, D>;
+  using Copy = MaskCopy<T, D, NW>;
+  using Frag = typename AttnType<T>::Frag;
+  constexpr int STAGE = 2 * S::BYTES, RING = mask_ring<T, D>();
+  prefetch_args<sizeof(p)>();
+  int bx, z;
+  p.locate(bx, z);
+  const int b = z / p.HK, hk = z - b * p.HK, L = p.L;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int blk0 = bx * 32 * NW, row0 = blk0 + wave * 32, row = row0 + (lane & 31);
+  Frag kf[D / 16], vf[D / 16];
+  mask_own_rows<T, D>(kf, p.k + b * p.bsk + hk * D, p.ldk, row, L);
+  mask_own_rows<T, D>(vf, p.v + b * p.bsv + hk * D, p.ldv, row, L);
+  const int2 own = p.col_range(b, row);
+  WaveReach reach;
+  reach.init(own);
+  int first = 0x7fffffff, last = 0;
+#pragma unroll
+  for (int i = 0; i < NW / 2; ++i) {
+    const int2 r = p.col_range(b, blk0 + i * 64 + lane);
+    first = min(first, r.x); last = max(last, r.y);
+  }
+  first = wave_min(first); last = wave_max(last);
+  MaskFrag<T, D> fr;
+  fr.init();
+  f32x16 ok[D / 32], ov[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) ok[i][j] = ov[i][j] = 0.f;
+  first = min(first, L) / 64 * 64;
+  const int tiles = last > first ? (last - first + 63) / 64 : 0, all = tiles * p.group;
+  const uint32_t lds0 = lds_addr(smem);
+  const char* stats = smem + RING * STAGE;             // per ring slot: 64 lse, 64 delta
+  const int h0 = hk * p.group;
+  Copy cq, cg;
+  cq.init(wave, p.q + b * p.bsq + h0 * D, p.ldq, first, tiles, L);
+  cg.init(wave, p.dout + b * p.bsdo + h0 * D, p.lddo, first, tiles, L);
+  // the even waves bring the slot's lse, the odd ones its delta: the same bytes from each, one copy per wave
+  const float* st_src = (wave & 1 ? p.delta : p.lse) + (size_t)(b * p.H + h0) * L;
+  int ih = 0, it = 0, bh = 0, bt = 0;                  // head and tile of the next copies, and of the next use
+  float poison = 0.f;
+  Scores<T> sc;
+  sc.init(p.scale, p.cap, p.slopes, h0);
+  const float c = sc.unit();
+  mask_arrived(kf);
+  mask_arrived(vf);
+  mask_walk<2 * Copy::NC + 1, RING>(all,
+    [&](int t) LACT_INLINE_LAMBDA {
+      const uint32_t slot = t % RING;
+      cq.issue(it, cq.base + ih * D, lds0 + slot * STAGE, wave);
+      cg.issue(it, cg.base + ih * D, lds0 + slot * STAGE + S::BYTES, wave);
+      const int q0 = first + it * 64;
+      dma4(st_src + (size_t)ih * L + q0, (uint32_t)min(lane, L - 1 - q0) * 4, lds0 + RING * STAGE + slot * 512 + (wave & 1) * 256);
+      if (++it == tiles) { it = 0; ++ih; }
+    },
+    [&](int t) LACT_INLINE_LAMBDA {
+      const int slot = t % RING, t0 = first + bt * 64;
+      if (bt == 0 && p.slopes) sc.slope = p.slopes[h0 + bh] * ATTN_LOG2E;
+      if (++bt == tiles) { bt = 0; ++bh; }
+      const char* qt = smem + slot * STAGE;
+      const char* gt = qt + S::BYTES;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int q0 = t0 + i * 32;
+        if (!reach.sees(q0, 32)) continue;
+        f32x16 s, ds;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = ds[j] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          s = mma32(fr.rows(qt, i, ks), kf[ks], s);
+          ds = mma32(fr.rows(gt, i, ks), vf[ks], ds);
+        }
+        const float* ls = reinterpret_cast<const float*>(stats + slot * 512) + i * 32 + 4 * (lane >> 5);
+        const int at = q0 + 4 * (lane >> 5);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 d4 = *reinterpret_cast<const float4*>(ls + 64 + 8 * g);
+          ds[4 * g] -= d4.x; ds[4 * g + 1] -= d4.y; ds[4 * g + 2] -= d4.z; ds[4 * g + 3] -= d4.w;
+        }
+        sc.apply(s, ds, at - row);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 l4 = *reinterpret_cast<const float4*>(ls + 8 * g);
+          const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            s[4 * g + j] = __builtin_amdgcn_exp2f(fmaf(s[4 * g + j], c, -lv[j]));
+            ds[4 * g + j] *= s[4 * g + j];
+          }
+        }
+        const bool masked = reach.masked(q0, 32);
+        const int lo = own.x - at, hi = own.y - at;
+        if (masked) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int qi = 8 * (j / 4) + j % 4;
+            const bool seen = qi >= lo && qi < hi;
+            s[j] = seen ? s[j] : 0.f;
+            ds[j] = seen ? ds[j] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const Frag pf = mask_pack<T>(s, st), df = mask_pack<T>(ds, st);
+          Frag fb[D / 32];
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt) fb[dt] = fr.cols(gt, dt, 2 * i + st);
+          if (masked && __any(any_unfinite(fb))) {
+            const uint32_t bad = make_finite(fb);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int qi = 16 * st + (j < 4 ? j : 4 + j);
+              if ((bad >> j & 1) && qi >= lo && qi < hi) poison = __builtin_nanf("");
+            }
+          }
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt) ov[dt] = mma32(fb[dt], pf, ov[dt]);
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt) fb[dt] = fr.cols(qt, dt, 2 * i + st);
+          if (masked && __any(any_unfinite(fb))) make_finite(fb);
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt) ok[dt] = mma32(fb[dt], df, ok[dt]);
+        }
+      }
+    });
+  poison += __shfl_xor(poison, 32, 64);
+  __syncthreads();
+  const size_t o = ((size_t)b * L * p.HK + hk) * D;
+  char* stage = smem + wave * 32 * (D + 16 / sizeof(T)) * sizeof(T);
+  mask_store_rows<T, D>(stage, ok, p.scale, p.dk + o, (size_t)p.HK * D, row0, L);
+  mask_store_rows<T, D>(stage, ov, 1.f + poison, p.dv + o, (size_t)p.HK * D, row0, L);
+}
+
+}  // namespace lact

@@ -1,0 +1,439 @@
+// Host side of the token mixers of liblact_hip.so (masked_attention.h, attention_step.h, linear_attention.h): checks the arguments and
+// enqueues the kernels on the caller's stream.  No allocation, no synchronisation.
+#include "../../include/lact_hip.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "host_common.h"
+#include "attention_step.h"
+#include "linear_attention.h"
+
+using namespace lact;
+
+namespace {
+
+constexpr int COMPUTE_UNITS = 256;
+constexpr long long MAX_GRID = (1LL << 31) - 1;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+int check_type(int act) { return act == LACT_BF16 || act == LACT_F32 ? 0 : fail("act_dtype must be LACT_BF16 or LACT_F32"); }
+
+// [B, L, heads, D] with heads contiguous inside a token
+int check_rows(const void* ptr, int ld, long long bs, int width, int act, const char* what) {
+  const int al = act == LACT_BF16 ? 8 : 4;
+  if (!ptr) return fail(std::string("null pointer: ") + what);
+  if (ld % al || bs % al || ld < width || bs < 0 || !aligned16(ptr)) return fail(std::string(what) + ": rows must be 16-byte aligned and hold all heads");
+  if (ld > (1 << 23)) return fail(std::string(what) + ": row stride too large");
+  return 0;
+}
+
+// ---- attention ----------------------------------------------------------------------------------
+int check_attention(const lact_attention_desc_t* d) {
+  if (!d) return fail("null descriptor");
+  if (check_type(d->act_dtype)) return -1;
+  if (d->B <= 0 || d->L <= 0 || d->H <= 0 || d->HK <= 0 || d->window <= 0) return fail("masked attention: B, L, H, HK and window must be positive");
+  if (d->D != 64 && d->D != 128) return fail("masked attention: head size must be 64 or 128");
+  if (d->H % d->HK) return fail("masked attention: the number of key heads must divide that of query heads");
+  if (d->L > (1 << 24) || (long long)d->B * d->H > (1 << 20) || (long long)d->B * d->H * ceil_div(d->L, 128) > MAX_GRID || d->B > 65535)
+    return fail("masked attention: sequence or batch too large");
+  if (!(d->scale > 0.f) || !std::isfinite(d->scale)) return fail("masked attention: the scale must be positive");
+  if (!(d->score_cap >= 0.f) || !std::isfinite(d->score_cap)) return fail("masked attention: the score cap must be positive, or 0 for none");
+  if (d->n_documents < 0 || d->n_documents > (1 << 24)) return fail("masked attention: bad number of documents");
+  if (!d->n_documents && (d->documents || d->prefixes)) return fail("masked attention: documents or prefixes without their number");
+  return 0;
+}
+
+template <typename T>
+int attention_params(const lact_attention_desc_t* d, const void* q, const void* k, const void* v, void* ranges, MaskedAttnParams<T>* p) {
+  memset(p, 0, sizeof(*p));
+  if (check_rows(q, d->q_ld, d->q_bs, d->H * d->D, d->act_dtype, "q") || check_rows(k, d->k_ld, d->k_bs, d->HK * d->D, d->act_dtype, "k") ||
+      check_rows(v, d->v_ld, d->v_bs, d->HK * d->D, d->act_dtype, "v"))
+    return -1;
+  if (d->n_documents && !ranges) return fail("null pointer: ranges");
+  p->B = d->B; p->L = d->L; p->H = d->H; p->HK = d->HK; p->group = d->H / d->HK;
+  p->window = std::min(d->window, d->L);
+  p->q = static_cast<const T*>(q); p->k = static_cast<const T*>(k); p->v = static_cast<const T*>(v);
+  p->ldq = d->q_ld; p->ldk = d->k_ld; p->ldv = d->v_ld;
+  p->bsq = d->q_bs; p->bsk = d->k_bs; p->bsv = d->v_bs;
+  if (d->n_documents) {
+    p->rows = static_cast<const int2*>(ranges);
+    p->cols = p->rows + (size_t)d->B * d->L;
+  }
+  p->slopes = d->slopes; p->scale = d->scale; p->cap = d->score_cap;
+  p->by_kv = make_udiv(d->B * d->HK);
+  return 0;
+}
+
+// Waves per block: 8 (256 rows) once that gives every compute unit a block, else 4.  which: 0 forward, 1 dq, 2 dk and dv
+template <typename T, int D, int NW>
+void launch_attention(int which, MaskedAttnParams<T> p, hipStream_t s) {
+  const int heads = p.B * (which == 2 ? p.HK : p.H);
+  p.by_heads = make_udiv(heads);
+  const dim3 grid(ceil_div(p.L, 32 * NW) * heads), block(64 * NW);
+  constexpr int SM = mask_lds_bytes<T, D, NW>(false), SMS = mask_lds_bytes<T, D, NW>(true);
+  const double w = p.window, f = 2.0 * ((double)p.L * w - w * (w - 1) / 2) * D * p.B * p.H;      // without documents
+  if (which == 0) {
+    LACT_BIG_LDS((k_masked_attn_fwd<T, D, NW>), SM);
+    LACT_LAUNCH_SMEM("k_masked_attn_fwd", "masked_attn", 2 * f, (k_masked_attn_fwd<T, D, NW>), grid, block, SM, s, p);
+  } else if (which == 1) {
+    LACT_BIG_LDS((k_masked_attn_dq<T, D, NW>), SM);
+    LACT_LAUNCH_SMEM("k_masked_attn_dq", "masked_attn_bwd", 3 * f, (k_masked_attn_dq<T, D, NW>), grid, block, SM, s, p);
+  } else {
+    LACT_BIG_LDS((k_masked_attn_dkv<T, D, NW>), SMS);
+    LACT_LAUNCH_SMEM("k_masked_attn_dkv", "masked_attn_bwd", 4 * f, (k_masked_attn_dkv<T, D, NW>), grid, block, SMS, s, p);
+  }
+}
+template <typename T, int D>
+void launch_attention(int which, const MaskedAttnParams<T>& p, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if ((long long)ceil_div(p.L, 256) * p.B * (which == 2 ? p.HK : p.H) >= COMPUTE_UNITS) return launch_attention<T, D, 8>(which, p, s);
+  }
+  launch_attention<T, D, 4>(which, p, s);
+}
+template <typename T>
+void launch_attention(int which, int D, const MaskedAttnParams<T>& p, hipStream_t s) {
+  if (D == 128) launch_attention<T, 128>(which, p, s);
+  else launch_attention<T, 64>(which, p, s);
+}
+
+template <typename T>
+int attention_forward(const lact_attention_desc_t* d, const void* q, const void* k, const void* v, void* out, float* lse, void* ranges, hipStream_t s) {
+  MaskedAttnParams<T> p;
+  if (d->n_documents > 1 && !d->documents) return fail("null pointer: documents");
+  if (attention_params(d, q, k, v, ranges, &p) || check_ptrs({out, lse}, "masked attention outputs")) return -1;
+  p.out = static_cast<T*>(out); p.lse = lse;
+  if (d->n_documents)
+    LACT_LAUNCH("k_attn_ranges", "masked_attn", 0.0, k_attn_ranges, dim3(ceil_div(d->L, 256), d->B), dim3(256), s, d->B, d->L, d->n_documents, p.window, d->documents,
+                d->prefixes, const_cast<int2*>(p.rows), const_cast<int2*>(p.cols));
+  launch_attention(0, d->D, p, s);
+  LACT_CHECK_LAUNCH();
+  return 0;
+}
+template <typename T>
+int attention_backward(const lact_attention_desc_t* d, const void* q, const void* k, const void* v, const void* out, const float* lse, const void* ranges,
+                       const void* dout, float* delta, void* dq, void* dk, void* dv, hipStream_t s) {
+  MaskedAttnParams<T> p;
+  if (attention_params(d, q, k, v, const_cast<void*>(ranges), &p) || check_rows(dout, d->do_ld, d->do_bs, d->H * d->D, d->act_dtype, "dout") ||
+      check_ptrs({out, lse, delta, dq, dk, dv}, "masked attention backward tensors"))
+    return -1;
+  p.o = static_cast<const T*>(out); p.lse = const_cast<float*>(lse); p.delta = delta;
+  p.dout = static_cast<const T*>(dout); p.lddo = d->do_ld; p.bsdo = d->do_bs;
+  p.dq = static_cast<T*>(dq); p.dk = static_cast<T*>(dk); p.dv = static_cast<T*>(dv);
+  launch_attention(1, d->D, p, s);
+  launch_attention(2, d->D, p, s);
+  LACT_CHECK_LAUNCH();
+  return 0;
+}
+
+// ---- one token of it ----------------------------------------------------------------------------
+int check_step(const lact_attention_step_desc_t* d) {
+  if (!d) return fail("null descriptor");
+  if (check_type(d->act_dtype)) return -1;
+  if (d->B <= 0 || d->N <= 0 || d->H <= 0 || d->HK <= 0 || d->window <= 0) return fail("attention step: B, N, H, HK and window must be positive");
+  if (d->D != 64 && d->D != 128) return fail("attention step: head size must be 64 or 128");
+  if (d->H % d->HK) return fail("attention step: the number of key heads must divide that of query heads");
+  if ((long long)d->B * d->H > (1 << 20) || d->N > (1 << 24)) return fail("attention step: cache or batch too large");
+  if (!(d->scale > 0.f) || !std::isfinite(d->scale)) return fail("attention step: the scale must be positive");
+  if (!(d->score_cap >= 0.f) || !std::isfinite(d->score_cap)) return fail("attention step: the score cap must be positive, or 0 for none");
+  const int al = d->act_dtype == LACT_BF16 ? 8 : 4;
+  if (d->q_bs % al || d->k_ld % al || d->k_bs % al || d->k_hs % al || d->v_ld % al || d->v_bs % al || d->v_hs % al)
+    return fail("attention step: rows must be 16-byte aligned");
+  if (d->k_ld < 0 || d->v_ld < 0 || d->k_bs < 0 || d->v_bs < 0 || d->k_hs < 0 || d->v_hs < 0 || d->q_bs < 0 || d->k_ld > (1 << 23) || d->v_ld > (1 << 23))
+    return fail("attention step: strides must be positive, those between tokens at most 2^23");
+  return 0;
+}
+template <typename T, int D>
+int step_blocks(const lact_attention_step_desc_t* d) {
+  const long long tiles = ceil_div(d->H / d->HK, 32), steps = ceil_div(std::min(d->N, d->window), AttnStepShape<T, D>::KEYS);
+  return (int)std::min<long long>(COMPUTE_UNITS, d->B * d->HK * tiles * steps);
+}
+template <typename T, int D>
+size_t step_workspace(const lact_attention_step_desc_t* d) {
+  return (size_t)2 * step_blocks<T, D>(d) * std::min(d->H / d->HK, 32) * (D + 2) * sizeof(float);
+}
+template <typename T, int D>
+int step_run(const lact_attention_step_desc_t* d, const void* q, const void* k, const void* v, const int32_t* lengths, void* out, void* workspace, hipStream_t s) {
+  AttnStepParams<T> p;
+  memset(&p, 0, sizeof(p));
+  p.B = d->B; p.N = d->N; p.H = d->H; p.HK = d->HK; p.group = d->H / d->HK; p.tiles = ceil_div(p.group, 32);
+  p.window = std::min(d->window, d->N);
+  p.blocks = step_blocks<T, D>(d);
+  p.q = static_cast<const T*>(q); p.bsq = d->q_bs;
+  p.k = static_cast<const T*>(k); p.ldk = d->k_ld; p.bsk = d->k_bs; p.hsk = d->k_hs;
+  p.v = static_cast<const T*>(v); p.ldv = d->v_ld; p.bsv = d->v_bs; p.hsv = d->v_hs;
+  p.lengths = lengths; p.slopes = d->slopes; p.scale = d->scale; p.cap = d->score_cap;
+  p.out = static_cast<T*>(out); p.part = static_cast<float*>(workspace);
+  constexpr int SM = AttnStepShape<T, D>::LDS;
+  LACT_BIG_LDS((k_attn_step<T, D>), SM);
+  LACT_LAUNCH_SMEM("k_attn_step", "attn_step", 0.0, (k_attn_step<T, D>), dim3(p.blocks), dim3(64 * AttnStepShape<T, D>::NW), SM, s, p);
+  LACT_LAUNCH("k_attn_step_join", "attn_step", 0.0, (k_attn_step_join<T, D>), dim3(p.B * p.H), dim3(512), s, p);
+  LACT_CHECK_LAUNCH();
+  return 0;
+}
+
+// ---- linear attention ---------------------------------------------------------------------------
+int check_linear(const lact_linear_desc_t* d) {
+  if (!d) return fail("null descriptor");
+  if (check_type(d->act_dtype)) return -1;
+  if (d->b <= 0 || d->l <= 0 || d->h <= 0) return fail("linear attention: b, l and h must be positive");
+  if ((d->dk != 64 && d->dk != 128) || (d->dv != 64 && d->dv != 128)) return fail("linear attention: key and value sizes must be 64 or 128");
+  if ((long long)d->b * d->h > (1 << 20) || d->l > (1 << 30)) return fail("linear attention: sequence or batch too large");
+  if (!std::isfinite(d->scale)) return fail("linear attention: the scale must be finite");
+  return 0;
+}
+
+struct LinCut { int segments, chunks; };      // chunks of a segment
+// One block walks a segment of a head; enough segments that the walks of all heads fill the chip once.
+LinCut lin_cut(const lact_linear_desc_t* d) {
+  const int chunks = ceil_div(d->l, LIN_CHUNK), heads = d->b * d->h;
+  const int want = std::max(1, std::min(chunks, COMPUTE_UNITS / heads)), per = ceil_div(chunks, want);
+  return LinCut{ceil_div(chunks, per), per};
+}
+struct LinBuffers {
+  size_t states, sums, end;              // of `states`: where segments start; sums of their decays
+  size_t ends, rsums, up, down, crossing, part, scratch;
+};
+LinBuffers lin_buffers(const lact_linear_desc_t* d) {
+  const LinCut cut = lin_cut(d);
+  const size_t heads = (size_t)d->b * d->h, elems = (size_t)d->dk * d->dv, tokens = (size_t)d->l * heads;
+  auto round = [](size_t n) { return (n + 255) & ~size_t(255); };
+  LinBuffers o;
+  size_t at = 0;
+  auto take = [&](size_t n) { const size_t a = at; at += round(n); return a; };
+  const size_t several = cut.segments > 1;
+  o.states = take(several * cut.segments * heads * elems * 4);
+  o.sums = take(several * cut.segments * heads * 4);
+  o.end = at;
+  at = 0;
+  o.ends = take(several * cut.segments * heads * elems * 4);
+  o.rsums = take(several * cut.segments * heads * 4);
+  o.up = take(tokens * 4);
+  o.down = take(tokens * 4);
+  o.crossing = take(cut.segments * heads * 4);
+  o.part = take(d->decay_per_token ? 0 : cut.segments * heads * 8);
+  o.scratch = at;
+  return o;
+}
+
+template <typename T>
+LinParams<T> lin_params(const lact_linear_desc_t* d, const float* g) {
+  LinParams<T> p;
+  memset(&p, 0, sizeof(p));
+  const LinCut cut = lin_cut(d);
+  p.B = d->b; p.L = d->l; p.H = d->h; p.segments = cut.segments; p.seg_chunks = cut.chunks;
+  p.decay.g = g; p.decay.per_token = d->decay_per_token;
+  p.by_heads = make_udiv(d->h);
+  return p;
+}
+
+template <typename T, int DX, int DZ, bool REV>
+void lin_segments(const LinParams<T>& p, const float* initial, float* states, float* sums, hipStream_t s) {
+  constexpr int SM = 2 * (MaskTile<T, DX>::BYTES + MaskTile<T, DZ>::BYTES) + 4 * 64 * 16;
+  LACT_BIG_LDS((k_lin_segments<T, DX, DZ, REV>), SM);
+  const int heads = p.B * p.H;
+  LACT_LAUNCH_SMEM("k_lin_segments", "linear_attn", 2.0 * heads * p.L * DX * DZ, (k_lin_segments<T, DX, DZ, REV>), dim3((p.segments - 1) * heads), dim3(256), SM, s, p,
+                   states, sums);
+  LACT_LAUNCH("k_lin_scan", "linear_attn", 0.0, k_lin_scan, dim3((unsigned)(((long long)heads * DX * DZ / 4 + 255) / 256)), dim3(256), s, p.segments, (long long)heads,
+              DX * DZ, (int)REV, initial, sums, states);
+}
+template <typename T, int DX, int DZ, bool REV, bool GATE>
+void lin_walk(const LinParams<T>& p, hipStream_t s) {
+  constexpr int SM = LinShape<T, DX, DZ, GATE>::LDS;
+  LACT_BIG_LDS((k_lin_walk<T, DX, DZ, REV, GATE>), SM);
+  LACT_LAUNCH_SMEM("k_lin_walk", "linear_attn", 4.0 * p.B * p.H * p.L * DX * DZ, (k_lin_walk<T, DX, DZ, REV, GATE>), dim3(p.segments * p.B * p.H), dim3(256), SM, s, p);
+}
+
+template <typename T, int DK, int DV>
+int lin_forward(const lact_linear_desc_t* d, const void* q, const void* k, const void* v, const float* g, const float* state, void* out, float* last, char* states,
+                hipStream_t s) {
+  const LinBuffers buf = lin_buffers(d);
+  LinParams<T> p = lin_params<T>(d, g);
+  p.x = {static_cast<const T*>(q), d->q_ld, d->q_bs};
+  p.y = {static_cast<const T*>(k), d->k_ld, d->k_bs};
+  p.z = {static_cast<const T*>(v), d->v_ld, d->v_bs};
+  p.pair_scale = p.state_scale = d->scale; p.source_scale = 1.f;
+  p.out = static_cast<T*>(out); p.last = last;
+  if (p.segments > 1) {
+    float* at = reinterpret_cast<float*>(states + buf.states);
+    lin_segments<T, DK, DV, false>(p, state, at, reinterpret_cast<float*>(states + buf.sums), s);
+    p.states = at;
+  } else {
+    p.state0 = state;
+  }
+  lin_walk<T, DK, DV, false, false>(p, s);
+  LACT_CHECK_LAUNCH();
+  return 0;
+}
+
+template <typename T, int DK, int DV>
+int lin_backward(const lact_linear_desc_t* d, const void* q, const void* k, const void* v, const float* g, const float* state, const float* last, const char* states,
+                 const void* dout, const float* dlast, void* dq, void* dk, void* dv, float* dg, float* dstate, char* scratch, hipStream_t s) {
+  const LinBuffers buf = lin_buffers(d);
+  const LinRows<T> rq{static_cast<const T*>(q), d->q_ld, d->q_bs}, rk{static_cast<const T*>(k), d->k_ld, d->k_bs}, rv{static_cast<const T*>(v), d->v_ld, d->v_bs},
+      ro{static_cast<const T*>(dout), d->do_ld, d->do_bs};
+  const LinParams<T> base = lin_params<T>(d, g);
+  float* up = reinterpret_cast<float*>(scratch + buf.up);
+  float* down = reinterpret_cast<float*>(scratch + buf.down);
+  float* ends = reinterpret_cast<float*>(scratch + buf.ends);
+  const float* starts = reinterpret_cast<const float*>(states + buf.states);
+  const bool several = base.segments > 1;
+  {      // dq: forwards with dout, v, k and the transposed state
+    LinParams<T> p = base;
+    p.x = ro; p.y = rv; p.z = rk; p.w = rq;
+    p.pair_scale = p.state_scale = d->scale; p.source_scale = 1.f;
+    p.out = static_cast<T*>(dq); p.transposed = 1; p.dots = up;
+    if (several) p.states = starts;
+    else p.state0 = state;
+    if (dg) lin_walk<T, DV, DK, false, true>(p, s);
+    else lin_walk<T, DV, DK, false, false>(p, s);
+  }
+  LinParams<T> p = base;      // backwards in time
+  p.x = rk; p.y = rq; p.z = ro; p.w = rv;
+  p.pair_scale = d->scale; p.state_scale = 1.f; p.source_scale = d->scale;
+  if (several) {
+    lin_segments<T, DK, DV, true>(p, dlast, ends, reinterpret_cast<float*>(scratch + buf.rsums), s);
+    p.states = ends;
+  } else {
+    p.state0 = dlast;
+  }
+  p.out = static_cast<T*>(dv); p.last = dstate; p.dots = down;
+  if (dg) lin_walk<T, DK, DV, true, true>(p, s);
+  else lin_walk<T, DK, DV, true, false>(p, s);
+  p.x = rv; p.y = ro; p.z = rq;
+  p.out = static_cast<T*>(dk); p.last = nullptr; p.dots = nullptr; p.transposed = 1;
+  lin_walk<T, DV, DK, true, false>(p, s);
+  if (dg) {
+    const int heads = d->b * d->h;
+    float* crossing = reinterpret_cast<float*>(scratch + buf.crossing);
+    double* part = reinterpret_cast<double*>(scratch + buf.part);
+    LACT_LAUNCH("k_lin_crossing", "linear_attn_bwd", 0.0, k_lin_crossing, dim3(base.segments * heads), dim3(256), s, base.segments, (long long)heads, DK * DV, starts, ends,
+                last, dlast, crossing);
+    LACT_LAUNCH("k_lin_decay_grad", "linear_attn_bwd", 0.0, k_lin_decay_grad, dim3(base.segments * heads), dim3(64), s, d->b, d->l, d->h, base.segments,
+                base.seg_chunks * LIN_CHUNK, up, down, crossing, base.decay, dg, part);
+    if (!d->decay_per_token)
+      LACT_LAUNCH("k_lin_decay_sum", "linear_attn_bwd", 0.0, k_lin_decay_sum, dim3(d->h), dim3(64), s, base.segments * d->b, d->h, part, dg);
+  }
+  LACT_CHECK_LAUNCH();
+  return 0;
+}
+
+// f(T(), key size, value size as integral constants) for the descriptor's
+template <typename F>
+int by_sizes(int act, int dk, int dv, F f) {
+  using C64 = std::integral_constant<int, 64>;
+  using C128 = std::integral_constant<int, 128>;
+  auto values = [&](auto t, auto k) { return dv == 64 ? f(t, k, C64()) : f(t, k, C128()); };
+  auto keys = [&](auto t) { return dk == 64 ? values(t, C64()) : values(t, C128()); };
+  return act == LACT_BF16 ? keys(uint16_t()) : keys(float());
+}
+int check_linear_rows(const lact_linear_desc_t* d, const void* q, const void* k, const void* v) {
+  return check_rows(q, d->q_ld, d->q_bs, d->h * d->dk, d->act_dtype, "q") || check_rows(k, d->k_ld, d->k_bs, d->h * d->dk, d->act_dtype, "k") ||
+         check_rows(v, d->v_ld, d->v_bs, d->h * d->dv, d->act_dtype, "v");
+}
+int check_states(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (!aligned16(p)) return fail("linear attention: states must be 16-byte aligned");
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t lact_attention_ranges_bytes(const lact_attention_desc_t* d) {
+  return d && d->n_documents > 0 && d->B > 0 && d->L > 0 ? (size_t)d->B * d->L * 2 * sizeof(int2) : 0;
+}
+
+int lact_masked_attention_forward(const lact_attention_desc_t* d, const void* q, const void* k, const void* v, void* out, float* lse, void* ranges, void* stream) {
+  if (check_attention(d)) return -1;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return d->act_dtype == LACT_BF16 ? attention_forward<uint16_t>(d, q, k, v, out, lse, ranges, s) : attention_forward<float>(d, q, k, v, out, lse, ranges, s);
+}
+
+int lact_masked_attention_backward(const lact_attention_desc_t* d, const void* q, const void* k, const void* v, const void* out, const float* lse, const void* ranges,
+                                   const void* dout, float* delta, void* dq, void* dk, void* dv, void* stream) {
+  if (check_attention(d)) return -1;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return d->act_dtype == LACT_BF16 ? attention_backward<uint16_t>(d, q, k, v, out, lse, ranges, dout, delta, dq, dk, dv, s)
+                                   : attention_backward<float>(d, q, k, v, out, lse, ranges, dout, delta, dq, dk, dv, s);
+}
+
+size_t lact_attention_step_workspace_bytes(const lact_attention_step_desc_t* d) {
+  if (check_step(d)) return 0;
+  if (d->act_dtype == LACT_BF16) return d->D == 128 ? step_workspace<uint16_t, 128>(d) : step_workspace<uint16_t, 64>(d);
+  return d->D == 128 ? step_workspace<float, 128>(d) : step_workspace<float, 64>(d);
+}
+
+int lact_attention_step(const lact_attention_step_desc_t* d, const void* q, const void* k, const void* v, const int32_t* lengths, void* out, void* workspace,
+                        void* stream) {
+  if (check_step(d) || check_ptrs({q, k, v, lengths, out, workspace}, "attention step tensors")) return -1;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v)) return fail("attention step: rows must be 16-byte aligned");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (d->act_dtype == LACT_BF16)
+    return d->D == 128 ? step_run<uint16_t, 128>(d, q, k, v, lengths, out, workspace, s) : step_run<uint16_t, 64>(d, q, k, v, lengths, out, workspace, s);
+  return d->D == 128 ? step_run<float, 128>(d, q, k, v, lengths, out, workspace, s) : step_run<float, 64>(d, q, k, v, lengths, out, workspace, s);
+}
+
+int lact_linear_attention_sizes(const lact_linear_desc_t* d, size_t* states_bytes, size_t* scratch_bytes) {
+  if (check_linear(d)) return -1;
+  const LinBuffers buf = lin_buffers(d);
+  if (states_bytes) *states_bytes = buf.end;
+  if (scratch_bytes) *scratch_bytes = buf.scratch;
+  return 0;
+}
+
+int lact_linear_attention_forward(const lact_linear_desc_t* d, const void* q, const void* k, const void* v, const float* g, const float* state, void* out, float* last,
+                                  void* states, void* stream) {
+  if (check_linear(d) || check_linear_rows(d, q, k, v) || check_ptrs({g, out}, "linear attention tensors") || check_states({state, last, states})) return -1;
+  if (lin_buffers(d).end && !states) return fail("null pointer: linear attention states");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return by_sizes(d->act_dtype, d->dk, d->dv, [&](auto t, auto dk, auto dv) {
+    return lin_forward<decltype(t), decltype(dk)::value, decltype(dv)::value>(d, q, k, v, g, state, out, last, static_cast<char*>(states), s);
+  });
+}
+
+int lact_linear_attention_backward(const lact_linear_desc_t* d, const void* q, const void* k, const void* v, const float* g, const float* state, const float* last,
+                                   const void* states, const void* dout, const float* dlast, void* dq, void* dk_, void* dv_, float* dg, float* dstate, void* scratch,
+                                   void* stream) {
+  if (check_linear(d) || check_linear_rows(d, q, k, v) || check_rows(dout, d->do_ld, d->do_bs, d->h * d->dv, d->act_dtype, "dout") ||
+      check_ptrs({g, dq, dk_, dv_, scratch}, "linear attention backward tensors") || check_states({state, last, states, dlast, dstate, scratch}))
+    return -1;
+  if (lin_buffers(d).end && !states) return fail("null pointer: linear attention states");
+  if (dg && dlast && !last) return fail("null pointer: the last state, for the gradient of the decays");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return by_sizes(d->act_dtype, d->dk, d->dv, [&](auto t, auto dk, auto dv) {
+    return lin_backward<decltype(t), decltype(dk)::value, decltype(dv)::value>(d, q, k, v, g, state, last, static_cast<const char*>(states), dout, dlast, dq, dk_, dv_, dg,
+                                                                               dstate, static_cast<char*>(scratch), s);
+  });
+}
+
+int lact_linear_attention_step(int32_t act_dtype, int32_t b, int32_t h, int32_t dk, int32_t dv, int32_t decay_per_token, float scale, const void* q, int64_t q_bs,
+                               const void* k, int64_t k_bs, const void* v, int64_t v_bs, const float* g, const float* state, float* state_out, void* out,
+                               void* stream) {
+  if (check_type(act_dtype)) return -1;
+  if (b <= 0 || h <= 0 || (long long)b * h > (1 << 20)) return fail("linear attention step: b and h must be positive, with at most 2^20 states");
+  if ((dk != 64 && dk != 128) || (dv != 64 && dv != 128)) return fail("linear attention step: key and value sizes must be 64 or 128");
+  if (!std::isfinite(scale)) return fail("linear attention step: the scale must be finite");
+  if (check_ptrs({q, k, v, g, state, state_out, out}, "linear attention step tensors") || check_states({state, state_out})) return -1;
+  const int al = act_dtype == LACT_BF16 ? 8 : 4;
+  if (v_bs % al || v_bs < 0 || q_bs < 0 || k_bs < 0 || !aligned16(v)) return fail("linear attention step: rows of v must be 16-byte aligned");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  auto run = [&](auto t) {
+    using T = decltype(t);
+    LinStepParams<T> p;
+    memset(&p, 0, sizeof(p));
+    p.H = h; p.DK = dk; p.DV = dv; p.per_token = decay_per_token != 0;
+    p.q = static_cast<const T*>(q); p.k = static_cast<const T*>(k); p.v = static_cast<const T*>(v);
+    p.bsq = q_bs; p.bsk = k_bs; p.bsv = v_bs;
+    p.g = g; p.state = state; p.state_out = state_out; p.scale = scale; p.out = static_cast<T*>(out);
+    LACT_LAUNCH("k_lin_step", "linear_attn_step", 0.0, (k_lin_step<T>), dim3(b * h * (dv / 32)), dim3(256), s, p);
+  };
+  if (act_dtype == LACT_BF16) run(uint16_t());
+  else run(float());
+  LACT_CHECK_LAUNCH();
+  return 0;
+}
+
+}  // extern "C"

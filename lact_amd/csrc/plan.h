@@ -8,15 +8,11 @@
 
 #include "../../include/lact_hip.h"
 #include "gemm_dma_kernels.h"
+#include "host_common.h"
 #include "state_kernels.h"
 
 namespace lact {
 
-inline thread_local std::string g_err;
-inline int fail(const std::string& m) {
-  g_err = m;
-  return -1;
-}
 inline int g_keep_pre = -1;       // LACT_OPT_KEEP_PREACTIVATIONS: -1 by shape, 0 never, 1 whenever the kernels allow it
 
 template <typename T> using TSG = typename AsyncTile<T>::TS;   // tile of the kernels in gemm_kernels.h
@@ -29,8 +25,6 @@ struct Bump {
     return o;
   }
 };
-
-inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 struct Split {
   int n, len;

@@ -4,6 +4,7 @@
 // forward call and made the GPU wait.  All arithmetic stays behind the C ABI (include/lact_hip.h).
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/autocast_mode.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -633,6 +634,245 @@ struct LayerInFn : torch::autograd::Function<LayerInFn> {
   }
 };
 
+// ---- attention and linear attention -----------------------------------------------------------------------------------
+// [b, l, h, d] as the kernels read it: heads next to each other inside a token, rows on 16-byte boundaries
+Tensor head_rows(const Tensor& t) {
+  const int64_t al = t.scalar_type() == at::kBFloat16 ? 8 : 4, d = t.size(3);
+  const bool ok = t.stride(3) == 1 && t.stride(2) == d && t.stride(1) % al == 0 && t.stride(0) % al == 0 && t.stride(0) >= 0 && t.stride(1) >= t.size(2) * d &&
+                  t.stride(1) <= (1 << 23) && aligned16(t);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+void expect_same(const Tensor& t, const Tensor& like, const char* name) {
+  if (t.device() != like.device()) throw std::runtime_error(std::string("expected all tensors to be on the same device: ") + name);
+  TORCH_CHECK_TYPE(t.scalar_type() == like.scalar_type(), name, " is ", t.scalar_type(), ", q is ", like.scalar_type());
+}
+// whole numbers that the kernels read as int32
+Tensor indices(const OptTensor& t, const Tensor& like, at::IntArrayRef shape, const char* name) {
+  if (!t) return Tensor();
+  expect(*t, like, shape, name);
+  TORCH_CHECK_TYPE(t->scalar_type() == at::kInt || t->scalar_type() == at::kLong, name, " must be int32 or int64, got ", t->scalar_type());
+  return t->to(at::kInt).contiguous();
+}
+
+struct AttentionCall {      // what a forward hands to its backward
+  lact_attention_desc_t desc{};
+  Tensor q, k, v, out, lse, ranges, slopes;
+};
+AttentionCall attention_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t window, double scale, double cap, const OptTensor& slopes,
+                                const OptTensor& documents_, const OptTensor& prefixes_) {
+  on_gpu(q_);
+  const c10::hip::HIPGuard guard(q_.device().index());
+  AttentionCall c;
+  auto& D = c.desc;
+  D.act_dtype = act_code(q_);
+  const int64_t b = q_.size(0), l = q_.size(1), h = q_.size(2), hk = k_.size(2), d = q_.size(3);
+  expect_same(k_, q_, "k");
+  expect_same(v_, q_, "v");
+  expect(k_, q_, {b, l, hk, d}, "k");
+  expect(v_, q_, {b, l, hk, d}, "v");
+  if (slopes) {
+    expect(*slopes, q_, {h}, "distance_slopes");
+    c.slopes = plain_f32(*slopes);
+  }
+  const int64_t n = documents_ ? documents_->size(1) - 1 : prefixes_ ? 1 : 0;
+  const Tensor documents = indices(documents_, q_, {b, n + 1}, "documents"), prefixes = indices(prefixes_, q_, {b, n}, "prefixes");
+  c.q = head_rows(q_); c.k = head_rows(k_); c.v = head_rows(v_);
+  D.B = (int)b; D.L = (int)l; D.H = (int)h; D.HK = (int)hk; D.D = (int)d; D.window = (int)std::min<int64_t>(window, l); D.n_documents = (int)n;
+  D.scale = (float)scale; D.score_cap = (float)cap;
+  D.q_ld = (int)c.q.stride(1); D.k_ld = (int)c.k.stride(1); D.v_ld = (int)c.v.stride(1);
+  D.q_bs = c.q.stride(0); D.k_bs = c.k.stride(0); D.v_bs = c.v.stride(0);
+  D.slopes = fptr(c.slopes); D.documents = fptr<int32_t>(documents); D.prefixes = fptr<int32_t>(prefixes);
+  c.out = at::empty({b, l, h, d}, q_.options());
+  c.lse = at::empty({b, h, l}, q_.options().dtype(at::kFloat));
+  if (const size_t bytes = lact_attention_ranges_bytes(&D)) c.ranges = at::empty({(int64_t)bytes}, q_.options().dtype(at::kByte));
+  check(lact_masked_attention_forward(&D, ptr(c.q), ptr(c.k), ptr(c.v), ptr(c.out), fptr(c.lse), ptr(c.ranges), stream()));
+  return c;
+}
+
+struct AttentionFn : torch::autograd::Function<AttentionFn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, double scale, double cap, const OptTensor& slopes,
+                        const OptTensor& documents, const OptTensor& prefixes) {
+    auto c = attention_forward(q, k, v, window, scale, cap, slopes, documents, prefixes);
+    ctx->save_for_backward({c.q, c.k, c.v, c.out, c.lse, c.ranges, c.slopes});
+    ctx->saved_data["dims"] = std::vector<int64_t>{c.desc.window, c.desc.n_documents};
+    ctx->saved_data["scale"] = scale; ctx->saved_data["cap"] = cap;
+    return c.out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool twice = at::GradMode::is_enabled();
+    const at::AutoGradMode off(false);
+    const auto t = ctx->get_saved_variables();
+    const Tensor &q = t[0], &k = t[1], &v = t[2], &out = t[3], &lse = t[4], &ranges = t[5], &slopes = t[6];
+    const c10::hip::HIPGuard guard(q.device().index());
+    const auto dims = ctx->saved_data["dims"].toIntVector();
+    const Tensor g = head_rows(cast(grads[0], q.scalar_type())), delta = at::empty_like(lse);
+    lact_attention_desc_t D{};
+    D.act_dtype = act_code(q);
+    D.B = (int)q.size(0); D.L = (int)q.size(1); D.H = (int)q.size(2); D.HK = (int)k.size(2); D.D = (int)q.size(3);
+    D.window = (int)dims[0]; D.n_documents = (int)dims[1];
+    D.scale = (float)ctx->saved_data["scale"].toDouble(); D.score_cap = (float)ctx->saved_data["cap"].toDouble();
+    D.q_ld = (int)q.stride(1); D.k_ld = (int)k.stride(1); D.v_ld = (int)v.stride(1); D.do_ld = (int)g.stride(1);
+    D.q_bs = q.stride(0); D.k_bs = k.stride(0); D.v_bs = v.stride(0); D.do_bs = g.stride(0);
+    D.slopes = fptr(slopes);
+    const auto c = at::MemoryFormat::Contiguous;
+    const Tensor dq = at::empty_like(q, q.options(), c), dk = at::empty_like(k, k.options(), c), dv = at::empty_like(v, v.options(), c);
+    check(lact_masked_attention_backward(&D, ptr(q), ptr(k), ptr(v), ptr(out), fptr(lse), ptr(ranges), ptr(g), fptr(delta), ptr(dq), ptr(dk), ptr(dv), stream()));
+    return finish({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, twice);
+  }
+};
+
+// One token of every sequence against its cache; inference.
+Tensor attention_step(const Tensor& q_, const Tensor& k, const Tensor& v, const Tensor& lengths_, int64_t window, double scale, double cap, const OptTensor& slopes_) {
+  on_gpu(q_);
+  const c10::hip::HIPGuard guard(q_.device().index());
+  const at::AutoGradMode off(false);
+  lact_attention_step_desc_t D{};
+  D.act_dtype = act_code(q_);
+  const int64_t b = q_.size(0), h = q_.size(1), d = q_.size(2), n = k.size(1), hk = k.size(2);
+  expect_same(k, q_, "k_cache");
+  expect_same(v, q_, "v_cache");
+  expect(k, q_, {b, n, hk, d}, "k_cache");
+  expect(v, q_, {b, n, hk, d}, "v_cache");
+  const Tensor lengths = indices(lengths_, q_, {b}, "lengths"), q = dense(q_);
+  Tensor slopes;
+  if (slopes_) {
+    expect(*slopes_, q_, {h}, "distance_slopes");
+    slopes = plain_f32(*slopes_);
+  }
+  const Tensor out = at::empty({b, h, d}, q_.options());
+  if (out.numel() == 0 || n == 0) return out.zero_();
+  // (a cache is not copied to fit: that would read all of it)
+  const int64_t al = D.act_dtype == LACT_BF16 ? 8 : 4;
+  for (const auto* t : {&k, &v}) {
+    bool ok = t->stride(3) == 1 && aligned16(*t);
+    for (int i = 0; i < 3; ++i) ok = ok && (t->size(i) == 1 || (t->stride(i) % al == 0 && t->stride(i) >= 0));
+    if (!ok) throw std::invalid_argument("a cache must have its last dimension contiguous and its rows on 16-byte boundaries");
+    if (t->size(1) > 1 && t->stride(1) > (1 << 23)) throw std::invalid_argument("a cache's tokens must lie at most 2^23 elements apart");
+  }
+  auto stride = [](const Tensor& t, int i) { return t.size(i) == 1 ? 0 : t.stride(i); };
+  D.B = (int)b; D.N = (int)std::min<int64_t>(n, INT32_MAX); D.H = (int)h; D.HK = (int)hk; D.D = (int)d; D.window = (int)std::min<int64_t>(window, n);
+  D.scale = (float)scale; D.score_cap = (float)cap;
+  D.q_bs = h * d;
+  D.k_ld = stride(k, 1); D.k_bs = stride(k, 0); D.k_hs = stride(k, 2);
+  D.v_ld = stride(v, 1); D.v_bs = stride(v, 0); D.v_hs = stride(v, 2);
+  D.slopes = fptr(slopes);
+  const int64_t bytes = (int64_t)lact_attention_step_workspace_bytes(&D);
+  if (bytes == 0) check(-1);
+  const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  check(lact_attention_step(&D, ptr(q), ptr(k), ptr(v), fptr<int32_t>(lengths), ptr(out), ptr(ws), stream()));
+  return out;
+}
+
+struct LinearCall {
+  lact_linear_desc_t desc{};
+  Tensor q, k, v, g, state, out, last, states;
+};
+lact_linear_desc_t linear_desc(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, double scale) {
+  lact_linear_desc_t D{};
+  D.act_dtype = act_code(q);
+  D.b = (int)q.size(0); D.l = (int)q.size(1); D.h = (int)q.size(2); D.dk = (int)q.size(3); D.dv = (int)v.size(3);
+  D.decay_per_token = g.dim() == 3; D.scale = (float)scale;
+  D.q_ld = (int)q.stride(1); D.k_ld = (int)k.stride(1); D.v_ld = (int)v.stride(1);
+  D.q_bs = q.stride(0); D.k_bs = k.stride(0); D.v_bs = v.stride(0);
+  return D;
+}
+LinearCall linear_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, const OptTensor& state_, double scale, bool return_state) {
+  on_gpu(q_);
+  const c10::hip::HIPGuard guard(q_.device().index());
+  LinearCall c;
+  act_code(q_);
+  const int64_t b = q_.size(0), l = q_.size(1), h = q_.size(2), dk = q_.size(3), dv = v_.size(3);
+  expect_same(k_, q_, "k");
+  expect_same(v_, q_, "v");
+  expect(k_, q_, {b, l, h, dk}, "k");
+  expect(v_, q_, {b, l, h, dv}, "v");
+  if (g_.dim() == 1) expect(g_, q_, {h}, "log_decay");
+  else expect(g_, q_, {b, l, h}, "log_decay");
+  if (state_) {
+    expect(*state_, q_, {b, h, dk, dv}, "state");
+    c.state = plain_f32(*state_);
+  }
+  c.q = head_rows(q_); c.k = head_rows(k_); c.v = head_rows(v_); c.g = plain_f32(g_);
+  const auto& D = c.desc = linear_desc(c.q, c.k, c.v, c.g, scale);
+  c.out = at::empty({b, l, h, dv}, q_.options());
+  const auto f32 = q_.options().dtype(at::kFloat);
+  if (return_state) c.last = at::empty({b, h, dk, dv}, f32);
+  size_t bytes = 0;
+  check(lact_linear_attention_sizes(&D, &bytes, nullptr));
+  if (bytes) c.states = at::empty({(int64_t)bytes}, f32.dtype(at::kByte));
+  check(lact_linear_attention_forward(&D, ptr(c.q), ptr(c.k), ptr(c.v), fptr(c.g), fptr(c.state), ptr(c.out), fptr(c.last), ptr(c.states), stream()));
+  return c;
+}
+struct LinearAttentionFn : torch::autograd::Function<LinearAttentionFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const OptTensor& state, double scale,
+                               bool return_state) {
+    auto c = linear_forward(q, k, v, g, state, scale, return_state);
+    ctx->save_for_backward({c.q, c.k, c.v, c.g, c.state, c.last, c.states});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)g.scalar_type(), (int64_t)(state ? state->scalar_type() : at::kFloat), g.requires_grad(),
+                                                    state && state->requires_grad()};
+    ctx->set_materialize_grads(false);
+    variable_list res{c.out};
+    if (return_state) res.push_back(c.last);
+    return res;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool twice = at::GradMode::is_enabled();
+    const at::AutoGradMode off(false);
+    const auto t = ctx->get_saved_variables();
+    const Tensor &q = t[0], &k = t[1], &v = t[2], &g = t[3], &state = t[4], &last = t[5], &states = t[6];
+    const c10::hip::HIPGuard guard(q.device().index());
+    const auto types = ctx->saved_data["types"].toIntVector();
+    lact_linear_desc_t D = linear_desc(q, k, v, g, ctx->saved_data["scale"].toDouble());
+    const auto c = at::MemoryFormat::Contiguous;
+    const Tensor go = grads[0].defined() ? head_rows(cast(grads[0], q.scalar_type())) : at::zeros(v.sizes(), v.options());
+    const Tensor dlast = grads.size() > 1 && grads[1].defined() ? plain_f32(grads[1]) : Tensor();
+    D.do_ld = (int)go.stride(1); D.do_bs = go.stride(0);
+    const Tensor dq = at::empty_like(q, q.options(), c), dk = at::empty_like(k, k.options(), c), dv = at::empty_like(v, v.options(), c);
+    const Tensor dg = types[2] ? at::empty_like(g) : Tensor(), ds = types[3] ? at::empty_like(state) : Tensor();
+    size_t bytes = 0;
+    check(lact_linear_attention_sizes(&D, nullptr, &bytes));
+    const Tensor scratch = at::empty({(int64_t)bytes}, g.options().dtype(at::kByte));
+    check(lact_linear_attention_backward(&D, ptr(q), ptr(k), ptr(v), fptr(g), fptr(state), fptr(last), ptr(states), ptr(go), fptr(dlast), ptr(dq), ptr(dk), ptr(dv),
+                                         fptr(dg), fptr(ds), ptr(scratch), stream()));
+    return finish({dq, dk, dv, cast(dg, (at::ScalarType)types[0]), cast(ds, (at::ScalarType)types[1]), Tensor(), Tensor()}, twice);
+  }
+};
+
+// One token: the output, and the new state in state_out (which may be the state).
+std::vector<Tensor> linear_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, const Tensor& state_, const OptTensor& state_out, double scale) {
+  on_gpu(q_);
+  const c10::hip::HIPGuard guard(q_.device().index());
+  const at::AutoGradMode off(false);
+  const int act = act_code(q_);
+  const int64_t b = q_.size(0), h = q_.size(1), dk = q_.size(2), dv = v_.size(2);
+  expect_same(k_, q_, "k");
+  expect_same(v_, q_, "v");
+  expect(k_, q_, {b, h, dk}, "k");
+  expect(v_, q_, {b, h, dv}, "v");
+  if (g_.dim() == 1) expect(g_, q_, {h}, "log_decay");
+  else expect(g_, q_, {b, h}, "log_decay");
+  expect(state_, q_, {b, h, dk, dv}, "state");
+  const Tensor q = dense(q_), k = dense(k_), v = dense(v_), g = plain_f32(g_), state = plain_f32(state_);
+  Tensor next;
+  if (state_out) {
+    next = *state_out;
+    expect(next, q_, {b, h, dk, dv}, "state_out");
+    TORCH_CHECK_TYPE(next.scalar_type() == at::kFloat, "state_out must be fp32");
+    if (!next.is_contiguous() || !aligned16(next)) throw std::invalid_argument("state_out must be contiguous, on a 16-byte boundary");
+    for (const Tensor* t : {&state, &q, &k, &v, &g})
+      if (t == &state) at::assert_no_partial_overlap(next, *t);
+      else at::assert_no_overlap(next, *t);
+  } else {
+    next = at::empty({b, h, dk, dv}, q_.options().dtype(at::kFloat));
+  }
+  const Tensor out = at::empty({b, h, dv}, q_.options());
+  if (out.numel() == 0) return {out, next};
+  check(lact_linear_attention_step(act, (int)b, (int)h, (int)dk, (int)dv, g.dim() == 2, (float)scale, ptr(q), h * dk, ptr(k), h * dk, ptr(v), h * dv, fptr(g),
+                                   fptr(state), fptr(next), ptr(out), stream()));
+  return {out, next};
+}
+
 template <class F, class... Args>
 auto apply_released(Args&&... args) {
   const py::gil_scoped_release nogil;
@@ -655,6 +895,24 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("layer_post", [](const Tensor& o, const OptTensor& weight, const OptTensor& gate, int64_t B, int64_t H, bool use_norm, double eps, const OptTensor& add) {
     return apply_released<LayerPostFn>(o, weight, gate, B, H, use_norm, eps, add);
   });
+  m.def("masked_attention", [](const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, double scale, double cap, const OptTensor& slopes,
+                               const OptTensor& documents, const OptTensor& prefixes) {
+    const py::gil_scoped_release nogil;
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+      return AttentionFn::apply(q, k, v, window, scale, cap, slopes, documents, prefixes);
+    const at::AutoGradMode off(false);
+    return attention_forward(q, k, v, window, scale, cap, slopes, documents, prefixes).out;
+  });
+  m.def("attention_step", &attention_step, py::call_guard<py::gil_scoped_release>());
+  m.def("linear_attention", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const OptTensor& state, double scale, bool return_state) {
+    const py::gil_scoped_release nogil;
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || g.requires_grad() || wants_grad(state)))
+      return LinearAttentionFn::apply(q, k, v, g, state, scale, return_state);
+    const at::AutoGradMode off(false);
+    auto c = linear_forward(q, k, v, g, state, scale, return_state);
+    return return_state ? variable_list{c.out, c.last} : variable_list{c.out};
+  });
+  m.def("linear_attention_step", &linear_step, py::call_guard<py::gil_scoped_release>());
   m.def("linear", [](const Tensor& x, const Tensor& weight) { return apply_released<LinearFn>(autocast_bf16(x), weight, autocast_bf16(weight)); });
   m.def("layer_in", [](const Tensor& x, const Tensor& qkv_w, const Tensor& lr_w, const OptTensor& lr_b, const OptTensor& mom_w, const OptTensor& mom_b,
                        const OptTensor& gate_w, const OptTensor& gate_b) { return apply_released<LayerInFn>(x, qkv_w, autocast_bf16(qkv_w), lr_w, lr_b, mom_w, mom_b, gate_w, gate_b); });

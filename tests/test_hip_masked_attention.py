@@ -1,0 +1,412 @@
+"""masked_window_attention and window_attention_step (csrc/masked_attention.h, csrc/attention_step.h) against their definition in float64:
+every mask, at the edges of the 32-row waves, 64-row tiles and 128 / 256-row blocks, output and gradients."""
+import pytest
+import torch
+
+from oracle import mixers_oracle as MO
+
+pytestmark = pytest.mark.gpu
+
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+
+
+def errors(dtype, l, d, size=8.0):
+    """Relative errors of a probability and of a stored value.  bf16: probabilities are rounded for the product (2^-8), scores are summed in fp32.
+    fp32: the sums of d and of l terms, and the exponential of a score of `size` off by the roundings of its d terms."""
+    fp32 = (2 * d + l + 16 * size + 64) * 2.0 ** -24
+    return (HALF[dtype] if dtype == torch.bfloat16 else 0.0) + fp32, HALF[dtype]
+
+
+def near(got, ref, bound, name):
+    got = got.detach().double().cpu()
+    assert got.shape == ref.shape and bool(torch.isfinite(got).all()), name
+    worst = ((got - ref).abs() / (bound + 1e-7)).max() if got.numel() else 0.0
+    print(f"[gpu-test]   {name}: {float(worst):.3f} of the bound", flush=True)
+    assert worst <= 1.0, (name, float(worst))
+
+
+def make(b, l, hq, hkv, d, dtype, seed=3, growth=1.0):
+    g = torch.Generator().manual_seed(seed)
+    packed = torch.randn(b, l, (hq + 2 * hkv) * d, generator=g)
+    packed[..., hq * d:(hq + hkv) * d] *= torch.linspace(1.0, growth, max(l, 1))[None, :, None]
+    go = torch.randn(b, l, hq, d, generator=g).to(dtype)
+    return packed.to(dtype), go
+
+
+def parts(packed, hq, hkv, d):
+    b, l = packed.shape[:2]
+    return [t.reshape(b, l, -1, d) for t in packed.split((hq * d, hkv * d, hkv * d), -1)]
+
+
+def ints(rows, dtype=torch.int32):
+    return None if rows is None else torch.tensor(rows, dtype=dtype)
+
+
+def check(b, l, hq, hkv, d, dtype, window=None, cap=None, slopes=False, documents=None, prefixes=None, growth=1.0, scale=None):
+    import lact_amd
+    print("[gpu-test] masked attention", b, l, hq, hkv, d, dtype, window, cap, slopes, documents, prefixes, flush=True)
+    packed, go = make(b, l, hq, hkv, d, dtype, growth=growth)
+    sl = 2.0 ** -torch.arange(1, hq + 1).float() if slopes else None
+    docs, pre = ints(documents), ints(prefixes)
+    dev = lambda t: None if t is None else t.to("cuda")  # noqa: E731
+    x = packed.to("cuda").requires_grad_(True)
+    out = lact_amd.masked_window_attention(*parts(x, hq, hkv, d), window, score_cap=cap, distance_slopes=dev(sl), documents=dev(docs), prefixes=dev(pre), scale=scale)
+    gx, = torch.autograd.grad(out, x, go.to("cuda"))
+    p_err, out_err = errors(dtype, l, d, 8.0 * growth + (l if slopes else 0))
+    ref, bound = MO.attention(*parts(packed, hq, hkv, d), window, cap, sl, docs, pre, scale, go, p_err, out_err)
+    assert out.dtype == dtype
+    for name, a, r, e in zip(("out", "dq", "dk", "dv"), [out, *parts(gx, hq, hkv, d)], ref, bound):
+        near(a, r, e, name)
+    seen = MO.visible(l, window, docs, pre).any(-1)
+    for i in range(b):
+        assert not out[i][~seen[i if len(seen) > 1 else 0].to("cuda")].any()
+    return out, gx
+
+
+BOTH = pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+
+
+@BOTH
+@pytest.mark.parametrize("b,l,hq,hkv,d,window", [
+    (1, 1, 1, 1, 64, None), (2, 5, 2, 1, 128, 2), (1, 64, 1, 1, 128, 64), (2, 129, 3, 3, 128, 33), (1, 257, 4, 2, 64, 65), (2, 333, 6, 2, 128, 200),
+    (1, 300, 5, 5, 64, None), (1, 70, 2, 2, 64, 1)])
+def test_causal_windows(b, l, hq, hkv, d, window, dtype):
+    check(b, l, hq, hkv, d, dtype, window)
+
+
+@BOTH
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("documents,prefixes,window", [
+    ([[0, 40, 41, 41, 150, 200]], None, None),                      # one token, none, and an edge inside a tile
+    ([[3, 64, 128, 190]], None, 50),                                # padded on both sides, edges on tiles
+    ([[0, 200]], [[200]], None),                                    # all of it a prefix: bidirectional
+    ([[0, 90, 200]], [[0, 70]], 30),                                # a prefix wider than the window
+    ([[0, 0, 0]], None, None),                                      # no token in any document
+    ([[0, 1, 2, 3, 64, 65, 199, 200]], [[1, 0, 1, 61, 1, 2, 1]], 64),
+    (None, [[33]], 70)])
+def test_documents_and_prefixes(documents, prefixes, window, d, dtype):
+    check(1, 200, 4, 2, d, dtype, window, documents=documents, prefixes=prefixes)
+
+
+@BOTH
+def test_documents_of_a_batch_differ(dtype):
+    check(3, 150, 2, 1, 64, dtype, None, documents=[[0, 150, 150], [20, 30, 100], [0, 75, 150]], prefixes=[[10, 0], [10, 3], [0, 75]])
+
+
+@BOTH
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cap,slopes,scale", [(20.0, False, None), (None, True, None), (2.0, True, 0.3)])
+def test_capped_scores_and_distance(cap, slopes, scale, d, dtype):
+    check(2, 170, 4, 4, d, dtype, 100, cap, slopes, documents=[[0, 60, 170], [5, 100, 165]], prefixes=[[20, 0], [0, 33]], scale=scale)
+
+
+@pytest.mark.parametrize("b,l,hq,hkv,d,window", [(2, 1030, 26, 26, 128, 256), (1, 1100, 64, 64, 64, 300), (2, 520, 64, 16, 128, None)])
+def test_blocks_of_256_rows(b, l, hq, hkv, d, window):
+    check(b, l, hq, hkv, d, torch.bfloat16, window, documents=[[0, 200, l - 3]] * b)
+
+
+@BOTH
+@pytest.mark.parametrize("growth", [40.0, 300.0])
+def test_scores_that_grow_along_the_sequence(growth, dtype):
+    """The rows' maxima follow by far more than exp2 reaches."""
+    check(1, 515, 3, 3, 128, dtype, 190, growth=growth)
+
+
+@BOTH
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), "lowest"])
+def test_what_is_masked_reaches_nothing(bad, dtype):
+    """Padding and another document hold values that are not finite, or the type's lowest: the outputs and gradients of the rest are those without."""
+    import lact_amd
+    print("[gpu-test] masked attention, masked places hold", bad, dtype, flush=True)
+    b, l, hq, hkv, d = 1, 230, 4, 2, 128
+    value = torch.finfo(dtype).min if bad == "lowest" else bad
+    docs = torch.tensor([[10, 100, 140, 200]], dtype=torch.int32, device="cuda")
+    spoilt = torch.zeros(l, dtype=torch.bool)
+    spoilt[:10] = spoilt[100:140] = spoilt[200:] = True
+    packed, go = make(b, l, hq, hkv, d, dtype)
+    results = []
+    for spoil in (False, True):
+        x, g = packed.clone(), go.clone()
+        if spoil:
+            x[:, spoilt], g[:, spoilt] = value, value
+        x = x.to("cuda").requires_grad_(True)
+        out = lact_amd.masked_window_attention(*parts(x, hq, hkv, d), None, score_cap=30.0, documents=docs, prefixes=torch.tensor([[30, 0, 0]], device="cuda"))
+        gx, = torch.autograd.grad(out, x, g.to("cuda"))
+        results.append((out.detach().cpu(), gx.cpu()))
+    for clean, other in zip(*results):
+        assert torch.equal(clean[:, ~spoilt], other[:, ~spoilt])
+    alone = torch.zeros(l, dtype=torch.bool)
+    alone[:10] = alone[200:] = True            # in no document
+    assert not results[1][0][:, alone].any() and not results[1][1][:, alone].any()
+
+
+@BOTH
+def test_future_values_reach_nothing_and_seen_ones_do(dtype):
+    import lact_amd
+    b, l, h, d = 1, 100, 2, 64
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(b, l, h, d, generator=g).to(dtype).to("cuda") for _ in range(3))
+    ref = lact_amd.masked_window_attention(q, k, v)
+    v2, k2 = v.clone(), k.clone()
+    v2[0, 70, 0, 3] = float("nan")
+    out = lact_amd.masked_window_attention(q, k2, v2)
+    assert torch.equal(out[:, :70], ref[:, :70]) and torch.equal(out[:, :, 1], ref[:, :, 1])
+    assert bool(torch.isnan(out[0, 70:, 0, 3]).all())
+    k2[0, 70, 0, 3] = float("nan")
+    out = lact_amd.masked_window_attention(q, k2, v)
+    assert torch.equal(out[:, :70], ref[:, :70]) and bool(torch.isnan(out[0, 70:, 0]).all())
+
+
+@BOTH
+def test_bounds_that_are_not_in_order_stay_inside(dtype):
+    """Nobody checks the bounds: whatever they hold, no read leaves the sequence and no token outside is attended to."""
+    import lact_amd
+    b, l, h, d = 2, 90, 2, 64
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.randn(b, l, h, d, generator=g).to(dtype).to("cuda").requires_grad_(True) for _ in range(3))
+    docs = torch.tensor([[50, -7, 400, 20], [2 ** 31 - 1, 0, -2 ** 31, 90]], dtype=torch.int32, device="cuda")
+    pre = torch.tensor([[1000, -5, 2 ** 31 - 1]] * 2, dtype=torch.int32, device="cuda")
+    out = lact_amd.masked_window_attention(q, k, v, documents=docs, prefixes=pre)
+    grads = torch.autograd.grad(out, (q, k, v), torch.ones_like(out))
+    assert all(bool(torch.isfinite(t).all()) for t in (out, *grads))
+
+
+def test_views_strides_and_alignment():
+    """Operands that the kernels do not read as they lie give what their copies give."""
+    import lact_amd
+    b, l, h, d = 2, 77, 3, 64
+    g = torch.Generator().manual_seed(1)
+    base = [torch.randn(b, h, l, d, generator=g).bfloat16().to("cuda") for _ in range(3)]
+    q, k, v = (t.transpose(1, 2) for t in base)                      # heads outside tokens
+    ref = lact_amd.masked_window_attention(*(t.contiguous() for t in (q, k, v)), 40)
+    assert torch.equal(lact_amd.masked_window_attention(q, k, v, 40), ref)
+    odd = torch.empty(b * l * h * d + 1, dtype=torch.bfloat16, device="cuda")[1:].view(b, l, h, d)
+    odd.copy_(k)
+    assert odd.data_ptr() % 16 and torch.equal(lact_amd.masked_window_attention(q, odd, v, 40), ref)
+    one = v[:, :, :1]
+    wide = lact_amd.masked_window_attention(q, k[:, :, :1].expand(b, l, 1, d), one.expand(b, l, 1, d), 40)
+    assert torch.equal(wide, lact_amd.masked_window_attention(q, k[:, :, :1].contiguous(), one.contiguous(), 40))
+    same = lact_amd.masked_window_attention(q[:1].expand(2, l, h, d), k[:1].expand(2, l, h, d), v[:1].expand(2, l, h, d), 40)
+    assert torch.equal(same[0], same[1]) and torch.equal(same[0], ref[0])
+
+
+def test_empty_sequences_and_batches():
+    import lact_amd
+    for b, l in ((0, 5), (2, 0)):
+        q, k, v = (torch.randn(b, l, n, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True) for n in (4, 2, 2))
+        out = lact_amd.masked_window_attention(q, k, v)
+        assert out.shape == q.shape and all(t.shape == x.shape for t, x in zip(torch.autograd.grad(out, (q, k, v), torch.empty_like(out)), (q, k, v)))
+
+
+def test_gradient_against_differences():
+    import lact_amd
+    b, l, hq, hkv, d = 1, 40, 2, 1, 64
+    g = torch.Generator().manual_seed(5)
+    q, k, v = (torch.randn(b, l, n, d, generator=g).to("cuda") for n in (hq, hkv, hkv))
+    w = torch.randn(b, l, hq, d, generator=g).double().to("cuda")
+    docs, sl = torch.tensor([[0, 17, 38]], device="cuda"), torch.tensor([0.1, 0.02], device="cuda")
+    f = lambda *a: lact_amd.masked_window_attention(*a, 20, score_cap=5.0, distance_slopes=sl, documents=docs)  # noqa: E731
+    x = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(f(*x), x, w.float())
+    for i in range(3):
+        step = torch.randn(x[i].shape, generator=g).to("cuda")
+        h = 2.0 ** -7
+        moved = [[t + (s * h * step if j == i else 0) for j, t in enumerate((q, k, v))] for s in (1, -1)]
+        diff = ((f(*moved[0]).double() - f(*moved[1]).double()) * w).sum() / (2 * h)
+        exact = (grads[i].double() * step.double()).sum()
+        # the third derivative times h^2 / 6, and fp32 outputs off by 2^-20 over 2 h
+        scale = (grads[i].double().abs() * step.double().abs()).sum()
+        assert abs(diff - exact) < 2e-3 * scale, (i, float(diff), float(exact))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16])
+def test_captured_training_step(dtype):
+    """Forward and backward captured into one graph and replayed with other inputs, eager work between the replays."""
+    import lact_amd
+    b, l, hq, hkv, d = 2, 200, 4, 2, 64
+    docs = torch.tensor([[0, 90, 200], [10, 20, 190]], dtype=torch.int32, device="cuda")
+    x = torch.randn(b, l, (hq + 2 * hkv) * d, device="cuda").to(dtype)
+    go = torch.randn(b, l, hq, d, device="cuda").to(dtype)
+
+    def step(x):
+        leaf = x.detach().requires_grad_(True)
+        out = lact_amd.masked_window_attention(*parts(leaf, hq, hkv, d), 64, documents=docs)
+        return out.detach(), torch.autograd.grad(out, leaf, go)[0]
+
+    step(x)
+    torch.cuda.synchronize()
+    static = x.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step(static)
+    for i in range(3):
+        fresh = torch.randn_like(x)
+        static.copy_(fresh)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, r in zip(res, step(fresh)):
+            assert torch.equal(a, r), i
+
+
+def test_other_streams_give_the_same():
+    import lact_amd
+    q, k, v = (torch.randn(1, 300, n, 128, device="cuda").bfloat16() for n in (8, 2, 2))
+    ref = lact_amd.masked_window_attention(q, k, v, 77)
+    lengths = torch.tensor([300], dtype=torch.int32, device="cuda")
+    ref1 = lact_amd.window_attention_step(q[:, -1], k, v, lengths, 77)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            outs.append((lact_amd.masked_window_attention(q, k, v, 77), lact_amd.window_attention_step(q[:, -1], k, v, lengths, 77)))
+    torch.cuda.synchronize()
+    for a, c in outs:
+        assert torch.equal(a, ref) and torch.equal(c, ref1)
+
+
+# ---- single tokens
+
+def check_step(b, n, hq, hkv, d, dtype, lengths, window=None, cap=None, slopes=False, layout="tokens"):
+    import lact_amd
+    print("[gpu-test] attention step", b, n, hq, hkv, d, dtype, lengths, window, cap, slopes, layout, flush=True)
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(b, hq, d, generator=g).to(dtype)
+    k, v = (torch.randn(b, n, hkv, d, generator=g).to(dtype) for _ in range(2))
+    sl = 2.0 ** -torch.arange(1, hq + 1).float() if slopes else None
+    kc, vc = (t.to("cuda") for t in (k, v))
+    for i, m in enumerate(lengths):                                  # what lies behind the lengths is not read
+        kc[i, max(0, min(m, n)):] = float("nan")
+        vc[i, max(0, min(m, n)):] = float("nan")
+    if layout == "heads":
+        kc, vc = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (kc, vc))
+    out = lact_amd.window_attention_step(q.to("cuda"), kc, vc, torch.tensor(lengths, device="cuda"), window, score_cap=cap,
+                                         distance_slopes=None if sl is None else sl.to("cuda"))
+    p_err, out_err = errors(dtype, n, d, 8.0 + (n if slopes else 0))
+    ref, bound = MO.attention_step(q, k, v, lengths, window, cap, sl, None, p_err, out_err)
+    assert out.dtype == dtype
+    near(out, ref, bound, "out")
+
+
+@BOTH
+@pytest.mark.parametrize("b,n,hq,hkv,d,lengths,window", [
+    (1, 1, 1, 1, 64, [1], None), (1, 300, 12, 12, 64, [300], 256), (3, 200, 4, 2, 128, [0, 1, 200], None), (2, 500, 7, 1, 128, [33, 499], 1),
+    (5, 129, 8, 8, 64, [-3, 128, 129, 1000, 32], 100), (2, 3000, 32, 4, 128, [2999, 31], None), (1, 4100, 40, 1, 64, [4097], None),
+    (70, 40, 2, 1, 64, [i % 41 for i in range(70)], 33)])
+def test_step(b, n, hq, hkv, d, lengths, window, dtype):
+    check_step(b, n, hq, hkv, d, dtype, lengths, window)
+
+
+@BOTH
+@pytest.mark.parametrize("layout", ["tokens", "heads"])
+def test_step_with_cap_and_distance(layout, dtype):
+    check_step(3, 700, 8, 2, 128, dtype, [700, 5, 333], 400, 20.0, True, layout)
+    check_step(2, 150, 4, 4, 64, dtype, [150, 64], None, 2.0, True, layout)
+
+
+def test_step_of_many_parts_is_joined():
+    """One long sequence over all compute units, and one block's share over many short ones."""
+    check_step(1, 20000, 2, 1, 128, torch.bfloat16, [19999])
+    check_step(600, 9, 4, 4, 64, torch.bfloat16, [i % 10 for i in range(600)])
+
+
+def test_step_of_a_cache_past_32_bits():
+    """The last sequence's cache lies more than 2^32 bytes behind the tensor's start, and its tokens more than 2^31 elements apart."""
+    import lact_amd
+    print("[gpu-test] attention step, far cache", flush=True)
+    b, n, hkv, d = 2, 70000, 256, 128
+    k = torch.zeros(b, n, hkv, d, dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(b, hkv, d, generator=g).bfloat16()
+    kk, vv = (torch.randn(6, 2, d, generator=g).bfloat16() for _ in range(2))
+    lengths = [n, n - 3]
+    for i in range(b):
+        k[i, lengths[i] - 6:lengths[i], -2:], v[i, lengths[i] - 6:lengths[i], -2:] = kk.to("cuda"), vv.to("cuda")
+    out = lact_amd.window_attention_step(q.to("cuda"), k, v, torch.tensor(lengths, device="cuda"), 6)
+    p_err, out_err = errors(torch.bfloat16, 6, d)
+    for i in range(b):
+        ref, bound = MO.attention_step(q[i:i + 1, -2:], kk[None], vv[None], [6], None, None, None, None, p_err, out_err)
+        near(out[i:i + 1, -2:], ref, bound, f"sequence {i}")
+    assert not out[:, :-2].any()
+
+
+def test_prompt_and_tokens_agree():
+    """A prompt through the attention, then token after token through the step, is the attention over all of it."""
+    import lact_amd
+    b, l, hq, hkv, d, prompt, window = 2, 90, 4, 2, 64, 70, 50
+    g = torch.Generator().manual_seed(9)
+    q, k, v = (torch.randn(b, l, n, d, generator=g).to("cuda") for n in (hq, hkv, hkv))
+    sl = torch.tensor([0.5, 0.25, 0.125, 0.0625], device="cuda")
+    opts = dict(score_cap=10.0, distance_slopes=sl)
+    whole = lact_amd.masked_window_attention(q, k, v, window, **opts)
+    kc, vc = (torch.full((b, 128, hkv, d), float("nan"), device="cuda") for _ in range(2))
+    kc[:, :prompt], vc[:, :prompt] = k[:, :prompt], v[:, :prompt]
+    outs = [lact_amd.masked_window_attention(q[:, :prompt], k[:, :prompt], v[:, :prompt], window, **opts)]
+    for t in range(prompt, l):
+        kc[:, t], vc[:, t] = k[:, t], v[:, t]
+        lengths = torch.full((b,), t + 1, dtype=torch.int32, device="cuda")
+        outs.append(lact_amd.window_attention_step(q[:, t], kc, vc, lengths, window, **opts)[:, None])
+    # both sides sum up to 50 probabilities in fp32, in another order
+    assert float((torch.cat(outs, 1) - whole).abs().max()) < (2 * d + 2 * l + 128) * 2.0 ** -24 * float(v.abs().max()) * 2
+
+
+def test_captured_steps():
+    """A step captured once and replayed while the sequences grow."""
+    import lact_amd
+    b, n, hq, hkv, d = 3, 400, 8, 2, 128
+    q, k, v = (torch.randn(*s, device="cuda").bfloat16() for s in ((b, hq, d), (b, n, hkv, d), (b, n, hkv, d)))
+    lengths = torch.tensor([1, 100, 250], dtype=torch.int32, device="cuda")
+    lact_amd.window_attention_step(q, k, v, lengths, 300)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = lact_amd.window_attention_step(q, k, v, lengths, 300)
+    for i in range(4):
+        q.copy_(torch.randn_like(q.float()))
+        lengths += 37
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, lact_amd.window_attention_step(q, k, v, lengths, 300)), i
+
+
+def test_refusals_on_the_gpu():
+    import lact_amd
+    f = lact_amd.masked_window_attention
+    q, k = torch.zeros(2, 8, 4, 64, device="cuda", dtype=torch.bfloat16), torch.zeros(2, 8, 2, 64, device="cuda", dtype=torch.bfloat16)
+    for bad, error in ((dict(k=k.float()), TypeError), (dict(v=k[:, :7]), ValueError), (dict(k=q), ValueError), (dict(distance_slopes=torch.zeros(2, device="cuda")), ValueError),
+                       (dict(distance_slopes=torch.zeros(4)), RuntimeError), (dict(documents=torch.zeros(1, 2, device="cuda", dtype=torch.int32)), ValueError),
+                       (dict(documents=torch.zeros(2, 2, device="cuda")), TypeError), (dict(prefixes=torch.zeros(2, 2, device="cuda", dtype=torch.int32)), ValueError),
+                       (dict(documents=torch.zeros(2, 2, dtype=torch.int32)), RuntimeError)):
+        with pytest.raises(error):
+            f(**{**dict(q=q, k=k, v=k), **bad})
+    with pytest.raises(TypeError):
+        f(q.half(), k.half(), k.half())
+    with pytest.raises(RuntimeError, match="divide"):
+        f(q[:, :, :3], k, k)
+    wide = torch.zeros(1, 8, 2, 96, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="64 or 128"):
+        f(wide, wide, wide)
+    leaf = q.clone().requires_grad_(True)
+    first, = torch.autograd.grad(f(leaf, k, k).float().sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(first.float().sum(), leaf)
+    step, n = lact_amd.window_attention_step, torch.ones(2, dtype=torch.int32, device="cuda")
+    for bad, error in ((dict(lengths=n.float()), TypeError), (dict(lengths=n[:1]), ValueError), (dict(v_cache=k[:, :7]), ValueError), (dict(lengths=n.cpu()), RuntimeError),
+                       (dict(k_cache=torch.zeros(2, 8, 2, 128, device="cuda", dtype=torch.bfloat16)[..., ::2]), ValueError),
+                       (dict(k_cache=torch.zeros(2 * 8 * 2 * 64 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(2, 8, 2, 64)), ValueError)):
+        with pytest.raises(error):
+            step(**{**dict(q=q[:, 0], k_cache=k, v_cache=k, lengths=n), **bad})
+    assert not step(q[:, 0], k[:, :0], k[:, :0], n).any()
+
+
+def test_autocast_casts_the_operands():
+    import lact_amd
+    x = torch.randn(1, 40, 2, 64, device="cuda", requires_grad=True)
+    with torch.autocast("cuda", torch.bfloat16):
+        out = lact_amd.masked_window_attention(x, x, x, 9)
+    g, = torch.autograd.grad(out.float().sum(), x)
+    b = x.detach().bfloat16()
+    assert out.dtype == torch.bfloat16 and g.dtype == torch.float32 and torch.equal(out, lact_amd.masked_window_attention(b, b, b, 9))
+    with torch.autocast("cuda", torch.float16), pytest.raises(TypeError):
+        lact_amd.masked_window_attention(x, x, x)
