@@ -261,7 +261,7 @@ int lact_window_attention_backward(int32_t B, int32_t L, int32_t H, int32_t D, i
  * n_documents 1: one of L tokens), where document n covers the tokens [documents[n], documents[n + 1]) (not falling; device memory, so not checked: bounds outside the sequence are cut
  * to it), and prefixes [B, n_documents] or null.  slopes: [H] fp32 or null, without a gradient.
  * out, dq, dk, dv contiguous; lse, delta: [B, H, L] fp32; ranges: lact_attention_ranges_bytes bytes (0 without documents), written by the
- * forward, read by the backward. */
+ * forward, read by the backward; workspace: the backward's own, lact_masked_attention_workspace_bytes bytes (often 0). */
 typedef struct lact_attention_desc {
   int32_t act_dtype, B, L, H, HK, D, window, n_documents;
   float scale, score_cap;
@@ -272,11 +272,12 @@ typedef struct lact_attention_desc {
   const int32_t* prefixes;
 } lact_attention_desc_t;
 size_t lact_attention_ranges_bytes(const lact_attention_desc_t* desc);
+size_t lact_masked_attention_workspace_bytes(const lact_attention_desc_t* desc);
 int lact_masked_attention_forward(const lact_attention_desc_t* desc, const void* q, const void* k, const void* v, void* out, float* lse,
                                   void* ranges, void* stream);
 int lact_masked_attention_backward(const lact_attention_desc_t* desc, const void* q, const void* k, const void* v, const void* out,
                                    const float* lse, const void* ranges, const void* dout, float* delta, void* dq, void* dk, void* dv,
-                                   void* stream);
+                                   void* workspace, void* stream);
 
 /* The same for one new token of every sequence: q, out [B, H, D]; k, v: caches [B, N, HK, D] with token (*_ld), batch (*_bs) and head (*_hs)
  * strides in elements, rows 16-byte aligned; lengths [B] int32 in device memory: the first lengths[b] entries are the sequence, the last of them

@@ -61,7 +61,7 @@ EXPORTS = ("lact_last_error", "lact_version", "lact_query_sizes", "lact_forward"
            "lact_layer_lr_backward", "lact_layer_post_forward", "lact_layer_post_dw_rows", "lact_layer_post_backward",
            "lact_window_attention_forward", "lact_window_attention_backward", "lact_layer_pre_attn_forward",
            "lact_layer_pre_attn_part_rows", "lact_layer_pre_attn_backward", "lact_layer_post_add_forward",
-           "lact_attention_ranges_bytes", "lact_masked_attention_forward", "lact_masked_attention_backward", "lact_attention_step_workspace_bytes",
+           "lact_attention_ranges_bytes", "lact_masked_attention_workspace_bytes", "lact_masked_attention_forward", "lact_masked_attention_backward", "lact_attention_step_workspace_bytes",
            "lact_attention_step", "lact_linear_attention_sizes", "lact_linear_attention_forward", "lact_linear_attention_backward",
            "lact_linear_attention_step")
 
@@ -145,10 +145,12 @@ def lib():
     for fn in ("lact_layer_post_add_forward", "lact_layer_pre_attn_forward", "lact_layer_pre_attn_part_rows", "lact_layer_pre_attn_backward", "lact_window_attention_forward", "lact_window_attention_backward", "lact_layer_pre_forward", "lact_layer_pre_backward", "lact_layer_lr_forward", "lact_layer_lr_backward",
                "lact_layer_post_forward", "lact_layer_post_dw_rows", "lact_layer_post_backward"):
         getattr(L, fn).restype = c_int32
+    L.lact_masked_attention_workspace_bytes.argtypes = [POINTER(AttentionDesc)]
+    L.lact_masked_attention_workspace_bytes.restype = c_size_t
     L.lact_attention_ranges_bytes.argtypes = [POINTER(AttentionDesc)]
     L.lact_attention_ranges_bytes.restype = c_size_t
     L.lact_masked_attention_forward.argtypes = [POINTER(AttentionDesc)] + [vp] * 7
-    L.lact_masked_attention_backward.argtypes = [POINTER(AttentionDesc)] + [vp] * 12
+    L.lact_masked_attention_backward.argtypes = [POINTER(AttentionDesc)] + [vp] * 13
     L.lact_attention_step_workspace_bytes.argtypes = [POINTER(AttentionStepDesc)]
     L.lact_attention_step_workspace_bytes.restype = c_size_t
     L.lact_attention_step.argtypes = [POINTER(AttentionStepDesc)] + [vp] * 7

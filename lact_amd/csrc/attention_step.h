@@ -193,11 +193,11 @@ __global__ __launch_bounds__((64 * AttnStepShape<T, D>::NW), 1) void k_attn_step
       sc.apply(s, at - (len - 1));
       if (k0 + 32 > len) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = 8 * (j / 4) + j % 4 < len - at ? s[j] : -__builtin_inff();
+        for (int j = 0; j < 16; ++j) s[j] = Seen(0, len - at).or_nothing(s[j], j);
       }
-      float mx = s[0];
+      float mx = max3(s[0], s[1], s[15]);
 #pragma unroll
-      for (int j = 1; j < 16; ++j) mx = __builtin_amdgcn_fmed3f(mx, s[j], __builtin_inff());
+      for (int j = 1; j < 8; ++j) mx = max3(mx, s[2 * j], s[2 * j + 1]);
       mx *= c;
       if (__any(mx > mc + 8.f)) {
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));

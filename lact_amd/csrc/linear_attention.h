@@ -424,7 +424,12 @@ __global__ __launch_bounds__(256, 1) void k_lin_walk(const LinParams<T> p) {
         p.dots[((size_t)b * L + t0 + lane) * p.H + h] = d;
       }
     // A value that is not finite must not reach the outputs that do not see its token (0 * inf): those chunks are summed term by term.
-    if (__any(any_unfinite(zf[0]) || any_unfinite(zf[1]))) {
+    bool bad = false;
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) bad |= unfinite(zf[v][nt]);
+    if (__any(bad)) {
       for (int j = 0; j < 64; ++j) {
         if (t0 + j >= L) break;
 #pragma unroll

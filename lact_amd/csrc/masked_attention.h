@@ -15,9 +15,8 @@
 // product as they lie: k slots 0..3 / 4..7 of lane half h stand for rows 4h + i / 8 + 4h + i of 16, on both operands.  fp32 runs the same
 // code: eight 32x32x2 products for one 32x32x16.
 //
-// A masked place weighs exactly nothing, whatever lies there: scores, probabilities and their gradients are selected, not multiplied,
-// and where a tile is masked for some row, values that are not finite are taken out of the product's other operand (0 * inf is NaN) and given
-// back as NaN to the rows that see them.
+// A masked place weighs exactly nothing, whatever lies there: scores, probabilities and their gradients are selected, not multiplied, and rows that
+// are not finite throughout are taken out of the products (0 * inf is NaN); a row that sees one of them has NaN for an output (Spoilt).
 #pragma once
 #include "gemm_dma.h"
 #include "window_attention.h"
@@ -41,6 +40,7 @@ struct MaskedAttnParams {
   const T* o;
   float* delta;                      // [B, H, L]: sum_d dout * out, written by dq, read by dk/dv
   T* dq; T* dk; T* dv;               // contiguous
+  float* part;                       // [2][splits][B, L, HK, D]: dk and dv of every split, where there are several
   UDiv by_heads, by_kv;              // B * (blocks' heads), B * HK
   __device__ __forceinline__ void locate(int& x, int& z) const {
     x = by_heads.div(blockIdx.x);
@@ -210,73 +210,62 @@ __device__ __forceinline__ typename AttnType<T>::Frag mask_pack(const f32x16& s,
   else return f32x8{s[8 * st], s[8 * st + 1], s[8 * st + 2], s[8 * st + 3], s[8 * st + 4], s[8 * st + 5], s[8 * st + 6], s[8 * st + 7]};
 }
 
-// Whether an operand holds something that is not finite; bit j of the result: slot j does.
-__device__ __forceinline__ uint32_t unfinite(const bf16x8& f) {
+// Whether eight elements hold something that is not finite.
+__device__ __forceinline__ bool unfinite(const bf16x8& f) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
   const uint4 u = __builtin_bit_cast(uint4, f);
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m |= ((w[i] & 0x7f80u) == 0x7f80u ? 1u << (2 * i) : 0u) | ((w[i] & 0x7f800000u) == 0x7f800000u ? 2u << (2 * i) : 0u);
-  return m;
-}
-__device__ __forceinline__ uint32_t unfinite(const f32x8& f) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m |= (__float_as_uint(f[i]) & 0x7f800000u) == 0x7f800000u ? 1u << i : 0u;
-  return m;
-}
-template <int N>
-__device__ __forceinline__ bool any_unfinite(const bf16x8 (&f)[N]) {
-  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
   u16x2 m = {0, 0};
 #pragma unroll
-  for (int s = 0; s < N; ++s) {
-    const uint4 u = __builtin_bit_cast(uint4, f[s]);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
-  }
-  return m[0] >= 0x7f80 || m[1] >= 0x7f80;
+  for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+  return max(m[0], m[1]) >= 0x7f80;
 }
-template <int N>
-__device__ __forceinline__ bool any_unfinite(const f32x8 (&f)[N]) {
+__device__ __forceinline__ bool unfinite(const f32x8& f) {
   uint32_t m = 0;
 #pragma unroll
-  for (int s = 0; s < N; ++s)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[s][i]) & 0x7fffffffu);
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
   return m >= 0x7f800000u;
 }
-__device__ __forceinline__ void drop(bf16x8& f, uint32_t bad) {
-  uint4 u = __builtin_bit_cast(uint4, f);
-  uint32_t* w = &u.x;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] &= (bad >> (2 * i) & 1 ? 0u : 0xffffu) | (bad >> (2 * i) & 2 ? 0u : 0xffff0000u);
-  f = __builtin_bit_cast(bf16x8, u);
-}
-__device__ __forceinline__ void drop(f32x8& f, uint32_t bad) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = bad >> i & 1 ? 0.f : f[i];
-}
-// Takes what is not finite out of the operands of 16 tile rows; bit j of the result: the row of this lane's slot j held such a value
-// in any column.
-template <typename F, int N>
-__device__ __forceinline__ uint32_t make_finite(F (&f)[N]) {
-  uint32_t bad = 0, rows = 0;
-#pragma unroll
-  for (int s = 0; s < N; ++s) {
-    const uint32_t m = unfinite(f[s]);
-    drop(f[s], m);
-    bad |= m;
+// What lies in a tile and is not finite must not meet the zero weight of a row that does not see it.  The wave that copied 1 KB of a tile looks it over
+// once it is there, clears rows that hold such a value and writes down which; every wave gives the rows of its own that see one of them NaN.
+// (Selecting in the products' operands instead, where a tile is masked, cost a tenth of the forward: a branch at every operand, or registers for two loops.)
+template <typename T, int D, int NW>
+struct Spoilt {
+  using S = MaskTile<T, D>;
+  static constexpr int BYTES = 64;
+  uint32_t* words;        // rows [0, 32) and [32, 64) of every ring slot; behind them whether there ever were any
+  __device__ __forceinline__ void init(char* lds) {
+    words = reinterpret_cast<uint32_t*>(lds);
+    if (threadIdx.x < 16) words[threadIdx.x] = 0;
+    __syncthreads();
   }
-  const int half = (threadIdx.x & 63) >> 5;
+  __device__ __forceinline__ void look(char* tile, int slot, int wave) const {
+    const int l = threadIdx.x & 63;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint64_t who = __ballot(bad >> j & 1);
-    rows |= (uint32_t)(who >> (32 * half)) ? 1u << j : 0u;
+    for (int i = 0; i < S::G / NW; ++i) {
+      uint4* at = reinterpret_cast<uint4*>(tile + (wave + i * NW) * 1024 + l * 16);
+      const uint4 u = *at;
+      bool bad;
+      if constexpr (sizeof(T) == 2) bad = unfinite(__builtin_bit_cast(bf16x8, u));
+      else bad = ((u.x & 0x7f800000u) == 0x7f800000u) | ((u.y & 0x7f800000u) == 0x7f800000u) | ((u.z & 0x7f800000u) == 0x7f800000u) | ((u.w & 0x7f800000u) == 0x7f800000u);
+      const uint64_t who = __ballot(bad);
+      if (who) {
+        const int in = l / S::G, row = (wave + i * NW) * (64 / S::G) + in;      // G lanes hold a row
+        if (who >> (in * S::G) & ((1ull << S::G) - 1)) {
+          *at = make_uint4(0, 0, 0, 0);
+          if (l % S::G == 0) atomicOr(words + 2 * slot + (row >> 5), 1u << (row & 31));
+          words[15] = 1;
+        }
+      }
+    }
   }
-  return rows;
-}
+  // behind the barrier: the slot's rows; and room for those of the slot that the next copies go to
+  __device__ __forceinline__ bool any() const { return __builtin_amdgcn_readfirstlane(*(volatile uint32_t*)(words + 15)) != 0; }
+  __device__ __forceinline__ uint64_t rows(int slot) const { return (uint64_t)words[2 * slot] | (uint64_t)words[2 * slot + 1] << 32; }
+  __device__ __forceinline__ void clear(int slot) const {
+    if (threadIdx.x < 2) words[2 * slot + threadIdx.x] = 0;
+  }
+};
 
 // tanh in fp32.  Small x: Lambert's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + x^2 / (7 + x^2 / 9)))), relative error below 1e-8
 // up to 0.8; 1 - 2 / (1 + e^2x) there loses the bits that x has below 1.
@@ -321,13 +310,17 @@ struct Scores {
   // the same, and the gradients dp (of what the softmax weighs) times the derivative of the cap
   __device__ __forceinline__ void apply(f32x16& s, f32x16& dp, int first) const {
     if (cap) {
-      f32x16 t;
+      // (in steps of four: one loop over both vectors leaves them in memory)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) t[j] = bent(s[j]);
+      for (int g = 0; g < 4; ++g) {
+        f32x4 t;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) s[j] = t[j] * k2;
+        for (int j = 0; j < 4; ++j) t[j] = bent(s[4 * g + j]);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) dp[j] *= fmaf(-t[j], t[j], 1.f);
+        for (int j = 0; j < 4; ++j) s[4 * g + j] = t[j] * k2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dp[4 * g + j] *= fmaf(-t[j], t[j], 1.f);
+      }
     } else if (bias) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[j] *= c;
@@ -346,21 +339,30 @@ template <typename T, int D> constexpr int mask_ring() { return sizeof(T) == 2 ?
 template <typename T, int D, int NW>
 constexpr int mask_lds_bytes(bool stats) {
   constexpr int R = mask_ring<T, D>();
-  return cmax(R * 2 * MaskTile<T, D>::BYTES + (stats ? R * 512 : 0), NW * 32 * (D + 16 / (int)sizeof(T)) * (int)sizeof(T));
+  const int ring = R * 2 * MaskTile<T, D>::BYTES + (stats ? R * 512 : 0) + Spoilt<T, D, NW>::BYTES;
+  // what the rows are stored through, for splits in fp32
+  return cmax(ring, NW * 32 * cmax((D + 16 / (int)sizeof(T)) * (int)sizeof(T), stats && NW == 4 ? (D + 4) * 4 : 0));
 }
 
-// Walks the tiles [0, n): issue(t) starts the copies of tile t, COPIES of a wave, RING - 1 tiles ahead; body(t) uses it.
-template <int COPIES, int RING, typename Issue, typename Body>
-__device__ __forceinline__ void mask_walk(int n, Issue issue, Body body) {
+// Walks the tiles [0, n): issue(t) starts the copies of tile t, COPIES of a wave, RING - 1 tiles ahead; look(t) sees the wave's own when they are there;
+// body(t, rows) uses the tile, `rows` of which are spoilt.
+template <int COPIES, int RING, typename Sp, typename Issue, typename Look, typename Body>
+__device__ __forceinline__ void mask_walk(int n, const Sp& spoilt, Issue issue, Look look, Body body) {
 #pragma unroll
   for (int t = 0; t < RING - 1; ++t)
     if (t < n) issue(t);
   for (int t = 0; t < n; ++t) {
     if (RING == 3 && t + 1 < n) wait_vmcnt<COPIES>();
     else wait_vmcnt<0>();
+    look(t);
     __syncthreads();      // tile t is there for every wave, and all are through with t - 1, whose place the next one takes
     if (t + RING - 1 < n) issue(t + RING - 1);
-    body(t);
+    uint64_t rows = 0;
+    if (spoilt.any()) {
+      rows = spoilt.rows(t % RING);
+      spoilt.clear((t + RING - 1) % RING);
+    }
+    body(t, rows);
   }
 }
 
@@ -404,8 +406,38 @@ struct WaveReach {
   __device__ __forceinline__ bool masked(int a, int n) const { return a < full_lo || a + n > full_hi; }
 };
 
+// Which of a lane's 16 elements of 32 tile rows lie in [lo, hi): element j is row 8 (j / 4) + j % 4, lo and hi count from the lane's first.  Two
+// instructions an element to apply (a bit spread over a word, a select by it) where comparisons take four.
+struct Seen {
+  uint32_t bits;
+  __device__ __forceinline__ Seen(int lo, int hi) {
+    const uint32_t below = hi >= 32 ? 0xffffffffu : hi <= 0 ? 0u : (1u << hi) - 1u, under = lo >= 32 ? 0xffffffffu : lo <= 0 ? 0u : (1u << lo) - 1u;
+    bits = below & ~under;
+  }
+  // whether a row among `rows` (of the 32) is one of them
+  __device__ __forceinline__ bool any_of(uint32_t rows) const { return (bits & 0x0f0f0f0fu & rows >> (4 * ((threadIdx.x & 63) >> 5))) != 0; }
+  // all ones or zero; computed here and now, not kept in a register for every j
+  __device__ __forceinline__ uint32_t word(int j) const {
+    uint32_t w;
+    asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(w) : "v"(bits), "n"(8 * (j / 4) + j % 4));
+    return w;
+  }
+  __device__ __forceinline__ float or_nothing(float s, int j) const {      // s, or -infinity
+    float r;
+    asm("v_bfi_b32 %0, %1, %2, %3" : "=v"(r) : "v"(word(j)), "v"(s), "s"(0xff800000u));
+    return r;
+  }
+  __device__ __forceinline__ float or_zero(float s, int j) const { return __uint_as_float(__float_as_uint(s) & word(j)); }
+};
+// One instruction; fmaxf quiets its operands first.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_fwd(const MaskedAttnParams<T> p) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_fwd(const MaskedAttnParams<T> p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using S = MaskTile<T, D>;
   using Copy = MaskCopy<T, D, NW>;
@@ -448,15 +480,17 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_fwd(co
   ck.init(wave, p.k + b * p.bsk + hk * D, p.ldk, first, tiles, L);
   cv.init(wave, p.v + b * p.bsv + hk * D, p.ldv, first, tiles, L);
   const uint32_t lds0 = lds_addr(smem);
-  auto larger = [](float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_inff()); };
+  Spoilt<T, D, NW> spoilt;
+  spoilt.init(smem + RING * STAGE);
   mask_arrived(qf);
-  mask_walk<2 * Copy::NC, RING>(tiles,
+  mask_walk<2 * Copy::NC, RING>(tiles, spoilt,
     [&](int t) LACT_INLINE_LAMBDA {
       const uint32_t slot = lds0 + t % RING * STAGE;
       ck.issue(t, ck.base, slot, wave);
       cv.issue(t, cv.base, slot + S::BYTES, wave);
     },
-    [&](int t) LACT_INLINE_LAMBDA {
+    [&](int t) LACT_INLINE_LAMBDA { spoilt.look(smem + t % RING * STAGE + S::BYTES, t % RING, wave); },
+    [&](int t, uint64_t bad) LACT_INLINE_LAMBDA {
       const int k0 = first + t * 64;
       if (!reach.sees(k0, 64)) return;
       const char* kt = smem + t % RING * STAGE;
@@ -473,20 +507,23 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_fwd(co
       const int at = k0 + 4 * (lane >> 5);
 #pragma unroll
       for (int i = 0; i < 2; ++i) sc.apply(s[i], at + 32 * i - row);
-      const bool masked = reach.masked(k0, 64);
-      if (masked) {
-        const int lo = own.x - at, hi = own.y - at;
+      if (reach.masked(k0, 64)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const Seen seen(own.x - at - 32 * i, own.y - at - 32 * i);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[i][j] = seen.or_nothing(s[i][j], j);
+        }
+      }
+      if (bad) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int key = i * 32 + 8 * (j / 4) + j % 4;
-            s[i][j] = (key >= lo && key < hi) ? s[i][j] : -__builtin_inff();
-          }
+          if (Seen(own.x - at - 32 * i, own.y - at - 32 * i).any_of((uint32_t)(bad >> (32 * i)))) sum = __builtin_nanf("");
       }
-      float mx = larger(s[0][0], s[1][0]);
+      float mx = s[0][0];
+      mx = max3(mx, s[1][0], s[1][1]);
 #pragma unroll
-      for (int j = 1; j < 16; ++j) mx = larger(mx, larger(s[0][j], s[1][j]));
+      for (int j = 1; j < 16; ++j) mx = max3(mx, s[0][j], s[1][j]);
       mx *= c;
       // The maximum only has to keep exp2 in range: it follows the row when it is exceeded by more than 2^8 (its own row only: what a row
       // gives does not depend on the others).
@@ -512,19 +549,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_fwd(co
 #pragma unroll
       for (int st = 0; st < 4; ++st) {
         const Frag pf = mask_pack<T>(s[st >> 1], st & 1);
-        Frag vb[D / 32];
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) vb[dt] = fr.cols(vt, dt, st);
-        if (masked && __any(any_unfinite(vb))) {
-          const uint32_t bad = make_finite(vb);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int key = at + 16 * st + (j < 4 ? j : 4 + j);
-            if ((bad >> j & 1) && key >= own.x && key < own.y) sum = __builtin_nanf("");
-          }
-        }
-#pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) o[dt] = mma32(vb[dt], pf, o[dt]);
+        for (int dt = 0; dt < D / 32; ++dt) o[dt] = mma32(fr.cols(vt, dt, st), pf, o[dt]);
       }
     });
   sum += __shfl_xor(sum, 32, 64);
@@ -536,7 +562,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_fwd(co
 
 // dq = scale * sum_keys ds k with ds = p (dp - delta) f', and delta itself.
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dq(const MaskedAttnParams<T> p) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_dq(const MaskedAttnParams<T> p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using S = MaskTile<T, D>;
   using Copy = MaskCopy<T, D, NW>;
@@ -595,13 +621,17 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dq(con
   mask_arrived(qf);
   mask_arrived(gf);
   asm volatile("" : "+v"(lse), "+v"(delta));
-  mask_walk<2 * Copy::NC, RING>(tiles,
+  Spoilt<T, D, NW> spoilt;
+  spoilt.init(smem + RING * STAGE);
+  float poison = 0.f;
+  mask_walk<2 * Copy::NC, RING>(tiles, spoilt,
     [&](int t) LACT_INLINE_LAMBDA {
       const uint32_t slot = lds0 + t % RING * STAGE;
       ck.issue(t, ck.base, slot, wave);
       cv.issue(t, cv.base, slot + S::BYTES, wave);
     },
-    [&](int t) LACT_INLINE_LAMBDA {
+    [&](int t) LACT_INLINE_LAMBDA { spoilt.look(smem + t % RING * STAGE, t % RING, wave); },
+    [&](int t, uint64_t bad) LACT_INLINE_LAMBDA {
       const char* kt = smem + t % RING * STAGE;
       const char* vt = kt + S::BYTES;
 #pragma unroll
@@ -622,34 +652,27 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dq(con
         sc.apply(s, dp, at - row);
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], c, -lse)) * dp[j];
-        const bool masked = reach.masked(k0, 32);
-        if (masked) {
-          const int lo = own.x - at, hi = own.y - at;
+        if (reach.masked(k0, 32)) {
+          const Seen seen(own.x - at, own.y - at);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int key = 8 * (j / 4) + j % 4;
-            s[j] = (key >= lo && key < hi) ? s[j] : 0.f;
-          }
+          for (int j = 0; j < 16; ++j) s[j] = seen.or_zero(s[j], j);
         }
+        if (bad && Seen(own.x - at, own.y - at).any_of((uint32_t)(bad >> (32 * i)))) poison = __builtin_nanf("");
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
           const Frag pf = mask_pack<T>(s, st);
-          Frag kb[D / 32];
 #pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) kb[dt] = fr.cols(kt, dt, 2 * i + st);
-          // (a row that sees such a key has a gradient of its score that is not finite)
-          if (masked && __any(any_unfinite(kb))) make_finite(kb);
-#pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) o[dt] = mma32(kb[dt], pf, o[dt]);
+          for (int dt = 0; dt < D / 32; ++dt) o[dt] = mma32(fr.cols(kt, dt, 2 * i + st), pf, o[dt]);
         }
       }
     });
+  poison += __shfl_xor(poison, 32, 64);
   __syncthreads();
-  mask_store_rows<T, D>(smem + wave * 32 * (D + 16 / sizeof(T)) * sizeof(T), o, p.scale, p.dq + ((size_t)b * L * p.H + h) * D, (size_t)p.H * D, row0, L);
+  mask_store_rows<T, D>(smem + wave * 32 * (D + 16 / sizeof(T)) * sizeof(T), o, p.scale + poison, p.dq + ((size_t)b * L * p.H + h) * D, (size_t)p.H * D, row0, L);
 }
 
 // dv = sum_queries p dout, dk = scale * sum_queries ds q, over the queries of all heads that share the key head: a wave owns 32 keys and
-// walks the queries that see them, head after head.
+// walks the queries that see them, head after head.  With few keys (blocks) the walk is cut into gridDim.y splits, whose sums k_attn_sum adds.
 template <typename T, int D, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dkv(const MaskedAttnParams<T> p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -684,7 +707,8 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dkv(co
 #pragma unroll
     for (int j = 0; j < 16; ++j) ok[i][j] = ov[i][j] = 0.f;
   first = min(first, L) / 64 * 64;
-  const int tiles = last > first ? (last - first + 63) / 64 : 0, all = tiles * p.group;
+  const int tiles = last > first ? (last - first + 63) / 64 : 0, steps = tiles * p.group;
+  const int splits = gridDim.y, from = (int)((long long)steps * blockIdx.y / splits), all = (int)((long long)steps * (blockIdx.y + 1) / splits) - from;
   const uint32_t lds0 = lds_addr(smem);
   const char* stats = smem + RING * STAGE;             // per ring slot: 64 lse, 64 delta
   const int h0 = hk * p.group;
@@ -693,14 +717,16 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dkv(co
   cg.init(wave, p.dout + b * p.bsdo + h0 * D, p.lddo, first, tiles, L);
   // the even waves bring the slot's lse, the odd ones its delta: the same bytes from each, one copy per wave
   const float* st_src = (wave & 1 ? p.delta : p.lse) + (size_t)(b * p.H + h0) * L;
-  int ih = 0, it = 0, bh = 0, bt = 0;                  // head and tile of the next copies, and of the next use
+  int ih = tiles ? from / tiles : 0, it = from - ih * tiles, bh = ih, bt = it;      // head and tile of the next copies, and of the next use
   float poison = 0.f;
   Scores<T> sc;
   sc.init(p.scale, p.cap, p.slopes, h0);
   const float c = sc.unit();
   mask_arrived(kf);
   mask_arrived(vf);
-  mask_walk<2 * Copy::NC + 1, RING>(all,
+  Spoilt<T, D, NW> spoilt;
+  spoilt.init(smem + RING * (STAGE + 512));
+  mask_walk<2 * Copy::NC + 1, RING>(all, spoilt,
     [&](int t) LACT_INLINE_LAMBDA {
       const uint32_t slot = t % RING;
       cq.issue(it, cq.base + ih * D, lds0 + slot * STAGE, wave);
@@ -710,8 +736,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dkv(co
       if (++it == tiles) { it = 0; ++ih; }
     },
     [&](int t) LACT_INLINE_LAMBDA {
+      spoilt.look(smem + t % RING * STAGE, t % RING, wave);
+      spoilt.look(smem + t % RING * STAGE + S::BYTES, t % RING, wave);
+    },
+    [&](int t, uint64_t bad) LACT_INLINE_LAMBDA {
       const int slot = t % RING, t0 = first + bt * 64;
-      if (bt == 0 && p.slopes) sc.slope = p.slopes[h0 + bh] * ATTN_LOG2E;
+      if ((bt == 0 || t == 0) && p.slopes) sc.slope = p.slopes[h0 + bh] * ATTN_LOG2E;
       if (++bt == tiles) { bt = 0; ++bh; }
       const char* qt = smem + slot * STAGE;
       const char* gt = qt + S::BYTES;
@@ -745,47 +775,54 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dkv(co
             ds[4 * g + j] *= s[4 * g + j];
           }
         }
-        const bool masked = reach.masked(q0, 32);
-        const int lo = own.x - at, hi = own.y - at;
-        if (masked) {
+        if (reach.masked(q0, 32)) {
+          const Seen seen(own.x - at, own.y - at);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            const int qi = 8 * (j / 4) + j % 4;
-            const bool seen = qi >= lo && qi < hi;
-            s[j] = seen ? s[j] : 0.f;
-            ds[j] = seen ? ds[j] : 0.f;
+            s[j] = seen.or_zero(s[j], j);
+            ds[j] = seen.or_zero(ds[j], j);
           }
         }
+        if (bad && Seen(own.x - at, own.y - at).any_of((uint32_t)(bad >> (32 * i)))) poison = __builtin_nanf("");
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
           const Frag pf = mask_pack<T>(s, st), df = mask_pack<T>(ds, st);
-          Frag fb[D / 32];
 #pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) fb[dt] = fr.cols(gt, dt, 2 * i + st);
-          if (masked && __any(any_unfinite(fb))) {
-            const uint32_t bad = make_finite(fb);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int qi = 16 * st + (j < 4 ? j : 4 + j);
-              if ((bad >> j & 1) && qi >= lo && qi < hi) poison = __builtin_nanf("");
-            }
+          for (int dt = 0; dt < D / 32; ++dt) {
+            ov[dt] = mma32(fr.cols(gt, dt, 2 * i + st), pf, ov[dt]);
+            ok[dt] = mma32(fr.cols(qt, dt, 2 * i + st), df, ok[dt]);
           }
-#pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) ov[dt] = mma32(fb[dt], pf, ov[dt]);
-#pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) fb[dt] = fr.cols(qt, dt, 2 * i + st);
-          if (masked && __any(any_unfinite(fb))) make_finite(fb);
-#pragma unroll
-          for (int dt = 0; dt < D / 32; ++dt) ok[dt] = mma32(fb[dt], df, ok[dt]);
         }
       }
     });
   poison += __shfl_xor(poison, 32, 64);
   __syncthreads();
-  const size_t o = ((size_t)b * L * p.HK + hk) * D;
+  const size_t o = ((size_t)b * L * p.HK + hk) * D, ld = (size_t)p.HK * D;
+  if (NW == 4 && splits > 1) {
+    float* stage = reinterpret_cast<float*>(smem) + wave * 32 * (D + 4);
+    const size_t all_keys = (size_t)p.B * L * ld, at = blockIdx.y * all_keys + o;
+    mask_store_rows<float, D>(reinterpret_cast<char*>(stage), ok, p.scale + poison, p.part + at, ld, row0, L);
+    mask_store_rows<float, D>(reinterpret_cast<char*>(stage), ov, 1.f + poison, p.part + splits * all_keys + at, ld, row0, L);
+    return;
+  }
   char* stage = smem + wave * 32 * (D + 16 / sizeof(T)) * sizeof(T);
-  mask_store_rows<T, D>(stage, ok, p.scale, p.dk + o, (size_t)p.HK * D, row0, L);
-  mask_store_rows<T, D>(stage, ov, 1.f + poison, p.dv + o, (size_t)p.HK * D, row0, L);
+  mask_store_rows<T, D>(stage, ok, p.scale + poison, p.dk + o, ld, row0, L);
+  mask_store_rows<T, D>(stage, ov, 1.f + poison, p.dv + o, ld, row0, L);
+}
+
+// dk (blockIdx.y 0) and dv (1): the sums of their splits, four elements a thread, in the splits' order.
+template <typename T>
+__global__ __launch_bounds__(256) void k_attn_sum(long long n, int splits, const float* part, T* dk, T* dv) {
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  const float* src = part + (blockIdx.y ? splits * n : 0) + i;
+  float4 a = *reinterpret_cast<const float4*>(src);
+#pragma unroll 4
+  for (int s = 1; s < splits; ++s) {
+    const float4 u = *reinterpret_cast<const float4*>(src + s * n);
+    a.x += u.x; a.y += u.y; a.z += u.z; a.w += u.w;
+  }
+  Elem<T>::store4((blockIdx.y ? dv : dk) + i, a.x, a.y, a.z, a.w);
 }
 
 }  // namespace lact

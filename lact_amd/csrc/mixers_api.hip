@@ -66,36 +66,55 @@ int attention_params(const lact_attention_desc_t* d, const void* q, const void* 
   return 0;
 }
 
-// Waves per block: 8 (256 rows) once that gives every compute unit a block, else 4.  which: 0 forward, 1 dq, 2 dk and dv
-template <typename T, int D, int NW>
-void launch_attention(int which, MaskedAttnParams<T> p, hipStream_t s) {
-  const int heads = p.B * (which == 2 ? p.HK : p.H);
+// Splits of the queries that a block of keys walks, where the blocks of 128 keys of all heads are fewer than the compute units: two blocks to a unit,
+// four tiles of 64 queries at least to a block.
+int key_splits(const lact_attention_desc_t* d) {
+  const long long blocks = (long long)ceil_div(d->L, 128) * d->B * d->HK;
+  if (blocks >= COMPUTE_UNITS) return 1;
+  const long long tiles = (long long)ceil_div(std::min(d->L, std::min(d->window, d->L) + 127), 64) * (d->H / d->HK);
+  return (int)std::max<long long>(1, std::min<long long>({2 * COMPUTE_UNITS / blocks, tiles / 4, 16}));
+}
+size_t attention_workspace(const lact_attention_desc_t* d) {
+  const int n = key_splits(d);
+  return n > 1 ? (size_t)2 * n * d->B * d->L * d->HK * d->D * sizeof(float) : 0;
+}
+
+// WHICH: 0 forward, 1 dq, 2 dk and dv (in `splits`)
+template <int WHICH, typename T, int D, int NW>
+void launch_attention(int splits, MaskedAttnParams<T> p, hipStream_t s) {
+  const int heads = p.B * (WHICH == 2 ? p.HK : p.H);
   p.by_heads = make_udiv(heads);
-  const dim3 grid(ceil_div(p.L, 32 * NW) * heads), block(64 * NW);
-  constexpr int SM = mask_lds_bytes<T, D, NW>(false), SMS = mask_lds_bytes<T, D, NW>(true);
+  const dim3 grid(ceil_div(p.L, 32 * NW) * heads, splits), block(64 * NW);
+  constexpr int SM = mask_lds_bytes<T, D, NW>(WHICH == 2);
   const double w = p.window, f = 2.0 * ((double)p.L * w - w * (w - 1) / 2) * D * p.B * p.H;      // without documents
-  if (which == 0) {
+  if constexpr (WHICH == 0) {
     LACT_BIG_LDS((k_masked_attn_fwd<T, D, NW>), SM);
     LACT_LAUNCH_SMEM("k_masked_attn_fwd", "masked_attn", 2 * f, (k_masked_attn_fwd<T, D, NW>), grid, block, SM, s, p);
-  } else if (which == 1) {
+  } else if constexpr (WHICH == 1) {
     LACT_BIG_LDS((k_masked_attn_dq<T, D, NW>), SM);
     LACT_LAUNCH_SMEM("k_masked_attn_dq", "masked_attn_bwd", 3 * f, (k_masked_attn_dq<T, D, NW>), grid, block, SM, s, p);
   } else {
-    LACT_BIG_LDS((k_masked_attn_dkv<T, D, NW>), SMS);
-    LACT_LAUNCH_SMEM("k_masked_attn_dkv", "masked_attn_bwd", 4 * f, (k_masked_attn_dkv<T, D, NW>), grid, block, SMS, s, p);
+    LACT_BIG_LDS((k_masked_attn_dkv<T, D, NW>), SM);
+    LACT_LAUNCH_SMEM("k_masked_attn_dkv", "masked_attn_bwd", 4 * f, (k_masked_attn_dkv<T, D, NW>), grid, block, SM, s, p);
+    if (splits > 1) {
+      const long long n = (long long)p.B * p.L * p.HK * D;
+      LACT_LAUNCH("k_attn_sum", "masked_attn_bwd", 0.0, (k_attn_sum<T>), dim3((unsigned)((n / 4 + 255) / 256), 2), dim3(256), s, n, splits, p.part, p.dk, p.dv);
+    }
   }
 }
-template <typename T, int D>
-void launch_attention(int which, const MaskedAttnParams<T>& p, hipStream_t s) {
-  if constexpr (sizeof(T) == 2) {
-    if ((long long)ceil_div(p.L, 256) * p.B * (which == 2 ? p.HK : p.H) >= COMPUTE_UNITS) return launch_attention<T, D, 8>(which, p, s);
+// Waves per block: 8 (256 rows) once that gives every compute unit a block, else 4.  dk and dv of heads of 128 take more registers than two waves of
+// a SIMD have: 4.
+template <int WHICH, typename T, int D>
+void launch_attention(int splits, const MaskedAttnParams<T>& p, hipStream_t s) {
+  if constexpr (sizeof(T) == 2 && (WHICH < 2 || D == 64)) {
+    if ((long long)ceil_div(p.L, 256) * p.B * (WHICH == 2 ? p.HK : p.H) >= COMPUTE_UNITS) return launch_attention<WHICH, T, D, 8>(1, p, s);
   }
-  launch_attention<T, D, 4>(which, p, s);
+  launch_attention<WHICH, T, D, 4>(splits, p, s);
 }
-template <typename T>
-void launch_attention(int which, int D, const MaskedAttnParams<T>& p, hipStream_t s) {
-  if (D == 128) launch_attention<T, 128>(which, p, s);
-  else launch_attention<T, 64>(which, p, s);
+template <int WHICH, typename T>
+void launch_attention(int splits, int D, const MaskedAttnParams<T>& p, hipStream_t s) {
+  if (D == 128) launch_attention<WHICH, T, 128>(splits, p, s);
+  else launch_attention<WHICH, T, 64>(splits, p, s);
 }
 
 template <typename T>
@@ -107,22 +126,23 @@ int attention_forward(const lact_attention_desc_t* d, const void* q, const void*
   if (d->n_documents)
     LACT_LAUNCH("k_attn_ranges", "masked_attn", 0.0, k_attn_ranges, dim3(ceil_div(d->L, 256), d->B), dim3(256), s, d->B, d->L, d->n_documents, p.window, d->documents,
                 d->prefixes, const_cast<int2*>(p.rows), const_cast<int2*>(p.cols));
-  launch_attention(0, d->D, p, s);
+  launch_attention<0>(1, d->D, p, s);
   LACT_CHECK_LAUNCH();
   return 0;
 }
 template <typename T>
 int attention_backward(const lact_attention_desc_t* d, const void* q, const void* k, const void* v, const void* out, const float* lse, const void* ranges,
-                       const void* dout, float* delta, void* dq, void* dk, void* dv, hipStream_t s) {
+                       const void* dout, float* delta, void* dq, void* dk, void* dv, void* workspace, hipStream_t s) {
   MaskedAttnParams<T> p;
+  if (attention_workspace(d) && !workspace) return fail("null pointer: masked attention workspace");
   if (attention_params(d, q, k, v, const_cast<void*>(ranges), &p) || check_rows(dout, d->do_ld, d->do_bs, d->H * d->D, d->act_dtype, "dout") ||
       check_ptrs({out, lse, delta, dq, dk, dv}, "masked attention backward tensors"))
     return -1;
   p.o = static_cast<const T*>(out); p.lse = const_cast<float*>(lse); p.delta = delta;
   p.dout = static_cast<const T*>(dout); p.lddo = d->do_ld; p.bsdo = d->do_bs;
-  p.dq = static_cast<T*>(dq); p.dk = static_cast<T*>(dk); p.dv = static_cast<T*>(dv);
-  launch_attention(1, d->D, p, s);
-  launch_attention(2, d->D, p, s);
+  p.dq = static_cast<T*>(dq); p.dk = static_cast<T*>(dk); p.dv = static_cast<T*>(dv); p.part = static_cast<float*>(workspace);
+  launch_attention<1>(1, d->D, p, s);
+  launch_attention<2>(key_splits(d), d->D, p, s);
   LACT_CHECK_LAUNCH();
   return 0;
 }
@@ -346,6 +366,8 @@ size_t lact_attention_ranges_bytes(const lact_attention_desc_t* d) {
   return d && d->n_documents > 0 && d->B > 0 && d->L > 0 ? (size_t)d->B * d->L * 2 * sizeof(int2) : 0;
 }
 
+size_t lact_masked_attention_workspace_bytes(const lact_attention_desc_t* d) { return check_attention(d) ? 0 : attention_workspace(d); }
+
 int lact_masked_attention_forward(const lact_attention_desc_t* d, const void* q, const void* k, const void* v, void* out, float* lse, void* ranges, void* stream) {
   if (check_attention(d)) return -1;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
@@ -353,11 +375,11 @@ int lact_masked_attention_forward(const lact_attention_desc_t* d, const void* q,
 }
 
 int lact_masked_attention_backward(const lact_attention_desc_t* d, const void* q, const void* k, const void* v, const void* out, const float* lse, const void* ranges,
-                                   const void* dout, float* delta, void* dq, void* dk, void* dv, void* stream) {
+                                   const void* dout, float* delta, void* dq, void* dk, void* dv, void* workspace, void* stream) {
   if (check_attention(d)) return -1;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  return d->act_dtype == LACT_BF16 ? attention_backward<uint16_t>(d, q, k, v, out, lse, ranges, dout, delta, dq, dk, dv, s)
-                                   : attention_backward<float>(d, q, k, v, out, lse, ranges, dout, delta, dq, dk, dv, s);
+  return d->act_dtype == LACT_BF16 ? attention_backward<uint16_t>(d, q, k, v, out, lse, ranges, dout, delta, dq, dk, dv, workspace, s)
+                                   : attention_backward<float>(d, q, k, v, out, lse, ranges, dout, delta, dq, dk, dv, workspace, s);
 }
 
 size_t lact_attention_step_workspace_bytes(const lact_attention_step_desc_t* d) {

@@ -716,7 +716,9 @@ struct AttentionFn : torch::autograd::Function<AttentionFn> {
     D.slopes = fptr(slopes);
     const auto c = at::MemoryFormat::Contiguous;
     const Tensor dq = at::empty_like(q, q.options(), c), dk = at::empty_like(k, k.options(), c), dv = at::empty_like(v, v.options(), c);
-    check(lact_masked_attention_backward(&D, ptr(q), ptr(k), ptr(v), ptr(out), fptr(lse), ptr(ranges), ptr(g), fptr(delta), ptr(dq), ptr(dk), ptr(dv), stream()));
+    const int64_t bytes = (int64_t)lact_masked_attention_workspace_bytes(&D);
+    const Tensor ws = bytes ? at::empty({bytes}, q.options().dtype(at::kByte)) : Tensor();
+    check(lact_masked_attention_backward(&D, ptr(q), ptr(k), ptr(v), ptr(out), fptr(lse), ptr(ranges), ptr(g), fptr(delta), ptr(dq), ptr(dk), ptr(dv), ptr(ws), stream()));
     return finish({dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, twice);
   }
 };

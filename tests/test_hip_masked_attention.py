@@ -89,6 +89,13 @@ def test_documents_and_prefixes(documents, prefixes, window, d, dtype):
 
 
 @BOTH
+@pytest.mark.parametrize("d", [64, 128])
+def test_keys_gradients_in_splits(d, dtype):
+    """Few key heads: the queries are walked in parts, which end inside heads and tiles."""
+    check(1, 700, 8, 1, d, dtype, 300, 30.0, True, documents=[[3, 250, 690]], prefixes=[[50, 100]])
+
+
+@BOTH
 def test_documents_of_a_batch_differ(dtype):
     check(3, 150, 2, 1, 64, dtype, None, documents=[[0, 150, 150], [20, 30, 100], [0, 75, 150]], prefixes=[[10, 0], [10, 3], [0, 75]])
 

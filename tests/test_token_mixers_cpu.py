@@ -47,7 +47,16 @@ def test_attention_pointers():
     d = attention_desc(n_documents=1)
     assert L.lact_attention_ranges_bytes(ctypes.byref(d)) == 2 * 100 * 16 and L.lact_attention_ranges_bytes(ctypes.byref(attention_desc())) == 0
     assert L.lact_masked_attention_forward(ctypes.byref(d), *[P] * 5, None, None) < 0 and "ranges" in lib_error()
-    assert L.lact_masked_attention_backward(ctypes.byref(attention_desc(do_ld=8)), *[P] * 11, None) < 0 and "dout" in lib_error()
+    assert L.lact_masked_attention_backward(ctypes.byref(attention_desc(do_ld=8)), *[P] * 12, None) < 0 and "dout" in lib_error()
+
+
+def test_attention_workspace():
+    """Few blocks of 128 keys: the sums of dk and dv over the queries come in splits of their own."""
+    L = _lib.lib()
+    size = lambda **kw: L.lact_masked_attention_workspace_bytes(ctypes.byref(attention_desc(**kw)))  # noqa: E731
+    assert size() == 0                                                     # four tiles of queries for one split
+    assert size(L=1024, window=1024) == 2 * 8 * 2 * 1024 * 2 * 64 * 4      # 2 heads x 16 tiles
+    assert size(L=1 << 20, window=1 << 20) == 0 and size(D=32) == 0
 
 
 def step_desc(**kw):
