@@ -149,7 +149,7 @@ __global__ __launch_bounds__((64 * AttnStepShape<T, D>::NW), 1) void k_attn_step
     const T* V = p.v + b * p.bsv + hk * p.hsv;
     Frag qf[D / 16];
     mask_own_rows<T, D>(qf, p.q + b * p.bsq, D, h, p.H);
-    Scores<T> sc;
+    Scores<T, true> sc;
     sc.init(p.scale, p.cap, p.slopes, h);
     const float c = sc.unit();
     f32x16 o[D / 32];

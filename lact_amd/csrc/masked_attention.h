@@ -113,6 +113,8 @@ __device__ __forceinline__ f32x16 mma32(const f32x8& a, const f32x8& b, f32x16 c
   return c;
 }
 
+constexpr int MASK_WAVES = 4;     // of a block; two blocks of the forward and of dq to a compute unit
+
 template <typename T, int D>
 struct MaskTile {       // 64 x D, the 16-byte granule g of row r at slot g ^ key(r): 16 rows of one granule fall into different banks
   static constexpr int ROWB = D * (int)sizeof(T), G = ROWB / 16, BYTES = 64 * ROWB;
@@ -122,8 +124,9 @@ struct MaskTile {       // 64 x D, the 16-byte granule g of row r at slot g ^ ke
   }
 };
 
-template <typename T, int D, int NW>
+template <typename T, int D>
 struct MaskCopy {
+  static constexpr int NW = MASK_WAVES;
   using S = MaskTile<T, D>;
   static constexpr int NC = S::G / NW;      // copies of a wave and tile
   static_assert(S::G % NW == 0, "copies must split evenly over the waves");
@@ -229,8 +232,9 @@ __device__ __forceinline__ bool unfinite(const f32x8& f) {
 // What lies in a tile and is not finite must not meet the zero weight of a row that does not see it.  The wave that copied 1 KB of a tile looks it over
 // once it is there, clears rows that hold such a value and writes down which; every wave gives the rows of its own that see one of them NaN.
 // (Selecting in the products' operands instead, where a tile is masked, cost a tenth of the forward: a branch at every operand, or registers for two loops.)
-template <typename T, int D, int NW>
+template <typename T, int D>
 struct Spoilt {
+  static constexpr int NW = MASK_WAVES;
   using S = MaskTile<T, D>;
   static constexpr int BYTES = 64;
   uint32_t* words;        // rows [0, 32) and [32, 64) of every ring slot; behind them whether there ever were any
@@ -277,31 +281,34 @@ __device__ __forceinline__ float tanh_f32(float x) {
 }
 
 // Scores as they come out of the product -> what 2^ is taken of, times `unit` (see below)
-template <typename T>
+template <typename T, bool BENT>      // BENT: with a cap or a distance
 struct Scores {
   float c;          // log2(e) / sqrt(D) without a cap: the scores then keep it out until they meet the maximum
   float k1, k2;     // with a cap: 2 log2(e) scale / cap, cap log2(e)
   float slope;      // times log2(e)
   bool cap, bias;
+  bool bounded;     // 2^s and its sums stay in range whatever the scores are: |s| <= k2 (a row sees itself, where the distance takes nothing off)
   __device__ __forceinline__ void init(float scale, float cap_, const float* slopes, int h) {
-    cap = cap_ > 0.f; bias = slopes != nullptr;
+    cap = BENT && cap_ > 0.f; bias = BENT && slopes != nullptr;
     k1 = sizeof(T) == 2 ? 2.f * ATTN_LOG2E * scale / cap_ : scale / cap_;
     k2 = cap_ * ATTN_LOG2E;
     slope = bias ? slopes[h] * ATTN_LOG2E : 0.f;
+    bounded = cap && k2 <= 90.f && slope >= 0.f;
     c = scale * ATTN_LOG2E;
   }
   // what is left to multiply by behind apply()
-  __device__ __forceinline__ float unit() const { return cap || bias ? 1.f : c; }
+  __device__ __forceinline__ float unit() const { return BENT ? 1.f : c; }
   __device__ __forceinline__ float bent(float s) const {      // tanh of the score over the cap
     if constexpr (sizeof(T) == 2) return fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * k1)), -2.f, 1.f);   // to 2^-23
     else return tanh_f32(s * k1);
   }
   // `first`: the place of the lane's element 0 minus the place of its own row
   __device__ __forceinline__ void apply(f32x16& s, int first) const {
+    if constexpr (!BENT) return;
     if (cap) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[j] = bent(s[j]) * k2;
-    } else if (bias) {
+    } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[j] *= c;
     }
@@ -309,6 +316,7 @@ struct Scores {
   }
   // the same, and the gradients dp (of what the softmax weighs) times the derivative of the cap
   __device__ __forceinline__ void apply(f32x16& s, f32x16& dp, int first) const {
+    if constexpr (!BENT) return;
     if (cap) {
       // (in steps of four: one loop over both vectors leaves them in memory)
 #pragma unroll
@@ -321,7 +329,7 @@ struct Scores {
 #pragma unroll
         for (int j = 0; j < 4; ++j) dp[4 * g + j] *= fmaf(-t[j], t[j], 1.f);
       }
-    } else if (bias) {
+    } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[j] *= c;
     }
@@ -335,13 +343,15 @@ struct Scores {
   }
 };
 
-template <typename T, int D> constexpr int mask_ring() { return sizeof(T) == 2 ? 3 : 2; }      // 64-row tiles of both operands in LDS
-template <typename T, int D, int NW>
+// 64-row tiles of both operands in LDS
+template <typename T, int D> constexpr int mask_ring(bool keys) { return sizeof(T) == 4 || (D == 128 && !keys) ? 2 : 3; }
+template <typename T, int D>
 constexpr int mask_lds_bytes(bool stats) {
-  constexpr int R = mask_ring<T, D>();
-  const int ring = R * 2 * MaskTile<T, D>::BYTES + (stats ? R * 512 : 0) + Spoilt<T, D, NW>::BYTES;
+  constexpr int NW = MASK_WAVES;
+  const int R = mask_ring<T, D>(stats);
+  const int ring = R * 2 * MaskTile<T, D>::BYTES + (stats ? R * 512 : 0) + Spoilt<T, D>::BYTES;
   // what the rows are stored through, for splits in fp32
-  return cmax(ring, NW * 32 * cmax((D + 16 / (int)sizeof(T)) * (int)sizeof(T), stats && NW == 4 ? (D + 4) * 4 : 0));
+  return cmax(ring, NW * 32 * cmax((D + 16 / (int)sizeof(T)) * (int)sizeof(T), stats ? (D + 4) * 4 : 0));
 }
 
 // Walks the tiles [0, n): issue(t) starts the copies of tile t, COPIES of a wave, RING - 1 tiles ahead; look(t) sees the wave's own when they are there;
@@ -387,20 +397,24 @@ __device__ __forceinline__ void mask_store_rows(char* lds, const f32x16 (&acc)[D
   wave_lds_fence();
 }
 
-// Intervals of the rows [row0, row0 + 32 N) that a wave sees as one: union (x, y), and for its own 32 the largest lower and least upper end.
-__device__ __forceinline__ int wave_min(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-  return __builtin_amdgcn_readfirstlane(v);
-}
-__device__ __forceinline__ int wave_max(int v) { return -wave_min(-v); }
-
-struct WaveReach {
-  int lo, hi;          // union over the wave's rows
-  int full_lo, full_hi;  // what every one of them sees
-  __device__ __forceinline__ void init(int2 own) {
-    lo = wave_min(own.x); hi = wave_max(own.y);
-    full_lo = wave_max(own.x); full_hi = wave_min(own.y);
+// What rows see, over a wave.  Neither end of the intervals falls from one row to the next, but rows may see nothing, which have {INT_MAX, 0}.
+struct Reach {
+  int lo, hi;            // of all of them: no tile outside
+  int full_lo, full_hi;  // of every one of them: no mask inside
+  // `rows`: one row a lane, in order, in the first COUNT lanes
+  template <int COUNT>
+  __device__ __forceinline__ void init(int2 rows) {
+    const uint64_t all = ~0ull >> (64 - COUNT), some = __ballot(rows.x < rows.y) & all;
+    lo = full_lo = 0x7fffffff;
+    hi = full_hi = 0;
+    if (some) {
+      lo = __builtin_amdgcn_readlane(rows.x, __builtin_ctzll(some));
+      hi = __builtin_amdgcn_readlane(rows.y, 63 - __builtin_clzll(some));
+    }
+    if (some == all) {
+      full_lo = __builtin_amdgcn_readlane(rows.x, COUNT - 1);
+      full_hi = __builtin_amdgcn_readlane(rows.y, 0);
+    }
   }
   __device__ __forceinline__ bool sees(int a, int n) const { return a < hi && a + n > lo; }
   __device__ __forceinline__ bool masked(int a, int n) const { return a < full_lo || a + n > full_hi; }
@@ -436,13 +450,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_fwd(const MaskedAttnParams<T> p) {
+template <typename T, int D, bool BENT>
+__global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_fwd(const MaskedAttnParams<T> p) {
+  constexpr int NW = MASK_WAVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using S = MaskTile<T, D>;
-  using Copy = MaskCopy<T, D, NW>;
+  using Copy = MaskCopy<T, D>;
   using Frag = typename AttnType<T>::Frag;
-  constexpr int STAGE = 2 * S::BYTES, RING = mask_ring<T, D>();
+  constexpr int STAGE = 2 * S::BYTES, RING = mask_ring<T, D>(false);
   prefetch_args<sizeof(p)>();
   int bx, z, b, h, hk;
   p.locate(bx, z);
@@ -454,16 +469,16 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_masked_attn
   Frag qf[D / 16];
   mask_own_rows<T, D>(qf, p.q + b * p.bsq + h * D, p.ldq, row, L);
   const int2 own = p.row_range(b, row);
-  WaveReach reach;
-  reach.init(own);
   int first = 0x7fffffff, last = 0;
 #pragma unroll
   for (int i = 0; i < NW / 2; ++i) {
-    const int2 r = p.row_range(b, blk0 + i * 64 + lane);
-    first = min(first, r.x); last = max(last, r.y);
+    Reach part;
+    part.init<64>(p.row_range(b, blk0 + i * 64 + lane));
+    first = min(first, part.lo); last = max(last, part.hi);
   }
-  first = wave_min(first); last = wave_max(last);
-  Scores<T> sc;
+  Reach reach;
+  reach.init<32>(own);
+  Scores<T, BENT> sc;
   sc.init(p.scale, p.cap, p.slopes, h);
   MaskFrag<T, D> fr;
   fr.init();
@@ -473,14 +488,14 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_masked_attn
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
   const float c = sc.unit();
-  float mc = -1e30f, sum = 0.f;        // running row maximum (of what 2^ is taken of) and this lane's share of the row sum
+  float mc = sc.bounded ? 0.f : -1e30f, sum = 0.f;        // running row maximum (of what 2^ is taken of) and this lane's share of the row sum
   first = min(first, L) / 64 * 64;
   const int tiles = last > first ? (last - first + 63) / 64 : 0;
   Copy ck, cv;
   ck.init(wave, p.k + b * p.bsk + hk * D, p.ldk, first, tiles, L);
   cv.init(wave, p.v + b * p.bsv + hk * D, p.ldv, first, tiles, L);
   const uint32_t lds0 = lds_addr(smem);
-  Spoilt<T, D, NW> spoilt;
+  Spoilt<T, D> spoilt;
   spoilt.init(smem + RING * STAGE);
   mask_arrived(qf);
   mask_walk<2 * Copy::NC, RING>(tiles, spoilt,
@@ -520,22 +535,25 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_masked_attn
         for (int i = 0; i < 2; ++i)
           if (Seen(own.x - at - 32 * i, own.y - at - 32 * i).any_of((uint32_t)(bad >> (32 * i)))) sum = __builtin_nanf("");
       }
-      float mx = s[0][0];
-      mx = max3(mx, s[1][0], s[1][1]);
+      // (a cap that bounds them saves the row maximum)
+      if (!sc.bounded) {
+        float mx = s[0][0];
+        mx = max3(mx, s[1][0], s[1][1]);
 #pragma unroll
-      for (int j = 1; j < 16; ++j) mx = max3(mx, s[0][j], s[1][j]);
-      mx *= c;
-      // The maximum only has to keep exp2 in range: it follows the row when it is exceeded by more than 2^8 (its own row only: what a row
-      // gives does not depend on the others).
-      if (__any(mx > mc + 8.f)) {
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float nm = mx > mc + 8.f ? mx : mc, f = __builtin_amdgcn_exp2f(mc - nm);
-        mc = nm;
-        sum *= f;
+        for (int j = 1; j < 16; ++j) mx = max3(mx, s[0][j], s[1][j]);
+        mx *= c;
+        // The maximum only has to keep exp2 in range: it follows the row when it is exceeded by more than 2^8 (its own row only: what a row
+        // gives does not depend on the others).
+        if (__any(mx > mc + 8.f)) {
+          mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+          const float nm = mx > mc + 8.f ? mx : mc, f = __builtin_amdgcn_exp2f(mc - nm);
+          mc = nm;
+          sum *= f;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i)
+          for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-          for (int j = 0; j < 16; ++j) o[i][j] *= f;
+            for (int j = 0; j < 16; ++j) o[i][j] *= f;
+        }
       }
       float part[2] = {0.f, 0.f};
 #pragma unroll
@@ -561,13 +579,14 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_masked_attn
 }
 
 // dq = scale * sum_keys ds k with ds = p (dp - delta) f', and delta itself.
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_dq(const MaskedAttnParams<T> p) {
+template <typename T, int D, bool BENT>
+__global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_dq(const MaskedAttnParams<T> p) {
+  constexpr int NW = MASK_WAVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using S = MaskTile<T, D>;
-  using Copy = MaskCopy<T, D, NW>;
+  using Copy = MaskCopy<T, D>;
   using Frag = typename AttnType<T>::Frag;
-  constexpr int STAGE = 2 * S::BYTES, RING = mask_ring<T, D>();
+  constexpr int STAGE = 2 * S::BYTES, RING = mask_ring<T, D>(false);
   prefetch_args<sizeof(p)>();
   int bx, z, b, h, hk;
   p.locate(bx, z);
@@ -593,16 +612,16 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_masked_attn
   mask_own_rows<T, D>(qf, p.q + b * p.bsq + h * D, p.ldq, row, L);
   float lse = p.lse[stat + min(row, L - 1)];
   const int2 own = p.row_range(b, row);
-  WaveReach reach;
-  reach.init(own);
   int first = 0x7fffffff, last = 0;
 #pragma unroll
   for (int i = 0; i < NW / 2; ++i) {
-    const int2 r = p.row_range(b, blk0 + i * 64 + lane);
-    first = min(first, r.x); last = max(last, r.y);
+    Reach part;
+    part.init<64>(p.row_range(b, blk0 + i * 64 + lane));
+    first = min(first, part.lo); last = max(last, part.hi);
   }
-  first = wave_min(first); last = wave_max(last);
-  Scores<T> sc;
+  Reach reach;
+  reach.init<32>(own);
+  Scores<T, BENT> sc;
   sc.init(p.scale, p.cap, p.slopes, h);
   MaskFrag<T, D> fr;
   fr.init();
@@ -621,7 +640,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_masked_attn
   mask_arrived(qf);
   mask_arrived(gf);
   asm volatile("" : "+v"(lse), "+v"(delta));
-  Spoilt<T, D, NW> spoilt;
+  Spoilt<T, D> spoilt;
   spoilt.init(smem + RING * STAGE);
   float poison = 0.f;
   mask_walk<2 * Copy::NC, RING>(tiles, spoilt,
@@ -673,13 +692,14 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_masked_attn
 
 // dv = sum_queries p dout, dk = scale * sum_queries ds q, over the queries of all heads that share the key head: a wave owns 32 keys and
 // walks the queries that see them, head after head.  With few keys (blocks) the walk is cut into gridDim.y splits, whose sums k_attn_sum adds.
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dkv(const MaskedAttnParams<T> p) {
+template <typename T, int D, bool BENT>
+__global__ __launch_bounds__(64 * MASK_WAVES, D == 64 && sizeof(T) == 2 ? 2 : 1) void k_masked_attn_dkv(const MaskedAttnParams<T> p) {
+  constexpr int NW = MASK_WAVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using S = MaskTile<T, D>;
-  using Copy = MaskCopy<T, D, NW>;
+  using Copy = MaskCopy<T, D>;
   using Frag = typename AttnType<T>::Frag;
-  constexpr int STAGE = 2 * S::BYTES, RING = mask_ring<T, D>();
+  constexpr int STAGE = 2 * S::BYTES, RING = mask_ring<T, D>(true);
   prefetch_args<sizeof(p)>();
   int bx, z;
   p.locate(bx, z);
@@ -690,15 +710,15 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dkv(co
   mask_own_rows<T, D>(kf, p.k + b * p.bsk + hk * D, p.ldk, row, L);
   mask_own_rows<T, D>(vf, p.v + b * p.bsv + hk * D, p.ldv, row, L);
   const int2 own = p.col_range(b, row);
-  WaveReach reach;
-  reach.init(own);
   int first = 0x7fffffff, last = 0;
 #pragma unroll
   for (int i = 0; i < NW / 2; ++i) {
-    const int2 r = p.col_range(b, blk0 + i * 64 + lane);
-    first = min(first, r.x); last = max(last, r.y);
+    Reach part;
+    part.init<64>(p.col_range(b, blk0 + i * 64 + lane));
+    first = min(first, part.lo); last = max(last, part.hi);
   }
-  first = wave_min(first); last = wave_max(last);
+  Reach reach;
+  reach.init<32>(own);
   MaskFrag<T, D> fr;
   fr.init();
   f32x16 ok[D / 32], ov[D / 32];
@@ -719,12 +739,12 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dkv(co
   const float* st_src = (wave & 1 ? p.delta : p.lse) + (size_t)(b * p.H + h0) * L;
   int ih = tiles ? from / tiles : 0, it = from - ih * tiles, bh = ih, bt = it;      // head and tile of the next copies, and of the next use
   float poison = 0.f;
-  Scores<T> sc;
+  Scores<T, BENT> sc;
   sc.init(p.scale, p.cap, p.slopes, h0);
   const float c = sc.unit();
   mask_arrived(kf);
   mask_arrived(vf);
-  Spoilt<T, D, NW> spoilt;
+  Spoilt<T, D> spoilt;
   spoilt.init(smem + RING * (STAGE + 512));
   mask_walk<2 * Copy::NC + 1, RING>(all, spoilt,
     [&](int t) LACT_INLINE_LAMBDA {
@@ -798,7 +818,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 2 : 1) void k_masked_attn_dkv(co
   poison += __shfl_xor(poison, 32, 64);
   __syncthreads();
   const size_t o = ((size_t)b * L * p.HK + hk) * D, ld = (size_t)p.HK * D;
-  if (NW == 4 && splits > 1) {
+  if (splits > 1) {
     float* stage = reinterpret_cast<float*>(smem) + wave * 32 * (D + 4);
     const size_t all_keys = (size_t)p.B * L * ld, at = blockIdx.y * all_keys + o;
     mask_store_rows<float, D>(reinterpret_cast<char*>(stage), ok, p.scale + poison, p.part + at, ld, row0, L);

@@ -80,41 +80,33 @@ size_t attention_workspace(const lact_attention_desc_t* d) {
 }
 
 // WHICH: 0 forward, 1 dq, 2 dk and dv (in `splits`)
-template <int WHICH, typename T, int D, int NW>
+template <int WHICH, typename T, int D, bool BENT>
 void launch_attention(int splits, MaskedAttnParams<T> p, hipStream_t s) {
   const int heads = p.B * (WHICH == 2 ? p.HK : p.H);
   p.by_heads = make_udiv(heads);
-  const dim3 grid(ceil_div(p.L, 32 * NW) * heads, splits), block(64 * NW);
-  constexpr int SM = mask_lds_bytes<T, D, NW>(WHICH == 2);
+  const dim3 grid(ceil_div(p.L, 32 * MASK_WAVES) * heads, splits), block(64 * MASK_WAVES);
+  constexpr int SM = mask_lds_bytes<T, D>(WHICH == 2);
   const double w = p.window, f = 2.0 * ((double)p.L * w - w * (w - 1) / 2) * D * p.B * p.H;      // without documents
   if constexpr (WHICH == 0) {
-    LACT_BIG_LDS((k_masked_attn_fwd<T, D, NW>), SM);
-    LACT_LAUNCH_SMEM("k_masked_attn_fwd", "masked_attn", 2 * f, (k_masked_attn_fwd<T, D, NW>), grid, block, SM, s, p);
+    LACT_BIG_LDS((k_masked_attn_fwd<T, D, BENT>), SM);
+    LACT_LAUNCH_SMEM("k_masked_attn_fwd", "masked_attn", 2 * f, (k_masked_attn_fwd<T, D, BENT>), grid, block, SM, s, p);
   } else if constexpr (WHICH == 1) {
-    LACT_BIG_LDS((k_masked_attn_dq<T, D, NW>), SM);
-    LACT_LAUNCH_SMEM("k_masked_attn_dq", "masked_attn_bwd", 3 * f, (k_masked_attn_dq<T, D, NW>), grid, block, SM, s, p);
+    LACT_BIG_LDS((k_masked_attn_dq<T, D, BENT>), SM);
+    LACT_LAUNCH_SMEM("k_masked_attn_dq", "masked_attn_bwd", 3 * f, (k_masked_attn_dq<T, D, BENT>), grid, block, SM, s, p);
   } else {
-    LACT_BIG_LDS((k_masked_attn_dkv<T, D, NW>), SM);
-    LACT_LAUNCH_SMEM("k_masked_attn_dkv", "masked_attn_bwd", 4 * f, (k_masked_attn_dkv<T, D, NW>), grid, block, SM, s, p);
+    LACT_BIG_LDS((k_masked_attn_dkv<T, D, BENT>), SM);
+    LACT_LAUNCH_SMEM("k_masked_attn_dkv", "masked_attn_bwd", 4 * f, (k_masked_attn_dkv<T, D, BENT>), grid, block, SM, s, p);
     if (splits > 1) {
       const long long n = (long long)p.B * p.L * p.HK * D;
       LACT_LAUNCH("k_attn_sum", "masked_attn_bwd", 0.0, (k_attn_sum<T>), dim3((unsigned)((n / 4 + 255) / 256), 2), dim3(256), s, n, splits, p.part, p.dk, p.dv);
     }
   }
 }
-// Waves per block: 8 (256 rows) once that gives every compute unit a block, else 4.  dk and dv of heads of 128 take more registers than two waves of
-// a SIMD have: 4.
-template <int WHICH, typename T, int D>
-void launch_attention(int splits, const MaskedAttnParams<T>& p, hipStream_t s) {
-  if constexpr (sizeof(T) == 2 && (WHICH < 2 || D == 64)) {
-    if ((long long)ceil_div(p.L, 256) * p.B * (WHICH == 2 ? p.HK : p.H) >= COMPUTE_UNITS) return launch_attention<WHICH, T, D, 8>(1, p, s);
-  }
-  launch_attention<WHICH, T, D, 4>(splits, p, s);
-}
 template <int WHICH, typename T>
 void launch_attention(int splits, int D, const MaskedAttnParams<T>& p, hipStream_t s) {
-  if (D == 128) launch_attention<WHICH, T, 128>(splits, p, s);
-  else launch_attention<WHICH, T, 64>(splits, p, s);
+  const bool bent = p.cap > 0.f || p.slopes;
+  if (D == 128) bent ? launch_attention<WHICH, T, 128, true>(splits, p, s) : launch_attention<WHICH, T, 128, false>(splits, p, s);
+  else bent ? launch_attention<WHICH, T, 64, true>(splits, p, s) : launch_attention<WHICH, T, 64, false>(splits, p, s);
 }
 
 template <typename T>
