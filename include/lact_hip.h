@@ -296,7 +296,7 @@ int lact_attention_step(const lact_attention_step_desc_t* desc, const void* q, c
 /* Linear attention with a decay: S_t = e^(g_t) S_(t-1) + k_t v_t^T, out_t = scale S_t^T q_t; dk, dv = 64 or 128.
  * q, k: [b, l, h, dk], v, dout: [b, l, h, dv] as above; g: fp32 log decays, contiguous [b, l, h] (decay_per_token) or [h]; -infinity (anything
  * below -200) forgets the state.  state: [b, h, dk, dv] fp32 in front of the first token, null: zero; last (nullable): behind the last one.
- * states: states_bytes bytes kept from the forward for the backward (may be 0); scratch: scratch_bytes bytes, the backward's own.
+ * states: states_bytes bytes kept from the forward for the backward; scratch: scratch_bytes bytes, the backward's own.
  * Backward: dlast nullable; dg (nullable, shape of g) and dstate (nullable) fp32; with dlast and dg it reads `last`. */
 typedef struct lact_linear_desc {
   int32_t act_dtype, b, l, h, dk, dv, decay_per_token;

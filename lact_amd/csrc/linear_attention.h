@@ -11,9 +11,9 @@
 //
 // Only differences of later and earlier sums are exponentiated, so no decay overflows; the sums are formed in fp64 and kept in two floats.
 // The gradients are the same recurrence with other operands: of q with (dout, v, k) and the transposed state; of k with (v, dout, q) and of v with (k, q, dout)
-// backwards in time from the gradient of the last state.  One kernel, k_lin_walk, is all four.
+// backwards in time from the gradient of the last state.  One function, lin_walk, is all four.
 //
-// A block walks the chunks of a segment of one head; a wave owns a quarter of the state's columns, in accumulators, from where they are
+// A block walks the chunks of a segment of one head (lin_walk); a wave owns a quarter of the state's columns, in accumulators, from where they are
 // packed as the next product's operand where they lie (an accumulator's rows are k slots there; which row of the state an accumulator row
 // holds is chosen so that the queries' operand is 8 neighbours).  Segments start from states that k_lin_segments and k_lin_scan form first, where heads
 // and batch alone do not fill the chip.
@@ -21,9 +21,8 @@
 // The state is held, and added to, in fp32: what is added is a product of bf16 inputs with a weight, which goes into the matrix product
 // as three bf16 parts (24 bits).  Probabilities and, where only rounded outputs depend on it, the state as an operand are rounded to bf16.
 //
-// A gradient of the decays adds what crosses a token: dg_s = sum_(i >= s > j) M_ij + ..., M_ij = e^(G_i - G_j) (q_i . k_j)(dout_i . v_j) scale.
-// Rows and columns of M are summed from the same products (they cancel outside the crossing), the state's shares likewise, and the sum over a
-// segment starts from <dS, S> at its end.
+// A gradient of the decays adds what crosses a token (k_lin_decay_grad): pairs M_ij = e^(G_i - G_j) (q_i . k_j)(dout_i . v_j) scale of a source in front and an
+// output behind it, and the states' shares.
 #pragma once
 #include "masked_attention.h"
 
@@ -52,15 +51,15 @@ struct LinRows {          // [B, L, H, D]
 template <typename T>
 struct LinParams {
   int B, L, H, segments, seg_chunks;     // chunks of a segment
-  LinRows<T> x, y, z, w;                 // out_i = sum_j (x_i . y_j) z_j + x_i S, S += y_j z_j^T; w: see k_lin_walk
-  LinDecay decay;
+  LinRows<T> x, y, z, w;                 // out_i = sum_j (x_i . y_j) z_j + x_i S, S += y_j z_j^T; w: see lin_walk
+  const float4* weights;                 // [B * H][chunks * 64], see k_lin_weights
   float pair_scale, state_scale, source_scale;
   T* out;                                // [B, L, H, DZ]
   const float* states;                   // [segments][B * H][DX * DZ] (or transposed): where each segment starts, null: from zero
   const float* state0;                   // [B * H][..]: the same for a single segment
   int transposed;                        // the states in memory are [DZ][DX]
   float* last;                           // [B * H][..]: state behind the walk's last chunk, nullable
-  float* dots;                           // [B, L, H] fp32, for the gradient of the decays
+  float* dots;                           // [B * H][L] fp32, forwards two of them, for the gradient of the decays
   UDiv by_heads;                         // H
 };
 
@@ -137,43 +136,39 @@ template <typename T, int D> struct LinFrag {
   }
 };
 
-// What the tokens of a chunk weigh, in LDS of a wave's own: sums of log2 decays in two floats, weight of the state in an output, weight of a token
-// in the state.
-struct LinWeights {
-  float4* w;
-  float whole;       // decay of the state over the chunk
-  template <bool REV>
-  __device__ __forceinline__ void form(float4* lds, float g, bool valid, float state_scale, float source_scale) {
-    w = lds;
-    double s = (double)g * 1.4426950408889634;
-    const int l = threadIdx.x & 63;
+// What the tokens of a chunk weigh, for every walk over it: the sum of log2 decays from the chunk's start in two floats, 2 to it (the weight of the
+// state in front in the token's output, forwards) and 2 to the rest of the chunk (the weight of the token in the state behind); both weights 0 past the
+// sequence's end.  One wave per chunk and head.
+__global__ __launch_bounds__(256) void k_lin_weights(int B, int L, int H, LinDecay decay, float4* weights) {
+  const int chunks = (L + 63) / 64, lane = threadIdx.x & 63;
+  const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (id >= (long long)B * H * chunks) return;
+  const int bh = (int)(id / chunks), t = (int)(id - (long long)bh * chunks) * 64 + lane, b = bh / H, h = bh - b * H;
+  double s = (double)decay.at(b, t, h, L, H) * 1.4426950408889634;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double u = __shfl_up(s, o, 64);
-      if (l >= o) s += u;
-    }
-    const double end = __shfl(s, 63, 64);
-    const float hi = (float)s, lo = (float)(s - (double)hi);
-    const float to = __builtin_amdgcn_exp2f((float)s), from = __builtin_amdgcn_exp2f((float)(end - s));
-    whole = __builtin_amdgcn_exp2f((float)end);
-    w[l] = make_float4(hi, lo, (REV ? from : to) * state_scale, valid ? (REV ? to : from) * source_scale : 0.f);
-    wave_lds_fence();
+  for (int o = 1; o < 64; o <<= 1) {
+    const double u = __shfl_up(s, o, 64);
+    if (lane >= o) s += u;
   }
-  // 2^(later - earlier)
-  __device__ static __forceinline__ float between(const float4& later, const float4& earlier) {
-    return __builtin_amdgcn_exp2f((later.x - earlier.x) + (later.y - earlier.y));
-  }
-};
+  const double end = __shfl(s, 63, 64);
+  const float hi = (float)s, lo = (float)(s - (double)hi);
+  weights[id * 64 + lane] = make_float4(hi, lo, t < L ? __builtin_amdgcn_exp2f(hi) : 0.f, t < L ? __builtin_amdgcn_exp2f((float)(end - s)) : 0.f);
+}
+
+// 2^(later - earlier) of the sums of two tokens
+__device__ __forceinline__ float lin_between(const float4& later, const float4& earlier) {
+  return __builtin_amdgcn_exp2f((later.x - earlier.x) + (later.y - earlier.y));
+}
 
 template <typename T, int DX, int DZ, bool GATE>
 struct LinShape {
   static constexpr int X = MaskTile<T, DX>::BYTES, Z = MaskTile<T, DZ>::BYTES;
-  static constexpr int STAGE = 2 * X + (GATE ? 2 : 1) * Z;                // x, y, z (, w)
-  static constexpr int BUFFERS = sizeof(T) == 2 ? 2 : 1;
+  static constexpr int STAGE = 2 * X + (GATE ? 2 : 1) * Z + 1024;         // x, y, z (, w), weights
   static constexpr int PAIRS = MaskTile<T, 64>::BYTES;
-  static constexpr int WEIGHTS = 4 * 64 * 16;
   static constexpr int SUMS = GATE ? 4 * 64 * 4 * 2 : 0;                  // per wave: what its columns, and its pairs, add to the dots
-  static constexpr int LDS = BUFFERS * STAGE + PAIRS + WEIGHTS + SUMS;
+  // two chunks where two blocks of them fit a compute unit
+  static constexpr int BUFFERS = 2 * STAGE + PAIRS + SUMS <= 80 * 1024 ? 2 : 1;
+  static constexpr int LDS = BUFFERS * STAGE + PAIRS + SUMS;
   static_assert(LDS <= 160 * 1024, "LDS");
 };
 
@@ -217,22 +212,26 @@ struct LinState {        // columns [wave * DZ / 4, + DZ / 4): accumulator a, ro
       }
   }
   // decays by `whole` and adds y^T (weight z); zf: the wave's columns of z
-  template <typename Frag>
-  __device__ __forceinline__ void update(const char* y, const Frag (&zf)[2][NT], const LinWeights& lw) {
+  template <bool REV, typename Frag>
+  __device__ __forceinline__ void update(const char* y, const Frag (&zf)[2][NT], const float4* w, float source_scale) {
     constexpr int PARTS = lin_parts<T>();
+    const float whole = __builtin_amdgcn_exp2f(w[63].x + w[63].y);
 #pragma unroll
     for (int a = 0; a < AT; ++a)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) s[a][n] *= lw.whole;
+      for (int n = 0; n < NT; ++n) s[a][n] *= whole;
     const int c = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
       Frag zw[NT][PARTS];
+      float weight[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) weight[j] = (REV ? w[32 * v + 8 * c + j].z : w[32 * v + 8 * c + j].w) * source_scale;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (float)zf[v][n][j] * lw.w[32 * v + 8 * c + j].w;
+        for (int j = 0; j < 8; ++j) x[j] = (float)zf[v][n][j] * weight[j];
         lin_split<T, PARTS>(x, zw[n]);
       }
 #pragma unroll
@@ -260,11 +259,10 @@ __device__ __forceinline__ void lin_copy(const LinRows<T>& m, int b, int h, int 
 }
 
 // The walk over a segment.  REV: from its end to its beginning, sources are the later tokens.
-// GATE: also dots[t], for the gradient of the decays.  Forwards (x, y, z, w = dout, v, k, q): row sum minus column sum of M at t, and the state's share in
-// q_t . dq_t; backwards (x, y, z, w = k, q, dout, v): the state's share in v_t . dv_t.
+// GATE: also dots[t], for the gradient of the decays.  Forwards (x, y, z, w = dout, v, k, q): the state's share in q_t . dq_t, and row sum minus column sum
+// of M at t; backwards (x, y, z, w = k, q, dout, v): the state's share in v_t . dv_t.
 template <typename T, int DX, int DZ, bool REV, bool GATE>
-__global__ __launch_bounds__(256, 1) void k_lin_walk(const LinParams<T> p) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+__device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* smem) {
   using Sh = LinShape<T, DX, DZ, GATE>;
   using St = LinState<T, DX, DZ>;
   using Frag = typename AttnType<T>::Frag;
@@ -272,13 +270,12 @@ __global__ __launch_bounds__(256, 1) void k_lin_walk(const LinParams<T> p) {
   using FZ = LinFrag<T, DZ>;
   using FP = LinFrag<T, 64>;
   constexpr int NT = St::NT, UX = DX / 32, UZ = DZ / 32, SP = GATE ? lin_parts<T>() : 1;
-  prefetch_args<sizeof(p)>();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane >> 4, li = lane & 15;
-  const int seg = blockIdx.x % p.segments, bh = blockIdx.x / p.segments, b = p.by_heads.div(bh), h = bh - b * p.H;
+  const int seg = item % p.segments, bh = item / p.segments, b = p.by_heads.div(bh), h = bh - b * p.H;
   const int L = p.L, chunks = (L + 63) / 64, first = seg * p.seg_chunks, n = min(p.seg_chunks, chunks - first);
   char* pairs = smem + Sh::BUFFERS * Sh::STAGE;
-  float4* weights = reinterpret_cast<float4*>(pairs + Sh::PAIRS) + wave * 64;
-  float* sums = reinterpret_cast<float*>(pairs + Sh::PAIRS + Sh::WEIGHTS);
+  float* sums = reinterpret_cast<float*>(pairs + Sh::PAIRS);
+  const float4* weights = uniform(p.weights + (size_t)bh * chunks * 64);
   const uint32_t lds0 = lds_addr(smem);
   auto token = [&](int i) { return (first + (REV ? n - 1 - i : i)) * 64; };
   auto issue = [&](int i) LACT_INLINE_LAMBDA {
@@ -288,18 +285,16 @@ __global__ __launch_bounds__(256, 1) void k_lin_walk(const LinParams<T> p) {
     lin_copy<T, DX>(p.y, b, h, t, L, to + Sh::X, wave);
     lin_copy<T, DZ>(p.z, b, h, t, L, to + 2 * Sh::X, wave);
     if (GATE) lin_copy<T, DZ>(p.w, b, h, t, L, to + 2 * Sh::X + Sh::Z, wave);
+    if (wave == 0) dma16<false>(weights + t, lane * 16, to + Sh::STAGE - 1024);
   };
   St st;
   const float* start = p.states ? p.states + ((size_t)seg * p.B * p.H + bh) * (DX * DZ) : p.state0 ? p.state0 + (size_t)bh * (DX * DZ) : nullptr;
   if (start) st.load(start, p.transposed, wave);
   else st.zero();
   const bool final = p.last && seg == (REV ? 0 : p.segments - 1);
-  float g_next = p.decay.at(b, token(0) + lane, h, L, p.H);
   issue(0);
   for (int i = 0; i < n; ++i) {
     const int t0 = token(i);
-    const float g = g_next;
-    if (i + 1 < n) g_next = p.decay.at(b, token(i + 1) + lane, h, L, p.H);
     if (Sh::BUFFERS == 1 || i == 0) wait_vmcnt<0>();
     __syncthreads();      // the chunk is there, and every wave is through with the one before
     if (Sh::BUFFERS == 2 && i + 1 < n) issue(i + 1);
@@ -307,11 +302,10 @@ __global__ __launch_bounds__(256, 1) void k_lin_walk(const LinParams<T> p) {
     const char* y = x + Sh::X;
     const char* z = y + Sh::X;
     const char* w = z + Sh::Z;
-    LinWeights lw;
-    lw.form<REV>(weights, g, t0 + lane < L, p.state_scale, p.source_scale);
+    const float4* lw = reinterpret_cast<const float4*>(x + Sh::STAGE - 1024);
     // Pairs of outputs [16 wave, +16) with their sources, [output][source] in LDS
     {
-      const float4 mine = lw.w[16 * wave + li];
+      const float4 mine = lw[16 * wave + li];
       float rowsum = 0.f;
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt) {
@@ -330,8 +324,8 @@ __global__ __launch_bounds__(256, 1) void k_lin_walk(const LinParams<T> p) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int j = 16 * jt + 4 * c + r, o = 16 * wave + li;
-            const float4 theirs = lw.w[j];
-            const float e = REV ? LinWeights::between(theirs, mine) : LinWeights::between(mine, theirs);
+            const float4 theirs = lw[j];
+            const float e = REV ? lin_between(theirs, mine) : lin_between(mine, theirs);
             const bool on = (REV ? j >= o : j <= o) && t0 + max(j, o) < L;
             v[r] = on ? acc[r] * e * p.pair_scale : 0.f;
             if constexpr (GATE && !REV) {
@@ -390,7 +384,7 @@ __global__ __launch_bounds__(256, 1) void k_lin_walk(const LinParams<T> p) {
     }
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
-      const float e = lw.w[16 * it + li].z;
+      const float e = (REV ? lw[16 * it + li].w : lw[16 * it + li].z) * p.state_scale;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) o[it][nt] *= e;
       if constexpr (GATE) {
@@ -415,13 +409,9 @@ __global__ __launch_bounds__(256, 1) void k_lin_walk(const LinParams<T> p) {
     __syncthreads();      // the pairs of all waves
     if constexpr (GATE)
       if (wave == 0 && t0 + lane < L) {
-        float d = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) d += sums[k * 64 + lane];
-        if constexpr (!REV)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) d -= sums[256 + k * 64 + lane];
-        p.dots[((size_t)b * L + t0 + lane) * p.H + h] = d;
+        float* to = p.dots + (size_t)bh * L + t0 + lane;
+        *to = (sums[lane] + sums[64 + lane]) + (sums[128 + lane] + sums[192 + lane]);
+        if constexpr (!REV) to[(size_t)p.B * p.H * L] = -((sums[256 + lane] + sums[320 + lane]) + (sums[384 + lane] + sums[448 + lane]));
       }
     // A value that is not finite must not reach the outputs that do not see its token (0 * inf): those chunks are summed term by term.
     bool bad = false;
@@ -466,7 +456,7 @@ __global__ __launch_bounds__(256, 1) void k_lin_walk(const LinParams<T> p) {
         for (int nt = 0; nt < NT; ++nt)
           Elem<T>::store4(p.out + (((size_t)b * L + t) * p.H + h) * DZ + wave * (DZ / 4) + nt * 16 + 4 * c, o[it][nt][0], o[it][nt][1], o[it][nt][2], o[it][nt][3]);
     }
-    if (i + 1 < n || final) st.update(y, zf, lw);
+    if (i + 1 < n || final) st.template update<REV>(y, zf, lw, p.source_scale);
     if (Sh::BUFFERS == 1 && i + 1 < n) {
       __syncthreads();
       issue(i + 1);
@@ -475,48 +465,69 @@ __global__ __launch_bounds__(256, 1) void k_lin_walk(const LinParams<T> p) {
   if (final) st.store(p.last + (size_t)bh * (DX * DZ), p.transposed, wave);
 }
 
+template <typename T> constexpr int lin_waves() { return sizeof(T) == 2 ? 2 : 1; }      // a SIMD's
+template <typename T, int DK, int DV>
+__global__ __launch_bounds__(256, lin_waves<T>()) void k_lin_forward(const LinParams<T> p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  prefetch_args<sizeof(p)>();
+  lin_walk<T, DK, DV, false, false>(p, blockIdx.x, smem);
+}
+// All three gradients in one launch: the blocks of an item (segment and head) for dq, dv and dk lie eight apart, on one die and at about the same time, so
+// that the inputs of the three come through its L2 once.
+template <typename T>
+struct LinBackward {
+  LinParams<T> dq, dv, dk;
+  int items;
+};
+template <typename T, int DK, int DV, bool GATE>
+__global__ __launch_bounds__(256, lin_waves<T>()) void k_lin_backward(const LinBackward<T> p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  prefetch_args<sizeof(p)>();
+  const int what = blockIdx.x / 8 % 3, item = blockIdx.x / 24 * 8 + blockIdx.x % 8;
+  if (item >= p.items) return;
+  if (what == 0) lin_walk<T, DV, DK, false, GATE>(p.dq, item, smem);
+  else if (what == 1) lin_walk<T, DK, DV, true, GATE>(p.dv, item, smem);
+  else lin_walk<T, DV, DK, true, false>(p.dk, item, smem);
+}
+
 // What the tokens of a segment add to the state, into entry `seg + 1` (REV: `seg - 1`) of states, and the segment's sum of log2 decays.
 template <typename T, int DX, int DZ, bool REV>
-__global__ __launch_bounds__(256, 1) void k_lin_segments(const LinParams<T> p, float* states, float* sums) {
+__global__ __launch_bounds__(256, lin_waves<T>()) void k_lin_segments(const LinParams<T> p, float* states, float* sums) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using St = LinState<T, DX, DZ>;
   using Frag = typename AttnType<T>::Frag;
-  constexpr int NT = St::NT, STAGE = MaskTile<T, DX>::BYTES + MaskTile<T, DZ>::BYTES;
+  constexpr int NT = St::NT, STAGE = MaskTile<T, DX>::BYTES + MaskTile<T, DZ>::BYTES + 1024;
   prefetch_args<sizeof(p)>();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int count = p.segments - 1, seg = blockIdx.x % count + (REV ? 1 : 0), bh = blockIdx.x / count, b = p.by_heads.div(bh), h = bh - b * p.H;
   const int L = p.L, chunks = (L + 63) / 64, first = seg * p.seg_chunks, n = min(p.seg_chunks, chunks - first);
-  float4* weights = reinterpret_cast<float4*>(smem + 2 * STAGE) + wave * 64;
+  const float4* weights = uniform(p.weights + (size_t)bh * chunks * 64);
   const uint32_t lds0 = lds_addr(smem);
   auto token = [&](int i) { return (first + (REV ? n - 1 - i : i)) * 64; };
   auto issue = [&](int i) LACT_INLINE_LAMBDA {
     const uint32_t to = lds0 + i % 2 * STAGE;
     lin_copy<T, DX>(p.y, b, h, token(i), L, to, wave);
     lin_copy<T, DZ>(p.z, b, h, token(i), L, to + MaskTile<T, DX>::BYTES, wave);
+    if (wave == 0) dma16<false>(weights + token(i), lane * 16, to + STAGE - 1024);
   };
   St st;
   st.zero();
   double total = 0.0;
-  float g_next = p.decay.at(b, token(0) + lane, h, L, p.H);
   issue(0);
   for (int i = 0; i < n; ++i) {
-    const int t0 = token(i);
-    const float g = g_next;
-    if (i + 1 < n) g_next = p.decay.at(b, token(i + 1) + lane, h, L, p.H);
     wait_vmcnt<0>();
     __syncthreads();
     if (i + 1 < n) issue(i + 1);
     const char* y = smem + i % 2 * STAGE;
     const char* z = y + MaskTile<T, DX>::BYTES;
-    LinWeights lw;
-    lw.form<REV>(weights, g, t0 + lane < L, p.state_scale, p.source_scale);
+    const float4* lw = reinterpret_cast<const float4*>(y + STAGE - 1024);
     Frag zf[2][NT];
 #pragma unroll
     for (int v = 0; v < 2; ++v)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) zf[v][nt] = LinFrag<T, DZ>::template cols<4>(z, wave * (DZ / 4) + nt * 16, v);
-    st.update(y, zf, lw);
-    total += (double)lw.w[63].x + (double)lw.w[63].y;
+    st.template update<REV>(y, zf, lw, p.source_scale);
+    total += (double)lw[63].x + (double)lw[63].y;
   }
   st.store(states + ((size_t)(seg + (REV ? -1 : 1)) * p.B * p.H + bh) * (DX * DZ), p.transposed, wave);
   if (threadIdx.x == 0) sums[(size_t)seg * p.B * p.H + bh] = (float)total;
@@ -541,54 +552,97 @@ __global__ __launch_bounds__(256) void k_lin_scan(int segments, long long matric
   }
 }
 
-// <gradient of the state, state> at the end of every segment: states [segments][n], the state in front of each; ends, the gradients behind each;
-// last: the state behind the last one (null: its gradient is zero).
-__global__ __launch_bounds__(256) void k_lin_crossing(int segments, long long matrices, int elems, const float* states, const float* ends, const float* last,
-                                                      const float* dlast, float* out) {
-  __shared__ float red[16];
-  const int seg = blockIdx.x % segments;
-  const long long m = blockIdx.x / segments, n = matrices * elems;
-  const bool end = seg == segments - 1;
-  const float* a = end ? (last ? last + m * elems : nullptr) : states + (size_t)(seg + 1) * n + m * elems;
-  const float* d = end ? (dlast ? dlast + m * elems : nullptr) : ends + (size_t)seg * n + m * elems;
-  float s = 0.f;
+// The gradient of a decay is what crosses its token.  In a chunk with the state S in front, the state's gradient dS behind, the state's shares a_i of its
+// outputs (in q . dq) and b_j of its tokens (in v . dv):
+//   dg_t = sum_(i >= t > j) M_ij + sum_(i >= t) a_i + sum_(j < t) b_j + e^G <dS, S>;
+// the last term is X - sum b with X the crossing at the chunk's end, or nothing where the whole chunk's decay G leaves less than 2^-30: no rounding of a large
+// crossing is then carried to tokens that it does not reach.  X of the chunk before is the last term + sum a; of a segment's last chunk, <dS, S> there.
+// M's part is summed as rows minus columns from t on.  0 where the decay forgets everything.
+// Where the decay is the head's, the segment's sum instead, into part [segment][B * H].  states [segments][n]: the state in front of each segment; ends: the
+// gradient behind each (null with one segment); last, dlast: behind the last one (either null: no crossing).  One block per segment and head.
+__global__ __launch_bounds__(256) void k_lin_decay_grad(int B, int L, int H, int segments, int seg_tokens, int elems, const float4* weights, const float* up,
+                                                        const float* down, const float* states, const float* ends, const float* last, const float* dlast,
+                                                        LinDecay decay, float* dg, double* part) {
+  __shared__ double tail[16], source[16], sums[4];
+  __shared__ int cut[16];
+  const int seg = blockIdx.x % segments, bh = blockIdx.x / segments, b = bh / H, h = bh - b * H, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const size_t n = (size_t)B * H * elems;
+  const bool end_of_all = seg == segments - 1;
+  const float* a = end_of_all ? (last ? last + (size_t)bh * elems : nullptr) : states + (size_t)(seg + 1) * n + (size_t)bh * elems;
+  const float* d = end_of_all ? (dlast ? dlast + (size_t)bh * elems : nullptr) : ends + (size_t)seg * n + (size_t)bh * elems;
+  double crossing = 0.0;
   if (a && d)
+#pragma unroll 4
     for (int i = threadIdx.x * 4; i < elems; i += 1024) {
       const float4 u = *reinterpret_cast<const float4*>(a + i), v = *reinterpret_cast<const float4*>(d + i);
-      s += u.x * v.x + u.y * v.y + u.z * v.z + u.w * v.w;
+      crossing += (double)u.x * v.x + (double)u.y * v.y + (double)u.z * v.z + (double)u.w * v.w;
     }
-  s = block_sum(s, red);
-  if (threadIdx.x == 0) out[blockIdx.x] = s;      // [matrix][segment]
-}
-
-// dg_t = crossing at the segment's end + sum over the segment's tokens from t on of (dq's dots - dv's); per_head: their sums over a segment instead,
-// into part [segment][B * H].  0 where the decay forgets everything.  One wave per segment and head.
-__global__ __launch_bounds__(64) void k_lin_decay_grad(int B, int L, int H, int segments, int seg_tokens, const float* up, const float* down, const float* crossing,
-                                                       LinDecay decay, float* dg, double* part) {
-  const int seg = blockIdx.x % segments, bh = blockIdx.x / segments, b = bh / H, h = bh - b * H, lane = threadIdx.x;
-  const int first = seg * seg_tokens, end = min(L, first + seg_tokens);
-  double run = crossing[blockIdx.x], sum = 0.0;
-  for (int t0 = first + (end - first - 1) / 64 * 64; t0 >= first; t0 -= 64) {
-    const int t = t0 + 63 - lane;                   // lane 0 holds the latest
-    const size_t at = ((size_t)b * L + t) * H + h;
-    double v = t < end ? (double)up[at] - (double)down[at] : 0.0;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const double u = __shfl_up(v, o, 64);
-      if (lane >= o) v += u;
+  for (int o = 32; o > 0; o >>= 1) crossing += __shfl_xor(crossing, o, 64);
+  if (lane == 0) sums[wave] = crossing;
+  __syncthreads();
+  double run = (sums[0] + sums[1]) + (sums[2] + sums[3]), sum = 0.0;
+  __syncthreads();
+  const int first = seg * seg_tokens, end = min(L, first + seg_tokens);
+  const float4* ends_of = weights + ((size_t)bh * ((L + 63) / 64) + first / 64) * 64 + 63;
+  // sixteen chunks at a time, the latest first, four to a wave; lane 0 holds a chunk's latest token
+  for (int c0 = (end - first - 1) / 64; c0 >= 0; c0 -= 16) {
+    double v[4], from[4], pairs[4];      // a - b, b, M
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = c0 - wave * 4 - k, t = first + c * 64 + 63 - lane;
+      const size_t at = (size_t)bh * L + t;
+      const bool on = c >= 0 && t < end;
+      from[k] = on ? (double)down[at] : 0.0;
+      v[k] = on ? (double)up[at] - from[k] : 0.0;
+      pairs[k] = on ? (double)up[at + (size_t)B * H * L] : 0.0;
+      if (lane == 0 && c >= 0) {
+        const float4 w = ends_of[c * 64];
+        cut[wave * 4 + k] = w.x + w.y < -30.f;
+      }
     }
-    v += run;
-    run = __shfl(v, 63, 64);
-    if (t < end) {
-      if (decay.at(b, t, h, L, H) <= LIN_MIN_LOG) v = 0.0;
-      if (decay.per_token) dg[at] = (float)v;
-      else sum += v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const double u = __shfl_up(v[k], o, 64), w = __shfl_up(pairs[k], o, 64);
+        if (lane >= o) {
+          v[k] += u;
+          pairs[k] += w;
+        }
+        from[k] += __shfl_xor(from[k], o, 64);
+      }
+      if (lane == 63) {
+        tail[wave * 4 + k] = v[k];
+        source[wave * 4 + k] = from[k];
+      }
     }
+    __syncthreads();
+    double base[4];
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (c0 - k >= 0) {
+        const double x = cut[k] ? source[k] : run;
+        if (k >> 2 == wave) base[k & 3] = x;
+        run = x + tail[k];
+      }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int c = c0 - wave * 4 - k, t = first + c * 64 + 63 - lane;
+      if (c >= 0 && t < end) {
+        const double x = decay.at(b, t, h, L, H) <= LIN_MIN_LOG ? 0.0 : base[k] + v[k] + pairs[k];
+        if (decay.per_token) dg[((size_t)b * L + t) * H + h] = (float)x;
+        else sum += x;
+      }
+    }
+    __syncthreads();
   }
   if (!decay.per_token) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-    if (lane == 0) part[(size_t)seg * B * H + bh] = sum;
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) part[(size_t)seg * B * H + bh] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   }
 }
 // One wave per head: the sum of part [rows][H].

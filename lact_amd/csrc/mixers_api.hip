@@ -197,15 +197,17 @@ int check_linear(const lact_linear_desc_t* d) {
 }
 
 struct LinCut { int segments, chunks; };      // chunks of a segment
-// One block walks a segment of a head; enough segments that the walks of all heads fill the chip once.
+// One block walks a segment of a head; enough segments that the walks of all heads give every compute unit two blocks.  Sequences of a few chunks
+// are walked as a whole: two launches less.
 LinCut lin_cut(const lact_linear_desc_t* d) {
   const int chunks = ceil_div(d->l, LIN_CHUNK), heads = d->b * d->h;
-  const int want = std::max(1, std::min(chunks, COMPUTE_UNITS / heads)), per = ceil_div(chunks, want);
+  if (chunks <= 8) return LinCut{1, chunks};
+  const int want = std::max(1, std::min(chunks, 2 * COMPUTE_UNITS / heads)), per = ceil_div(chunks, want);
   return LinCut{ceil_div(chunks, per), per};
 }
 struct LinBuffers {
-  size_t states, sums, end;              // of `states`: where segments start; sums of their decays
-  size_t ends, rsums, up, down, crossing, part, scratch;
+  size_t weights, states, sums, end;     // of `states`: what tokens weigh, where segments start, sums of their decays
+  size_t ends, rsums, up, down, part, scratch;
 };
 LinBuffers lin_buffers(const lact_linear_desc_t* d) {
   const LinCut cut = lin_cut(d);
@@ -215,34 +217,34 @@ LinBuffers lin_buffers(const lact_linear_desc_t* d) {
   size_t at = 0;
   auto take = [&](size_t n) { const size_t a = at; at += round(n); return a; };
   const size_t several = cut.segments > 1;
+  o.weights = take(heads * ceil_div(d->l, LIN_CHUNK) * LIN_CHUNK * sizeof(float4));
   o.states = take(several * cut.segments * heads * elems * 4);
   o.sums = take(several * cut.segments * heads * 4);
   o.end = at;
   at = 0;
   o.ends = take(several * cut.segments * heads * elems * 4);
   o.rsums = take(several * cut.segments * heads * 4);
-  o.up = take(tokens * 4);
+  o.up = take(tokens * 8);
   o.down = take(tokens * 4);
-  o.crossing = take(cut.segments * heads * 4);
   o.part = take(d->decay_per_token ? 0 : cut.segments * heads * 8);
   o.scratch = at;
   return o;
 }
 
 template <typename T>
-LinParams<T> lin_params(const lact_linear_desc_t* d, const float* g) {
+LinParams<T> lin_params(const lact_linear_desc_t* d, const char* states) {
   LinParams<T> p;
   memset(&p, 0, sizeof(p));
   const LinCut cut = lin_cut(d);
   p.B = d->b; p.L = d->l; p.H = d->h; p.segments = cut.segments; p.seg_chunks = cut.chunks;
-  p.decay.g = g; p.decay.per_token = d->decay_per_token;
+  p.weights = reinterpret_cast<const float4*>(states + lin_buffers(d).weights);
   p.by_heads = make_udiv(d->h);
   return p;
 }
 
 template <typename T, int DX, int DZ, bool REV>
 void lin_segments(const LinParams<T>& p, const float* initial, float* states, float* sums, hipStream_t s) {
-  constexpr int SM = 2 * (MaskTile<T, DX>::BYTES + MaskTile<T, DZ>::BYTES) + 4 * 64 * 16;
+  constexpr int SM = 2 * (MaskTile<T, DX>::BYTES + MaskTile<T, DZ>::BYTES + 1024);
   LACT_BIG_LDS((k_lin_segments<T, DX, DZ, REV>), SM);
   const int heads = p.B * p.H;
   LACT_LAUNCH_SMEM("k_lin_segments", "linear_attn", 2.0 * heads * p.L * DX * DZ, (k_lin_segments<T, DX, DZ, REV>), dim3((p.segments - 1) * heads), dim3(256), SM, s, p,
@@ -250,23 +252,20 @@ void lin_segments(const LinParams<T>& p, const float* initial, float* states, fl
   LACT_LAUNCH("k_lin_scan", "linear_attn", 0.0, k_lin_scan, dim3((unsigned)(((long long)heads * DX * DZ / 4 + 255) / 256)), dim3(256), s, p.segments, (long long)heads,
               DX * DZ, (int)REV, initial, sums, states);
 }
-template <typename T, int DX, int DZ, bool REV, bool GATE>
-void lin_walk(const LinParams<T>& p, hipStream_t s) {
-  constexpr int SM = LinShape<T, DX, DZ, GATE>::LDS;
-  LACT_BIG_LDS((k_lin_walk<T, DX, DZ, REV, GATE>), SM);
-  LACT_LAUNCH_SMEM("k_lin_walk", "linear_attn", 4.0 * p.B * p.H * p.L * DX * DZ, (k_lin_walk<T, DX, DZ, REV, GATE>), dim3(p.segments * p.B * p.H), dim3(256), SM, s, p);
-}
 
 template <typename T, int DK, int DV>
 int lin_forward(const lact_linear_desc_t* d, const void* q, const void* k, const void* v, const float* g, const float* state, void* out, float* last, char* states,
                 hipStream_t s) {
   const LinBuffers buf = lin_buffers(d);
-  LinParams<T> p = lin_params<T>(d, g);
+  LinParams<T> p = lin_params<T>(d, states);
   p.x = {static_cast<const T*>(q), d->q_ld, d->q_bs};
   p.y = {static_cast<const T*>(k), d->k_ld, d->k_bs};
   p.z = {static_cast<const T*>(v), d->v_ld, d->v_bs};
   p.pair_scale = p.state_scale = d->scale; p.source_scale = 1.f;
   p.out = static_cast<T*>(out); p.last = last;
+  const int heads = d->b * d->h;
+  LACT_LAUNCH("k_lin_weights", "linear_attn", 0.0, k_lin_weights, dim3((unsigned)(((long long)heads * ceil_div(d->l, LIN_CHUNK) + 3) / 4)), dim3(256), s, d->b, d->l, d->h,
+              (LinDecay{g, d->decay_per_token}), const_cast<float4*>(p.weights));
   if (p.segments > 1) {
     float* at = reinterpret_cast<float*>(states + buf.states);
     lin_segments<T, DK, DV, false>(p, state, at, reinterpret_cast<float*>(states + buf.sums), s);
@@ -274,9 +273,19 @@ int lin_forward(const lact_linear_desc_t* d, const void* q, const void* k, const
   } else {
     p.state0 = state;
   }
-  lin_walk<T, DK, DV, false, false>(p, s);
+  constexpr int SM = LinShape<T, DK, DV, false>::LDS;
+  LACT_BIG_LDS((k_lin_forward<T, DK, DV>), SM);
+  LACT_LAUNCH_SMEM("k_lin_forward", "linear_attn", 4.0 * heads * p.L * DK * DV, (k_lin_forward<T, DK, DV>), dim3(p.segments * heads), dim3(256), SM, s, p);
   LACT_CHECK_LAUNCH();
   return 0;
+}
+
+template <typename T, int DK, int DV, bool GATE>
+void lin_gradients(const LinBackward<T>& p, hipStream_t s) {
+  constexpr int SM = std::max({LinShape<T, DV, DK, GATE>::LDS, LinShape<T, DK, DV, GATE>::LDS, LinShape<T, DV, DK, false>::LDS});
+  LACT_BIG_LDS((k_lin_backward<T, DK, DV, GATE>), SM);
+  LACT_LAUNCH_SMEM("k_lin_backward", "linear_attn_bwd", 12.0 * p.dq.B * p.dq.H * p.dq.L * DK * DV, (k_lin_backward<T, DK, DV, GATE>), dim3(ceil_div(p.items, 8) * 24),
+                   dim3(256), SM, s, p);
 }
 
 template <typename T, int DK, int DV>
@@ -285,45 +294,40 @@ int lin_backward(const lact_linear_desc_t* d, const void* q, const void* k, cons
   const LinBuffers buf = lin_buffers(d);
   const LinRows<T> rq{static_cast<const T*>(q), d->q_ld, d->q_bs}, rk{static_cast<const T*>(k), d->k_ld, d->k_bs}, rv{static_cast<const T*>(v), d->v_ld, d->v_bs},
       ro{static_cast<const T*>(dout), d->do_ld, d->do_bs};
-  const LinParams<T> base = lin_params<T>(d, g);
+  const LinParams<T> base = lin_params<T>(d, states);
   float* up = reinterpret_cast<float*>(scratch + buf.up);
   float* down = reinterpret_cast<float*>(scratch + buf.down);
   float* ends = reinterpret_cast<float*>(scratch + buf.ends);
   const float* starts = reinterpret_cast<const float*>(states + buf.states);
   const bool several = base.segments > 1;
-  {      // dq: forwards with dout, v, k and the transposed state
-    LinParams<T> p = base;
-    p.x = ro; p.y = rv; p.z = rk; p.w = rq;
-    p.pair_scale = p.state_scale = d->scale; p.source_scale = 1.f;
-    p.out = static_cast<T*>(dq); p.transposed = 1; p.dots = up;
-    if (several) p.states = starts;
-    else p.state0 = state;
-    if (dg) lin_walk<T, DV, DK, false, true>(p, s);
-    else lin_walk<T, DV, DK, false, false>(p, s);
-  }
-  LinParams<T> p = base;      // backwards in time
-  p.x = rk; p.y = rq; p.z = ro; p.w = rv;
-  p.pair_scale = d->scale; p.state_scale = 1.f; p.source_scale = d->scale;
+  const int heads = d->b * d->h;
+  LinBackward<T> all{base, base, base, base.segments * heads};
+  LinParams<T>& a = all.dq;      // forwards with dout, v, k and the transposed state
+  a.x = ro; a.y = rv; a.z = rk; a.w = rq;
+  a.pair_scale = a.state_scale = d->scale; a.source_scale = 1.f;
+  a.out = static_cast<T*>(dq); a.transposed = 1; a.dots = up;
+  if (several) a.states = starts;
+  else a.state0 = state;
+  LinParams<T>& r = all.dv;      // backwards in time
+  r.x = rk; r.y = rq; r.z = ro; r.w = rv;
+  r.pair_scale = d->scale; r.state_scale = 1.f; r.source_scale = d->scale;
   if (several) {
-    lin_segments<T, DK, DV, true>(p, dlast, ends, reinterpret_cast<float*>(scratch + buf.rsums), s);
-    p.states = ends;
+    lin_segments<T, DK, DV, true>(r, dlast, ends, reinterpret_cast<float*>(scratch + buf.rsums), s);
+    r.states = ends;
   } else {
-    p.state0 = dlast;
+    r.state0 = dlast;
   }
-  p.out = static_cast<T*>(dv); p.last = dstate; p.dots = down;
-  if (dg) lin_walk<T, DK, DV, true, true>(p, s);
-  else lin_walk<T, DK, DV, true, false>(p, s);
-  p.x = rv; p.y = ro; p.z = rq;
-  p.out = static_cast<T*>(dk); p.last = nullptr; p.dots = nullptr; p.transposed = 1;
-  lin_walk<T, DV, DK, true, false>(p, s);
+  all.dk = r;
+  r.out = static_cast<T*>(dv); r.last = dstate; r.dots = down;
+  LinParams<T>& c = all.dk;
+  c.x = rv; c.y = ro; c.z = rq;
+  c.out = static_cast<T*>(dk); c.transposed = 1;
+  if (dg) lin_gradients<T, DK, DV, true>(all, s);
+  else lin_gradients<T, DK, DV, false>(all, s);
   if (dg) {
-    const int heads = d->b * d->h;
-    float* crossing = reinterpret_cast<float*>(scratch + buf.crossing);
     double* part = reinterpret_cast<double*>(scratch + buf.part);
-    LACT_LAUNCH("k_lin_crossing", "linear_attn_bwd", 0.0, k_lin_crossing, dim3(base.segments * heads), dim3(256), s, base.segments, (long long)heads, DK * DV, starts, ends,
-                last, dlast, crossing);
-    LACT_LAUNCH("k_lin_decay_grad", "linear_attn_bwd", 0.0, k_lin_decay_grad, dim3(base.segments * heads), dim3(64), s, d->b, d->l, d->h, base.segments,
-                base.seg_chunks * LIN_CHUNK, up, down, crossing, base.decay, dg, part);
+    LACT_LAUNCH("k_lin_decay_grad", "linear_attn_bwd", 0.0, k_lin_decay_grad, dim3(base.segments * heads), dim3(256), s, d->b, d->l, d->h, base.segments,
+                base.seg_chunks * LIN_CHUNK, DK * DV, base.weights, up, down, starts, ends, last, dlast, (LinDecay{g, d->decay_per_token}), dg, part);
     if (!d->decay_per_token)
       LACT_LAUNCH("k_lin_decay_sum", "linear_attn_bwd", 0.0, k_lin_decay_sum, dim3(d->h), dim3(64), s, base.segments * d->b, d->h, part, dg);
   }
@@ -401,7 +405,7 @@ int lact_linear_attention_sizes(const lact_linear_desc_t* d, size_t* states_byte
 int lact_linear_attention_forward(const lact_linear_desc_t* d, const void* q, const void* k, const void* v, const float* g, const float* state, void* out, float* last,
                                   void* states, void* stream) {
   if (check_linear(d) || check_linear_rows(d, q, k, v) || check_ptrs({g, out}, "linear attention tensors") || check_states({state, last, states})) return -1;
-  if (lin_buffers(d).end && !states) return fail("null pointer: linear attention states");
+  if (!states) return fail("null pointer: linear attention states");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return by_sizes(d->act_dtype, d->dk, d->dv, [&](auto t, auto dk, auto dv) {
     return lin_forward<decltype(t), decltype(dk)::value, decltype(dv)::value>(d, q, k, v, g, state, out, last, static_cast<char*>(states), s);
@@ -414,7 +418,7 @@ int lact_linear_attention_backward(const lact_linear_desc_t* d, const void* q, c
   if (check_linear(d) || check_linear_rows(d, q, k, v) || check_rows(dout, d->do_ld, d->do_bs, d->h * d->dv, d->act_dtype, "dout") ||
       check_ptrs({g, dq, dk_, dv_, scratch}, "linear attention backward tensors") || check_states({state, last, states, dlast, dstate, scratch}))
     return -1;
-  if (lin_buffers(d).end && !states) return fail("null pointer: linear attention states");
+  if (!states) return fail("null pointer: linear attention states");
   if (dg && dlast && !last) return fail("null pointer: the last state, for the gradient of the decays");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   return by_sizes(d->act_dtype, d->dk, d->dv, [&](auto t, auto dk, auto dv) {

@@ -801,7 +801,7 @@ LinearCall linear_forward(const Tensor& q_, const Tensor& k_, const Tensor& v_, 
   if (return_state) c.last = at::empty({b, h, dk, dv}, f32);
   size_t bytes = 0;
   check(lact_linear_attention_sizes(&D, &bytes, nullptr));
-  if (bytes) c.states = at::empty({(int64_t)bytes}, f32.dtype(at::kByte));
+  c.states = at::empty({(int64_t)bytes}, f32.dtype(at::kByte));
   check(lact_linear_attention_forward(&D, ptr(c.q), ptr(c.k), ptr(c.v), fptr(c.g), fptr(c.state), ptr(c.out), fptr(c.last), ptr(c.states), stream()));
   return c;
 }
