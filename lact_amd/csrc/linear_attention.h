@@ -167,8 +167,8 @@ struct LinShape {
   static constexpr int PAIRS = MaskTile<T, 64>::BYTES;
   static constexpr int SUMS = GATE ? 4 * 64 * 4 * 2 : 0;                  // per wave: what its columns, and its pairs, add to the dots
   // two chunks where two blocks of them fit a compute unit
-  static constexpr int BUFFERS = 2 * STAGE + PAIRS + SUMS <= 80 * 1024 ? 2 : 1;
-  static constexpr int LDS = BUFFERS * STAGE + PAIRS + SUMS;
+  static constexpr int BUFFERS = 2 * STAGE + PAIRS + SUMS + 16 <= 80 * 1024 ? 2 : 1;
+  static constexpr int LDS = BUFFERS * STAGE + PAIRS + SUMS + 16;
   static_assert(LDS <= 160 * 1024, "LDS");
 };
 
@@ -212,9 +212,8 @@ struct LinState {        // columns [wave * DZ / 4, + DZ / 4): accumulator a, ro
       }
   }
   // decays by `whole` and adds y^T (weight z); zf: the wave's columns of z
-  template <bool REV, typename Frag>
+  template <bool REV, int PARTS, typename Frag>
   __device__ __forceinline__ void update(const char* y, const Frag (&zf)[2][NT], const float4* w, float source_scale) {
-    constexpr int PARTS = lin_parts<T>();
     const float whole = __builtin_amdgcn_exp2f(w[63].x + w[63].y);
 #pragma unroll
     for (int a = 0; a < AT; ++a)
@@ -261,7 +260,8 @@ __device__ __forceinline__ void lin_copy(const LinRows<T>& m, int b, int h, int 
 // The walk over a segment.  REV: from its end to its beginning, sources are the later tokens.
 // GATE: also dots[t], for the gradient of the decays.  Forwards (x, y, z, w = dout, v, k, q): the state's share in q_t . dq_t, and row sum minus column sum
 // of M at t; backwards (x, y, z, w = k, q, dout, v): the state's share in v_t . dv_t.
-template <typename T, int DX, int DZ, bool REV, bool GATE>
+// ROUNDED: only rounded outputs depend on the state, which then is added to in products of one part.
+template <typename T, int DX, int DZ, bool REV, bool GATE, bool ROUNDED>
 __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* smem) {
   using Sh = LinShape<T, DX, DZ, GATE>;
   using St = LinState<T, DX, DZ>;
@@ -275,6 +275,8 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
   const int L = p.L, chunks = (L + 63) / 64, first = seg * p.seg_chunks, n = min(p.seg_chunks, chunks - first);
   char* pairs = smem + Sh::BUFFERS * Sh::STAGE;
   float* sums = reinterpret_cast<float*>(pairs + Sh::PAIRS);
+  volatile int* spoilt = reinterpret_cast<volatile int*>(pairs + Sh::PAIRS + Sh::SUMS);
+  if (threadIdx.x == 0) *spoilt = 0;
   const float4* weights = uniform(p.weights + (size_t)bh * chunks * 64);
   const uint32_t lds0 = lds_addr(smem);
   auto token = [&](int i) { return (first + (REV ? n - 1 - i : i)) * 64; };
@@ -295,8 +297,8 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
   issue(0);
   for (int i = 0; i < n; ++i) {
     const int t0 = token(i);
-    if (Sh::BUFFERS == 1 || i == 0) wait_vmcnt<0>();
-    __syncthreads();      // the chunk is there, and every wave is through with the one before
+    if (i == 0) wait_vmcnt<0>();
+    __syncthreads();      // the chunk is there, and every wave is through with the pairs of the one before
     if (Sh::BUFFERS == 2 && i + 1 < n) issue(i + 1);
     const char* x = smem + i % Sh::BUFFERS * Sh::STAGE;
     const char* y = x + Sh::X;
@@ -406,7 +408,14 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
     for (int v = 0; v < 2; ++v)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) zf[v][nt] = FZ::template cols<4>(z, wave * (DZ / 4) + nt * 16, v);
-    __syncthreads();      // the pairs of all waves
+    bool bad = false;
+#pragma unroll
+    for (int v = 0; v < 2; ++v)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) bad |= unfinite(zf[v][nt]);
+    if (__any(bad)) *spoilt = 1;
+    if (i + 1 < n || final) st.template update<REV, ROUNDED ? 1 : lin_parts<T>()>(y, zf, lw, p.source_scale);
+    __syncthreads();      // the pairs of all waves; nobody reads the chunk any more
     if constexpr (GATE)
       if (wave == 0 && t0 + lane < L) {
         float* to = p.dots + (size_t)bh * L + t0 + lane;
@@ -414,12 +423,7 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
         if constexpr (!REV) to[(size_t)p.B * p.H * L] = -((sums[256 + lane] + sums[320 + lane]) + (sums[384 + lane] + sums[448 + lane]));
       }
     // A value that is not finite must not reach the outputs that do not see its token (0 * inf): those chunks are summed term by term.
-    bool bad = false;
-#pragma unroll
-    for (int v = 0; v < 2; ++v)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) bad |= unfinite(zf[v][nt]);
-    if (__any(bad)) {
+    if (__builtin_amdgcn_readfirstlane(*spoilt)) {
       for (int j = 0; j < 64; ++j) {
         if (t0 + j >= L) break;
 #pragma unroll
@@ -436,7 +440,11 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
             }
         }
       }
+      __syncthreads();
+      if (threadIdx.x == 0) *spoilt = 0;
+      if (Sh::BUFFERS == 1 && i + 1 < n) issue(i + 1);
     } else {
+      if (Sh::BUFFERS == 1 && i + 1 < n) issue(i + 1);
 #pragma unroll
       for (int it = 0; it < 4; ++it)
 #pragma unroll
@@ -447,7 +455,7 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
           for (int nt = 0; nt < NT; ++nt) o[it][nt] = mma16(zf[v][nt], pf, o[it][nt]);
         }
     }
-    if (Sh::BUFFERS == 2) wait_vmcnt<0>();      // for the next chunk, here and not behind the stores
+    wait_vmcnt<0>();      // for the next chunk, here and not behind the stores
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
       const int t = t0 + 16 * it + li;
@@ -455,11 +463,6 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           Elem<T>::store4(p.out + (((size_t)b * L + t) * p.H + h) * DZ + wave * (DZ / 4) + nt * 16 + 4 * c, o[it][nt][0], o[it][nt][1], o[it][nt][2], o[it][nt][3]);
-    }
-    if (i + 1 < n || final) st.template update<REV>(y, zf, lw, p.source_scale);
-    if (Sh::BUFFERS == 1 && i + 1 < n) {
-      __syncthreads();
-      issue(i + 1);
     }
   }
   if (final) st.store(p.last + (size_t)bh * (DX * DZ), p.transposed, wave);
@@ -470,7 +473,7 @@ template <typename T, int DK, int DV>
 __global__ __launch_bounds__(256, lin_waves<T>()) void k_lin_forward(const LinParams<T> p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   prefetch_args<sizeof(p)>();
-  lin_walk<T, DK, DV, false, false>(p, blockIdx.x, smem);
+  lin_walk<T, DK, DV, false, false, false>(p, blockIdx.x, smem);
 }
 // All three gradients in one launch: the blocks of an item (segment and head) for dq, dv and dk lie eight apart, on one die and at about the same time, so
 // that the inputs of the three come through its L2 once.
@@ -485,9 +488,9 @@ __global__ __launch_bounds__(256, lin_waves<T>()) void k_lin_backward(const LinB
   prefetch_args<sizeof(p)>();
   const int what = blockIdx.x / 8 % 3, item = blockIdx.x / 24 * 8 + blockIdx.x % 8;
   if (item >= p.items) return;
-  if (what == 0) lin_walk<T, DV, DK, false, GATE>(p.dq, item, smem);
-  else if (what == 1) lin_walk<T, DK, DV, true, GATE>(p.dv, item, smem);
-  else lin_walk<T, DV, DK, true, false>(p.dk, item, smem);
+  if (what == 0) lin_walk<T, DV, DK, false, GATE, !GATE>(p.dq, item, smem);
+  else if (what == 1) lin_walk<T, DK, DV, true, GATE, false>(p.dv, item, smem);
+  else lin_walk<T, DV, DK, true, false, true>(p.dk, item, smem);
 }
 
 // What the tokens of a segment add to the state, into entry `seg + 1` (REV: `seg - 1`) of states, and the segment's sum of log2 decays.
@@ -526,7 +529,7 @@ __global__ __launch_bounds__(256, lin_waves<T>()) void k_lin_segments(const LinP
     for (int v = 0; v < 2; ++v)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) zf[v][nt] = LinFrag<T, DZ>::template cols<4>(z, wave * (DZ / 4) + nt * 16, v);
-    st.template update<REV>(y, zf, lw, p.source_scale);
+    st.template update<REV, lin_parts<T>()>(y, zf, lw, p.source_scale);
     total += (double)lw[63].x + (double)lw[63].y;
   }
   st.store(states + ((size_t)(seg + (REV ? -1 : 1)) * p.B * p.H + bh) * (DX * DZ), p.transposed, wave);

@@ -201,7 +201,7 @@ struct LinCut { int segments, chunks; };      // chunks of a segment
 // are walked as a whole: two launches less.
 LinCut lin_cut(const lact_linear_desc_t* d) {
   const int chunks = ceil_div(d->l, LIN_CHUNK), heads = d->b * d->h;
-  if (chunks <= 8) return LinCut{1, chunks};
+  if (chunks <= (d->act_dtype == LACT_BF16 ? 4 : 2)) return LinCut{1, chunks};      // (fp32 products take some seven times as long)
   const int want = std::max(1, std::min(chunks, 2 * COMPUTE_UNITS / heads)), per = ceil_div(chunks, want);
   return LinCut{ceil_div(chunks, per), per};
 }
