@@ -275,7 +275,7 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
   const int L = p.L, chunks = (L + 63) / 64, first = seg * p.seg_chunks, n = min(p.seg_chunks, chunks - first);
   char* pairs = smem + Sh::BUFFERS * Sh::STAGE;
   float* sums = reinterpret_cast<float*>(pairs + Sh::PAIRS);
-  volatile int* spoilt = reinterpret_cast<volatile int*>(pairs + Sh::PAIRS + Sh::SUMS);
+  int* spoilt = reinterpret_cast<int*>(pairs + Sh::PAIRS + Sh::SUMS);
   if (threadIdx.x == 0) *spoilt = 0;
   const float4* weights = uniform(p.weights + (size_t)bh * chunks * 64);
   const uint32_t lds0 = lds_addr(smem);
@@ -423,7 +423,7 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
         if constexpr (!REV) to[(size_t)p.B * p.H * L] = -((sums[256 + lane] + sums[320 + lane]) + (sums[384 + lane] + sums[448 + lane]));
       }
     // A value that is not finite must not reach the outputs that do not see its token (0 * inf): those chunks are summed term by term.
-    if (__builtin_amdgcn_readfirstlane(*spoilt)) {
+    if (__builtin_amdgcn_readfirstlane(lds_word(spoilt))) {
       for (int j = 0; j < 64; ++j) {
         if (t0 + j >= L) break;
 #pragma unroll

@@ -229,6 +229,11 @@ __device__ __forceinline__ bool unfinite(const f32x8& f) {
   for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
   return m >= 0x7f800000u;
 }
+// A word of LDS that other waves write.
+__device__ __forceinline__ uint32_t lds_word(const void* p) {
+  typedef __attribute__((address_space(3))) const volatile uint32_t lds_u32;
+  return *(lds_u32*)(const __attribute__((address_space(3))) char*)(const char*)p;
+}
 // What lies in a tile and is not finite must not meet the zero weight of a row that does not see it.  The wave that copied 1 KB of a tile looks it over
 // once it is there, clears rows that hold such a value and writes down which; every wave gives the rows of its own that see one of them NaN.
 // (Selecting in the products' operands instead, where a tile is masked, cost a tenth of the forward: a branch at every operand, or registers for two loops.)
@@ -263,8 +268,9 @@ struct Spoilt {
       }
     }
   }
-  // behind the barrier: the slot's rows; and room for those of the slot that the next copies go to
-  __device__ __forceinline__ bool any() const { return __builtin_amdgcn_readfirstlane(*(volatile uint32_t*)(words + 15)) != 0; }
+  // behind the barrier: the slot's rows; and room for those of the slot that the next copies go to.  (Read as LDS by its address space: through a generic
+  // pointer the load counts as one of global memory too, and its wait is one for the copies just issued.)
+  __device__ __forceinline__ bool any() const { return __builtin_amdgcn_readfirstlane(lds_word(words + 15)) != 0; }
   __device__ __forceinline__ uint64_t rows(int slot) const { return (uint64_t)words[2 * slot] | (uint64_t)words[2 * slot + 1] << 32; }
   __device__ __forceinline__ void clear(int slot) const {
     if (threadIdx.x < 2) words[2 * slot + threadIdx.x] = 0;
