@@ -124,31 +124,36 @@ struct MaskTile {       // 64 x D, the 16-byte granule g of row r at slot g ^ ke
   }
 };
 
-template <typename T, int D>
+template <typename T, int D, int NW = MASK_WAVES>
 struct MaskCopy {
-  static constexpr int NW = MASK_WAVES;
   using S = MaskTile<T, D>;
   static constexpr int NC = S::G / NW;      // copies of a wave and tile
   static_assert(S::G % NW == 0, "copies must split evenly over the waves");
-  uint32_t voff[NC], vlast[NC];
+  uint32_t voff[NC];
   const T* base;
-  int step, last;
+  int ld, last, rows;
+  __device__ __forceinline__ int row(int wave, int i) const { return ((wave + i * NW) * 64 + (int)(threadIdx.x & 63)) / S::G; }
   // the 64-row tiles [0, n) from row `first` on of a head whose rows end at L
-  __device__ __forceinline__ void init(int wave, const T* head, int ld, int first, int n, int L) {
-    base = uniform(head + (size_t)first * ld);
-    step = 64 * ld; last = n - 1;
-    const int rows = L - 1 - (first + last * 64);
+  __device__ __forceinline__ void init(int wave, const T* head, int ld_, int first, int n, int L) {
+    base = uniform(head + (size_t)first * ld_);
+    ld = ld_; last = n - 1;
+    rows = L - 1 - (first + last * 64);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int c = (wave + i * NW) * 64 + (threadIdx.x & 63), row = c / S::G, slot = c % S::G;
-      const uint32_t col = (uint32_t)(slot ^ S::key(row)) * 16;
-      voff[i] = (uint32_t)row * ld * sizeof(T) + col;
-      vlast[i] = (uint32_t)min(row, rows) * ld * sizeof(T) + col;      // rows past the end repeat the last one
+      const int r = row(wave, i), slot = (threadIdx.x & 63) % S::G;
+      voff[i] = (uint32_t)r * ld * sizeof(T) + (uint32_t)(slot ^ S::key(r)) * 16;
     }
   }
   __device__ __forceinline__ void issue(int t, const T* from, uint32_t lds, int wave) const {
+    const T* at = from + (long long)t * 64 * ld;
+    if (t < last || rows >= 63) {
 #pragma unroll
-    for (int i = 0; i < NC; ++i) dma16<false>(from + (long long)t * step, t == last ? vlast[i] : voff[i], lds + (wave + i * NW) * 1024);
+      for (int i = 0; i < NC; ++i) dma16<false>(at, voff[i], lds + (wave + i * NW) * 1024);
+    } else {      // rows past the end repeat the last one
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        dma16<false>(at, voff[i] - (uint32_t)max(0, row(wave, i) - rows) * ld * (uint32_t)sizeof(T), lds + (wave + i * NW) * 1024);
+    }
   }
 };
 
@@ -237,9 +242,8 @@ __device__ __forceinline__ uint32_t lds_word(const void* p) {
 // What lies in a tile and is not finite must not meet the zero weight of a row that does not see it.  The wave that copied 1 KB of a tile looks it over
 // once it is there, clears rows that hold such a value and writes down which; every wave gives the rows of its own that see one of them NaN.
 // (Selecting in the products' operands instead, where a tile is masked, cost a tenth of the forward: a branch at every operand, or registers for two loops.)
-template <typename T, int D>
+template <typename T, int D, int NW = MASK_WAVES>
 struct Spoilt {
-  static constexpr int NW = MASK_WAVES;
   using S = MaskTile<T, D>;
   static constexpr int BYTES = 64;
   uint32_t* words;        // rows [0, 32) and [32, 64) of every ring slot; behind them whether there ever were any
@@ -349,13 +353,18 @@ struct Scores {
   }
 };
 
+// Waves of dk/dv that share 32 keys: heads of 128 in bf16 take two, one for the queries [0, 32) of every tile and one for [32, 64), whose sums are added at the
+// end.  A wave's two accumulators (128 registers) and its own keys and values (64) leave too little of the 256 that two waves of a SIMD have each: here
+// the values are read from LDS.  One wave with all of them in 400 registers: 148 us at 2 x 4096 tokens in documents, 12 heads.
+// With a cap or a distance there are too many for that as well: 969 us as one wave, 1075 as two, the backward of 4 x 4096 tokens of 12 heads.
+template <typename T, int D, bool BENT> constexpr int mask_halves() { return sizeof(T) == 2 && D == 128 && !BENT ? 2 : 1; }
 // 64-row tiles of both operands in LDS
 template <typename T, int D> constexpr int mask_ring(bool keys) { return sizeof(T) == 4 || (D == 128 && !keys) ? 2 : 3; }
-template <typename T, int D>
+template <typename T, int D, bool BENT>
 constexpr int mask_lds_bytes(bool stats) {
   constexpr int NW = MASK_WAVES;
   const int R = mask_ring<T, D>(stats);
-  const int ring = R * 2 * MaskTile<T, D>::BYTES + (stats ? R * 512 : 0) + Spoilt<T, D>::BYTES;
+  const int ring = R * 2 * MaskTile<T, D>::BYTES + (stats ? R * 512 + (mask_halves<T, D, BENT>() - 1) * 2 * MaskTile<T, D>::BYTES : 0) + Spoilt<T, D>::BYTES;
   // what the rows are stored through, for splits in fp32
   return cmax(ring, NW * 32 * cmax((D + 16 / (int)sizeof(T)) * (int)sizeof(T), stats ? (D + 4) * 4 : 0));
 }
@@ -436,7 +445,7 @@ struct Seen {
   }
   // whether a row among `rows` (of the 32) is one of them
   __device__ __forceinline__ bool any_of(uint32_t rows) const { return (bits & 0x0f0f0f0fu & rows >> (4 * ((threadIdx.x & 63) >> 5))) != 0; }
-  // all ones or zero; computed here and now, not kept in a register for every j
+  // all ones or zero
   __device__ __forceinline__ uint32_t word(int j) const {
     uint32_t w;
     asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(w) : "v"(bits), "n"(8 * (j / 4) + j % 4));
@@ -699,11 +708,11 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
 // dv = sum_queries p dout, dk = scale * sum_queries ds q, over the queries of all heads that share the key head: a wave owns 32 keys and
 // walks the queries that see them, head after head.  With few keys (blocks) the walk is cut into gridDim.y splits, whose sums k_attn_sum adds.
 template <typename T, int D, bool BENT>
-__global__ __launch_bounds__(64 * MASK_WAVES, D == 64 && sizeof(T) == 2 ? 2 : 1) void k_masked_attn_dkv(const MaskedAttnParams<T> p) {
-  constexpr int NW = MASK_WAVES;
+__global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (sizeof(T) == 2 && (D == 64 || !BENT) ? 2 : 1)) void k_masked_attn_dkv(const MaskedAttnParams<T> p) {
+  constexpr int KW = MASK_WAVES, HALVES = mask_halves<T, D, BENT>(), NW = KW * HALVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using S = MaskTile<T, D>;
-  using Copy = MaskCopy<T, D>;
+  using Copy = MaskCopy<T, D, NW>;
   using Frag = typename AttnType<T>::Frag;
   constexpr int STAGE = 2 * S::BYTES, RING = mask_ring<T, D>(true);
   prefetch_args<sizeof(p)>();
@@ -711,14 +720,23 @@ __global__ __launch_bounds__(64 * MASK_WAVES, D == 64 && sizeof(T) == 2 ? 2 : 1)
   p.locate(bx, z);
   const int b = z / p.HK, hk = z - b * p.HK, L = p.L;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int blk0 = bx * 32 * NW, row0 = blk0 + wave * 32, row = row0 + (lane & 31);
-  Frag kf[D / 16], vf[D / 16];
+  const int group = wave % KW, half = wave / KW;        // of keys; of a tile's queries
+  const int blk0 = bx * 32 * KW, row0 = blk0 + group * 32, row = row0 + (lane & 31);
+  Frag kf[D / 16], vf[HALVES == 1 ? D / 16 : 1];
   mask_own_rows<T, D>(kf, p.k + b * p.bsk + hk * D, p.ldk, row, L);
-  mask_own_rows<T, D>(vf, p.v + b * p.bsv + hk * D, p.ldv, row, L);
+  char* values = smem + RING * (STAGE + 512) + Spoilt<T, D>::BYTES;      // of all of the block's keys, as two tiles
+  if constexpr (HALVES == 1) {
+    mask_own_rows<T, D>(vf, p.v + b * p.bsv + hk * D, p.ldv, row, L);
+  } else {
+    const int n = blk0 + 64 < L ? 2 : 1;      // (keys past the end have nothing in LDS, and nobody looks at their sums)
+    Copy cv;
+    cv.init(wave, p.v + b * p.bsv + hk * D, p.ldv, blk0, n, L);
+    for (int i = 0; i < n; ++i) cv.issue(i, cv.base, lds_addr(values) + i * S::BYTES, wave);
+  }
   const int2 own = p.col_range(b, row);
   int first = 0x7fffffff, last = 0;
 #pragma unroll
-  for (int i = 0; i < NW / 2; ++i) {
+  for (int i = 0; i < KW / 2; ++i) {
     Reach part;
     part.init<64>(p.col_range(b, blk0 + i * 64 + lane));
     first = min(first, part.lo); last = max(last, part.hi);
@@ -749,8 +767,8 @@ __global__ __launch_bounds__(64 * MASK_WAVES, D == 64 && sizeof(T) == 2 ? 2 : 1)
   sc.init(p.scale, p.cap, p.slopes, h0);
   const float c = sc.unit();
   mask_arrived(kf);
-  mask_arrived(vf);
-  Spoilt<T, D> spoilt;
+  if constexpr (HALVES == 1) mask_arrived(vf);
+  Spoilt<T, D, NW> spoilt;
   spoilt.init(smem + RING * (STAGE + 512));
   mask_walk<2 * Copy::NC + 1, RING>(all, spoilt,
     [&](int t) LACT_INLINE_LAMBDA {
@@ -772,8 +790,8 @@ __global__ __launch_bounds__(64 * MASK_WAVES, D == 64 && sizeof(T) == 2 ? 2 : 1)
       const char* qt = smem + slot * STAGE;
       const char* gt = qt + S::BYTES;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int q0 = t0 + i * 32;
+      for (int part = 0; part < 2 / HALVES; ++part) {
+        const int i = HALVES == 1 ? part : half, q0 = t0 + i * 32;
         if (!reach.sees(q0, 32)) continue;
         f32x16 s, ds;
 #pragma unroll
@@ -781,7 +799,7 @@ __global__ __launch_bounds__(64 * MASK_WAVES, D == 64 && sizeof(T) == 2 ? 2 : 1)
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           s = mma32(fr.rows(qt, i, ks), kf[ks], s);
-          ds = mma32(fr.rows(gt, i, ks), vf[ks], ds);
+          ds = mma32(fr.rows(gt, i, ks), HALVES == 1 ? vf[HALVES == 1 ? ks : 0] : fr.rows(values + (group >> 1) * S::BYTES, group & 1, ks), ds);
         }
         const float* ls = reinterpret_cast<const float*>(stats + slot * 512) + i * 32 + 4 * (lane >> 5);
         const int at = q0 + 4 * (lane >> 5);
@@ -823,15 +841,43 @@ __global__ __launch_bounds__(64 * MASK_WAVES, D == 64 && sizeof(T) == 2 ? 2 : 1)
     });
   poison += __shfl_xor(poison, 32, 64);
   __syncthreads();
+  if constexpr (HALVES == 2) {      // the second half's sums to the first
+    float4* sums = reinterpret_cast<float4*>(smem) + group * 32 * 64 + lane;
+    float* spoils = reinterpret_cast<float*>(smem + KW * 32 * 1024) + group * 64 + lane;
+    if (half == 1) {
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          sums[(dt * 4 + g) * 64] = make_float4(ok[dt][4 * g], ok[dt][4 * g + 1], ok[dt][4 * g + 2], ok[dt][4 * g + 3]);
+          sums[(16 + dt * 4 + g) * 64] = make_float4(ov[dt][4 * g], ov[dt][4 * g + 1], ov[dt][4 * g + 2], ov[dt][4 * g + 3]);
+        }
+      *spoils = poison;
+    }
+    __syncthreads();
+    if (half == 0) {
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float4 a = sums[(dt * 4 + g) * 64], c = sums[(16 + dt * 4 + g) * 64];
+          ok[dt][4 * g] += a.x; ok[dt][4 * g + 1] += a.y; ok[dt][4 * g + 2] += a.z; ok[dt][4 * g + 3] += a.w;
+          ov[dt][4 * g] += c.x; ov[dt][4 * g + 1] += c.y; ov[dt][4 * g + 2] += c.z; ov[dt][4 * g + 3] += c.w;
+        }
+      poison += *spoils;
+    }
+    __syncthreads();
+    if (half == 1) return;
+  }
   const size_t o = ((size_t)b * L * p.HK + hk) * D, ld = (size_t)p.HK * D;
   if (splits > 1) {
-    float* stage = reinterpret_cast<float*>(smem) + wave * 32 * (D + 4);
+    float* stage = reinterpret_cast<float*>(smem) + group * 32 * (D + 4);
     const size_t all_keys = (size_t)p.B * L * ld, at = blockIdx.y * all_keys + o;
     mask_store_rows<float, D>(reinterpret_cast<char*>(stage), ok, p.scale + poison, p.part + at, ld, row0, L);
     mask_store_rows<float, D>(reinterpret_cast<char*>(stage), ov, 1.f + poison, p.part + splits * all_keys + at, ld, row0, L);
     return;
   }
-  char* stage = smem + wave * 32 * (D + 16 / sizeof(T)) * sizeof(T);
+  char* stage = smem + group * 32 * (D + 16 / sizeof(T)) * sizeof(T);
   mask_store_rows<T, D>(stage, ok, p.scale + poison, p.dk + o, ld, row0, L);
   mask_store_rows<T, D>(stage, ov, 1.f + poison, p.dv + o, ld, row0, L);
 }

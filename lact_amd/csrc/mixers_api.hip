@@ -84,8 +84,8 @@ template <int WHICH, typename T, int D, bool BENT>
 void launch_attention(int splits, MaskedAttnParams<T> p, hipStream_t s) {
   const int heads = p.B * (WHICH == 2 ? p.HK : p.H);
   p.by_heads = make_udiv(heads);
-  const dim3 grid(ceil_div(p.L, 32 * MASK_WAVES) * heads, splits), block(64 * MASK_WAVES);
-  constexpr int SM = mask_lds_bytes<T, D>(WHICH == 2);
+  const dim3 grid(ceil_div(p.L, 32 * MASK_WAVES) * heads, splits), block(64 * MASK_WAVES * (WHICH == 2 ? mask_halves<T, D, BENT>() : 1));
+  constexpr int SM = mask_lds_bytes<T, D, BENT>(WHICH == 2);
   const double w = p.window, f = 2.0 * ((double)p.L * w - w * (w - 1) / 2) * D * p.B * p.H;      // without documents
   if constexpr (WHICH == 0) {
     LACT_BIG_LDS((k_masked_attn_fwd<T, D, BENT>), SM);
