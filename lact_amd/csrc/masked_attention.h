@@ -252,23 +252,29 @@ struct Spoilt {
     if (threadIdx.x < 16) words[threadIdx.x] = 0;
     __syncthreads();
   }
+  __device__ __forceinline__ static bool bad(const uint4& u) {
+    if constexpr (sizeof(T) == 2) return unfinite(__builtin_bit_cast(bf16x8, u));
+    else return ((u.x & 0x7f800000u) == 0x7f800000u) | ((u.y & 0x7f800000u) == 0x7f800000u) | ((u.z & 0x7f800000u) == 0x7f800000u) | ((u.w & 0x7f800000u) == 0x7f800000u);
+  }
   __device__ __forceinline__ void look(char* tile, int slot, int wave) const {
+    constexpr int NC = S::G / NW;
     const int l = threadIdx.x & 63;
+    uint4 u[NC];
 #pragma unroll
-    for (int i = 0; i < S::G / NW; ++i) {
+    for (int i = 0; i < NC; ++i) u[i] = *reinterpret_cast<uint4*>(tile + (wave + i * NW) * 1024 + l * 16);
+    bool some = false;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) some |= bad(u[i]);
+    if (!__any(some)) return;
+#pragma unroll 1
+    for (int i = 0; i < NC; ++i) {
       uint4* at = reinterpret_cast<uint4*>(tile + (wave + i * NW) * 1024 + l * 16);
-      const uint4 u = *at;
-      bool bad;
-      if constexpr (sizeof(T) == 2) bad = unfinite(__builtin_bit_cast(bf16x8, u));
-      else bad = ((u.x & 0x7f800000u) == 0x7f800000u) | ((u.y & 0x7f800000u) == 0x7f800000u) | ((u.z & 0x7f800000u) == 0x7f800000u) | ((u.w & 0x7f800000u) == 0x7f800000u);
-      const uint64_t who = __ballot(bad);
-      if (who) {
-        const int in = l / S::G, row = (wave + i * NW) * (64 / S::G) + in;      // G lanes hold a row
-        if (who >> (in * S::G) & ((1ull << S::G) - 1)) {
-          *at = make_uint4(0, 0, 0, 0);
-          if (l % S::G == 0) atomicOr(words + 2 * slot + (row >> 5), 1u << (row & 31));
-          words[15] = 1;
-        }
+      const uint64_t who = __ballot(bad(*at));
+      const int in = l / S::G, row = (wave + i * NW) * (64 / S::G) + in;      // G lanes hold a row
+      if (who >> (in * S::G) & ((1ull << S::G) - 1)) {
+        *at = make_uint4(0, 0, 0, 0);
+        if (l % S::G == 0) atomicOr(words + 2 * slot + (row >> 5), 1u << (row & 31));
+        words[15] = 1;
       }
     }
   }
@@ -317,7 +323,10 @@ struct Scores {
     if constexpr (!BENT) return;
     if (cap) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) s[j] = bent(s[j]) * k2;
+      for (int j = 0; j < 16; ++j) {
+        if constexpr (sizeof(T) == 2) s[j] = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[j] * k1)), -2.f * k2, k2);
+        else s[j] = bent(s[j]) * k2;
+      }
     } else {
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[j] *= c;
