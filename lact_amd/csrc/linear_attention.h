@@ -24,6 +24,8 @@
 // A gradient of the decays adds what crosses a token (k_lin_decay_grad): pairs M_ij = e^(G_i - G_j) (q_i . k_j)(dout_i . v_j) scale of a source in front and an
 // output behind it, and the states' shares.
 #pragma once
+#include <type_traits>
+
 #include "masked_attention.h"
 
 namespace lact {
@@ -76,6 +78,17 @@ __device__ __forceinline__ bf16x8 lin_pack(const float (&v)[8], uint16_t) {
   return __builtin_bit_cast(bf16x8, make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])));
 }
 __device__ __forceinline__ f32x8 lin_pack(const float (&v)[8], float) { return f32x8{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}; }
+// Sum over 16 neighbouring lanes, without a way through LDS
+__device__ __forceinline__ float sum16(float v) {
+  auto turned = [](float x, auto by) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x120 + decltype(by)::value, 0xf, 0xf, false));      // row_ror
+  };
+  v += turned(v, std::integral_constant<int, 8>());
+  v += turned(v, std::integral_constant<int, 4>());
+  v += turned(v, std::integral_constant<int, 2>());
+  v += turned(v, std::integral_constant<int, 1>());
+  return v;
+}
 // Eight floats as PARTS operands whose sum they are, largest first; fp32 needs one.
 template <typename T, int PARTS>
 __device__ __forceinline__ void lin_split(float (&v)[8], typename AttnType<T>::Frag (&f)[PARTS]) {
@@ -233,13 +246,18 @@ struct LinState {        // columns [wave * DZ / 4, + DZ / 4): accumulator a, ro
         for (int j = 0; j < 8; ++j) x[j] = (float)zf[v][n][j] * weight[j];
         lin_split<T, PARTS>(x, zw[n]);
       }
+      auto rows = [&](int a) LACT_INLINE_LAMBDA { return LinFrag<T, DX>::template cols<8>(y, 32 * (a >> 1) + 4 * (a & 1), v); };
+      Frag yf[3];
+      yf[0] = rows(0);
+      yf[1] = rows(1);
 #pragma unroll
       for (int a = 0; a < AT; ++a) {
-        const Frag yf = LinFrag<T, DX>::template cols<8>(y, 32 * (a >> 1) + 4 * (a & 1), v);
+        if (a + 2 < AT) yf[(a + 2) % 3] = rows(a + 2);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int p = 0; p < PARTS; ++p)      // (products of one sum after another wait for each other)
 #pragma unroll
-          for (int p = 0; p < PARTS; ++p) s[a][n] = mma16(yf, zw[n][p], s[a][n]);
+          for (int n = 0; n < NT; ++n) s[a][n] = mma16(yf[a % 3], zw[n][p], s[a][n]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -307,8 +325,15 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
     const float4* lw = reinterpret_cast<const float4*>(x + Sh::STAGE - 1024);
     // Pairs of outputs [16 wave, +16) with their sources, [output][source] in LDS
     {
+      constexpr bool PAIRED = GATE && !REV;
       const float4 mine = lw[16 * wave + li];
       float rowsum = 0.f;
+      Frag xr[UX], wr[PAIRED ? UZ : 1];
+#pragma unroll
+      for (int u = 0; u < UX; ++u) xr[u] = FX::rows(x, wave, u);
+      if constexpr (PAIRED)
+#pragma unroll
+        for (int u = 0; u < UZ; ++u) wr[u] = FZ::rows(w, wave, u);
 #pragma unroll
       for (int jt = 0; jt < 4; ++jt) {
         const bool none = REV ? jt < wave : jt > wave;
@@ -318,11 +343,17 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
           f32x4 acc, other;
           lin_zero(acc);
           lin_zero(other);
+          Frag yf[UX], zr[PAIRED ? UZ : 1];
 #pragma unroll
-          for (int u = 0; u < UX; ++u) acc = mma16(FX::rows(y, jt, u), FX::rows(x, wave, u), acc);
-          if constexpr (GATE && !REV)
+          for (int u = 0; u < UX; ++u) yf[u] = FX::rows(y, jt, u);
+          if constexpr (PAIRED)
 #pragma unroll
-            for (int u = 0; u < UZ; ++u) other = mma16(FZ::rows(z, jt, u), FZ::rows(w, wave, u), other);
+            for (int u = 0; u < UZ; ++u) zr[u] = FZ::rows(z, jt, u);
+#pragma unroll
+          for (int u = 0; u < UX; ++u) acc = mma16(yf[u], xr[u], acc);
+          if constexpr (PAIRED)
+#pragma unroll
+            for (int u = 0; u < UZ; ++u) other = mma16(zr[u], wr[u], other);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int j = 16 * jt + 4 * c + r, o = 16 * wave + li;
@@ -340,8 +371,7 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
         if constexpr (GATE && !REV) {      // columns of M over the wave's outputs
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-#pragma unroll
-            for (int s = 1; s < 16; s <<= 1) m[r] += __shfl_xor(m[r], s, 64);
+            m[r] = sum16(m[r]);
             if (li == 0) sums[256 + wave * 64 + 16 * jt + 4 * c + r] = m[r];
           }
         }
@@ -365,23 +395,29 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
     for (int it = 0; it < 4; ++it)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) lin_zero(o[it][nt]);
+    {
+      // operands two steps ahead of the products: a wave waits for LDS longer than for them
+      Frag xf[3], sf[NT][SP];
+      xf[0] = FX::rows(x, 0, 0);
+      xf[1] = FX::rows(x, 1, 0);
 #pragma unroll
-    for (int u = 0; u < UX; ++u) {
-      Frag sf[NT][SP];
+      for (int e = 0; e < 4 * UX; ++e) {
+        const int u = e / 4, it = e % 4;
+        if (e + 2 < 4 * UX) xf[(e + 2) % 3] = FX::rows(x, (e + 2) % 4, (e + 2) / 4);
+        if (it == 0) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float v[8];
+          for (int nt = 0; nt < NT; ++nt) {
+            float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = st.s[2 * u + (j >> 2)][nt][j & 3];
-        lin_split<T, SP>(v, sf[nt]);
-      }
+            for (int j = 0; j < 8; ++j) v[j] = st.s[2 * u + (j >> 2)][nt][j & 3];
+            lin_split<T, SP>(v, sf[nt]);
+          }
+        }
 #pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const Frag xf = FX::rows(x, it, u);
+        for (int q = 0; q < SP; ++q)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int q = 0; q < SP; ++q) o[it][nt] = mma16(sf[nt][q], xf, o[it][nt]);
+          for (int nt = 0; nt < NT; ++nt) o[it][nt] = mma16(sf[nt][q], xf[e % 3], o[it][nt]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
 #pragma unroll
