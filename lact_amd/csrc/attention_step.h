@@ -157,7 +157,7 @@ __global__ __launch_bounds__((64 * AttnStepShape<T, D>::NW), 1) void k_attn_step
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
       for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-    float mc = -1e30f, sum = 0.f;
+    float mc = ATTN_LOWEST, sum = 0.f;
     mask_arrived(qf);
     // the wave's tiles: 32 keys from lo + (step * NW + wave) * 32 on
     const int tiles = min(step1 - step0, max(0, (len - lo - wave * 32 - step0 * A::KEYS + A::KEYS - 1) / A::KEYS));

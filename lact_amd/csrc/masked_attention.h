@@ -41,7 +41,8 @@ struct MaskedAttnParams {
   float* delta;                      // [B, H, L]: sum_d dout * out, written by dq, read by dk/dv
   T* dq; T* dk; T* dv;               // contiguous
   float* part;                       // [2][splits][B, L, HK, D]: dk and dv of every split, where there are several
-  UDiv by_heads, by_kv;              // B * (blocks' heads), B * HK
+  int splits;
+  UDiv by_heads, by_kv;              // blocks at one place of the sequence: B * H, or splits * B * HK; B * HK
   __device__ __forceinline__ void locate(int& x, int& z) const {
     x = by_heads.div(blockIdx.x);
     z = blockIdx.x - x * (int)by_heads.d;
@@ -113,6 +114,8 @@ __device__ __forceinline__ f32x16 mma32(const f32x8& a, const f32x8& b, f32x16 c
   return c;
 }
 
+// A row maximum before there is one: below every score that is finite, and 2^(-infinity - it) is 0.
+constexpr float ATTN_LOWEST = -3e38f;
 constexpr int MASK_WAVES = 4;     // of a block; two blocks of the forward and of dq to a compute unit
 
 template <typename T, int D>
@@ -246,7 +249,9 @@ template <typename T, int D, int NW = MASK_WAVES>
 struct Spoilt {
   using S = MaskTile<T, D>;
   static constexpr int BYTES = 64;
-  uint32_t* words;        // rows [0, 32) and [32, 64) of every ring slot; behind them whether there ever were any
+  // Rows [0, 32) and [32, 64) of tile t at its place of four (with as many places as a ring of two has, a wave may write down those of the next tile before
+  // they are cleared); the last word: whether there ever were any.
+  uint32_t* words;
   __device__ __forceinline__ void init(char* lds) {
     words = reinterpret_cast<uint32_t*>(lds);
     if (threadIdx.x < 16) words[threadIdx.x] = 0;
@@ -256,7 +261,7 @@ struct Spoilt {
     if constexpr (sizeof(T) == 2) return unfinite(__builtin_bit_cast(bf16x8, u));
     else return ((u.x & 0x7f800000u) == 0x7f800000u) | ((u.y & 0x7f800000u) == 0x7f800000u) | ((u.z & 0x7f800000u) == 0x7f800000u) | ((u.w & 0x7f800000u) == 0x7f800000u);
   }
-  __device__ __forceinline__ void look(char* tile, int slot, int wave) const {
+  __device__ __forceinline__ void look(char* tile, int t, int wave) const {
     constexpr int NC = S::G / NW;
     const int l = threadIdx.x & 63;
     uint4 u[NC];
@@ -273,17 +278,17 @@ struct Spoilt {
       const int in = l / S::G, row = (wave + i * NW) * (64 / S::G) + in;      // G lanes hold a row
       if (who >> (in * S::G) & ((1ull << S::G) - 1)) {
         *at = make_uint4(0, 0, 0, 0);
-        if (l % S::G == 0) atomicOr(words + 2 * slot + (row >> 5), 1u << (row & 31));
+        if (l % S::G == 0) atomicOr(words + 2 * (t & 3) + (row >> 5), 1u << (row & 31));
         words[15] = 1;
       }
     }
   }
-  // behind the barrier: the slot's rows; and room for those of the slot that the next copies go to.  (Read as LDS by its address space: through a generic
+  // behind the barrier: the tile's rows; and room for those of the tile after the next, which nobody looks over before the next barrier.  (Read as LDS by its address space: through a generic
   // pointer the load counts as one of global memory too, and its wait is one for the copies just issued.)
   __device__ __forceinline__ bool any() const { return __builtin_amdgcn_readfirstlane(lds_word(words + 15)) != 0; }
-  __device__ __forceinline__ uint64_t rows(int slot) const { return (uint64_t)words[2 * slot] | (uint64_t)words[2 * slot + 1] << 32; }
-  __device__ __forceinline__ void clear(int slot) const {
-    if (threadIdx.x < 2) words[2 * slot + threadIdx.x] = 0;
+  __device__ __forceinline__ uint64_t rows(int t) const { return (uint64_t)words[2 * (t & 3)] | (uint64_t)words[2 * (t & 3) + 1] << 32; }
+  __device__ __forceinline__ void clear_after_next(int t) const {
+    if (threadIdx.x < 2) words[2 * ((t + 2) & 3) + threadIdx.x] = 0;
   }
 };
 
@@ -369,13 +374,35 @@ struct Scores {
 template <typename T, int D, bool BENT> constexpr int mask_halves() { return sizeof(T) == 2 && D == 128 && !BENT ? 2 : 1; }
 // 64-row tiles of both operands in LDS
 template <typename T, int D> constexpr int mask_ring(bool keys) { return sizeof(T) == 4 || (D == 128 && !keys) ? 2 : 3; }
-template <typename T, int D, bool BENT>
-constexpr int mask_lds_bytes(bool stats) {
-  constexpr int NW = MASK_WAVES;
+// stats: of dk/dv; groups of 32 rows; halves: waves that share them
+template <typename T, int D>
+constexpr int mask_lds_bytes(bool stats, int groups, int halves) {
   const int R = mask_ring<T, D>(stats);
-  const int ring = R * 2 * MaskTile<T, D>::BYTES + (stats ? R * 512 + (mask_halves<T, D, BENT>() - 1) * 2 * MaskTile<T, D>::BYTES : 0) + Spoilt<T, D>::BYTES;
-  // what the rows are stored through, for splits in fp32
-  return cmax(ring, NW * 32 * cmax((D + 16 / (int)sizeof(T)) * (int)sizeof(T), stats ? (D + 4) * 4 : 0));
+  const int ring = R * 2 * MaskTile<T, D>::BYTES + (stats ? R * 512 + (halves - 1) * 2 * MaskTile<T, D>::BYTES : 0) + Spoilt<T, D>::BYTES;
+  // what the rows are stored through, for splits in fp32, and what one half of the waves gives to the other
+  const int store = groups * 32 * cmax((D + 16 / (int)sizeof(T)) * (int)sizeof(T), stats ? (D + 4) * 4 : 0);
+  return cmax(cmax(ring, store), (halves - 1) * groups * 64 * ((stats ? 2 : 1) * D * 2 + 8));
+}
+// The second half's accumulators to the first, through LDS: a wave's [N][4][64 lanes] float4.
+template <int N>
+__device__ __forceinline__ void mask_give(float4* at, const f32x16 (&acc)[N]) {
+#pragma unroll
+  for (int dt = 0; dt < N; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) at[(dt * 4 + g) * 64] = make_float4(acc[dt][4 * g], acc[dt][4 * g + 1], acc[dt][4 * g + 2], acc[dt][4 * g + 3]);
+}
+template <int N>      // acc mine + theirs other
+__device__ __forceinline__ void mask_take(const float4* at, f32x16 (&acc)[N], float mine, float theirs) {
+#pragma unroll
+  for (int dt = 0; dt < N; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float4 u = at[(dt * 4 + g) * 64];
+      acc[dt][4 * g] = fmaf(acc[dt][4 * g], mine, u.x * theirs);
+      acc[dt][4 * g + 1] = fmaf(acc[dt][4 * g + 1], mine, u.y * theirs);
+      acc[dt][4 * g + 2] = fmaf(acc[dt][4 * g + 2], mine, u.z * theirs);
+      acc[dt][4 * g + 3] = fmaf(acc[dt][4 * g + 3], mine, u.w * theirs);
+    }
 }
 
 // Walks the tiles [0, n): issue(t) starts the copies of tile t, COPIES of a wave, RING - 1 tiles ahead; look(t) sees the wave's own when they are there;
@@ -393,8 +420,8 @@ __device__ __forceinline__ void mask_walk(int n, const Sp& spoilt, Issue issue, 
     if (t + RING - 1 < n) issue(t + RING - 1);
     uint64_t rows = 0;
     if (spoilt.any()) {
-      rows = spoilt.rows(t % RING);
-      spoilt.clear((t + RING - 1) % RING);
+      rows = spoilt.rows(t);
+      spoilt.clear_after_next(t);
     }
     body(t, rows);
   }
@@ -474,28 +501,29 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-template <typename T, int D, bool BENT>
+template <typename T, int D, bool BENT, int HALVES>
 __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_fwd(const MaskedAttnParams<T> p) {
-  constexpr int NW = MASK_WAVES;
+  constexpr int NW = MASK_WAVES, KW = NW / HALVES, N = 2 / HALVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using S = MaskTile<T, D>;
-  using Copy = MaskCopy<T, D>;
+  using Copy = MaskCopy<T, D, NW>;
   using Frag = typename AttnType<T>::Frag;
   constexpr int STAGE = 2 * S::BYTES, RING = mask_ring<T, D>(false);
   prefetch_args<sizeof(p)>();
   int bx, z, b, h, hk;
   p.locate(bx, z);
-  bx = (p.L - 1) / (32 * NW) - bx;      // the longest rows of a causal mask first
+  bx = (p.L - 1) / (32 * KW) - bx;      // the longest rows of a causal mask first
   p.query_head(z, b, h, hk);
   const int L = p.L;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int blk0 = bx * 32 * NW, row0 = blk0 + wave * 32, row = row0 + (lane & 31);
+  const int group = wave % KW, half = wave / KW;        // of rows; of a tile's keys
+  const int blk0 = bx * 32 * KW, row0 = blk0 + group * 32, row = row0 + (lane & 31);
   Frag qf[D / 16];
   mask_own_rows<T, D>(qf, p.q + b * p.bsq + h * D, p.ldq, row, L);
   const int2 own = p.row_range(b, row);
   int first = 0x7fffffff, last = 0;
 #pragma unroll
-  for (int i = 0; i < NW / 2; ++i) {
+  for (int i = 0; i < KW / 2; ++i) {
     Reach part;
     part.init<64>(p.row_range(b, blk0 + i * 64 + lane));
     first = min(first, part.lo); last = max(last, part.hi);
@@ -512,14 +540,19 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
   const float c = sc.unit();
-  float mc = sc.bounded ? 0.f : -1e30f, sum = 0.f;        // running row maximum (of what 2^ is taken of) and this lane's share of the row sum
+  float mc = sc.bounded ? 0.f : ATTN_LOWEST, sum = 0.f;        // running row maximum (of what 2^ is taken of) and this lane's share of the row sum
+  // Without a cap or a distance the maximum is rounded where it is multiplied by c, the scores in fma are not: past 2^20 the difference would reach 2^(the rounding).
+  // Such rows subtract `high`, the maximum before the product.
+  constexpr float FAR = 1048576.f;
+  float high = ATTN_LOWEST;
+  bool far = false;
   first = min(first, L) / 64 * 64;
   const int tiles = last > first ? (last - first + 63) / 64 : 0;
   Copy ck, cv;
   ck.init(wave, p.k + b * p.bsk + hk * D, p.ldk, first, tiles, L);
   cv.init(wave, p.v + b * p.bsv + hk * D, p.ldv, first, tiles, L);
   const uint32_t lds0 = lds_addr(smem);
-  Spoilt<T, D> spoilt;
+  Spoilt<T, D, NW> spoilt;
   spoilt.init(smem + RING * STAGE);
   mask_arrived(qf);
   mask_walk<2 * Copy::NC, RING>(tiles, spoilt,
@@ -528,27 +561,27 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
       ck.issue(t, ck.base, slot, wave);
       cv.issue(t, cv.base, slot + S::BYTES, wave);
     },
-    [&](int t) LACT_INLINE_LAMBDA { spoilt.look(smem + t % RING * STAGE + S::BYTES, t % RING, wave); },
+    [&](int t) LACT_INLINE_LAMBDA { spoilt.look(smem + t % RING * STAGE + S::BYTES, t, wave); },
     [&](int t, uint64_t bad) LACT_INLINE_LAMBDA {
-      const int k0 = first + t * 64;
-      if (!reach.sees(k0, 64)) return;
+      const int k0 = first + t * 64 + 32 * half;
+      if (!reach.sees(k0, 32 * N)) return;
       const char* kt = smem + t % RING * STAGE;
       const char* vt = kt + S::BYTES;
-      f32x16 s[2];
+      f32x16 s[N];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[i][j] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < D / 16; ++ks)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) s[i] = mma32(fr.rows(kt, i, ks), qf[ks], s[i]);
+        for (int i = 0; i < N; ++i) s[i] = mma32(fr.rows(kt, i + half, ks), qf[ks], s[i]);
       const int at = k0 + 4 * (lane >> 5);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) sc.apply(s[i], at + 32 * i - row);
-      if (reach.masked(k0, 64)) {
+      for (int i = 0; i < N; ++i) sc.apply(s[i], at + 32 * i - row);
+      if (reach.masked(k0, 32 * N)) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < N; ++i) {
           const Seen seen(own.x - at - 32 * i, own.y - at - 32 * i);
 #pragma unroll
           for (int j = 0; j < 16; ++j) s[i][j] = seen.or_nothing(s[i][j], j);
@@ -556,21 +589,36 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
       }
       if (bad) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (Seen(own.x - at - 32 * i, own.y - at - 32 * i).any_of((uint32_t)(bad >> (32 * i)))) sum = __builtin_nanf("");
+        for (int i = 0; i < N; ++i)
+          if (Seen(own.x - at - 32 * i, own.y - at - 32 * i).any_of((uint32_t)(bad >> (32 * (i + half))))) sum = __builtin_nanf("");
       }
       // (a cap that bounds them saves the row maximum)
       if (!sc.bounded) {
-        float mx = s[0][0];
-        mx = max3(mx, s[1][0], s[1][1]);
+        float mx;
+        if constexpr (N == 2) {
+          mx = max3(s[0][0], s[1][0], s[1][1]);
 #pragma unroll
-        for (int j = 1; j < 16; ++j) mx = max3(mx, s[0][j], s[1][j]);
+          for (int j = 1; j < 16; ++j) mx = max3(mx, s[0][j], s[N - 1][j]);
+        } else {
+          mx = max3(s[0][0], s[0][1], s[0][15]);
+#pragma unroll
+          for (int j = 1; j < 8; ++j) mx = max3(mx, s[0][2 * j], s[0][2 * j + 1]);
+        }
+        const float top = mx;
         mx *= c;
         // The maximum only has to keep exp2 in range: it follows the row when it is exceeded by more than 2^8 (its own row only: what a row
         // gives does not depend on the others).
         if (__any(mx > mc + 8.f)) {
           mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-          const float nm = mx > mc + 8.f ? mx : mc, f = __builtin_amdgcn_exp2f(mc - nm);
+          const bool moves = mx > mc + 8.f;
+          const float nm = moves ? mx : mc;
+          float f = __builtin_amdgcn_exp2f(mc - nm);
+          if constexpr (!BENT) {
+            const float was = high;
+            high = moves ? fmaxf(top, __shfl_xor(top, 32, 64)) : high;
+            if (fabsf(nm) > FAR) f = __builtin_amdgcn_exp2f((was - high) * c);
+            far = __any(nm > FAR || (nm < -FAR && nm > ATTN_LOWEST));
+          }
           mc = nm;
           sum *= f;
 #pragma unroll
@@ -579,46 +627,75 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
             for (int j = 0; j < 16; ++j) o[i][j] *= f;
         }
       }
+      float base = mc;
+      if constexpr (!BENT)
+        if (far) {
+          const bool mine = fabsf(mc) > FAR;
+          base = mine ? 0.f : mc;
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[i][j] -= mine ? high : 0.f;
+        }
       float part[2] = {0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < N; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          s[i][j] = __builtin_amdgcn_exp2f(fmaf(s[i][j], c, -mc));
+          s[i][j] = __builtin_amdgcn_exp2f(fmaf(s[i][j], c, -base));
           part[i] += s[i][j];
         }
       sum += part[0] + part[1];
 #pragma unroll
-      for (int st = 0; st < 4; ++st) {
+      for (int st = 0; st < 2 * N; ++st) {
         const Frag pf = mask_pack<T>(s[st >> 1], st & 1);
 #pragma unroll
-        for (int dt = 0; dt < D / 32; ++dt) o[dt] = mma32(fr.cols(vt, dt, st), pf, o[dt]);
+        for (int dt = 0; dt < D / 32; ++dt) o[dt] = mma32(fr.cols(vt, dt, st + 2 * half), pf, o[dt]);
       }
     });
   sum += __shfl_xor(sum, 32, 64);
+  __syncthreads();
+  if constexpr (HALVES == 2) {
+    float4* theirs = reinterpret_cast<float4*>(smem) + group * (D / 32) * 256 + lane;
+    float2* stats = reinterpret_cast<float2*>(smem + KW * D * 128) + group * 64 + lane;
+    if (half == 1) {
+      mask_give(theirs, o);
+      *stats = make_float2(mc, sum);
+    }
+    __syncthreads();
+    if (half == 0) {
+      const float2 u = *stats;
+      const float m = fmaxf(mc, u.x), f = __builtin_amdgcn_exp2f(mc - m), e = __builtin_amdgcn_exp2f(u.x - m);
+      mask_take(theirs, o, f, e);
+      mc = m;
+      sum = fmaf(sum, f, u.y * e);
+    }
+    __syncthreads();
+    if (half == 1) return;
+  }
   const bool empty = own.x >= own.y;
   if (lane < 32 && row < L) p.lse[(size_t)(b * p.H + h) * L + row] = empty ? 0.f : mc + __builtin_amdgcn_logf(sum);   // v_log_f32 is base 2
-  __syncthreads();
-  mask_store_rows<T, D>(smem + wave * 32 * (D + 16 / sizeof(T)) * sizeof(T), o, empty ? 0.f : 1.f / sum, p.out + ((size_t)b * L * p.H + h) * D, (size_t)p.H * D, row0, L);
+  mask_store_rows<T, D>(smem + group * 32 * (D + 16 / sizeof(T)) * sizeof(T), o, empty ? 0.f : 1.f / sum, p.out + ((size_t)b * L * p.H + h) * D, (size_t)p.H * D, row0, L);
 }
 
 // dq = scale * sum_keys ds k with ds = p (dp - delta) f', and delta itself.
-template <typename T, int D, bool BENT>
+template <typename T, int D, bool BENT, int HALVES>
 __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_dq(const MaskedAttnParams<T> p) {
-  constexpr int NW = MASK_WAVES;
+  constexpr int NW = MASK_WAVES, KW = NW / HALVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using S = MaskTile<T, D>;
-  using Copy = MaskCopy<T, D>;
+  using Copy = MaskCopy<T, D, NW>;
   using Frag = typename AttnType<T>::Frag;
   constexpr int STAGE = 2 * S::BYTES, RING = mask_ring<T, D>(false);
   prefetch_args<sizeof(p)>();
   int bx, z, b, h, hk;
   p.locate(bx, z);
-  bx = (p.L - 1) / (32 * NW) - bx;
+  bx = (p.L - 1) / (32 * KW) - bx;
   p.query_head(z, b, h, hk);
   const int L = p.L;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int blk0 = bx * 32 * NW, row0 = blk0 + wave * 32, row = row0 + (lane & 31);
+  const int group = wave % KW, half = wave / KW;        // of rows; of a tile's keys
+  const int blk0 = bx * 32 * KW, row0 = blk0 + group * 32, row = row0 + (lane & 31);
   Frag qf[D / 16], gf[D / 16];
   mask_own_rows<T, D>(gf, p.dout + b * p.bsdo + h * D, p.lddo, row, L);
   float delta = 0.f;
@@ -632,13 +709,13 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
     delta += __shfl_xor(delta, 32, 64);
   }
   const size_t stat = (size_t)(b * p.H + h) * L;
-  if (lane < 32 && row < L) p.delta[stat + row] = delta;
+  if (half == 0 && lane < 32 && row < L) p.delta[stat + row] = delta;
   mask_own_rows<T, D>(qf, p.q + b * p.bsq + h * D, p.ldq, row, L);
   float lse = p.lse[stat + min(row, L - 1)];
   const int2 own = p.row_range(b, row);
   int first = 0x7fffffff, last = 0;
 #pragma unroll
-  for (int i = 0; i < NW / 2; ++i) {
+  for (int i = 0; i < KW / 2; ++i) {
     Reach part;
     part.init<64>(p.row_range(b, blk0 + i * 64 + lane));
     first = min(first, part.lo); last = max(last, part.hi);
@@ -664,7 +741,7 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
   mask_arrived(qf);
   mask_arrived(gf);
   asm volatile("" : "+v"(lse), "+v"(delta));
-  Spoilt<T, D> spoilt;
+  Spoilt<T, D, NW> spoilt;
   spoilt.init(smem + RING * STAGE);
   float poison = 0.f;
   mask_walk<2 * Copy::NC, RING>(tiles, spoilt,
@@ -673,13 +750,13 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
       ck.issue(t, ck.base, slot, wave);
       cv.issue(t, cv.base, slot + S::BYTES, wave);
     },
-    [&](int t) LACT_INLINE_LAMBDA { spoilt.look(smem + t % RING * STAGE, t % RING, wave); },
+    [&](int t) LACT_INLINE_LAMBDA { spoilt.look(smem + t % RING * STAGE, t, wave); },
     [&](int t, uint64_t bad) LACT_INLINE_LAMBDA {
       const char* kt = smem + t % RING * STAGE;
       const char* vt = kt + S::BYTES;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int k0 = first + t * 64 + 32 * i;
+      for (int part = 0; part < 2 / HALVES; ++part) {
+        const int i = HALVES == 1 ? part : half, k0 = first + t * 64 + 32 * i;
         if (!reach.sees(k0, 32)) continue;
         f32x16 s, dp;
 #pragma unroll
@@ -711,11 +788,27 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
     });
   poison += __shfl_xor(poison, 32, 64);
   __syncthreads();
-  mask_store_rows<T, D>(smem + wave * 32 * (D + 16 / sizeof(T)) * sizeof(T), o, p.scale + poison, p.dq + ((size_t)b * L * p.H + h) * D, (size_t)p.H * D, row0, L);
+  if constexpr (HALVES == 2) {
+    float4* theirs = reinterpret_cast<float4*>(smem) + group * (D / 32) * 256 + lane;
+    float* spoils = reinterpret_cast<float*>(smem + KW * D * 128) + group * 64 + lane;
+    if (half == 1) {
+      mask_give(theirs, o);
+      *spoils = poison;
+    }
+    __syncthreads();
+    if (half == 0) {
+      mask_take(theirs, o, 1.f, 1.f);
+      poison += *spoils;
+    }
+    __syncthreads();
+    if (half == 1) return;
+  }
+  mask_store_rows<T, D>(smem + group * 32 * (D + 16 / sizeof(T)) * sizeof(T), o, p.scale + poison, p.dq + ((size_t)b * L * p.H + h) * D, (size_t)p.H * D, row0, L);
 }
 
 // dv = sum_queries p dout, dk = scale * sum_queries ds q, over the queries of all heads that share the key head: a wave owns 32 keys and
-// walks the queries that see them, head after head.  With few keys (blocks) the walk is cut into gridDim.y splits, whose sums k_attn_sum adds.
+// walks the queries that see them, head after head.  With few keys (blocks) the walk is cut into splits, whose sums k_attn_sum adds; all splits of the first
+// keys, whose walks are the longest under a causal mask, come first.
 template <typename T, int D, bool BENT>
 __global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (sizeof(T) == 2 && (D == 64 || !BENT) ? 2 : 1)) void k_masked_attn_dkv(const MaskedAttnParams<T> p) {
   constexpr int KW = MASK_WAVES, HALVES = mask_halves<T, D, BENT>(), NW = KW * HALVES;
@@ -727,6 +820,8 @@ __global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (siz
   prefetch_args<sizeof(p)>();
   int bx, z;
   p.locate(bx, z);
+  const int split = p.by_kv.div(z);
+  z -= split * (int)p.by_kv.d;
   const int b = z / p.HK, hk = z - b * p.HK, L = p.L;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int group = wave % KW, half = wave / KW;        // of keys; of a tile's queries
@@ -761,7 +856,7 @@ __global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (siz
     for (int j = 0; j < 16; ++j) ok[i][j] = ov[i][j] = 0.f;
   first = min(first, L) / 64 * 64;
   const int tiles = last > first ? (last - first + 63) / 64 : 0, steps = tiles * p.group;
-  const int splits = gridDim.y, from = (int)((long long)steps * blockIdx.y / splits), all = (int)((long long)steps * (blockIdx.y + 1) / splits) - from;
+  const int splits = p.splits, from = (int)((long long)steps * split / splits), all = (int)((long long)steps * (split + 1) / splits) - from;
   const uint32_t lds0 = lds_addr(smem);
   const char* stats = smem + RING * STAGE;             // per ring slot: 64 lse, 64 delta
   const int h0 = hk * p.group;
@@ -789,8 +884,8 @@ __global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (siz
       if (++it == tiles) { it = 0; ++ih; }
     },
     [&](int t) LACT_INLINE_LAMBDA {
-      spoilt.look(smem + t % RING * STAGE, t % RING, wave);
-      spoilt.look(smem + t % RING * STAGE + S::BYTES, t % RING, wave);
+      spoilt.look(smem + t % RING * STAGE, t, wave);
+      spoilt.look(smem + t % RING * STAGE + S::BYTES, t, wave);
     },
     [&](int t, uint64_t bad) LACT_INLINE_LAMBDA {
       const int slot = t % RING, t0 = first + bt * 64;
@@ -849,30 +944,20 @@ __global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (siz
       }
     });
   poison += __shfl_xor(poison, 32, 64);
+  if constexpr (HALVES == 2) wait_vmcnt<0>();      // the values', which a walk without tiles has not waited for
   __syncthreads();
   if constexpr (HALVES == 2) {      // the second half's sums to the first
-    float4* sums = reinterpret_cast<float4*>(smem) + group * 32 * 64 + lane;
-    float* spoils = reinterpret_cast<float*>(smem + KW * 32 * 1024) + group * 64 + lane;
+    float4* theirs = reinterpret_cast<float4*>(smem) + group * 2 * (D / 32) * 256 + lane;
+    float* spoils = reinterpret_cast<float*>(smem + 2 * KW * D * 128) + group * 64 + lane;
     if (half == 1) {
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          sums[(dt * 4 + g) * 64] = make_float4(ok[dt][4 * g], ok[dt][4 * g + 1], ok[dt][4 * g + 2], ok[dt][4 * g + 3]);
-          sums[(16 + dt * 4 + g) * 64] = make_float4(ov[dt][4 * g], ov[dt][4 * g + 1], ov[dt][4 * g + 2], ov[dt][4 * g + 3]);
-        }
+      mask_give(theirs, ok);
+      mask_give(theirs + (D / 32) * 256, ov);
       *spoils = poison;
     }
     __syncthreads();
     if (half == 0) {
-#pragma unroll
-      for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float4 a = sums[(dt * 4 + g) * 64], c = sums[(16 + dt * 4 + g) * 64];
-          ok[dt][4 * g] += a.x; ok[dt][4 * g + 1] += a.y; ok[dt][4 * g + 2] += a.z; ok[dt][4 * g + 3] += a.w;
-          ov[dt][4 * g] += c.x; ov[dt][4 * g + 1] += c.y; ov[dt][4 * g + 2] += c.z; ov[dt][4 * g + 3] += c.w;
-        }
+      mask_take(theirs, ok, 1.f, 1.f);
+      mask_take(theirs + (D / 32) * 256, ov, 1.f, 1.f);
       poison += *spoils;
     }
     __syncthreads();
@@ -881,7 +966,7 @@ __global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (siz
   const size_t o = ((size_t)b * L * p.HK + hk) * D, ld = (size_t)p.HK * D;
   if (splits > 1) {
     float* stage = reinterpret_cast<float*>(smem) + group * 32 * (D + 4);
-    const size_t all_keys = (size_t)p.B * L * ld, at = blockIdx.y * all_keys + o;
+    const size_t all_keys = (size_t)p.B * L * ld, at = split * all_keys + o;
     mask_store_rows<float, D>(reinterpret_cast<char*>(stage), ok, p.scale + poison, p.part + at, ld, row0, L);
     mask_store_rows<float, D>(reinterpret_cast<char*>(stage), ov, 1.f + poison, p.part + splits * all_keys + at, ld, row0, L);
     return;

@@ -67,32 +67,35 @@ int attention_params(const lact_attention_desc_t* d, const void* q, const void* 
 }
 
 // Splits of the queries that a block of keys walks, where the blocks of 128 keys of all heads are fewer than the compute units: two blocks to a unit,
-// four tiles of 64 queries at least to a block.
+// four tiles of 64 queries at least to a block (in fp32, whose tiles take some eight times as long, one: 300 tokens, 48 / 19 us and 4 for the sums).
 int key_splits(const lact_attention_desc_t* d) {
   const long long blocks = (long long)ceil_div(d->L, 128) * d->B * d->HK;
   if (blocks >= COMPUTE_UNITS) return 1;
   const long long tiles = (long long)ceil_div(std::min(d->L, std::min(d->window, d->L) + 127), 64) * (d->H / d->HK);
-  return (int)std::max<long long>(1, std::min<long long>({2 * COMPUTE_UNITS / blocks, tiles / 4, 16}));
+  return (int)std::max<long long>(1, std::min<long long>({2 * COMPUTE_UNITS / blocks, tiles / (d->act_dtype == LACT_BF16 ? 4 : 1), 16}));
 }
 size_t attention_workspace(const lact_attention_desc_t* d) {
   const int n = key_splits(d);
   return n > 1 ? (size_t)2 * n * d->B * d->L * d->HK * d->D * sizeof(float) : 0;
 }
 
+// Whether two waves share 32 queries, each with half of the keys of every tile, in blocks of 64 queries: where those of 128 leave places of the compute units
+// (two blocks to a unit) empty, so that a block's walk is what the time is.  Blocks of 128 / 64 queries, forward and backward, us: 1 x 4096 tokens, 12 heads of
+// 128 (384 blocks of 128) 108 + 324 / 95 + 282; 300 tokens in fp32 (12) 36 + 97 / 20 + 75; but 15 heads and a window of 512 (480) 48 + 151 / 57 + 160.
+bool half_rows(long long blocks) { return blocks <= COMPUTE_UNITS * 3 / 2; }
+
 // WHICH: 0 forward, 1 dq, 2 dk and dv (in `splits`)
-template <int WHICH, typename T, int D, bool BENT>
-void launch_attention(int splits, MaskedAttnParams<T> p, hipStream_t s) {
-  const int heads = p.B * (WHICH == 2 ? p.HK : p.H);
-  p.by_heads = make_udiv(heads);
-  const dim3 grid(ceil_div(p.L, 32 * MASK_WAVES) * heads, splits), block(64 * MASK_WAVES * (WHICH == 2 ? mask_halves<T, D, BENT>() : 1));
-  constexpr int SM = mask_lds_bytes<T, D, BENT>(WHICH == 2);
+template <int WHICH, typename T, int D, bool BENT, int HALVES>
+void launch_attention(int splits, const MaskedAttnParams<T>& p, dim3 grid, hipStream_t s) {
+  const dim3 block(64 * MASK_WAVES * (WHICH == 2 ? HALVES : 1));
+  constexpr int SM = mask_lds_bytes<T, D>(WHICH == 2, MASK_WAVES / (WHICH == 2 ? 1 : HALVES), HALVES);
   const double w = p.window, f = 2.0 * ((double)p.L * w - w * (w - 1) / 2) * D * p.B * p.H;      // without documents
   if constexpr (WHICH == 0) {
-    LACT_BIG_LDS((k_masked_attn_fwd<T, D, BENT>), SM);
-    LACT_LAUNCH_SMEM("k_masked_attn_fwd", "masked_attn", 2 * f, (k_masked_attn_fwd<T, D, BENT>), grid, block, SM, s, p);
+    LACT_BIG_LDS((k_masked_attn_fwd<T, D, BENT, HALVES>), SM);
+    LACT_LAUNCH_SMEM("k_masked_attn_fwd", "masked_attn", 2 * f, (k_masked_attn_fwd<T, D, BENT, HALVES>), grid, block, SM, s, p);
   } else if constexpr (WHICH == 1) {
-    LACT_BIG_LDS((k_masked_attn_dq<T, D, BENT>), SM);
-    LACT_LAUNCH_SMEM("k_masked_attn_dq", "masked_attn_bwd", 3 * f, (k_masked_attn_dq<T, D, BENT>), grid, block, SM, s, p);
+    LACT_BIG_LDS((k_masked_attn_dq<T, D, BENT, HALVES>), SM);
+    LACT_LAUNCH_SMEM("k_masked_attn_dq", "masked_attn_bwd", 3 * f, (k_masked_attn_dq<T, D, BENT, HALVES>), grid, block, SM, s, p);
   } else {
     LACT_BIG_LDS((k_masked_attn_dkv<T, D, BENT>), SM);
     LACT_LAUNCH_SMEM("k_masked_attn_dkv", "masked_attn_bwd", 4 * f, (k_masked_attn_dkv<T, D, BENT>), grid, block, SM, s, p);
@@ -101,6 +104,16 @@ void launch_attention(int splits, MaskedAttnParams<T> p, hipStream_t s) {
       LACT_LAUNCH("k_attn_sum", "masked_attn_bwd", 0.0, (k_attn_sum<T>), dim3((unsigned)((n / 4 + 255) / 256), 2), dim3(256), s, n, splits, p.part, p.dk, p.dv);
     }
   }
+}
+template <int WHICH, typename T, int D, bool BENT>
+void launch_attention(int splits, MaskedAttnParams<T> p, hipStream_t s) {
+  const int heads = p.B * (WHICH == 2 ? p.HK * splits : p.H);
+  p.splits = splits;
+  p.by_heads = make_udiv(heads);
+  const dim3 grid(ceil_div(p.L, 32 * MASK_WAVES) * heads);
+  if constexpr (WHICH == 2) launch_attention<WHICH, T, D, BENT, mask_halves<T, D, BENT>()>(splits, p, grid, s);
+  else if (half_rows(grid.x)) launch_attention<WHICH, T, D, BENT, 2>(splits, p, dim3(ceil_div(p.L, 16 * MASK_WAVES) * heads), s);
+  else launch_attention<WHICH, T, D, BENT, 1>(splits, p, grid, s);
 }
 template <int WHICH, typename T>
 void launch_attention(int splits, int D, const MaskedAttnParams<T>& p, hipStream_t s) {

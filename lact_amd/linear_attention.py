@@ -41,7 +41,7 @@ def decayed_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     q, k, v = _autocast(q, k, v)
     s = _scale(name, scale, q.shape[3])
     if q.is_cuda and 0 in q.shape[:2] and q.shape[:3] == k.shape[:3] == v.shape[:3]:
-        out = v + (q.sum() + k.sum())
+        out = v + (q.sum() + k.sum() + log_decay.sum())      # (empty: the sums keep every operand in the graph)
         last = state if state is not None else torch.zeros(q.shape[0], q.shape[2], q.shape[3], v.shape[3], device=q.device)
         return (out, last.float().clone()) if return_state else out
     res = _lib.host().linear_attention(q, k, v, log_decay, state, s, bool(return_state))

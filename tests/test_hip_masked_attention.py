@@ -165,6 +165,54 @@ def test_future_values_reach_nothing_and_seen_ones_do(dtype):
 
 
 @BOTH
+@pytest.mark.parametrize("cap", [None, 25.0])
+@pytest.mark.parametrize("d", [64, 128])
+def test_values_that_are_not_finite_in_every_tile(d, cap, dtype):
+    """One token of every 64: the tokens whose windows hold it are NaN, in all of its heads, and the others what they are without."""
+    import lact_amd
+    print("[gpu-test] masked attention, a NaN in every tile", d, cap, dtype, flush=True)
+    l, hq, hkv, window = 1500, 4, 2, 9
+    packed, go = make(1, l, hq, hkv, d, dtype)
+    at = torch.arange(5, l, 61)
+    hit = torch.zeros(l, dtype=torch.bool)
+    for i in range(window):
+        hit[(at + i).clamp(max=l - 1)] = True
+    docs = torch.tensor([[0, l]], dtype=torch.int32, device="cuda")
+    results = []
+    for spoil in (False, True):
+        x = packed.clone()
+        if spoil:
+            x[:, at, hq * d:] = float("nan")         # keys and values
+        x = x.to("cuda").requires_grad_(True)
+        out = lact_amd.masked_window_attention(*parts(x, hq, hkv, d), window, score_cap=cap, documents=docs)
+        gx, = torch.autograd.grad(out, x, go.to("cuda"))
+        results.append((out.detach().cpu(), gx.cpu()))
+    (ref, gref), (out, gx) = results
+    assert bool(torch.isnan(out[:, hit]).all()) and torch.equal(out[:, ~hit], ref[:, ~hit])
+    q = slice(0, hq * d)
+    assert bool(torch.isnan(gx[:, hit, q]).all()) and torch.equal(gx[:, ~hit, q], gref[:, ~hit, q])
+    reached = torch.zeros(l, dtype=torch.bool)       # keys that a query with a NaN sees
+    for i in range(window):
+        reached[(torch.nonzero(hit)[:, 0] - i).clamp(min=0)] = True
+    assert bool(torch.isnan(gx[:, reached, hq * d:]).all()) and torch.equal(gx[:, ~reached, hq * d:], gref[:, ~reached, hq * d:])
+
+
+@BOTH
+def test_scores_far_below_zero(dtype):
+    """Scores of -1e36 and below are ordinary ones to the softmax: the largest of them has the weight."""
+    import lact_amd
+    l, h, d = 70, 2, 64
+    q, k = torch.full((1, l, h, d), -1e18), torch.full((1, l, h, d), 1e18)
+    k[:, 1:] *= 4.0
+    v = torch.randn(1, l, h, d, generator=torch.Generator().manual_seed(2))
+    q, k, v = (t.to(dtype).to("cuda") for t in (q, k, v))
+    out = lact_amd.masked_window_attention(q, k, v)
+    assert torch.equal(out, v[:, :1].expand_as(out))
+    lengths = torch.tensor([l], dtype=torch.int32, device="cuda")
+    assert torch.equal(lact_amd.window_attention_step(q[:, -1], k, v, lengths), v[:, 0])
+
+
+@BOTH
 def test_bounds_that_are_not_in_order_stay_inside(dtype):
     """Nobody checks the bounds: whatever they hold, no read leaves the sequence and no token outside is attended to."""
     import lact_amd
