@@ -54,7 +54,7 @@ template <typename T>
 struct LinParams {
   int B, L, H, segments, seg_chunks;     // chunks of a segment
   LinRows<T> x, y, z, w;                 // out_i = sum_j (x_i . y_j) z_j + x_i S, S += y_j z_j^T; w: see lin_walk
-  const float4* weights;                 // [B * H][chunks * 64], see k_lin_weights
+  const float* weights;                  // [B * H][chunks][4][64], see k_lin_weights
   float pair_scale, state_scale, source_scale;
   T* out;                                // [B, L, H, DZ]
   const float* states;                   // [segments][B * H][DX * DZ] (or transposed): where each segment starts, null: from zero
@@ -149,10 +149,11 @@ template <typename T, int D> struct LinFrag {
   }
 };
 
-// What the tokens of a chunk weigh, for every walk over it: the sum of log2 decays from the chunk's start in two floats, 2 to it (the weight of the
+// What the tokens of a chunk weigh, for every walk over it, 64 of each: the sum of log2 decays from the chunk's start in two floats, 2 to it (the weight of the
 // state in front in the token's output, forwards) and 2 to the rest of the chunk (the weight of the token in the state behind); both weights 0 past the
 // sequence's end.  One wave per chunk and head.
-__global__ __launch_bounds__(256) void k_lin_weights(int B, int L, int H, LinDecay decay, float4* weights) {
+enum { LIN_HI = 0, LIN_LO = 64, LIN_FRONT = 128, LIN_BEHIND = 192 };
+__global__ __launch_bounds__(256) void k_lin_weights(int B, int L, int H, LinDecay decay, float* weights) {
   const int chunks = (L + 63) / 64, lane = threadIdx.x & 63;
   const long long id = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (id >= (long long)B * H * chunks) return;
@@ -165,12 +166,16 @@ __global__ __launch_bounds__(256) void k_lin_weights(int B, int L, int H, LinDec
   }
   const double end = __shfl(s, 63, 64);
   const float hi = (float)s, lo = (float)(s - (double)hi);
-  weights[id * 64 + lane] = make_float4(hi, lo, t < L ? __builtin_amdgcn_exp2f(hi) : 0.f, t < L ? __builtin_amdgcn_exp2f((float)(end - s)) : 0.f);
+  float* to = weights + id * 256 + lane;
+  to[LIN_HI] = hi;
+  to[LIN_LO] = lo;
+  to[LIN_FRONT] = t < L ? __builtin_amdgcn_exp2f(hi) : 0.f;
+  to[LIN_BEHIND] = t < L ? __builtin_amdgcn_exp2f((float)(end - s)) : 0.f;
 }
 
 // 2^(later - earlier) of the sums of two tokens
-__device__ __forceinline__ float lin_between(const float4& later, const float4& earlier) {
-  return __builtin_amdgcn_exp2f((later.x - earlier.x) + (later.y - earlier.y));
+__device__ __forceinline__ float lin_between(float later_hi, float later_lo, float earlier_hi, float earlier_lo) {
+  return __builtin_amdgcn_exp2f((later_hi - earlier_hi) + (later_lo - earlier_lo));
 }
 
 template <typename T, int DX, int DZ, bool GATE>
@@ -226,8 +231,8 @@ struct LinState {        // columns [wave * DZ / 4, + DZ / 4): accumulator a, ro
   }
   // decays by `whole` and adds y^T (weight z); zf: the wave's columns of z
   template <bool REV, int PARTS, typename Frag>
-  __device__ __forceinline__ void update(const char* y, const Frag (&zf)[2][NT], const float4* w, float source_scale) {
-    const float whole = __builtin_amdgcn_exp2f(w[63].x + w[63].y);
+  __device__ __forceinline__ void update(const char* y, const Frag (&zf)[2][NT], const float* w, float source_scale) {
+    const float whole = __builtin_amdgcn_exp2f(w[LIN_HI + 63] + w[LIN_LO + 63]);
 #pragma unroll
     for (int a = 0; a < AT; ++a)
 #pragma unroll
@@ -235,10 +240,14 @@ struct LinState {        // columns [wave * DZ / 4, + DZ / 4): accumulator a, ro
     const int c = (threadIdx.x & 63) >> 4;
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
+      __builtin_amdgcn_sched_barrier(0);
       Frag zw[NT][PARTS];
       float weight[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) weight[j] = (REV ? w[32 * v + 8 * c + j].z : w[32 * v + 8 * c + j].w) * source_scale;
+      for (int j = 0; j < 8; j += 4) {
+        const float4 u = *reinterpret_cast<const float4*>(w + (REV ? LIN_FRONT : LIN_BEHIND) + 32 * v + 8 * c + j);
+        weight[j] = u.x * source_scale; weight[j + 1] = u.y * source_scale; weight[j + 2] = u.z * source_scale; weight[j + 3] = u.w * source_scale;
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float x[8];
@@ -295,7 +304,7 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
   float* sums = reinterpret_cast<float*>(pairs + Sh::PAIRS);
   int* spoilt = reinterpret_cast<int*>(pairs + Sh::PAIRS + Sh::SUMS);
   if (threadIdx.x == 0) *spoilt = 0;
-  const float4* weights = uniform(p.weights + (size_t)bh * chunks * 64);
+  const float* weights = uniform(p.weights + (size_t)bh * chunks * 256);
   const uint32_t lds0 = lds_addr(smem);
   auto token = [&](int i) { return (first + (REV ? n - 1 - i : i)) * 64; };
   auto issue = [&](int i) LACT_INLINE_LAMBDA {
@@ -305,7 +314,7 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
     lin_copy<T, DX>(p.y, b, h, t, L, to + Sh::X, wave);
     lin_copy<T, DZ>(p.z, b, h, t, L, to + 2 * Sh::X, wave);
     if (GATE) lin_copy<T, DZ>(p.w, b, h, t, L, to + 2 * Sh::X + Sh::Z, wave);
-    if (wave == 0) dma16<false>(weights + t, lane * 16, to + Sh::STAGE - 1024);
+    if (wave == 0) dma16<false>(weights + (long long)t * 4, lane * 16, to + Sh::STAGE - 1024);
   };
   St st;
   const float* start = p.states ? p.states + ((size_t)seg * p.B * p.H + bh) * (DX * DZ) : p.state0 ? p.state0 + (size_t)bh * (DX * DZ) : nullptr;
@@ -322,11 +331,11 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
     const char* y = x + Sh::X;
     const char* z = y + Sh::X;
     const char* w = z + Sh::Z;
-    const float4* lw = reinterpret_cast<const float4*>(x + Sh::STAGE - 1024);
+    const float* lw = reinterpret_cast<const float*>(x + Sh::STAGE - 1024);
     // Pairs of outputs [16 wave, +16) with their sources, [output][source] in LDS
     {
       constexpr bool PAIRED = GATE && !REV;
-      const float4 mine = lw[16 * wave + li];
+      const float my_hi = lw[LIN_HI + 16 * wave + li], my_lo = lw[LIN_LO + 16 * wave + li];
       float rowsum = 0.f;
       Frag xr[UX], wr[PAIRED ? UZ : 1];
 #pragma unroll
@@ -354,11 +363,12 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
           if constexpr (PAIRED)
 #pragma unroll
             for (int u = 0; u < UZ; ++u) other = mma16(zr[u], wr[u], other);
+          const float4 h4 = *reinterpret_cast<const float4*>(lw + LIN_HI + 16 * jt + 4 * c), l4 = *reinterpret_cast<const float4*>(lw + LIN_LO + 16 * jt + 4 * c);
+          const float hi[4] = {h4.x, h4.y, h4.z, h4.w}, lo[4] = {l4.x, l4.y, l4.z, l4.w};
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int j = 16 * jt + 4 * c + r, o = 16 * wave + li;
-            const float4 theirs = lw[j];
-            const float e = REV ? lin_between(theirs, mine) : lin_between(mine, theirs);
+            const float e = REV ? lin_between(hi[r], lo[r], my_hi, my_lo) : lin_between(my_hi, my_lo, hi[r], lo[r]);
             const bool on = (REV ? j >= o : j <= o) && t0 + max(j, o) < L;
             v[r] = on ? acc[r] * e * p.pair_scale : 0.f;
             if constexpr (GATE && !REV) {
@@ -422,7 +432,7 @@ __device__ __forceinline__ void lin_walk(const LinParams<T>& p, int item, char* 
     }
 #pragma unroll
     for (int it = 0; it < 4; ++it) {
-      const float e = (REV ? lw[16 * it + li].w : lw[16 * it + li].z) * p.state_scale;
+      const float e = lw[(REV ? LIN_BEHIND : LIN_FRONT) + 16 * it + li] * p.state_scale;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) o[it][nt] *= e;
       if constexpr (GATE) {
@@ -540,14 +550,14 @@ __global__ __launch_bounds__(256, lin_waves<T>()) void k_lin_segments(const LinP
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int count = p.segments - 1, seg = blockIdx.x % count + (REV ? 1 : 0), bh = blockIdx.x / count, b = p.by_heads.div(bh), h = bh - b * p.H;
   const int L = p.L, chunks = (L + 63) / 64, first = seg * p.seg_chunks, n = min(p.seg_chunks, chunks - first);
-  const float4* weights = uniform(p.weights + (size_t)bh * chunks * 64);
+  const float* weights = uniform(p.weights + (size_t)bh * chunks * 256);
   const uint32_t lds0 = lds_addr(smem);
   auto token = [&](int i) { return (first + (REV ? n - 1 - i : i)) * 64; };
   auto issue = [&](int i) LACT_INLINE_LAMBDA {
     const uint32_t to = lds0 + i % 2 * STAGE;
     lin_copy<T, DX>(p.y, b, h, token(i), L, to, wave);
     lin_copy<T, DZ>(p.z, b, h, token(i), L, to + MaskTile<T, DX>::BYTES, wave);
-    if (wave == 0) dma16<false>(weights + token(i), lane * 16, to + STAGE - 1024);
+    if (wave == 0) dma16<false>(weights + (long long)token(i) * 4, lane * 16, to + STAGE - 1024);
   };
   St st;
   st.zero();
@@ -559,14 +569,14 @@ __global__ __launch_bounds__(256, lin_waves<T>()) void k_lin_segments(const LinP
     if (i + 1 < n) issue(i + 1);
     const char* y = smem + i % 2 * STAGE;
     const char* z = y + MaskTile<T, DX>::BYTES;
-    const float4* lw = reinterpret_cast<const float4*>(y + STAGE - 1024);
+    const float* lw = reinterpret_cast<const float*>(y + STAGE - 1024);
     Frag zf[2][NT];
 #pragma unroll
     for (int v = 0; v < 2; ++v)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) zf[v][nt] = LinFrag<T, DZ>::template cols<4>(z, wave * (DZ / 4) + nt * 16, v);
     st.template update<REV, lin_parts<T>()>(y, zf, lw, p.source_scale);
-    total += (double)lw[63].x + (double)lw[63].y;
+    total += (double)lw[LIN_HI + 63] + (double)lw[LIN_LO + 63];
   }
   st.store(states + ((size_t)(seg + (REV ? -1 : 1)) * p.B * p.H + bh) * (DX * DZ), p.transposed, wave);
   if (threadIdx.x == 0) sums[(size_t)seg * p.B * p.H + bh] = (float)total;
@@ -599,7 +609,7 @@ __global__ __launch_bounds__(256) void k_lin_scan(int segments, long long matric
 // M's part is summed as rows minus columns from t on.  0 where the decay forgets everything.
 // Where the decay is the head's, the segment's sum instead, into part [segment][B * H].  states [segments][n]: the state in front of each segment; ends: the
 // gradient behind each (null with one segment); last, dlast: behind the last one (either null: no crossing).  One block per segment and head.
-__global__ __launch_bounds__(256) void k_lin_decay_grad(int B, int L, int H, int segments, int seg_tokens, int elems, const float4* weights, const float* up,
+__global__ __launch_bounds__(256) void k_lin_decay_grad(int B, int L, int H, int segments, int seg_tokens, int elems, const float* weights, const float* up,
                                                         const float* down, const float* states, const float* ends, const float* last, const float* dlast,
                                                         LinDecay decay, float* dg, double* part) {
   __shared__ double tail[16], source[16], sums[4];
@@ -623,7 +633,7 @@ __global__ __launch_bounds__(256) void k_lin_decay_grad(int B, int L, int H, int
   double run = (sums[0] + sums[1]) + (sums[2] + sums[3]), sum = 0.0;
   __syncthreads();
   const int first = seg * seg_tokens, end = min(L, first + seg_tokens);
-  const float4* ends_of = weights + ((size_t)bh * ((L + 63) / 64) + first / 64) * 64 + 63;
+  const float* ends_of = weights + ((size_t)bh * ((L + 63) / 64) + first / 64) * 256 + 63;
   // sixteen chunks at a time, the latest first, four to a wave; lane 0 holds a chunk's latest token
   for (int c0 = (end - first - 1) / 64; c0 >= 0; c0 -= 16) {
     double v[4], from[4], pairs[4];      // a - b, b, M
@@ -636,8 +646,7 @@ __global__ __launch_bounds__(256) void k_lin_decay_grad(int B, int L, int H, int
       v[k] = on ? (double)up[at] - from[k] : 0.0;
       pairs[k] = on ? (double)up[at + (size_t)B * H * L] : 0.0;
       if (lane == 0 && c >= 0) {
-        const float4 w = ends_of[c * 64];
-        cut[wave * 4 + k] = w.x + w.y < -30.f;
+        cut[wave * 4 + k] = ends_of[(size_t)c * 256 + LIN_HI] + ends_of[(size_t)c * 256 + LIN_LO] < -30.f;
       }
     }
 #pragma unroll

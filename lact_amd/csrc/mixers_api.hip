@@ -250,7 +250,7 @@ LinParams<T> lin_params(const lact_linear_desc_t* d, const char* states) {
   memset(&p, 0, sizeof(p));
   const LinCut cut = lin_cut(d);
   p.B = d->b; p.L = d->l; p.H = d->h; p.segments = cut.segments; p.seg_chunks = cut.chunks;
-  p.weights = reinterpret_cast<const float4*>(states + lin_buffers(d).weights);
+  p.weights = reinterpret_cast<const float*>(states + lin_buffers(d).weights);
   p.by_heads = make_udiv(d->h);
   return p;
 }
@@ -278,7 +278,7 @@ int lin_forward(const lact_linear_desc_t* d, const void* q, const void* k, const
   p.out = static_cast<T*>(out); p.last = last;
   const int heads = d->b * d->h;
   LACT_LAUNCH("k_lin_weights", "linear_attn", 0.0, k_lin_weights, dim3((unsigned)(((long long)heads * ceil_div(d->l, LIN_CHUNK) + 3) / 4)), dim3(256), s, d->b, d->l, d->h,
-              (LinDecay{g, d->decay_per_token}), const_cast<float4*>(p.weights));
+              (LinDecay{g, d->decay_per_token}), const_cast<float*>(p.weights));
   if (p.segments > 1) {
     float* at = reinterpret_cast<float*>(states + buf.states);
     lin_segments<T, DK, DV, false>(p, state, at, reinterpret_cast<float*>(states + buf.sums), s);
