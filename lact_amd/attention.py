@@ -75,7 +75,8 @@ def masked_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, w
     What is not finite makes NaN of the heads of all tokens that see it, in every element (a key whose score is -infinity only of gradients).
 
     Differentiable in q, k and v, once.  The gradients use a row's log2 of its sum of 2^scores in fp32: they have lost 2^-24 of its size, and all digits
-    at scores past 2^20.  Under autocast the operands are cast to its type."""
+    at scores past 2^20.  Under autocast the operands are cast to its type.  While a stream is captured, leaves that a graph made on the default stream still
+    holds are refused."""
     name = "masked_window_attention"
     _plain_only(name, q, k, v, distance_slopes, documents, prefixes)
     _dims(name, 4, q=q, k=k, v=v)

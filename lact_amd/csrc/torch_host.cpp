@@ -3,9 +3,11 @@
 // call (one view rendered, one short sequence) is bound by this code: the same steps in Python cost 65 us of host time per
 // forward call and made the GPU wait.  All arithmetic stays behind the C ABI (include/lact_hip.h).
 #include <torch/extension.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <ATen/MemoryOverlap.h>
 #include <ATen/autocast_mode.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -13,6 +15,7 @@
 #include <memory>
 #include <optional>
 #include <string>
+#include <unordered_set>
 #include <utility>
 #include <vector>
 
@@ -654,6 +657,26 @@ Tensor indices(const OptTensor& t, const Tensor& like, at::IntArrayRef shape, co
   return t->to(at::kInt).contiguous();
 }
 
+// A leaf's node belongs to the stream on which the first graph that holds the leaf was made, and a backward waits for that stream.  The default stream cannot
+// be part of a capture, and the error of such a wait, raised inside autograd's threads, ends the process: a captured call refuses leaves that a graph made
+// there still holds.
+void refuse_leaves_of_eager_graphs(std::initializer_list<const Tensor*> ts) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  std::vector<std::shared_ptr<torch::autograd::Node>> todo;
+  std::unordered_set<const torch::autograd::Node*> seen;
+  for (const Tensor* t : ts)
+    if (t && t->defined() && t->requires_grad()) todo.push_back(t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t));
+  while (!todo.empty()) {
+    const auto node = todo.back();
+    todo.pop_back();
+    if (!node || !seen.insert(node.get()).second) continue;
+    const auto on = node->stream();
+    if (dynamic_cast<const torch::autograd::AccumulateGrad*>(node.get()) && on && on->id() == 0)
+      throw std::runtime_error("a captured call needs leaves that no graph made on the default stream holds: free that graph (its outputs) first, or detach the leaves");
+    for (const auto& e : node->next_edges()) todo.push_back(e.function);
+  }
+}
+
 struct AttentionCall {      // what a forward hands to its backward
   lact_attention_desc_t desc{};
   Tensor q, k, v, out, lse, ranges, slopes;
@@ -900,16 +923,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("masked_attention", [](const Tensor& q, const Tensor& k, const Tensor& v, int64_t window, double scale, double cap, const OptTensor& slopes,
                                const OptTensor& documents, const OptTensor& prefixes) {
     const py::gil_scoped_release nogil;
-    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) {
+      refuse_leaves_of_eager_graphs({&q, &k, &v});
       return AttentionFn::apply(q, k, v, window, scale, cap, slopes, documents, prefixes);
+    }
     const at::AutoGradMode off(false);
     return attention_forward(q, k, v, window, scale, cap, slopes, documents, prefixes).out;
   });
   m.def("attention_step", &attention_step, py::call_guard<py::gil_scoped_release>());
   m.def("linear_attention", [](const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const OptTensor& state, double scale, bool return_state) {
     const py::gil_scoped_release nogil;
-    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || g.requires_grad() || wants_grad(state)))
+    if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || g.requires_grad() || wants_grad(state))) {
+      refuse_leaves_of_eager_graphs({&q, &k, &v, &g, state ? &*state : nullptr});
       return LinearAttentionFn::apply(q, k, v, g, state, scale, return_state);
+    }
     const at::AutoGradMode off(false);
     auto c = linear_forward(q, k, v, g, state, scale, return_state);
     return return_state ? variable_list{c.out, c.last} : variable_list{c.out};

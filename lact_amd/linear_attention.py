@@ -32,7 +32,8 @@ def decayed_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     state: [b, h, dk, dv] fp32, S in front of the first token; None: zero.   return_state: also return S behind the last token, fp32.
     scale: 1 / sqrt(dk) if None.
 
-    Differentiable in q, k, v, log_decay and state, once.  Under autocast q, k and v are cast to its type."""
+    Differentiable in q, k, v, log_decay and state, once.  Under autocast q, k and v are cast to its type.  While a stream is captured, leaves that a
+    graph made on the default stream still holds are refused."""
     name = "decayed_linear_attention"
     _plain_only(name, q, k, v, log_decay, state)
     _dims(name, 4, q=q, k=k, v=v, state=state)

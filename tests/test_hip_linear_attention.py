@@ -210,6 +210,28 @@ def test_captured_training_step():
             assert torch.equal(a, r), i
 
 
+def test_capture_refuses_leaves_that_an_eager_graph_holds():
+    import lact_amd
+    x, go, _ = make(1, 100, 2, 64, 64, torch.bfloat16, "token", state=False)
+    leaves = {n: t.to("cuda").requires_grad_(n == "log_decay") for n, t in x.items() if t is not None}
+    out = lact_amd.decayed_linear_attention(**leaves)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="default stream"), torch.cuda.graph(graph):
+        lact_amd.decayed_linear_attention(**leaves)
+    assert torch.equal(out, lact_amd.decayed_linear_attention(**leaves))
+
+
+def test_empty_sequences_keep_every_operand_in_the_graph():
+    import lact_amd
+    q = torch.zeros(2, 0, 3, 64, device="cuda", requires_grad=True)
+    g, s = torch.zeros(3, device="cuda", requires_grad=True), torch.randn(2, 3, 64, 64, device="cuda", requires_grad=True)
+    out, last = lact_amd.decayed_linear_attention(q, q, q, g, state=s, return_state=True)
+    assert out.shape == (2, 0, 3, 64) and torch.equal(last, s)
+    dq, dg, ds = torch.autograd.grad((out, last), (q, g, s), (torch.zeros_like(out), torch.ones_like(last)))
+    assert dq.shape == q.shape and not dg.any() and bool((ds == 1).all())
+
+
 # ---- single tokens
 
 @BOTH

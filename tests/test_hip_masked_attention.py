@@ -303,6 +303,30 @@ def test_captured_training_step(dtype):
             assert torch.equal(a, r), i
 
 
+def test_capture_refuses_leaves_that_an_eager_graph_holds():
+    """Their nodes belong to the default stream, which a captured backward would wait for.  Without the eager graph the same leaves are captured."""
+    import lact_amd
+    leaf = torch.randn(1, 70, 6, 64, device="cuda").bfloat16().requires_grad_(True)
+    go = torch.randn(1, 70, 2, 64, device="cuda").bfloat16()
+    f = lambda: lact_amd.masked_window_attention(leaf[:, :, :2], leaf[:, :, 2:4], leaf[:, :, 4:], 20)  # noqa: E731
+    out = f()
+    ref, = torch.autograd.grad(out, leaf, go, retain_graph=True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="default stream"), torch.cuda.graph(graph):
+        f()
+    with torch.no_grad():
+        assert torch.equal(f(), out)
+    del out
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        g, = torch.autograd.grad(f(), leaf, go)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(g, ref)
+
+
 def test_other_streams_give_the_same():
     import lact_amd
     q, k, v = (torch.randn(1, 300, n, 128, device="cuda").bfloat16() for n in (8, 2, 2))
