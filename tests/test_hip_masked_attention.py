@@ -108,8 +108,16 @@ def test_capped_scores_and_distance(cap, slopes, scale, d, dtype):
 
 
 @pytest.mark.parametrize("b,l,hq,hkv,d,window", [(2, 1030, 26, 26, 128, 256), (1, 1100, 64, 64, 64, 300), (2, 520, 64, 16, 128, None)])
-def test_blocks_of_256_rows(b, l, hq, hkv, d, window):
+def test_many_blocks(b, l, hq, hkv, d, window):
     check(b, l, hq, hkv, d, torch.bfloat16, window, documents=[[0, 200, l - 3]] * b)
+
+
+@BOTH
+@pytest.mark.parametrize("cap,slopes", [(None, False), (25.0, False), (None, True)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_heads(d, cap, slopes, dtype):
+    """More blocks of 128 queries than the compute units hold at once, of few tokens: a wave has its queries for itself."""
+    check(2, 140, 160, 32, d, dtype, 90, cap, slopes, documents=[[0, 70, 70, 140], [3, 50, 100, 130]], prefixes=[[20, 0, 0], [0, 9, 30]])
 
 
 @BOTH
@@ -167,11 +175,12 @@ def test_future_values_reach_nothing_and_seen_ones_do(dtype):
 @BOTH
 @pytest.mark.parametrize("cap", [None, 25.0])
 @pytest.mark.parametrize("d", [64, 128])
-def test_values_that_are_not_finite_in_every_tile(d, cap, dtype):
+@pytest.mark.parametrize("hq,hkv", [(4, 2), (36, 36)])
+def test_values_that_are_not_finite_in_every_tile(hq, hkv, d, cap, dtype):
     """One token of every 64: the tokens whose windows hold it are NaN, in all of its heads, and the others what they are without."""
     import lact_amd
-    print("[gpu-test] masked attention, a NaN in every tile", d, cap, dtype, flush=True)
-    l, hq, hkv, window = 1500, 4, 2, 9
+    print("[gpu-test] masked attention, a NaN in every tile", hq, d, cap, dtype, flush=True)
+    l, window = 1500, 9
     packed, go = make(1, l, hq, hkv, d, dtype)
     at = torch.arange(5, l, 61)
     hit = torch.zeros(l, dtype=torch.bool)
