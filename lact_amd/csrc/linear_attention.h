@@ -612,12 +612,12 @@ __global__ __launch_bounds__(256) void k_lin_scan(int segments, long long matric
 //   dg_t = sum_(i >= t > j) M_ij + sum_(i >= t) a_i + sum_(j < t) b_j + e^G <dS, S>;
 // the last term is X - sum b with X the crossing at the chunk's end, or nothing where the whole chunk's decay G leaves less than 2^-30: no rounding of a large
 // crossing is then carried to tokens that it does not reach.  X of the chunk before is the last term + sum a; of a segment's last chunk, <dS, S> there.
-// M's part is summed as rows minus columns from t on.  0 where the decay forgets everything.
+// M's part is summed as rows minus columns from t on.  0 where the decay forgets everything, and where there is nothing in front to forget.
 // Where the decay is the head's, the segment's sum instead, into part [segment][B * H].  states [segments][n]: the state in front of each segment; ends: the
 // gradient behind each (null with one segment); last, dlast: behind the last one (either null: no crossing).  One block per segment and head.
 __global__ __launch_bounds__(256) void k_lin_decay_grad(int B, int L, int H, int segments, int seg_tokens, int elems, const float* weights, const float* up,
                                                         const float* down, const float* states, const float* ends, const float* last, const float* dlast,
-                                                        LinDecay decay, float* dg, double* part) {
+                                                        LinDecay decay, int from_zero, float* dg, double* part) {
   __shared__ double tail[16], source[16], sums[4];
   __shared__ int cut[16];
   const int seg = blockIdx.x % segments, bh = blockIdx.x / segments, b = bh / H, h = bh - b * H, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -684,7 +684,7 @@ __global__ __launch_bounds__(256) void k_lin_decay_grad(int B, int L, int H, int
     for (int k = 0; k < 4; ++k) {
       const int c = c0 - wave * 4 - k, t = first + c * 64 + 63 - lane;
       if (c >= 0 && t < end) {
-        const double x = decay.at(b, t, h, L, H) <= LIN_MIN_LOG ? 0.0 : base[k] + v[k] + pairs[k];
+        const double x = decay.at(b, t, h, L, H) <= LIN_MIN_LOG || (from_zero && t == 0) ? 0.0 : base[k] + v[k] + pairs[k];
         if (decay.per_token) dg[((size_t)b * L + t) * H + h] = (float)x;
         else sum += x;
       }

@@ -62,6 +62,8 @@ struct MaskedAttnParams {
     }
     return make_int2(max(0, i - window + 1), i + 1);
   }
+  // A row sees itself: of one key, its softmax is constant, and the scores' gradients are 0 (dp - delta would leave what the two sums round differently).
+  __device__ __forceinline__ static bool alone(int2 r) { return r.y - r.x == 1; }
   __device__ __forceinline__ int2 col_range(int b, int j) const {
     if (j >= L) return make_int2(0x7fffffff, 0);
     if (cols) {
@@ -808,13 +810,13 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
     __syncthreads();
     if (half == 1) return;
   }
-  mask_store_rows<T, D>(smem + group * 32 * (D + 16 / sizeof(T)) * sizeof(T), o, p.scale + poison, p.dq + ((size_t)b * L * p.H + h) * D, (size_t)p.H * D, row0, L);
+  mask_store_rows<T, D>(smem + group * 32 * (D + 16 / sizeof(T)) * sizeof(T), o, (p.alone(own) ? 0.f : p.scale) + poison, p.dq + ((size_t)b * L * p.H + h) * D, (size_t)p.H * D, row0, L);
 }
 
 // dv = sum_queries p dout, dk = scale * sum_queries ds q, over the queries of all heads that share the key head: a wave owns 32 keys and
 // walks the queries that see them, head after head.  With few keys (blocks) the walk is cut into splits, whose sums k_attn_sum adds; all splits of the first
 // keys, whose walks are the longest under a causal mask, come first.  (dq is not formed here as well: its sums over keys would be atomics, in no order.)
-// 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 114 us, bound as the outputs are and by LDS, which both operands are read from in both directions.
+// 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 117 us, bound as the outputs are and by LDS, which both operands are read from in both directions.
 template <typename T, int D, bool BENT>
 __global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (sizeof(T) == 2 && (D == 64 || !BENT) ? 2 : 1)) void k_masked_attn_dkv(const MaskedAttnParams<T> p) {
   constexpr int KW = MASK_WAVES, HALVES = mask_halves<T, D, BENT>(), NW = KW * HALVES;
@@ -844,6 +846,7 @@ __global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (siz
     for (int i = 0; i < n; ++i) cv.issue(i, cv.base, lds_addr(values) + i * S::BYTES, wave);
   }
   const int2 own = p.col_range(b, row);
+  const bool alone = p.alone(p.row_range(b, row));
   int first = 0x7fffffff, last = 0;
 #pragma unroll
   for (int i = 0; i < KW / 2; ++i) {
@@ -930,12 +933,13 @@ __global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (siz
           }
         }
         if (reach.masked(q0, 32)) {
-          const Seen seen(own.x - at, own.y - at);
+          Seen seen(own.x - at, own.y - at);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            s[j] = seen.or_zero(s[j], j);
-            ds[j] = seen.or_zero(ds[j], j);
-          }
+          for (int j = 0; j < 16; ++j) s[j] = seen.or_zero(s[j], j);
+          // (a query that sees its own key alone lies at an end of this key's interval, so that the tile is masked)
+          if (alone && (uint32_t)(row - at) < 32) seen.bits &= ~(1u << (row - at));
+#pragma unroll
+          for (int j = 0; j < 16; ++j) ds[j] = seen.or_zero(ds[j], j);
         }
         if (bad && Seen(own.x - at, own.y - at).any_of((uint32_t)(bad >> (32 * i)))) poison = __builtin_nanf("");
 #pragma unroll

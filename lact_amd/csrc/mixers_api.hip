@@ -340,7 +340,7 @@ int lin_backward(const lact_linear_desc_t* d, const void* q, const void* k, cons
   if (dg) {
     double* part = reinterpret_cast<double*>(scratch + buf.part);
     LACT_LAUNCH("k_lin_decay_grad", "linear_attn_bwd", 0.0, k_lin_decay_grad, dim3(base.segments * heads), dim3(256), s, d->b, d->l, d->h, base.segments,
-                base.seg_chunks * LIN_CHUNK, DK * DV, base.weights, up, down, starts, ends, last, dlast, (LinDecay{g, d->decay_per_token}), dg, part);
+                base.seg_chunks * LIN_CHUNK, DK * DV, base.weights, up, down, starts, ends, last, dlast, (LinDecay{g, d->decay_per_token}), state == nullptr, dg, part);
     if (!d->decay_per_token)
       LACT_LAUNCH("k_lin_decay_sum", "linear_attn_bwd", 0.0, k_lin_decay_sum, dim3(d->h), dim3(64), s, base.segments * d->b, d->h, part, dg);
   }

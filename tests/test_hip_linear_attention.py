@@ -222,6 +222,18 @@ def test_capture_refuses_leaves_that_an_eager_graph_holds():
     assert torch.equal(out, lact_amd.decayed_linear_attention(**leaves))
 
 
+@BOTH
+@pytest.mark.parametrize("l", [1, 130])
+def test_nothing_in_front_has_no_gradient_of_its_decay(l, dtype):
+    """Without a state in front, the first token's decay has nothing to act on."""
+    import lact_amd
+    x, go, gs = make(2, l, 2, 64, 128, dtype, "token", state=False)
+    x = {n: t.to("cuda").requires_grad_(True) for n, t in x.items() if t is not None}
+    res = lact_amd.decayed_linear_attention(**x, return_state=True)
+    dg, = torch.autograd.grad(res, x["log_decay"], [go.to("cuda"), torch.randn(2, 2, 64, 128, device="cuda")])
+    assert not dg[:, 0].any() and (l == 1 or bool(dg[:, 1:].all()))
+
+
 def test_empty_sequences_keep_every_operand_in_the_graph():
     import lact_amd
     q = torch.zeros(2, 0, 3, 64, device="cuda", requires_grad=True)

@@ -207,6 +207,38 @@ def test_values_that_are_not_finite_in_every_tile(hq, hkv, d, cap, dtype):
 
 
 @BOTH
+@pytest.mark.parametrize("cap,slopes", [(None, False), (20.0, False), (None, True)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_single_key_has_no_gradient_of_scores(d, cap, slopes, dtype):
+    """A window of one token, and documents of one: the softmax is constant, dq and dk are 0 and dv is the output's gradient."""
+    import lact_amd
+    print("[gpu-test] masked attention, one key", d, cap, slopes, dtype, flush=True)
+    l, h = 200, 3
+    packed, go = make(1, l, h, h, d, dtype)
+    sl = torch.tensor([0.5, 0.25, 0.1], device="cuda") if slopes else None
+    bounds = [0] + list(range(1, 65)) + [130, 131, 162, 163, 200]      # single tokens, and longer documents that start with one
+    for window, docs in ((1, None), (1, bounds), (None, bounds)):
+        x = packed.to("cuda").requires_grad_(True)
+        documents = None if docs is None else torch.tensor([docs], dtype=torch.int32, device="cuda")
+        out = lact_amd.masked_window_attention(*parts(x, h, h, d), window, score_cap=cap, distance_slopes=sl, documents=documents)
+        g, = torch.autograd.grad(out, x, go.to("cuda"))
+        q, k, v = (t[0] for t in parts(g, h, h, d))
+        single = torch.ones(l, dtype=torch.bool)
+        if window is None:
+            single[64:] = False
+            single[[130, 162]] = True
+            assert bool(k[64:130].any())
+            single[64] = single[131] = single[163] = False
+        alone = single.to("cuda")
+        assert not q[alone].any()
+        only = alone if window == 1 else torch.arange(l, device="cuda") < 64      # keys that nobody else sees either
+        assert not k[only].any()
+        tol = torch.finfo(dtype).eps * 4      # p / sum, rounded to the type, and the gradient
+        ref = go.to("cuda")[0, only].float()
+        assert float((v[only].float() - ref).abs().max()) <= tol * float(ref.abs().max())
+
+
+@BOTH
 def test_scores_far_below_zero(dtype):
     """Scores of -1e36 and below are ordinary ones to the softmax: the largest of them has the weight."""
     import lact_amd
