@@ -589,21 +589,31 @@ __global__ __launch_bounds__(256, lin_waves<T>()) void k_lin_segments(const LinP
 }
 
 // entry[s + 1] += 2^sums[s] entry[s] from entry[0] = initial on, or (reverse) entry[s - 1] += 2^sums[s] entry[s] from the last on; a
-// thread has four elements of one matrix.
+// thread has four elements of one matrix, and reads eight entries ahead: nothing but the sum depends on the one before (32
+// entries of 16 matrices of 64 x 128: 13.6 / 8.4 us).
 __global__ __launch_bounds__(256) void k_lin_scan(int segments, long long matrices, int elems, int reverse, const float* initial, const float* sums, float* states) {
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4, n = matrices * elems;
   if (i >= n) return;
   const long long m = i / elems;
   float4 s = initial ? *reinterpret_cast<const float4*>(initial + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k = 0; k < segments; ++k) {
-    const int e = reverse ? segments - 1 - k : k;
-    float4* at = reinterpret_cast<float4*>(states + (size_t)e * n + i);
-    if (k > 0) {
-      const float f = __builtin_amdgcn_exp2f(sums[(size_t)(reverse ? e + 1 : e - 1) * matrices + m]);
-      const float4 a = *at;
-      s = make_float4(fmaf(f, s.x, a.x), fmaf(f, s.y, a.y), fmaf(f, s.z, a.z), fmaf(f, s.w, a.w));
-    }
-    *at = s;
+  auto entry = [&](int k) { return reinterpret_cast<float4*>(states + (size_t)(reverse ? segments - 1 - k : k) * n + i); };
+  *entry(0) = s;
+  for (int k0 = 1; k0 < segments; k0 += 8) {
+    float4 a[8];
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (k0 + j < segments) {
+        a[j] = *entry(k0 + j);
+        f[j] = sums[(size_t)(reverse ? segments - k0 - j : k0 + j - 1) * matrices + m];
+      }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (k0 + j < segments) {
+        const float w = __builtin_amdgcn_exp2f(f[j]);
+        s = make_float4(fmaf(w, s.x, a[j].x), fmaf(w, s.y, a[j].y), fmaf(w, s.z, a[j].z), fmaf(w, s.w, a[j].w));
+        *entry(k0 + j) = s;
+      }
   }
 }
 

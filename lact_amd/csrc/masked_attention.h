@@ -76,7 +76,7 @@ struct MaskedAttnParams {
 
 // Intervals from the documents' bounds [B, n + 1] (null: one document) and the lengths of their prefixes [B, n] (null: none).  Whatever the bounds hold, the
 // intervals lie inside [0, L).
-__global__ void k_attn_ranges(int B, int L, int n, int window, const int* __restrict__ bounds, const int* __restrict__ prefixes, int2* rows, int2* cols) {
+__global__ void k_attn_ranges(int L, int n, int window, const int* __restrict__ bounds, const int* __restrict__ prefixes, int2* rows, int2* cols) {
   const int b = blockIdx.y, t = blockIdx.x * blockDim.x + threadIdx.x;
   if (t >= L) return;
   int lo = 1, start = 0, end = L;

@@ -129,7 +129,7 @@ int attention_forward(const lact_attention_desc_t* d, const void* q, const void*
   if (attention_params(d, q, k, v, ranges, &p) || check_ptrs({out, lse}, "masked attention outputs")) return -1;
   p.out = static_cast<T*>(out); p.lse = lse;
   if (d->n_documents)
-    LACT_LAUNCH("k_attn_ranges", "masked_attn", 0.0, k_attn_ranges, dim3(ceil_div(d->L, 256), d->B), dim3(256), s, d->B, d->L, d->n_documents, p.window, d->documents,
+    LACT_LAUNCH("k_attn_ranges", "masked_attn", 0.0, k_attn_ranges, dim3(ceil_div(d->L, 256), d->B), dim3(256), s, d->L, d->n_documents, p.window, d->documents,
                 d->prefixes, const_cast<int2*>(p.rows), const_cast<int2*>(p.cols));
   launch_attention<0>(1, d->D, p, s);
   LACT_CHECK_LAUNCH();
