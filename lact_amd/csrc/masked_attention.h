@@ -505,7 +505,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 
 // Outputs.  Bound by the vector instructions between the two products of a tile: for 64 scores of a wave some 70 cycles with a cap (two exponentials and a
 // reciprocal at a quarter of the rate) beside 32 of matrix products at D = 128, which the other wave of the SIMD covers in part.  A prompt of 8191 tokens in
-// a prefix, 32 heads of 128 over 8, cap 30: 772 us, 720 TFLOP/s; 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 57 us.
+// a prefix, 32 heads of 128 over 8, cap 30: 765 us, 720 TFLOP/s; 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 57 us.
 // HALVES: waves that share 32 queries, each with its half of every tile's keys; their sums are joined through LDS at the end.
 template <typename T, int D, bool BENT, int HALVES>
 __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_fwd(const MaskedAttnParams<T> p) {
