@@ -649,12 +649,14 @@ void expect_same(const Tensor& t, const Tensor& like, const char* name) {
   if (t.device() != like.device()) throw std::runtime_error(std::string("expected all tensors to be on the same device: ") + name);
   TORCH_CHECK_TYPE(t.scalar_type() == like.scalar_type(), name, " is ", t.scalar_type(), ", q is ", like.scalar_type());
 }
-// whole numbers that the kernels read as int32
+// Whole numbers that the kernels read as int32.  int64 beyond its range is cut to it, not wrapped: such a bound or length lies outside every sequence, and the
+// kernels cut it to theirs.
 Tensor indices(const OptTensor& t, const Tensor& like, at::IntArrayRef shape, const char* name) {
   if (!t) return Tensor();
   expect(*t, like, shape, name);
   TORCH_CHECK_TYPE(t->scalar_type() == at::kInt || t->scalar_type() == at::kLong, name, " must be int32 or int64, got ", t->scalar_type());
-  return t->to(at::kInt).contiguous();
+  const Tensor in = t->scalar_type() == at::kLong ? t->clamp(INT32_MIN, INT32_MAX) : *t;
+  return in.to(at::kInt).contiguous();
 }
 
 // A leaf's node belongs to the stream on which the first graph that holds the leaf was made, and a backward waits for that stream.  The default stream cannot

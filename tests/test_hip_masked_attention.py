@@ -530,3 +530,25 @@ def test_autocast_casts_the_operands():
     assert out.dtype == torch.bfloat16 and g.dtype == torch.float32 and torch.equal(out, lact_amd.masked_window_attention(b, b, b, 9))
     with torch.autocast("cuda", torch.float16), pytest.raises(TypeError):
         lact_amd.masked_window_attention(x, x, x)
+
+
+@BOTH
+def test_wide_integers_are_cut_to_the_sequence(dtype):
+    """Bounds, prefixes and lengths past 32 bits lie outside the sequence like any others."""
+    import lact_amd
+    b, l, h, d = 3, 150, 2, 64
+    packed, go = make(b, l, h, h, d, dtype)
+    far = 2 ** 63 - 1
+    wide = torch.tensor([[0, 40, 2 ** 40], [10, 2 ** 32 + 60, far], [-far - 1, 2 ** 31, far]])
+    plain = torch.tensor([[0, 40, l], [10, l, l], [0, l, l]])
+    wide_pre, plain_pre = torch.tensor([[far, 2 ** 32 + 1], [-far - 1, 5], [2 ** 32, 0]]), torch.tensor([[l, l], [0, 5], [l, 0]])
+    results = []
+    for docs, pre in ((wide, wide_pre), (plain.int(), plain_pre.int())):
+        x = packed.to("cuda").requires_grad_(True)
+        out = lact_amd.masked_window_attention(*parts(x, h, h, d), 70, documents=docs.to("cuda"), prefixes=pre.to("cuda"))
+        results.append((out.detach(), *torch.autograd.grad(out, x, go.to("cuda"))))
+    assert all(torch.equal(a, r) for a, r in zip(*results))
+    assert bool(results[0][0].any(-1).sum() == b * l * h - 10 * h)
+    q, k, v = (t.to("cuda") for t in parts(packed, h, h, d))
+    step = lambda *n: lact_amd.window_attention_step(q[:, 0], k, v, torch.tensor(n, device="cuda"), 40)  # noqa: E731
+    assert torch.equal(step(far, 2 ** 31, 2 ** 32 + 5), step(l, l, l)) and not step(-far - 1, -2 ** 32 + 9, -2 ** 31).any()
