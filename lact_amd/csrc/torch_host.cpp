@@ -897,6 +897,9 @@ std::vector<Tensor> linear_step(const Tensor& q_, const Tensor& k_, const Tensor
   if (out.numel() == 0) return {out, next};
   check(lact_linear_attention_step(act, (int)b, (int)h, (int)dk, (int)dv, g.dim() == 2, (float)scale, ptr(q), h * dk, ptr(k), h * dk, ptr(v), h * dv, fptr(g),
                                    fptr(state), fptr(next), ptr(out), stream()));
+  // A graph that has kept this memory (a sequence call's state or last state) has to see that it changed.  (What was made for inference has no version, and no
+  // graph keeps it.)
+  if (state_out && !next.is_inference()) torch::autograd::impl::bump_version(next);
   return {out, next};
 }
 

@@ -54,14 +54,15 @@ def decayed_linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Ten
                                   state_out: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """decayed_linear_attention for one token of every sequence: q, k [b, h, dk], v [b, h, dv], log_decay [h] or [b, h], state [b, h, dk, dv] ->
     (out [b, h, dv], the new state, fp32).  state_out: where the new state goes; it may be `state` itself (then nothing is
-    allocated for it), but must not overlap it otherwise.  For inference: under torch.no_grad(), or with operands that need no gradient."""
+    allocated for it), but must not overlap it otherwise; for autograd it is an operation in place.  For inference: under torch.no_grad(), or with operands
+    (and a state_out) that need no gradient."""
     name = "decayed_linear_attention_step"
     _plain_only(name, q, k, v, log_decay, state, state_out)
     _dims(name, 3, q=q, k=k, v=v)
     _dims(name, 4, state=state, state_out=state_out)
     if log_decay.dim() not in (1, 2):
         raise ValueError(f"{name}: log_decay must be [h] or [b, h], got {tuple(log_decay.shape)}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, log_decay, state, state_out)):
         raise RuntimeError(f"{name} is for inference: call it under torch.no_grad()")
     out, new = _lib.host().linear_attention_step(q, k, v, log_decay, state, state_out, _scale(name, scale, q.shape[2]))
     return out, new

@@ -343,3 +343,36 @@ def test_refusals_on_the_gpu():
     first, = torch.autograd.grad(f(leaf, q, q, g).float().sum(), leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(first.float().sum(), leaf)
+
+
+def test_steps_in_place_are_seen_by_autograd():
+    """The states that a sequence call keeps for its backward, stepped in place in front of it: the backward refuses, as behind any operation in place."""
+    import lact_amd
+    x, go, gs = make(1, 100, 2, 64, 64, torch.bfloat16, "token")
+    go, gs = go.to("cuda"), gs.to("cuda")
+    dev = {n: t.to("cuda").requires_grad_(n != "state") for n, t in x.items()}
+    one = [dev[n].detach()[:, 0] for n in ("q", "k", "v", "log_decay")]
+    for which in ("last", "state", "neither"):
+        out, last = lact_amd.decayed_linear_attention(**dev, return_state=True)
+        before = last._version, dev["state"]._version
+        with torch.no_grad():
+            target = {"last": last, "state": dev["state"], "neither": torch.empty_like(last)}[which]
+            _, new = lact_amd.decayed_linear_attention_step(*one, target if which != "neither" else last, state_out=target)
+        assert new is target or new.data_ptr() == target.data_ptr()
+        assert (last._version > before[0], dev["state"]._version > before[1]) == (which == "last", which == "state")
+        if which == "neither":
+            torch.autograd.grad([out, last], dev["q"], [go, gs])
+        else:
+            with pytest.raises(RuntimeError, match="inplace"):
+                torch.autograd.grad([out, last], dev["q"], [go, gs])
+    with torch.inference_mode():
+        state = torch.zeros(1, 2, 64, 64, device="cuda")
+        lact_amd.decayed_linear_attention_step(*one, state, state_out=state)
+    with torch.no_grad():      # a state made for inference, which no graph can keep
+        lact_amd.decayed_linear_attention_step(*one, state, state_out=state)
+    leaf = torch.zeros(1, 2, 64, 64, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="inference"):
+        lact_amd.decayed_linear_attention_step(*one, state.clone(), state_out=leaf)
+    with torch.no_grad():
+        lact_amd.decayed_linear_attention_step(*one, state.clone(), state_out=leaf)
+    assert leaf.any()

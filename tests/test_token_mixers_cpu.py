@@ -196,3 +196,9 @@ def test_oracle_recurrence_is_the_quadratic_form():
     ref = (torch.einsum("bihd,bjhd,bijh,bjhe->bihe", q, k, w, v) + torch.einsum("bih,bihd,bhde->bihe", run.exp(), q, s)) / math.sqrt(8)
     assert float((out - ref).abs().max()) < 1e-12
     assert float((last - (torch.einsum("bjhd,bjh,bjhe->bhde", k, (run[:, -1:] - run).exp(), v) + run[:, -1].exp()[..., None, None] * s)).abs().max()) < 1e-12
+
+
+def test_step_refuses_a_state_out_that_needs_a_gradient():
+    k, s = torch.zeros(1, 2, 64), torch.zeros(1, 2, 64, 64)
+    with pytest.raises(RuntimeError, match="inference"):
+        lact_amd.decayed_linear_attention_step(k, k, k, torch.zeros(2), s, state_out=s.clone().requires_grad_(True))
