@@ -107,7 +107,7 @@ struct StepWork {
   __device__ __forceinline__ int block_of(long long s) const { return (int)(((s + 1) * blocks - 1) / total); }
 };
 
-template <typename T, int D>
+template <typename T, int D, int BENT>
 __global__ __launch_bounds__((64 * AttnStepShape<T, D>::NW), 1) void k_attn_step(const AttnStepParams<T> p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using A = AttnStepShape<T, D>;
@@ -150,7 +150,7 @@ __global__ __launch_bounds__((64 * AttnStepShape<T, D>::NW), 1) void k_attn_step
     const T* V = p.v + b * p.bsv + hk * p.hsv;
     Frag qf[D / 16];
     mask_own_rows<T, D>(qf, p.q + b * p.bsq, D, h, p.H);
-    Scores<T, true> sc;
+    Scores<T, BENT> sc;
     sc.init(p.scale, p.cap, p.slopes, h);
     const float c = sc.unit();
     f32x16 o[D / 32];

@@ -294,26 +294,34 @@ struct Spoilt {
   }
 };
 
-// tanh in fp32.  Small x: Lambert's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + x^2 / (7 + x^2 / 9)))), relative error below 1e-8
+// tanh(x) / x and tanh(x) in fp32, of |x|.  Small x: Lambert's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + x^2 / (7 + x^2 / 9)))), relative error below 1e-8
 // up to 0.8; 1 - 2 / (1 + e^2x) there loses the bits that x has below 1.
-__device__ __forceinline__ float tanh_f32(float x) {
-  const float a = fabsf(x), y = a * a;
-  const float near = a * fmaf(y, fmaf(y, 1.f, 105.f), 945.f) / fmaf(y, fmaf(y, 15.f, 420.f), 945.f);
-  const float far = 1.f - 2.f / (1.f + __builtin_amdgcn_exp2f(a * (2.f * ATTN_LOG2E)));
-  return copysignf(a < 0.8f ? near : far, x);
+constexpr float TANH_NEAR = 0.8f;
+__device__ __forceinline__ float tanh_over_near(float a) {
+  const float y = a * a;
+  return fmaf(y, fmaf(y, 1.f, 105.f), 945.f) / fmaf(y, fmaf(y, 15.f, 420.f), 945.f);
 }
+__device__ __forceinline__ float tanh_far(float a) { return 1.f - 2.f / (1.f + __builtin_amdgcn_exp2f(a * (2.f * ATTN_LOG2E))); }
+
+// What the scores go through: nothing; a cap, a distance or both; the same with a cap past CAP_QUICK in bf16.  (A branch in one kernel takes 12 registers more, which cost the
+// heads of 64 a wave of a SIMD, and dq of heads of 128 spills.)
+enum { SCORES_PLAIN, SCORES_BENT, SCORES_FAR_CAP };
+constexpr float CAP_QUICK = 256.f / ATTN_LOG2E;
 
 // Scores as they come out of the product -> what 2^ is taken of, times `unit` (see below)
-template <typename T, bool BENT>      // BENT: with a cap or a distance
+template <typename T, int BENT>
 struct Scores {
-  float c;          // log2(e) / sqrt(D) without a cap: the scores then keep it out until they meet the maximum
-  float k1, k2;     // with a cap: 2 log2(e) scale / cap, cap log2(e)
+  // k2 - 2 k2 / (1 + e^2x) for the capped score, with an error of 2 k2 2^-23: in bf16 with caps to CAP_QUICK, where that is a sixty-fourth of what a probability is
+  // rounded by.  Otherwise the score itself times tanh(x) / x, whose error is relative however far the cap is.
+  static constexpr bool QUICK = sizeof(T) == 2 && BENT == SCORES_BENT;
+  float c;          // scale log2(e); without a cap the scores keep it out until they meet the maximum
+  float k1, k2;     // with a cap: scale / cap (QUICK: 2 log2(e) times it), cap log2(e)
   float slope;      // times log2(e)
   bool cap, bias;
   bool bounded;     // 2^s and its sums stay in range whatever the scores are: |s| <= k2 (a row sees itself, where the distance takes nothing off)
   __device__ __forceinline__ void init(float scale, float cap_, const float* slopes, int h) {
     cap = BENT && cap_ > 0.f; bias = BENT && slopes != nullptr;
-    k1 = sizeof(T) == 2 ? 2.f * ATTN_LOG2E * scale / cap_ : scale / cap_;
+    k1 = fminf(QUICK ? 2.f * ATTN_LOG2E * scale / cap_ : scale / cap_, 3e38f);      // (finite: a score of 0 stays 0 under the smallest caps)
     k2 = cap_ * ATTN_LOG2E;
     slope = bias ? slopes[h] * ATTN_LOG2E : 0.f;
     bounded = cap && k2 <= 90.f && slope >= 0.f;
@@ -321,18 +329,26 @@ struct Scores {
   }
   // what is left to multiply by behind apply()
   __device__ __forceinline__ float unit() const { return BENT ? 1.f : c; }
-  __device__ __forceinline__ float bent(float s) const {      // tanh of the score over the cap
-    if constexpr (sizeof(T) == 2) return fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * k1)), -2.f, 1.f);   // to 2^-23
-    else return tanh_f32(s * k1);
+  // the capped score times log2(e), and the tanh that the cap takes
+  __device__ __forceinline__ float capped(float s, float& t) const {
+    if constexpr (QUICK) {
+      t = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * k1)), -2.f, 1.f);      // to 2^-23
+      return t * k2;
+    } else {
+      const float a = fabsf(s * k1), r = tanh_over_near(a), far = tanh_far(a);
+      t = a < TANH_NEAR ? a * r : far;
+      return a < TANH_NEAR ? s * c * r : copysignf(k2 * far, s);
+    }
   }
   // `first`: the place of the lane's element 0 minus the place of its own row
   __device__ __forceinline__ void apply(f32x16& s, int first) const {
-    if constexpr (!BENT) return;
+    if constexpr (BENT == SCORES_PLAIN) return;
     if (cap) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        if constexpr (sizeof(T) == 2) s[j] = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[j] * k1)), -2.f * k2, k2);
-        else s[j] = bent(s[j]) * k2;
+        float t;
+        if constexpr (QUICK) s[j] = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[j] * k1)), -2.f * k2, k2);
+        else s[j] = capped(s[j], t);
       }
     } else {
 #pragma unroll
@@ -342,16 +358,14 @@ struct Scores {
   }
   // the same, and the gradients dp (of what the softmax weighs) times the derivative of the cap
   __device__ __forceinline__ void apply(f32x16& s, f32x16& dp, int first) const {
-    if constexpr (!BENT) return;
+    if constexpr (BENT == SCORES_PLAIN) return;
     if (cap) {
       // (in steps of four: one loop over both vectors leaves them in memory)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        f32x4 t;
+        float t[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) t[j] = bent(s[4 * g + j]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[4 * g + j] = t[j] * k2;
+        for (int j = 0; j < 4; ++j) s[4 * g + j] = capped(s[4 * g + j], t[j]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) dp[4 * g + j] *= fmaf(-t[j], t[j], 1.f);
       }
@@ -373,7 +387,7 @@ struct Scores {
 // end.  A wave's two accumulators (128 registers) and its own keys and values (64) leave too little of the 256 that two waves of a SIMD have each: here
 // the values are read from LDS.  One wave with all of them in 400 registers: 148 us at 2 x 4096 tokens in documents, 12 heads.
 // With a cap or a distance there are too many for that as well: 969 us as one wave, 1075 as two, the backward of 4 x 4096 tokens of 12 heads.
-template <typename T, int D, bool BENT> constexpr int mask_halves() { return sizeof(T) == 2 && D == 128 && !BENT ? 2 : 1; }
+template <typename T, int D, int BENT> constexpr int mask_halves() { return sizeof(T) == 2 && D == 128 && !BENT ? 2 : 1; }
 // 64-row tiles of both operands in LDS
 template <typename T, int D> constexpr int mask_ring(bool keys) { return sizeof(T) == 4 || (D == 128 && !keys) ? 2 : 3; }
 // stats: of dk/dv; groups of 32 rows; halves: waves that share them
@@ -507,7 +521,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // reciprocal at a quarter of the rate) beside 32 of matrix products at D = 128, which the other wave of the SIMD covers in part.  A prompt of 8191 tokens in
 // a prefix, 32 heads of 128 over 8, cap 30: 765 us, 720 TFLOP/s; 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 57 us.
 // HALVES: waves that share 32 queries, each with its half of every tile's keys; their sums are joined through LDS at the end.
-template <typename T, int D, bool BENT, int HALVES>
+template <typename T, int D, int BENT, int HALVES>
 __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_fwd(const MaskedAttnParams<T> p) {
   constexpr int NW = MASK_WAVES, KW = NW / HALVES, N = 2 / HALVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -686,7 +700,7 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
 
 // dq = scale * sum_keys ds k with ds = p (dp - delta) f', and delta itself.  The probabilities are formed again from lse: the scores are a product more, but
 // nothing of length L^2 is in memory.  Bound as the outputs are; 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 77 us.
-template <typename T, int D, bool BENT, int HALVES>
+template <typename T, int D, int BENT, int HALVES>
 __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_dq(const MaskedAttnParams<T> p) {
   constexpr int NW = MASK_WAVES, KW = NW / HALVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -817,7 +831,7 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
 // walks the queries that see them, head after head.  With few keys (blocks) the walk is cut into splits, whose sums k_attn_sum adds; all splits of the first
 // keys, whose walks are the longest under a causal mask, come first.  (dq is not formed here as well: its sums over keys would be atomics, in no order.)
 // 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 117 us, bound as the outputs are and by LDS, which both operands are read from in both directions.
-template <typename T, int D, bool BENT>
+template <typename T, int D, int BENT>
 __global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (sizeof(T) == 2 && (D == 64 || !BENT) ? 2 : 1)) void k_masked_attn_dkv(const MaskedAttnParams<T> p) {
   constexpr int KW = MASK_WAVES, HALVES = mask_halves<T, D, BENT>(), NW = KW * HALVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];

@@ -85,7 +85,7 @@ size_t attention_workspace(const lact_attention_desc_t* d) {
 bool half_rows(long long blocks) { return blocks <= COMPUTE_UNITS * 3 / 2; }
 
 // WHICH: 0 forward, 1 dq, 2 dk and dv (in `splits`)
-template <int WHICH, typename T, int D, bool BENT, int HALVES>
+template <int WHICH, typename T, int D, int BENT, int HALVES>
 void launch_attention(int splits, const MaskedAttnParams<T>& p, dim3 grid, hipStream_t s) {
   const dim3 block(64 * MASK_WAVES * (WHICH == 2 ? HALVES : 1));
   constexpr int SM = mask_lds_bytes<T, D>(WHICH == 2, MASK_WAVES / (WHICH == 2 ? 1 : HALVES), HALVES);
@@ -105,7 +105,7 @@ void launch_attention(int splits, const MaskedAttnParams<T>& p, dim3 grid, hipSt
     }
   }
 }
-template <int WHICH, typename T, int D, bool BENT>
+template <int WHICH, typename T, int D, int BENT>
 void launch_attention(int splits, MaskedAttnParams<T> p, hipStream_t s) {
   const int heads = p.B * (WHICH == 2 ? p.HK * splits : p.H);
   p.splits = splits;
@@ -115,11 +115,17 @@ void launch_attention(int splits, MaskedAttnParams<T> p, hipStream_t s) {
   else if (half_rows(grid.x)) launch_attention<WHICH, T, D, BENT, 2>(splits, p, dim3(ceil_div(p.L, 16 * MASK_WAVES) * heads), s);
   else launch_attention<WHICH, T, D, BENT, 1>(splits, p, grid, s);
 }
+template <int WHICH, typename T, int D>
+void launch_attention(int splits, const MaskedAttnParams<T>& p, hipStream_t s) {
+  if (!(p.cap > 0.f || p.slopes)) return launch_attention<WHICH, T, D, SCORES_PLAIN>(splits, p, s);
+  if constexpr (sizeof(T) == 2)
+    if (p.cap > CAP_QUICK) return launch_attention<WHICH, T, D, SCORES_FAR_CAP>(splits, p, s);
+  launch_attention<WHICH, T, D, SCORES_BENT>(splits, p, s);
+}
 template <int WHICH, typename T>
 void launch_attention(int splits, int D, const MaskedAttnParams<T>& p, hipStream_t s) {
-  const bool bent = p.cap > 0.f || p.slopes;
-  if (D == 128) bent ? launch_attention<WHICH, T, 128, true>(splits, p, s) : launch_attention<WHICH, T, 128, false>(splits, p, s);
-  else bent ? launch_attention<WHICH, T, 64, true>(splits, p, s) : launch_attention<WHICH, T, 64, false>(splits, p, s);
+  if (D == 128) launch_attention<WHICH, T, 128>(splits, p, s);
+  else launch_attention<WHICH, T, 64>(splits, p, s);
 }
 
 template <typename T>
@@ -190,9 +196,13 @@ int step_run(const lact_attention_step_desc_t* d, const void* q, const void* k, 
   p.v = static_cast<const T*>(v); p.ldv = d->v_ld; p.bsv = d->v_bs; p.hsv = d->v_hs;
   p.lengths = lengths; p.slopes = d->slopes; p.scale = d->scale; p.cap = d->score_cap;
   p.out = static_cast<T*>(out); p.part = static_cast<float*>(workspace);
-  constexpr int SM = AttnStepShape<T, D>::LDS;
-  LACT_BIG_LDS((k_attn_step<T, D>), SM);
-  LACT_LAUNCH_SMEM("k_attn_step", "attn_step", 0.0, (k_attn_step<T, D>), dim3(p.blocks), dim3(64 * AttnStepShape<T, D>::NW), SM, s, p);
+  auto launch = [&](auto kind) {
+    constexpr int SM = AttnStepShape<T, D>::LDS, BENT = decltype(kind)::value;
+    LACT_BIG_LDS((k_attn_step<T, D, BENT>), SM);
+    LACT_LAUNCH_SMEM("k_attn_step", "attn_step", 0.0, (k_attn_step<T, D, BENT>), dim3(p.blocks), dim3(64 * AttnStepShape<T, D>::NW), SM, s, p);
+  };
+  if (sizeof(T) == 2 && p.cap > CAP_QUICK) launch(std::integral_constant<int, sizeof(T) == 2 ? SCORES_FAR_CAP : SCORES_BENT>());
+  else launch(std::integral_constant<int, SCORES_BENT>());
   LACT_LAUNCH("k_attn_step_join", "attn_step", 0.0, (k_attn_step_join<T, D>), dim3(p.B * p.H), dim3(512), s, p);
   LACT_CHECK_LAUNCH();
   return 0;

@@ -552,3 +552,74 @@ def test_wide_integers_are_cut_to_the_sequence(dtype):
     q, k, v = (t.to("cuda") for t in parts(packed, h, h, d))
     step = lambda *n: lact_amd.window_attention_step(q[:, 0], k, v, torch.tensor(n, device="cuda"), 40)  # noqa: E731
     assert torch.equal(step(far, 2 ** 31, 2 ** 32 + 5), step(l, l, l)) and not step(-far - 1, -2 ** 32 + 9, -2 ** 31).any()
+
+
+def capped_errors(dtype, l, d, size, cap):
+    """bf16, caps up to 256 / log2(e): the exponential, 1 + it and its reciprocal are off by 2^-23, 2^-24 and 2^-23 of themselves, which the cap multiplies: in
+    units of cap log2(e) by 1/2, 1/2 and 1 of 2^-23, and the last sum by 2^-24 of it."""
+    p_err, out_err = errors(dtype, l, d, size)
+    return p_err + (2.5 * 2.0 ** -23 * cap if dtype == torch.bfloat16 and cap * 1.4427 <= 256 else 0.0), out_err
+
+
+@BOTH
+@pytest.mark.parametrize("hq", [3, 200])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cap", [150.0, 2000.0, 1e5, 1e7, 1e30, 3e38])
+def test_large_caps(cap, d, hq, dtype):
+    """A cap far above the scores leaves them as they are."""
+    import lact_amd
+    print("[gpu-test] masked attention, large cap", cap, d, hq, dtype, flush=True)
+    l = 140
+    packed, go = make(1, l, hq, hq, d, dtype)
+    x = packed.to("cuda").requires_grad_(True)
+    out = lact_amd.masked_window_attention(*parts(x, hq, hq, d), 90, score_cap=cap)
+    gx, = torch.autograd.grad(out, x, go.to("cuda"))
+    ref, bound = MO.attention(*parts(packed, hq, hq, d), 90, cap, None, None, None, None, go, *capped_errors(dtype, l, d, 8.0, cap))
+    for name, a, r, e in zip(("out", "dq", "dk", "dv"), [out, *parts(gx, hq, hq, d)], ref, bound):
+        near(a, r, e, name)
+
+
+@BOTH
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cap", [150.0, 2500.0])
+def test_large_caps_that_bend_scores(cap, d, dtype):
+    """Keys that grow along the sequence: scores from nothing to beyond the cap."""
+    import lact_amd
+    print("[gpu-test] masked attention, scores about a large cap", cap, d, dtype, flush=True)
+    l, h = 300, 3
+    growth = cap / 8
+    packed, go = make(1, l, h, h, d, dtype, growth=growth)
+    x = packed.to("cuda").requires_grad_(True)
+    out = lact_amd.masked_window_attention(*parts(x, h, h, d), 190, score_cap=cap)
+    gx, = torch.autograd.grad(out, x, go.to("cuda"))
+    ref, bound = MO.attention(*parts(packed, h, h, d), 190, cap, None, None, None, None, go, *capped_errors(dtype, l, d, 8.0 * growth, cap))
+    for name, a, r, e in zip(("out", "dq", "dk", "dv"), [out, *parts(gx, h, h, d)], ref, bound):
+        near(a, r, e, name)
+
+
+@BOTH
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("cap", [150.0, 1e5, 1e7, 3e38])
+def test_step_with_large_caps(cap, d, dtype):
+    import lact_amd
+    print("[gpu-test] attention step, large cap", cap, d, dtype, flush=True)
+    b, n, hq, hkv, lengths = 2, 300, 4, 2, [300, 77]
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(*s, generator=g).to(dtype) for s in ((b, hq, d), (b, n, hkv, d), (b, n, hkv, d)))
+    out = lact_amd.window_attention_step(*(t.to("cuda") for t in (q, k, v)), torch.tensor(lengths, device="cuda"), score_cap=cap)
+    near(out, *MO.attention_step(q, k, v, lengths, None, cap, None, None, *capped_errors(dtype, n, d, 8.0, cap)), "out")
+
+
+@BOTH
+def test_the_smallest_caps_leave_equal_weights(dtype):
+    """A cap of 1e-40: scores are nothing but their sign's, and a score of 0 is 0."""
+    import lact_amd
+    l, h, d = 100, 2, 64
+    packed, _ = make(1, l, h, h, d, dtype)
+    packed[:, ::3, :h * d] = 0.0
+    q, k, v = parts(packed, h, h, d)
+    out = lact_amd.masked_window_attention(*(t.to("cuda") for t in (q, k, v)), score_cap=1e-40)
+    near(out, *MO.attention(q, k, v, None, 1e-40, None, None, None, None, None, *errors(dtype, l, d)), "out")
+    lengths = torch.tensor([l], device="cuda")
+    one = lact_amd.window_attention_step(q[:, 3].to("cuda"), k.to("cuda"), v.to("cuda"), lengths, score_cap=1e-40)
+    near(one, *MO.attention_step(q[:, 3], k, v, [l], None, 1e-40, None, None, *errors(dtype, l, d)), "step")
