@@ -318,13 +318,11 @@ struct Scores {
   float k1, k2;     // with a cap: scale / cap (QUICK: 2 log2(e) times it), cap log2(e)
   float slope;      // times log2(e)
   bool cap, bias;
-  bool bounded;     // 2^s and its sums stay in range whatever the scores are: |s| <= k2 (a row sees itself, where the distance takes nothing off)
   __device__ __forceinline__ void init(float scale, float cap_, const float* slopes, int h) {
     cap = BENT && cap_ > 0.f; bias = BENT && slopes != nullptr;
     k1 = fminf(QUICK ? 2.f * ATTN_LOG2E * scale / cap_ : scale / cap_, 3e38f);      // (finite: a score of 0 stays 0 under the smallest caps)
     k2 = cap_ * ATTN_LOG2E;
     slope = bias ? slopes[h] * ATTN_LOG2E : 0.f;
-    bounded = cap && k2 <= 90.f && slope >= 0.f;
     c = scale * ATTN_LOG2E;
   }
   // what is left to multiply by behind apply()
@@ -560,7 +558,7 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
   const float c = sc.unit();
-  float mc = sc.bounded ? 0.f : ATTN_LOWEST, sum = 0.f;        // running row maximum (of what 2^ is taken of) and this lane's share of the row sum
+  float mc = ATTN_LOWEST, sum = 0.f;        // running row maximum (of what 2^ is taken of) and this lane's share of the row sum
   // Without a cap or a distance the maximum is rounded where it is multiplied by c, the scores in fma are not: past 2^20 the difference would reach 2^(the rounding).
   // Such rows subtract `high`, the maximum before the product.
   constexpr float FAR = 1048576.f;
@@ -612,40 +610,37 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
         for (int i = 0; i < N; ++i)
           if (Seen(own.x - at - 32 * i, own.y - at - 32 * i).any_of((uint32_t)(bad >> (32 * (i + half))))) sum = __builtin_nanf("");
       }
-      // (a cap that bounds them saves the row maximum)
-      if (!sc.bounded) {
-        float mx;
-        if constexpr (N == 2) {
-          mx = max3(s[0][0], s[1][0], s[1][1]);
+      float mx;
+      if constexpr (N == 2) {
+        mx = max3(s[0][0], s[1][0], s[1][1]);
 #pragma unroll
-          for (int j = 1; j < 16; ++j) mx = max3(mx, s[0][j], s[N - 1][j]);
-        } else {
-          mx = max3(s[0][0], s[0][1], s[0][15]);
+        for (int j = 1; j < 16; ++j) mx = max3(mx, s[0][j], s[N - 1][j]);
+      } else {
+        mx = max3(s[0][0], s[0][1], s[0][15]);
 #pragma unroll
-          for (int j = 1; j < 8; ++j) mx = max3(mx, s[0][2 * j], s[0][2 * j + 1]);
+        for (int j = 1; j < 8; ++j) mx = max3(mx, s[0][2 * j], s[0][2 * j + 1]);
+      }
+      const float top = mx;
+      mx *= c;
+      // The maximum only has to keep exp2 in range: it follows the row when it is exceeded by more than 2^8 (its own row only: what a row
+      // gives does not depend on the others).
+      if (__any(mx > mc + 8.f)) {
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const bool moves = mx > mc + 8.f;
+        const float nm = moves ? mx : mc;
+        float f = __builtin_amdgcn_exp2f(mc - nm);
+        if constexpr (!BENT) {
+          const float was = high;
+          high = moves ? fmaxf(top, __shfl_xor(top, 32, 64)) : high;
+          if (fabsf(nm) > FAR) f = __builtin_amdgcn_exp2f((was - high) * c);
+          far = __any(nm > FAR || (nm < -FAR && nm > ATTN_LOWEST));
         }
-        const float top = mx;
-        mx *= c;
-        // The maximum only has to keep exp2 in range: it follows the row when it is exceeded by more than 2^8 (its own row only: what a row
-        // gives does not depend on the others).
-        if (__any(mx > mc + 8.f)) {
-          mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-          const bool moves = mx > mc + 8.f;
-          const float nm = moves ? mx : mc;
-          float f = __builtin_amdgcn_exp2f(mc - nm);
-          if constexpr (!BENT) {
-            const float was = high;
-            high = moves ? fmaxf(top, __shfl_xor(top, 32, 64)) : high;
-            if (fabsf(nm) > FAR) f = __builtin_amdgcn_exp2f((was - high) * c);
-            far = __any(nm > FAR || (nm < -FAR && nm > ATTN_LOWEST));
-          }
-          mc = nm;
-          sum *= f;
+        mc = nm;
+        sum *= f;
 #pragma unroll
-          for (int i = 0; i < D / 32; ++i)
+        for (int i = 0; i < D / 32; ++i)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[i][j] *= f;
-        }
+          for (int j = 0; j < 16; ++j) o[i][j] *= f;
       }
       float base = mc;
       if constexpr (!BENT)

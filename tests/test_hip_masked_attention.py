@@ -623,3 +623,21 @@ def test_the_smallest_caps_leave_equal_weights(dtype):
     lengths = torch.tensor([l], device="cuda")
     one = lact_amd.window_attention_step(q[:, 3].to("cuda"), k.to("cuda"), v.to("cuda"), lengths, score_cap=1e-40)
     near(one, *MO.attention_step(q[:, 3], k, v, [l], None, 1e-40, None, None, *errors(dtype, l, d)), "step")
+
+
+@BOTH
+@pytest.mark.parametrize("hq", [3, 200])
+@pytest.mark.parametrize("size", [1e30, 1e-30])
+@pytest.mark.parametrize("cap,sign", [(12.0, 1.0), (30.0, 1.0), (60.0, 1.0), (30.0, -1.0), (60.0, -1.0)])
+def test_large_and_small_values_under_scores_at_their_cap(cap, sign, size, hq, dtype):
+    """All scores at the cap, or at its negative: the outputs are means of the values, whose sums stay far from the ends of what fp32 holds.  Values of 1e30 times 140
+    terms and the 2^8 that a row's largest probability may reach: 2^115; values of 1e-30 times a probability of 1 or more: 2^-100."""
+    import lact_amd
+    print("[gpu-test] masked attention, values and caps", cap, sign, size, hq, dtype, flush=True)
+    l, d = 140, 64
+    q, k = torch.full((1, l, hq, d), 16.0), torch.full((1, l, hq, d), 16.0 * sign)
+    v = torch.randn(1, l, hq, d, generator=torch.Generator().manual_seed(3)) * size
+    q, k, v = (t.to(dtype) for t in (q, k, v))
+    out = lact_amd.masked_window_attention(*(t.to("cuda") for t in (q, k, v)), score_cap=cap)
+    ref, bound = MO.attention(q, k, v, None, cap, None, None, None, None, None, *errors(dtype, l, d, cap))
+    near(out.double() / size, ref / size, bound / size, "out")
