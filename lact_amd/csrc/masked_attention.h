@@ -395,7 +395,7 @@ constexpr int mask_lds_bytes(bool stats, int groups, int halves) {
   const int ring = R * 2 * MaskTile<T, D>::BYTES + (stats ? R * 512 + (halves - 1) * 2 * MaskTile<T, D>::BYTES : 0) + Spoilt<T, D>::BYTES;
   // what the rows are stored through, for splits in fp32, and what one half of the waves gives to the other
   const int store = groups * 32 * cmax((D + 16 / (int)sizeof(T)) * (int)sizeof(T), stats ? (D + 4) * 4 : 0);
-  return cmax(cmax(ring, store), (halves - 1) * groups * 64 * ((stats ? 2 : 1) * D * 2 + 8));
+  return cmax(cmax(ring, store), (halves - 1) * groups * 64 * ((stats ? 2 : 1) * D * 2 + 16));
 }
 // The second half's accumulators to the first, through LDS: a wave's [N][4][64 lanes] float4.
 template <int N>
@@ -515,6 +515,16 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// Without a cap or a distance the maximum m of a row is rounded where the scores' maximum h is multiplied by c, the scores in fma are not: past 2^20 the difference would reach
+// 2^(the rounding).  Such rows, far ones, subtract h ahead of the product.
+constexpr float ATTN_FAR = 1048576.f;
+__device__ __forceinline__ bool attn_far(float m) { return fabsf(m) > ATTN_FAR && m > ATTN_LOWEST; }
+// How much more was taken off the scores of a row under (m, h) than under (n, i): exactly what either takes.
+__device__ __forceinline__ float attn_above(float m, float h, float n, float i, float c) {
+  if (attn_far(m)) return attn_far(n) ? (h - i) * c : fmaf(h, c, -n);
+  return attn_far(n) ? fmaf(-i, c, m) : m - n;
+}
+
 // Outputs.  Bound by the vector instructions between the two products of a tile: for 64 scores of a wave some 70 cycles with a cap (two exponentials and a
 // reciprocal at a quarter of the rate) beside 32 of matrix products at D = 128, which the other wave of the SIMD covers in part.  A prompt of 8191 tokens in
 // a prefix, 32 heads of 128 over 8, cap 30: 765 us, 720 TFLOP/s; 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 57 us.
@@ -559,10 +569,7 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
     for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
   const float c = sc.unit();
   float mc = ATTN_LOWEST, sum = 0.f;        // running row maximum (of what 2^ is taken of) and this lane's share of the row sum
-  // Without a cap or a distance the maximum is rounded where it is multiplied by c, the scores in fma are not: past 2^20 the difference would reach 2^(the rounding).
-  // Such rows subtract `high`, the maximum before the product.
-  constexpr float FAR = 1048576.f;
-  float high = ATTN_LOWEST;
+  float high = ATTN_LOWEST;      // that maximum ahead of the product with c, for far rows (attn_far)
   bool far = false;
   first = min(first, L) / 64 * 64;
   const int tiles = last > first ? (last - first + 63) / 64 : 0;
@@ -628,12 +635,14 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
         const bool moves = mx > mc + 8.f;
         const float nm = moves ? mx : mc;
-        float f = __builtin_amdgcn_exp2f(mc - nm);
-        if constexpr (!BENT) {
+        float f;
+        if constexpr (BENT) {
+          f = __builtin_amdgcn_exp2f(mc - nm);
+        } else {
           const float was = high;
           high = moves ? fmaxf(top, __shfl_xor(top, 32, 64)) : high;
-          if (fabsf(nm) > FAR) f = __builtin_amdgcn_exp2f((was - high) * c);
-          far = __any(nm > FAR || (nm < -FAR && nm > ATTN_LOWEST));
+          f = __builtin_amdgcn_exp2f(attn_above(mc, was, nm, high, c));
+          far = __any(attn_far(nm));
         }
         mc = nm;
         sum *= f;
@@ -645,7 +654,7 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
       float base = mc;
       if constexpr (!BENT)
         if (far) {
-          const bool mine = fabsf(mc) > FAR;
+          const bool mine = attn_far(mc);
           base = mine ? 0.f : mc;
 #pragma unroll
           for (int i = 0; i < N; ++i)
@@ -672,17 +681,19 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
   __syncthreads();
   if constexpr (HALVES == 2) {
     float4* theirs = reinterpret_cast<float4*>(smem) + group * (D / 32) * 256 + lane;
-    float2* stats = reinterpret_cast<float2*>(smem + KW * D * 128) + group * 64 + lane;
+    float4* stats = reinterpret_cast<float4*>(smem + KW * D * 128) + group * 64 + lane;
     if (half == 1) {
       mask_give(theirs, o);
-      *stats = make_float2(mc, sum);
+      *stats = make_float4(mc, sum, high, 0.f);
     }
     __syncthreads();
     if (half == 0) {
-      const float2 u = *stats;
-      const float m = fmaxf(mc, u.x), f = __builtin_amdgcn_exp2f(mc - m), e = __builtin_amdgcn_exp2f(u.x - m);
+      const float4 u = *stats;
+      float above = mc - u.x;
+      if constexpr (!BENT) above = attn_above(mc, high, u.x, u.z, c);
+      const float f = __builtin_amdgcn_exp2f(fminf(above, 0.f)), e = __builtin_amdgcn_exp2f(fminf(-above, 0.f));
       mask_take(theirs, o, f, e);
-      mc = m;
+      mc = above < 0.f ? u.x : mc;
       sum = fmaf(sum, f, u.y * e);
     }
     __syncthreads();

@@ -641,3 +641,27 @@ def test_large_and_small_values_under_scores_at_their_cap(cap, sign, size, hq, d
     out = lact_amd.masked_window_attention(*(t.to("cuda") for t in (q, k, v)), score_cap=cap)
     ref, bound = MO.attention(q, k, v, None, cap, None, None, None, None, None, *errors(dtype, l, d, cap))
     near(out.double() / size, ref / size, bound / size, "out")
+
+
+@BOTH
+@pytest.mark.parametrize("h", [2, 200])
+@pytest.mark.parametrize("lead,step,rise", [((2048.0, 16384.0, 0.0, 0.0, 0.0), 4.0, 0.0), ((-2048.0, 16384.0, 0.0, 0.0, 0.0), 4.0, 0.0),
+                                            ((354.0, 16384.0, 256.0, 57.0, 12.0), 0.5, 0.0), ((354.0, 16384.0, 256.0, 57.0, 12.0), 0.5, 48.0),
+                                            ((-354.0, 16384.0, -256.0, 57.0, -12.0), 0.5, 48.0)])
+def test_far_scores_that_nearly_tie(lead, step, rise, h, dtype):
+    """Scores about 2^22 (and about 2^20 / log2(e), where rows begin to subtract their maximum ahead of the product) that differ by some units: whichever
+    waves share a row and wherever its maximum moves to, what its keys weigh comes from the differences.  Every product and sum of a score is a whole number of
+    steps of fp32, and so exact."""
+    import lact_amd
+    print("[gpu-test] masked attention, far scores", lead, rise, h, dtype, flush=True)
+    l, d = 140, 64
+    g = torch.Generator().manual_seed(4)
+    q, k = torch.zeros(1, l, h, d), torch.zeros(1, l, h, d)
+    q[..., 0], k[..., 0], q[..., 1], k[..., 1], q[..., 2] = lead[0], lead[1], lead[2], lead[3], 1.0
+    k[..., 2] = lead[4] + step * torch.randint(-8, 9, (1, l, h), generator=g)
+    k[:, :64, :, 2] -= rise / 2
+    k[:, 64:, :, 2] += rise / 2
+    v = torch.randn(1, l, h, d, generator=g)
+    q, k, v = (t.to(dtype) for t in (q, k, v))
+    out = lact_amd.masked_window_attention(*(t.to("cuda") for t in (q, k, v)))
+    near(out, *MO.attention(q, k, v, None, None, None, None, None, None, None, *errors(dtype, l, d)), "out")
