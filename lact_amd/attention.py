@@ -13,6 +13,8 @@ from torch.autograd import forward_ad as fwad
 
 from . import _lib
 
+_SMALLEST, _LARGEST = 2.0 ** -149, (2.0 - 2.0 ** -23) * 2.0 ** 127      # of fp32
+
 
 def _plain_only(name: str, *ts: Optional[torch.Tensor]) -> None:
     """The kernels read memory: what needs to see tensor operations (function transforms, tracing, forward mode, subclasses) is refused."""
@@ -43,10 +45,11 @@ def _dims(name: str, n: int, **ts: Optional[torch.Tensor]) -> None:
 def _options(name, d, window, score_cap, scale, slopes):
     if window is not None and (int(window) != window or window < 1):
         raise ValueError(f"{name}: window must be a positive number of tokens or None, got {window}")
-    if score_cap is not None and not (0 < float(score_cap) < math.inf):
-        raise ValueError(f"{name}: score_cap must be positive or None, got {score_cap}")
-    if scale is not None and not (0 < float(scale) < math.inf):
-        raise ValueError(f"{name}: scale must be positive or None, got {scale}")
+    # (the kernels take both in fp32, where a smaller one would be 0, and a cap of 0 none)
+    if score_cap is not None and not (_SMALLEST <= float(score_cap) <= _LARGEST):
+        raise ValueError(f"{name}: score_cap must be positive and a number of fp32, or None, got {score_cap}")
+    if scale is not None and not (_SMALLEST <= float(scale) <= _LARGEST):
+        raise ValueError(f"{name}: scale must be positive and a number of fp32, or None, got {scale}")
     if slopes is not None and torch.is_grad_enabled() and slopes.requires_grad:
         raise RuntimeError(f"{name}: distance_slopes have no gradient; detach them")
     return (1 << 30 if window is None else int(window), 1.0 / math.sqrt(d) if scale is None else float(scale),

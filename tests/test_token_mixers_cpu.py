@@ -202,3 +202,16 @@ def test_step_refuses_a_state_out_that_needs_a_gradient():
     k, s = torch.zeros(1, 2, 64), torch.zeros(1, 2, 64, 64)
     with pytest.raises(RuntimeError, match="inference"):
         lact_amd.decayed_linear_attention_step(k, k, k, torch.zeros(2), s, state_out=s.clone().requires_grad_(True))
+
+
+@pytest.mark.parametrize("value", [1e-50, 1e39, -1e-50, 5e-324])
+def test_caps_and_scales_that_fp32_does_not_hold(value):
+    """The kernels take them in fp32, where these would be 0 (no cap at all) or infinite."""
+    q = torch.zeros(1, 8, 2, 64)
+    for kw in (dict(score_cap=value), dict(scale=value)):
+        with pytest.raises(ValueError):
+            lact_amd.masked_window_attention(q, q, q, **kw)
+        with pytest.raises(ValueError):
+            lact_amd.window_attention_step(q[:, 0], q, q, torch.ones(1, dtype=torch.int32), **kw)
+    with pytest.raises(RuntimeError, match="MI355X"):
+        lact_amd.masked_window_attention(q, q, q, score_cap=3e38, scale=1e-40)
