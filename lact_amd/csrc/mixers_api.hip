@@ -219,7 +219,10 @@ int check_linear(const lact_linear_desc_t* d) {
   return 0;
 }
 
-struct LinCut { int segments, chunks; };      // chunks of a segment
+struct LinCut {
+  int segments, chunks;      // chunks of a segment
+  int stretches() const { return ceil_div(chunks, LIN_STRETCH); }
+};
 // One block walks a segment of a head; enough segments that the walks of all heads give every compute unit two blocks.  Sequences of a few chunks
 // are walked as a whole: two launches less.
 LinCut lin_cut(const lact_linear_desc_t* d) {
@@ -230,7 +233,7 @@ LinCut lin_cut(const lact_linear_desc_t* d) {
 }
 struct LinBuffers {
   size_t weights, states, sums, end;     // of `states`: what tokens weigh, where segments start, sums of their decays
-  size_t ends, rsums, up, down, part, scratch;
+  size_t ends, rsums, up, down, part, between, dbetween, scratch;
 };
 LinBuffers lin_buffers(const lact_linear_desc_t* d) {
   const LinCut cut = lin_cut(d);
@@ -249,7 +252,10 @@ LinBuffers lin_buffers(const lact_linear_desc_t* d) {
   o.rsums = take(several * cut.segments * heads * 4);
   o.up = take(tokens * 8);
   o.down = take(tokens * 4);
-  o.part = take(d->decay_per_token ? 0 : cut.segments * heads * 8);
+  o.part = take(d->decay_per_token ? 0 : cut.segments * cut.stretches() * heads * 8);
+  const size_t between = (size_t)cut.segments * (cut.stretches() - 1) * heads * elems * 4;
+  o.between = take(between);
+  o.dbetween = take(between);
   o.scratch = at;
   return o;
 }
@@ -259,7 +265,7 @@ LinParams<T> lin_params(const lact_linear_desc_t* d, const char* states) {
   LinParams<T> p;
   memset(&p, 0, sizeof(p));
   const LinCut cut = lin_cut(d);
-  p.B = d->b; p.L = d->l; p.H = d->h; p.segments = cut.segments; p.seg_chunks = cut.chunks;
+  p.B = d->b; p.L = d->l; p.H = d->h; p.segments = cut.segments; p.seg_chunks = cut.chunks; p.stretches = cut.stretches();
   p.weights = reinterpret_cast<const float*>(states + lin_buffers(d).weights);
   p.by_heads = make_udiv(d->h);
   return p;
@@ -345,14 +351,20 @@ int lin_backward(const lact_linear_desc_t* d, const void* q, const void* k, cons
   LinParams<T>& c = all.dk;
   c.x = rv; c.y = ro; c.z = rq;
   c.out = static_cast<T*>(dk); c.transposed = 1;
+  float *between = reinterpret_cast<float*>(scratch + buf.between), *dbetween = reinterpret_cast<float*>(scratch + buf.dbetween);
+  if (base.stretches > 1) {
+    a.between = between;
+    r.between = dbetween;
+  }
   if (dg) lin_gradients<T, DK, DV, true>(all, s);
   else lin_gradients<T, DK, DV, false>(all, s);
   if (dg) {
     double* part = reinterpret_cast<double*>(scratch + buf.part);
-    LACT_LAUNCH("k_lin_decay_grad", "linear_attn_bwd", 0.0, k_lin_decay_grad, dim3(base.segments * heads), dim3(256), s, d->b, d->l, d->h, base.segments,
-                base.seg_chunks * LIN_CHUNK, DK * DV, base.weights, up, down, starts, ends, last, dlast, (LinDecay{g, d->decay_per_token}), state == nullptr, dg, part);
+    LACT_LAUNCH("k_lin_decay_grad", "linear_attn_bwd", 0.0, k_lin_decay_grad, dim3(base.segments * base.stretches * heads), dim3(256), s, d->b, d->l, d->h, base.segments,
+                base.seg_chunks, base.stretches, DK * DV, base.weights, up, down, starts, ends, last, dlast, between, dbetween, (LinDecay{g, d->decay_per_token}),
+                state == nullptr, dg, part);
     if (!d->decay_per_token)
-      LACT_LAUNCH("k_lin_decay_sum", "linear_attn_bwd", 0.0, k_lin_decay_sum, dim3(d->h), dim3(64), s, base.segments * d->b, d->h, part, dg);
+      LACT_LAUNCH("k_lin_decay_sum", "linear_attn_bwd", 0.0, k_lin_decay_sum, dim3(d->h), dim3(64), s, base.segments * base.stretches * d->b, d->h, part, dg);
   }
   LACT_CHECK_LAUNCH();
   return 0;

@@ -376,3 +376,28 @@ def test_steps_in_place_are_seen_by_autograd():
     with torch.no_grad():
         lact_amd.decayed_linear_attention_step(*one, state.clone(), state_out=leaf)
     assert leaf.any()
+
+
+@BOTH
+@pytest.mark.parametrize("gates", ["token", "head"])
+@pytest.mark.parametrize("b,l,h,d", [(2, 1100, 130, 64), (2, 1100, 130, 128), (1, 3000, 100, 64)])
+def test_long_walks(b, l, h, d, gates, dtype):
+    """260 heads: more than segments are made for, so that a block walks all 18 chunks of its head; 100 heads: five segments of ten chunks, seven in the last.  The decays'
+    gradient is carried over eight chunks at a time.  Some of the heads, which do not depend on each other, are compared."""
+    import lact_amd
+    print("[gpu-test] linear attention, long walks", b, l, h, d, gates, dtype, flush=True)
+    some = [0, h // 2 - 1, h - 1]
+    x, go, gs = make(b, l, h, d, d, dtype, gates)
+    dev = on_gpu(x)
+    out, last = lact_amd.decayed_linear_attention(dev["q"], dev["k"], dev["v"], dev["log_decay"], state=dev["state"], return_state=True)
+    grads = torch.autograd.grad([out, last], list(dev.values()), [go.to("cuda"), gs.to("cuda")])
+    at = {"state": 1, "log_decay": x["log_decay"].dim() - 1}
+    part = lambda t, n: t.index_select(at.get(n, 2), torch.tensor(some, device=t.device))  # noqa: E731
+    ref_in = {n: part(t, n).double().requires_grad_(True) for n, t in x.items()}
+    ref, ref_last = MO.linear(*ref_in.values())
+    ref_grads = torch.autograd.grad([ref, ref_last], list(ref_in.values()), [part(go, "q").double(), part(gs, "state").double()])
+    for name, a, r in zip(["q", "state"] + list(x), [out, last, *grads], [ref, ref_last, *ref_grads]):
+        bound = 1.5 * 2.0 ** -8 if a.dtype == torch.bfloat16 else 200 * 2.0 ** -24      # as in check()
+        e = rel_l2(part(a, name), r)
+        print(f"[gpu-test]   {name}: {e:.2e}", flush=True)
+        assert bool(torch.isfinite(a).all()) and e < bound, (name, e)
