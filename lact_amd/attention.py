@@ -67,17 +67,18 @@ def masked_window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, w
 
     times v.  Query i sees key j of its own document when j > i - window and (j <= i or j is in the document's prefix).
 
-    window: tokens that a query looks back on, its own included; None: all.   scale: positive, 1 / sqrt(d) if None.
+    window: tokens that a query looks back on, its own included; None: all.   score_cap, scale: positive numbers of fp32; scale 1 / sqrt(d) if None.
     distance_slopes: [hq], without a gradient.
     documents: [b, n + 1] int32 (int64 is converted): document i of a sequence is its tokens [documents[:, i], documents[:, i + 1]).  The bounds do not
     fall; equal ones are empty documents.  Tokens in front of the first and behind the last bound are in none: their output and their
     gradients are 0, and nothing of them reaches another token, whatever they hold.  The bounds are not checked (they stay on the device);
     what lies outside the sequence is cut off.  None: the whole sequence is one document.
     prefixes: [b, n] ([b, 1] without documents): how many of a document's first tokens all of its tokens see, in both directions; a prefix as
-    long as the document makes its attention bidirectional.
-    What is not finite makes NaN of the heads of all tokens that see it, in every element (a key whose score is -infinity only of gradients).
+    long as the document makes its attention bidirectional.  (A plain causal window of bf16 and equal heads is sliding_window_attention's as well, whose kernels are up to a
+    tenth faster there.)
+    What is not finite makes NaN of the heads of all tokens that see it, in every element (a key whose score is -infinity, or infinite under a cap, only of gradients).
 
-    Differentiable in q, k and v, once.  The gradients use a row's log2 of its sum of 2^scores in fp32: they have lost 2^-24 of its size, and all digits
+    Differentiable in q, k and v, once.  Scores are numbers of fp32.  The gradients use a row's log2 of its sum of 2^scores in fp32: they have lost 2^-24 of its size, and all digits
     at scores past 2^20.  Under autocast the operands are cast to its type.  While a stream is captured, leaves that a graph made on the default stream still
     holds are refused."""
     name = "masked_window_attention"

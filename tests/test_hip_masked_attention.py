@@ -665,3 +665,23 @@ def test_far_scores_that_nearly_tie(lead, step, rise, h, dtype):
     q, k, v = (t.to(dtype) for t in (q, k, v))
     out = lact_amd.masked_window_attention(*(t.to("cuda") for t in (q, k, v)))
     near(out, *MO.attention(q, k, v, None, None, None, None, None, None, None, *errors(dtype, l, d)), "out")
+
+
+@BOTH
+@pytest.mark.parametrize("cap", [20.0, 1e4])
+def test_keys_of_infinity_under_a_cap(cap, dtype):
+    """Their scores are the cap or its negative, as those of very large keys are: outputs are finite, gradients of the queries that see them NaN."""
+    import lact_amd
+    l, h, d = 90, 2, 64
+    packed, go = make(1, l, h, h, d, dtype)
+    results = []
+    for value in (1e30, float("inf")):
+        x = packed.clone()
+        x[:, 40, h * d:2 * h * d:d] = value           # one element of a key in every head
+        x = x.to("cuda").requires_grad_(True)
+        out = lact_amd.masked_window_attention(*parts(x, h, h, d), 30, score_cap=cap)
+        results.append((out.detach(), torch.autograd.grad(out, x, go.to("cuda"))[0]))
+    (ref, gref), (out, g) = results
+    assert bool(torch.isfinite(out).all()) and torch.equal(out, ref)
+    q = slice(0, h * d)
+    assert bool(torch.isnan(g[:, 40:70, q]).all()) and torch.equal(g[:, :40], gref[:, :40]) and torch.equal(g[:, 70:, q], gref[:, 70:, q])
