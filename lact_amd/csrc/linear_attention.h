@@ -19,13 +19,15 @@
 // and batch alone do not fill the chip.
 //
 // 4 x 4096 tokens, 12 heads of 128 x 128, decays per token, us: weights 5, segments 30 and scan 11 (the two of them also for the gradients, backwards), outputs
-// 57, gradients 216, decays' gradient 20.  The segments, the scan and the decays are bound by memory: 100 MB at 3.4 TB/s, 62 MB at 5.8 (out of the cache),
-// 63 MB at 3.1.  The walks are bound by the way from one dependent product to the next: a chunk's pairs, the state's share, the update and the outputs follow each
-// other, two waves of a SIMD cover what they can (the matrix units are busy for a fifth of the time, the vector units for a third).  Eight waves to a block with
-// half of the columns each (255 us for the gradients) read the shared operands from LDS twice as often, and have too few registers.
+// 57, gradients 217, decays' gradient 17.  The segments, the scan and the decays are bound by memory: 100 MB at 3.4 TB/s, 62 MB at 5.8 (out of the cache),
+// 63 MB at 3.7.  The walks are bound by the way from one dependent product to the next: a chunk's pairs, the state's share, the update and the outputs follow each
+// other, two waves of a SIMD cover what they can (gradients: the matrix units are busy for 17 % of the time, the vector units for 27 %, and waves wait for 38 % of theirs).  Eight
+// waves to a block with half of the columns each (255 us for the gradients) read the shared operands from LDS twice as often, and have too few registers.  In fp32 the
+// gradients of 128 x 128 keep 66 registers in memory with the decays' gradient, 13 without.
 //
 // The state is held, and added to, in fp32: what is added is a product of bf16 inputs with a weight, which goes into the matrix product
-// as three bf16 parts (24 bits).  Probabilities and, where only rounded outputs depend on it, the state as an operand are rounded to bf16.
+// as three bf16 parts (24 bits).  Where only rounded results depend on the state (dk, and dq without the decays' gradient) it is added to in one part, and as an operand it
+// is one part there and in the outputs; pairs are rounded to bf16 as well.
 //
 // A gradient of the decays adds what crosses a token (k_lin_decay_grad): pairs M_ij = e^(G_i - G_j) (q_i . k_j)(dout_i . v_j) scale of a source in front and an
 // output behind it, and the states' shares.

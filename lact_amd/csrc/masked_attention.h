@@ -527,7 +527,8 @@ __device__ __forceinline__ float attn_above(float m, float h, float n, float i, 
 
 // Outputs.  Bound by the vector instructions between the two products of a tile: for 64 scores of a wave some 70 cycles with a cap (two exponentials and a
 // reciprocal at a quarter of the rate) beside 32 of matrix products at D = 128, which the other wave of the SIMD covers in part.  A prompt of 8191 tokens in
-// a prefix, 32 heads of 128 over 8, cap 30: 765 us, 720 TFLOP/s; 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 57 us.
+// a prefix, 32 heads of 128 over 8, cap 30: 746 us, 743 TFLOP/s, the vector units busy for 69 % of the time and the matrix units for 34 %; 2 x 4096 tokens in documents, 12 heads
+// of 128, window 2048: 57 us.  (Where both apply, window_attention.h forms the scores a tile ahead: 4 x 4096 tokens, 12 heads of 128, window 2048, forward 180 / here 198 us.)
 // HALVES: waves that share 32 queries, each with its half of every tile's keys; their sums are joined through LDS at the end.
 template <typename T, int D, int BENT, int HALVES>
 __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_fwd(const MaskedAttnParams<T> p) {
@@ -836,7 +837,8 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
 // dv = sum_queries p dout, dk = scale * sum_queries ds q, over the queries of all heads that share the key head: a wave owns 32 keys and
 // walks the queries that see them, head after head.  With few keys (blocks) the walk is cut into splits, whose sums k_attn_sum adds; all splits of the first
 // keys, whose walks are the longest under a causal mask, come first.  (dq is not formed here as well: its sums over keys would be atomics, in no order.)
-// 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 117 us, bound as the outputs are and by LDS, which both operands are read from in both directions.
+// 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 117 us, bound as the outputs are and by LDS, which both operands are read from in both directions.  (bf16, heads of
+// 128, without a cap or a distance: 256 registers and 12 more in memory.)
 template <typename T, int D, int BENT>
 __global__ __launch_bounds__((64 * MASK_WAVES * mask_halves<T, D, BENT>()), (sizeof(T) == 2 && (D == 64 || !BENT) ? 2 : 1)) void k_masked_attn_dkv(const MaskedAttnParams<T> p) {
   constexpr int KW = MASK_WAVES, HALVES = mask_halves<T, D, BENT>(), NW = KW * HALVES;
