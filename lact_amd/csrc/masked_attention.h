@@ -294,14 +294,16 @@ struct Spoilt {
   }
 };
 
-// tanh(x) / x and tanh(x) in fp32, of |x|.  Small x: Lambert's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + x^2 / (7 + x^2 / 9)))), relative error below 1e-8
-// up to 0.8; 1 - 2 / (1 + e^2x) there loses the bits that x has below 1.
-constexpr float TANH_NEAR = 0.8f;
-__device__ __forceinline__ float tanh_over_near(float a) {
-  const float y = a * a;
-  return fmaf(y, fmaf(y, 1.f, 105.f), 945.f) / fmaf(y, fmaf(y, 15.f, 420.f), 945.f);
-}
-__device__ __forceinline__ float tanh_far(float a) { return 1.f - 2.f / (1.f + __builtin_amdgcn_exp2f(a * (2.f * ATTN_LOG2E))); }
+// tanh in fp32, of a = |x|, by one division: tanh(a) / a up to 0.8, by Lambert's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + x^2 / (7 + x^2 / 9)))), relative error
+// below 1e-8; past it what tanh lacks of 1, 2 / (1 + e^2a), which would lose the bits that x has below 1.
+struct Tanh {
+  bool near;
+  float q;
+  __device__ __forceinline__ explicit Tanh(float a) : near(a < 0.8f) {
+    const float y = a * a, e = 1.f + __builtin_amdgcn_exp2f(a * (2.f * ATTN_LOG2E));
+    q = (near ? fmaf(y, fmaf(y, 1.f, 105.f), 945.f) : 2.f) / (near ? fmaf(y, fmaf(y, 15.f, 420.f), 945.f) : e);
+  }
+};
 
 // What the scores go through: nothing; a cap, a distance or both; the same with a cap past CAP_QUICK in bf16.  (A branch in one kernel takes 12 registers more, which cost the
 // heads of 64 a wave of a SIMD, and dq of heads of 128 spills.)
@@ -327,15 +329,18 @@ struct Scores {
   }
   // what is left to multiply by behind apply()
   __device__ __forceinline__ float unit() const { return BENT ? 1.f : c; }
-  // the capped score times log2(e), and the tanh that the cap takes
-  __device__ __forceinline__ float capped(float s, float& t) const {
+  // the capped score times log2(e), and the derivative of the cap, 1 - tanh^2
+  __device__ __forceinline__ float capped(float s, float& slope) const {
     if constexpr (QUICK) {
-      t = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * k1)), -2.f, 1.f);      // to 2^-23
+      const float t = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * k1)), -2.f, 1.f);      // to 2^-23
+      slope = fmaf(-t, t, 1.f);
       return t * k2;
     } else {
-      const float a = fabsf(s * k1), r = tanh_over_near(a), far = tanh_far(a);
-      t = a < TANH_NEAR ? a * r : far;
-      return a < TANH_NEAR ? s * c * r : copysignf(k2 * far, s);
+      const float a = fabsf(s * k1);
+      const Tanh t(a);
+      const float lacks = t.near ? fmaf(-a, t.q, 1.f) : t.q;      // of 1, with all digits
+      slope = lacks * (2.f - lacks);
+      return t.near ? s * c * t.q : copysignf(fmaf(-k2, t.q, k2), s);
     }
   }
   // `first`: the place of the lane's element 0 minus the place of its own row
@@ -344,9 +349,9 @@ struct Scores {
     if (cap) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
-        float t;
+        float slope;
         if constexpr (QUICK) s[j] = fmaf(__builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s[j] * k1)), -2.f * k2, k2);
-        else s[j] = capped(s[j], t);
+        else s[j] = capped(s[j], slope);
       }
     } else {
 #pragma unroll
@@ -361,11 +366,11 @@ struct Scores {
       // (in steps of four: one loop over both vectors leaves them in memory)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        float t[4];
+        float by[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[4 * g + j] = capped(s[4 * g + j], t[j]);
+        for (int j = 0; j < 4; ++j) s[4 * g + j] = capped(s[4 * g + j], by[j]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) dp[4 * g + j] *= fmaf(-t[j], t[j], 1.f);
+        for (int j = 0; j < 4; ++j) dp[4 * g + j] *= by[j];
       }
     } else {
 #pragma unroll

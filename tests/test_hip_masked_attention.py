@@ -685,3 +685,25 @@ def test_keys_of_infinity_under_a_cap(cap, dtype):
     assert bool(torch.isfinite(out).all()) and torch.equal(out, ref)
     q = slice(0, h * d)
     assert bool(torch.isnan(g[:, 40:70, q]).all()) and torch.equal(g[:, :40], gref[:, :40]) and torch.equal(g[:, 70:, q], gref[:, 70:, q])
+
+
+@pytest.mark.parametrize("h", [2, 200])
+@pytest.mark.parametrize("d", [64, 128])
+def test_gradients_of_scores_past_their_cap_in_fp32(d, h):
+    """What is left of a gradient behind scores of 8 to 12 under a cap of 2, 1e-3 to 2e-5, keeps its digits.  The scores are one product each, and exact; the derivative's
+    exponent of up to 12 is off by two roundings, as the scores' of this size are allowed to be."""
+    import lact_amd
+    print("[gpu-test] masked attention, gradients past the cap", d, h, flush=True)
+    l = 140
+    packed, go = make(1, l, h, h, d, torch.float32)
+    q, k, _ = parts(packed, h, h, d)
+    q[:], q[..., 0] = 0.0, 1.0
+    g = torch.Generator().manual_seed(1)
+    k[..., 0] = torch.randint(64, 97, (1, l, h), generator=g) / 8 * (2 * torch.randint(0, 2, (1, l, h), generator=g) - 1)
+    packed = torch.cat([q.flatten(2), k.flatten(2), packed[..., 2 * h * d:]], -1)
+    x = packed.to("cuda").requires_grad_(True)
+    out = lact_amd.masked_window_attention(*parts(x, h, h, d), 90, score_cap=2.0, scale=1.0)
+    gx, = torch.autograd.grad(out, x, go.to("cuda"))
+    ref, bound = MO.attention(*parts(packed, h, h, d), 90, 2.0, None, None, None, 1.0, go, *errors(torch.float32, l, d))
+    for name, a, r, e in zip(("out", "dq", "dk", "dv"), [out, *parts(gx, h, h, d)], ref, bound):
+        near(a, r, e, name)
