@@ -710,9 +710,10 @@ __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_mas
   mask_store_rows<T, D>(smem + group * 32 * (D + 16 / sizeof(T)) * sizeof(T), o, empty ? 0.f : 1.f / sum, p.out + ((size_t)b * L * p.H + h) * D, (size_t)p.H * D, row0, L);
 }
 
-// dq = scale * sum_keys ds k with ds = p (dp - delta) f', and delta itself, from the output as it is stored: what that was rounded by is in all of a row's ds (bf16, relative errors of
-// dq: its own rounding 1.65e-3, with that of ds 2.37e-3, with the output's 2.46e-3; an output of 32 bits beside it would be written and read for the last).  The probabilities are formed again from lse: the scores are a product more, but
-// nothing of length L^2 is in memory.  Bound as the outputs are; 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 77 us.
+// dq = scale * sum_keys ds k with ds = p (dp - delta) f', and delta itself, from the output as it is stored: what that was rounded by is in all of a row's ds
+// (bf16, relative errors of dq: its own rounding 1.65e-3, with that of ds 2.37e-3, with the output's 2.46e-3; an output of 32 bits beside it would be written
+// and read for the last).  The probabilities are formed again from lse: the scores are a product more, but nothing of length L^2 is in memory.  Bound as the
+// outputs are; 2 x 4096 tokens in documents, 12 heads of 128, window 2048: 77 us.
 template <typename T, int D, int BENT, int HALVES>
 __global__ __launch_bounds__(64 * MASK_WAVES, sizeof(T) == 2 ? 2 : 1) void k_masked_attn_dq(const MaskedAttnParams<T> p) {
   constexpr int NW = MASK_WAVES, KW = NW / HALVES;
