@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-enum { LACT_BF16 = 0, LACT_F32 = 1 };
+enum { LACT_BF16 = 0, LACT_F32 = 1, LACT_E4M3 = 2 };      /* LACT_E4M3: pages of a cache only */
 enum { LACT_UPDATE = 0, LACT_APPLY = 1 };
 /* Newton-Schulz numerics.  AUTOCAST: bf16 GEMM operands, fp32 accumulation and fp32 iterate, what
  * ttt_operation.py:30-66 computes under torch.autocast(bf16).  PLAIN_BF16: the iterate itself is
@@ -292,6 +292,52 @@ typedef struct lact_attention_step_desc {
 size_t lact_attention_step_workspace_bytes(const lact_attention_step_desc_t* desc);
 int lact_attention_step(const lact_attention_step_desc_t* desc, const void* q, const void* k, const void* v, const int32_t* lengths, void* out,
                         void* workspace, void* stream);
+
+/* A cache of keys and values in pages: k, v [pages, HK, page_size, D], D = 64 or 128, page_size a multiple of 16, of act_dtype or e4m3 (LACT_E4M3), dense inside a page,
+ * 16-byte aligned pages *_page elements apart.  e4m3: an exponent (e8m0) beside every row, [pages, HK, page_size], pages *e_page bytes apart: the row is its numbers times
+ * 2^(e - 127).  Tables [B, width] int32 say on which page the places n * page_size ... of a sequence lie; entries outside 0 .. pages - 1 are no page.  They, lengths,
+ * starts and counts are device memory and not checked: places outside the table or on no page are not written, read as zeros and not seen. */
+typedef struct lact_paged_cache {
+  int32_t dtype, pages, page_size, HK, D, width;
+  int64_t k_page, v_page, ke_page, ve_page;
+  void* k;
+  void* v;
+  uint8_t* k_exponents;
+  uint8_t* v_exponents;
+} lact_paged_cache_t;
+
+/* Tokens into their places: k, v [B, L, HK, D] of act_dtype with token (*_ld) and batch (*_bs) strides in elements, heads contiguous, rows 16-byte aligned.  Token t of
+ * sequence b goes to place starts[b] + t (starts null: t) where t < counts[b] (counts null: all).  e4m3: to nearest, ties to even; the exponent is the smallest
+ * (0 .. 254) with which the row's largest finite magnitude is at most 448 * 2^(e - 127); what is not finite becomes NaN. */
+int lact_paged_cache_write(const lact_paged_cache_t* cache, int32_t act_dtype, int32_t B, int32_t L, const void* k, int64_t k_ld, int64_t k_bs, const void* v,
+                           int64_t v_ld, int64_t v_bs, const int32_t* table, const int32_t* starts, const int32_t* counts, void* stream);
+/* And back: k, v [B, L, HK, D] of act_dtype, contiguous: place starts[b] + t, zeros from lengths[b] on. */
+int lact_paged_cache_read(const lact_paged_cache_t* cache, int32_t act_dtype, int32_t B, int32_t L, const int32_t* table, const int32_t* starts, const int32_t* lengths,
+                          void* k, void* v, void* stream);
+
+/* lact_attention_step over pages: q, out [B, H, D] of act_dtype (q_bs between sequences); the first lengths[b] places are the sequence, the last of them the new token's.
+ * A sequence that sees no place has output 0.  workspace: lact_paged_attention_step_workspace_bytes bytes (0: an error). */
+typedef struct lact_paged_step_desc {
+  int32_t act_dtype, B, H, window;
+  float scale, score_cap;
+  int64_t q_bs;
+  const float* slopes;
+} lact_paged_step_desc_t;
+size_t lact_paged_attention_step_workspace_bytes(const lact_paged_cache_t* cache, const lact_paged_step_desc_t* desc, const int32_t* table);
+int lact_paged_attention_step(const lact_paged_cache_t* cache, const lact_paged_step_desc_t* desc, const void* q, const int32_t* table, const int32_t* lengths, void* out,
+                              void* workspace, void* stream);
+
+/* Rotary positions with several axes: pair p of a head's channels, (2 p, 2 p + 1) if interleaved, else (p, p + pairs), is turned by the angle
+ * positions[b, l, axis_of_pair[p]] * frequencies[p], backwards if inverse (which is the gradient); the channels from 2 * pairs on go through.
+ * q: [B, L, H, D], k: [B, L, HK, D] (HK 0: none) with batch, token and head strides in elements, D even and at most 256; outputs contiguous.  positions: int32, int64 or
+ * fp32 (position_type 0, 1, 2), batch and token strides in elements, axes contiguous.  frequencies and axis_of_pair are host memory, [pairs]. */
+typedef struct lact_rotary_desc {
+  int32_t act_dtype, B, L, H, HK, D, pairs, n_axes, interleaved, inverse, position_type;
+  int64_t q_bs, q_ls, q_hs, k_bs, k_ls, k_hs, p_bs, p_ls;
+  const double* frequencies;
+  const int32_t* axis_of_pair;
+} lact_rotary_desc_t;
+int lact_axial_rotary(const lact_rotary_desc_t* desc, const void* q, const void* k, const void* positions, void* q_out, void* k_out, void* stream);
 
 /* Linear attention with a decay: S_t = e^(g_t) S_(t-1) + k_t v_t^T, out_t = scale S_t^T q_t; dk, dv = 64 or 128.
  * q, k: [b, l, h, dk], v, dout: [b, l, h, dv] as above; g: fp32 log decays, contiguous [b, l, h] (decay_per_token) or [h]; -infinity (anything

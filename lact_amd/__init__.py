@@ -10,6 +10,8 @@ The package mirrors the reference's call signatures for this one path:
 and has token mixers to go beside it:
   lact_amd.attention         softmax attention over documents, and for single tokens against a cache
   lact_amd.linear_attention  linear attention with a decay, and for single tokens
+  lact_amd.paged_cache       a cache of keys and values in pages, in 8 bits too, and the attention of single tokens with it
+  lact_amd.rotary            rotary positions with several axes
 All arithmetic runs in lib/liblact_hip.so (built from csrc/ with hipcc for gfx950)."""
 from .ops import NS5_COEFFS, NS_CLASSIC, Program, block_causal_steps, check_async_error, run_program  # noqa: F401
 from .ttt_operation import (block_causal_lact_swiglu, l2_norm, prenorm_block_causal_lact_swiglu,  # noqa: F401
@@ -22,3 +24,5 @@ from .layers import (BidirectionalLaCTSwiGLU, CausalLaCTSwiGLUWithSlidingWindowA
                      sliding_window_attention)
 from .attention import masked_window_attention, window_attention_step  # noqa: F401
 from .linear_attention import decayed_linear_attention, decayed_linear_attention_step  # noqa: F401
+from .paged_cache import PagedCache, paged_attention_step, paged_cache_read, paged_cache_write  # noqa: F401
+from .rotary import axial_rotary  # noqa: F401

@@ -3,12 +3,12 @@
 There is no fallback: if the library has not been built, every operation raises."""
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_float, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_void_p
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "liblact_hip.so")
 
-LACT_BF16, LACT_F32 = 0, 1
+LACT_BF16, LACT_F32, LACT_E4M3 = 0, 1, 2
 LACT_UPDATE, LACT_APPLY = 0, 1
 
 
@@ -50,6 +50,21 @@ class LinearDesc(Structure):
                 [(n, c_int32) for n in ("q_ld", "k_ld", "v_ld", "do_ld")] + [(n, c_int64) for n in ("q_bs", "k_bs", "v_bs", "do_bs")])
 
 
+class PagedCacheDesc(Structure):
+    _fields_ = ([(n, c_int32) for n in ("dtype", "pages", "page_size", "HK", "D", "width")] + [(n, c_int64) for n in ("k_page", "v_page", "ke_page", "ve_page")] +
+                [(n, c_void_p) for n in ("k", "v", "k_exponents", "v_exponents")])
+
+
+class PagedStepDesc(Structure):
+    _fields_ = ([(n, c_int32) for n in ("act_dtype", "B", "H", "window")] + [("scale", c_float), ("score_cap", c_float), ("q_bs", c_int64), ("slopes", c_void_p)])
+
+
+class RotaryDesc(Structure):
+    _fields_ = ([(n, c_int32) for n in ("act_dtype", "B", "L", "H", "HK", "D", "pairs", "n_axes", "interleaved", "inverse", "position_type")] +
+                [(n, c_int64) for n in ("q_bs", "q_ls", "q_hs", "k_bs", "k_ls", "k_hs", "p_bs", "p_ls")] +
+                [("frequencies", POINTER(c_double)), ("axis_of_pair", POINTER(c_int32))])
+
+
 OPT_STREAM_OVERLAP, OPT_FUSED_NEWTON_SCHULZ, OPT_NS_BARRIER_SPIN_LIMIT, OPT_PERSISTENT_TILES, OPT_KEEP_PREACTIVATIONS = 0, 1, 2, 3, 4
 EXPORTS = ("lact_last_error", "lact_version", "lact_query_sizes", "lact_forward", "lact_forward_from_state", "lact_backward",
            "lact_forward_shared_weights", "lact_backward_shared_weights",
@@ -63,7 +78,8 @@ EXPORTS = ("lact_last_error", "lact_version", "lact_query_sizes", "lact_forward"
            "lact_layer_pre_attn_part_rows", "lact_layer_pre_attn_backward", "lact_layer_post_add_forward",
            "lact_attention_ranges_bytes", "lact_masked_attention_workspace_bytes", "lact_masked_attention_forward", "lact_masked_attention_backward", "lact_attention_step_workspace_bytes",
            "lact_attention_step", "lact_linear_attention_sizes", "lact_linear_attention_forward", "lact_linear_attention_backward",
-           "lact_linear_attention_step")
+           "lact_linear_attention_step", "lact_paged_cache_write", "lact_paged_cache_read", "lact_paged_attention_step_workspace_bytes", "lact_paged_attention_step",
+           "lact_axial_rotary")
 
 HOST_PATH = os.path.join(HERE, "lib", "_lact_host.so")
 
@@ -158,7 +174,13 @@ def lib():
     L.lact_linear_attention_forward.argtypes = [POINTER(LinearDesc)] + [vp] * 9
     L.lact_linear_attention_backward.argtypes = [POINTER(LinearDesc)] + [vp] * 16
     L.lact_linear_attention_step.argtypes = [i32] * 6 + [f32, vp, c_int64, vp, c_int64, vp, c_int64] + [vp] * 5
-    for fn in ("lact_masked_attention_forward", "lact_masked_attention_backward", "lact_attention_step", "lact_linear_attention_sizes",
+    L.lact_paged_cache_write.argtypes = [POINTER(PagedCacheDesc)] + [i32] * 3 + [vp, c_int64, c_int64] * 2 + [vp] * 4
+    L.lact_paged_cache_read.argtypes = [POINTER(PagedCacheDesc)] + [i32] * 3 + [vp] * 6
+    L.lact_paged_attention_step_workspace_bytes.argtypes = [POINTER(PagedCacheDesc), POINTER(PagedStepDesc), vp]
+    L.lact_paged_attention_step_workspace_bytes.restype = c_size_t
+    L.lact_paged_attention_step.argtypes = [POINTER(PagedCacheDesc), POINTER(PagedStepDesc)] + [vp] * 6
+    L.lact_axial_rotary.argtypes = [POINTER(RotaryDesc)] + [vp] * 6
+    for fn in ("lact_paged_cache_write", "lact_paged_cache_read", "lact_paged_attention_step", "lact_axial_rotary", "lact_masked_attention_forward", "lact_masked_attention_backward", "lact_attention_step", "lact_linear_attention_sizes",
                "lact_linear_attention_forward", "lact_linear_attention_backward", "lact_linear_attention_step"):
         getattr(L, fn).restype = c_int32
     L.lact_profile_enable.argtypes = [c_int32]

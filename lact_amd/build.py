@@ -6,7 +6,7 @@ import sys
 import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SOURCES = [os.path.join(HERE, "csrc", f) for f in ("lact_api.hip", "mixers_api.hip")]
+SOURCES = [os.path.join(HERE, "csrc", f) for f in ("lact_api.hip", "mixers_api.hip", "paged_api.hip")]
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "liblact_hip.so")
 HOST_SRC = os.path.join(HERE, "csrc", "torch_host.cpp")

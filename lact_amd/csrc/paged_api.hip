@@ -1,0 +1,275 @@
+// Host side of the paged cache and of rotary positions (paged_cache.h, paged_attention.h, rotary.h): checks the arguments and enqueues the kernels on the caller's
+// stream.  No allocation, no synchronisation.
+#include "../../include/lact_hip.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "host_common.h"
+#include "paged_attention.h"
+#include "rotary.h"
+
+using namespace lact;
+
+namespace {
+
+constexpr int COMPUTE_UNITS = 256;
+constexpr long long MAX_ROWS = (1LL << 31) - 1;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+int check_type(int act) { return act == LACT_BF16 || act == LACT_F32 ? 0 : fail("act_dtype must be LACT_BF16 or LACT_F32"); }
+
+int check_cache(const lact_paged_cache_t* c, int act, const int32_t* table) {
+  if (!c) return fail("null descriptor");
+  if (check_type(act)) return -1;
+  if (c->dtype != LACT_E4M3 && c->dtype != act) return fail("paged cache: pages must be of act_dtype or LACT_E4M3");
+  if (c->pages <= 0 || c->page_size <= 0 || c->HK <= 0 || c->width <= 0) return fail("paged cache: pages, page_size, HK and width must be positive");
+  if (c->D != 64 && c->D != 128) return fail("paged cache: head size must be 64 or 128");
+  if (c->page_size % 16) return fail("paged cache: the page size must be a multiple of 16");
+  if ((long long)c->width * c->page_size > (1 << 24) || (long long)c->HK * c->page_size > (1 << 24)) return fail("paged cache: too many places in a sequence, or rows in a page");
+  const long long al = c->dtype == LACT_E4M3 ? 16 : c->dtype == LACT_BF16 ? 8 : 4, rows = (long long)c->HK * c->page_size;
+  if (!c->k || !c->v || !table) return fail("null pointer: paged cache");
+  if (c->k_page % al || c->v_page % al || !aligned16(c->k) || !aligned16(c->v)) return fail("paged cache: pages must be 16-byte aligned");
+  if (c->k_page < rows * c->D || c->v_page < rows * c->D) return fail("paged cache: pages must not overlap");
+  if (c->dtype == LACT_E4M3) {
+    if (!c->k_exponents || !c->v_exponents) return fail("null pointer: paged cache exponents");
+    if (c->ke_page % 16 || c->ve_page % 16 || !aligned16(c->k_exponents) || !aligned16(c->v_exponents)) return fail("paged cache: exponents must be 16-byte aligned");
+    if (c->ke_page < rows || c->ve_page < rows) return fail("paged cache: pages of exponents must not overlap");
+  }
+  return 0;
+}
+Pages pages_of(const lact_paged_cache_t* c, const int32_t* table) {
+  Pages p;
+  memset(&p, 0, sizeof(p));
+  p.pages = c->pages; p.size = c->page_size; p.wide = c->width; p.HK = c->HK;
+  p.by_size = make_udiv(c->page_size);
+  p.table = table;
+  p.k_page = c->k_page; p.v_page = c->v_page; p.ks_page = c->ke_page; p.vs_page = c->ve_page;
+  p.k = c->k; p.v = c->v; p.ks = c->k_exponents; p.vs = c->v_exponents;
+  return p;
+}
+
+// Memory that is written, or that is read meanwhile: `n` pieces of `len` bytes, `stride` apart.
+struct Pieces {
+  uintptr_t at;
+  long long n, stride, len;
+  uintptr_t end() const { return at + (n - 1) * stride + len; }
+};
+bool disjoint(const Pieces& a, const Pieces& b) {
+  if (a.end() <= b.at || b.end() <= a.at) return true;
+  if (a.n == 1 || b.n == 1 || a.stride != b.stride) return false;      // (one inside the other's gaps: nobody's layout)
+  const long long d = (long long)((b.at - a.at) % (uintptr_t)a.stride);      // parts of the same page, however many pages apart they begin
+  return d >= a.len && a.stride - d >= b.len;
+}
+// What a write goes to, nothing of which may lie in another part of it or in what is read.
+int check_apart(const lact_paged_cache_t* c, std::initializer_list<Pieces> read) {
+  const long long rows = (long long)c->HK * c->page_size, size = c->dtype == LACT_E4M3 ? 1 : c->dtype == LACT_BF16 ? 2 : 4;
+  auto pages = [&](const void* p, long long stride, long long len) { return Pieces{reinterpret_cast<uintptr_t>(p), c->pages, stride, len}; };
+  const Pieces to[4] = {pages(c->k, c->k_page * size, rows * c->D * size), pages(c->v, c->v_page * size, rows * c->D * size), pages(c->k_exponents, c->ke_page, rows),
+                        pages(c->v_exponents, c->ve_page, rows)};
+  for (int i = 0, n = c->dtype == LACT_E4M3 ? 4 : 2; i < n; ++i) {
+    for (int j = 0; j < i; ++j)
+      if (!disjoint(to[i], to[j])) return fail("paged cache write: keys, values and exponents must not overlap");
+    for (const Pieces& r : read)
+      if (r.at && !disjoint(to[i], r)) return fail("paged cache write: what is read must not lie in the cache");
+  }
+  return 0;
+}
+
+// f(type of the tokens, type of the pages, head size)
+template <typename F>
+int by_types(int act, int held, int D, F f) {
+  auto with = [&](auto t, auto c) { return D == 128 ? f(t, c, std::integral_constant<int, 128>()) : f(t, c, std::integral_constant<int, 64>()); };
+  if (act == LACT_BF16) return held == LACT_E4M3 ? with(uint16_t(), uint8_t()) : with(uint16_t(), uint16_t());
+  return held == LACT_E4M3 ? with(float(), uint8_t()) : with(float(), float());
+}
+
+int check_tokens(const lact_paged_cache_t* c, int B, int L) {
+  if (B <= 0 || L <= 0) return fail("paged cache: B and L must be positive");
+  if ((long long)B * c->HK * L > MAX_ROWS) return fail("paged cache: too many tokens in one call");
+  return 0;
+}
+template <typename T, int D>
+dim3 row_blocks(int B, int HK, int L) {
+  const long long per = CACHE_ROWS * (256 / (D * (int)sizeof(T) / 16));
+  return dim3((unsigned)(((long long)B * HK * L + per - 1) / per), 2);
+}
+
+// ---- one token's attention --------------------------------------------------------------------------
+int check_step(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d, const int32_t* table) {
+  if (!d) return fail("null descriptor");
+  if (check_cache(c, d->act_dtype, table)) return -1;
+  if (d->B <= 0 || d->H <= 0 || d->window <= 0) return fail("paged attention step: B, H and window must be positive");
+  if (d->H % c->HK) return fail("paged attention step: the number of key heads must divide that of query heads");
+  if ((long long)d->B * d->H > (1 << 20)) return fail("paged attention step: batch too large");
+  if (!(d->scale > 0.f) || !std::isfinite(d->scale)) return fail("paged attention step: the scale must be positive");
+  if (!(d->score_cap >= 0.f) || !std::isfinite(d->score_cap)) return fail("paged attention step: the score cap must be positive, or 0 for none");
+  if (d->q_bs < 0 || d->q_bs % (d->act_dtype == LACT_BF16 ? 8 : 4)) return fail("paged attention step: queries must be 16-byte aligned");
+  return 0;
+}
+int places(const lact_paged_cache_t* c) { return c->width * c->page_size; }
+template <typename C, int D>
+int step_blocks(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) {
+  // (a window that begins inside a piece of 16 reaches up to 15 places further back)
+  const long long tiles = ceil_div(d->H / c->HK, 32), steps = ceil_div(std::min(places(c), std::min(d->window, places(c)) + 15), PagedShape<C, D>::KEYS);
+  return (int)std::min<long long>(COMPUTE_UNITS, d->B * c->HK * tiles * steps);
+}
+template <typename C, int D>
+size_t step_workspace(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) {
+  return (size_t)2 * step_blocks<C, D>(c, d) * std::min(d->H / c->HK, 32) * (D + 2) * sizeof(float);
+}
+template <typename T, typename C, int D>
+int step_run(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d, const void* q, const int32_t* table, const int32_t* lengths, void* out, void* workspace,
+             hipStream_t s) {
+  PagedStepParams<T> p;
+  memset(&p, 0, sizeof(p));
+  p.kv = pages_of(c, table);
+  p.B = d->B; p.N = places(c); p.H = d->H; p.HK = c->HK; p.group = d->H / c->HK; p.tiles = ceil_div(p.group, 32);
+  p.window = std::min(d->window, p.N);
+  p.blocks = step_blocks<C, D>(c, d);
+  p.q = static_cast<const T*>(q); p.bsq = d->q_bs;
+  p.lengths = lengths; p.slopes = d->slopes; p.scale = d->scale; p.cap = d->score_cap;
+  p.out = static_cast<T*>(out); p.part = static_cast<float*>(workspace);
+  using A = PagedShape<C, D>;
+  auto launch = [&](auto kind) {
+    constexpr int BENT = decltype(kind)::value;
+    LACT_BIG_LDS((k_paged_step<T, C, D, BENT>), A::LDS);
+    LACT_LAUNCH_SMEM("k_paged_step", "paged_step", 0.0, (k_paged_step<T, C, D, BENT>), dim3(p.blocks), dim3(64 * A::NW), A::LDS, s, p);
+  };
+  if (sizeof(T) == 2 && p.cap > CAP_QUICK) launch(std::integral_constant<int, sizeof(T) == 2 ? SCORES_FAR_CAP : SCORES_BENT>());
+  else launch(std::integral_constant<int, SCORES_BENT>());
+  LACT_LAUNCH("k_attn_step_join", "paged_step", 0.0, (k_attn_step_join<T, D, A::KEYS, PagedStepParams<T>>), dim3(p.B * p.H), dim3(512), s, p);
+  LACT_CHECK_LAUNCH();
+  return 0;
+}
+
+// ---- rotary positions -------------------------------------------------------------------------------
+int check_rotary(const lact_rotary_desc_t* d) {
+  if (!d) return fail("null descriptor");
+  if (check_type(d->act_dtype)) return -1;
+  if (d->B <= 0 || d->L <= 0 || d->H <= 0 || d->HK < 0) return fail("rotary: B, L and H must be positive");
+  if (d->D <= 0 || d->D % 2 || d->D > 2 * ROTARY_PAIRS) return fail("rotary: head size must be even and at most 256");
+  if (d->pairs <= 0 || 2 * d->pairs > d->D) return fail("rotary: pairs must be positive and fit the head");
+  if (d->n_axes <= 0 || d->n_axes > 256) return fail("rotary: 1 to 256 axes");
+  if ((long long)d->B * d->L > MAX_ROWS || (long long)d->H + d->HK > 65535) return fail("rotary: too many tokens or heads");
+  if (d->position_type < 0 || d->position_type > 2) return fail("rotary: positions must be int32, int64 or fp32");
+  if (!d->frequencies || !d->axis_of_pair) return fail("null pointer: rotary tables");
+  for (int i = 0; i < d->pairs; ++i)
+    if (d->axis_of_pair[i] < 0 || d->axis_of_pair[i] >= d->n_axes || !std::isfinite(d->frequencies[i])) return fail("rotary: axes of pairs or frequencies out of range");
+  return 0;
+}
+template <typename T, int V, bool SIDE>
+void launch_rotary(RotaryParams p, hipStream_t s) {
+  p.units = SIDE ? p.D / V : p.pairs / V + (p.D - 2 * p.pairs) / V;
+  p.by_units = make_udiv(p.units);
+  p.tokens = 256 / p.units;
+  const int heads = p.op[0].heads + p.op[1].heads;
+  const long long blocks = ((long long)p.B * p.L + p.tokens - 1) / p.tokens;
+  p.per = (int)std::max<long long>(1, std::min<long long>(heads, blocks * heads / (8 * COMPUTE_UNITS)));
+  LACT_LAUNCH("k_rotary", "rotary", 0.0, (k_rotary<T, V, SIDE>), dim3((unsigned)blocks, ceil_div(heads, p.per)), dim3(256), s, p);
+}
+template <typename T>
+void launch_rotary(const RotaryParams& p, bool side, hipStream_t s) {
+  constexpr int E = 16 / (int)sizeof(T);
+  bool wide = p.D % E == 0 && (side || p.pairs % E == 0);
+  for (const auto& o : p.op) wide = wide && (!o.heads || (aligned16(o.x) && aligned16(o.y) && o.bs % E == 0 && o.ls % E == 0 && o.hs % E == 0));
+  if (side) wide ? launch_rotary<T, E, true>(p, s) : launch_rotary<T, 2, true>(p, s);
+  else wide ? launch_rotary<T, E, false>(p, s) : launch_rotary<T, 1, false>(p, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int lact_paged_cache_write(const lact_paged_cache_t* c, int32_t act_dtype, int32_t B, int32_t L, const void* k, int64_t k_ld, int64_t k_bs, const void* v, int64_t v_ld,
+                           int64_t v_bs, const int32_t* table, const int32_t* starts, const int32_t* counts, void* stream) {
+  if (check_cache(c, act_dtype, table) || check_tokens(c, B, L) || check_ptrs({k, v}, "paged cache write tensors")) return -1;
+  const int al = act_dtype == LACT_BF16 ? 8 : 4;
+  if (k_ld % al || k_bs % al || v_ld % al || v_bs % al || !aligned16(k) || !aligned16(v) || k_ld < 0 || k_bs < 0 || v_ld < 0 || v_bs < 0)
+    return fail("paged cache write: rows must be 16-byte aligned");
+  const long long size = act_dtype == LACT_BF16 ? 2 : 4, row = (long long)c->HK * c->D;
+  auto whole = [](const void* p, long long bytes) { return Pieces{reinterpret_cast<uintptr_t>(p), 1, 0, bytes}; };
+  if (check_apart(c, {whole(k, ((B - 1) * k_bs + (L - 1) * k_ld + row) * size), whole(v, ((B - 1) * v_bs + (L - 1) * v_ld + row) * size),
+                      whole(table, (long long)B * c->width * 4), whole(starts, B * 4LL), whole(counts, B * 4LL)}))
+    return -1;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return by_types(act_dtype, c->dtype, c->D, [&](auto t, auto h, auto d) {
+    using T = decltype(t);
+    using C = decltype(h);
+    constexpr int D = decltype(d)::value;
+    CacheWriteParams<T> p;
+    memset(&p, 0, sizeof(p));
+    p.to = pages_of(c, table);
+    p.B = B; p.L = L; p.by_l = make_udiv(L); p.by_heads = make_udiv(c->HK);
+    p.k = static_cast<const T*>(k); p.v = static_cast<const T*>(v);
+    p.ldk = k_ld; p.bsk = k_bs; p.ldv = v_ld; p.bsv = v_bs;
+    p.starts = starts; p.counts = counts;
+    LACT_LAUNCH("k_cache_write", "paged_cache", 0.0, (k_cache_write<T, C, D>), (row_blocks<T, D>(B, c->HK, L)), dim3(256), s, p);
+    LACT_CHECK_LAUNCH();
+    return 0;
+  });
+}
+
+int lact_paged_cache_read(const lact_paged_cache_t* c, int32_t act_dtype, int32_t B, int32_t L, const int32_t* table, const int32_t* starts, const int32_t* lengths,
+                          void* k, void* v, void* stream) {
+  if (check_cache(c, act_dtype, table) || check_tokens(c, B, L) || check_ptrs({k, v, lengths}, "paged cache read tensors")) return -1;
+  if (!aligned16(k) || !aligned16(v)) return fail("paged cache read: rows must be 16-byte aligned");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  return by_types(act_dtype, c->dtype, c->D, [&](auto t, auto h, auto d) {
+    using T = decltype(t);
+    using C = decltype(h);
+    constexpr int D = decltype(d)::value;
+    CacheReadParams<T> p;
+    memset(&p, 0, sizeof(p));
+    p.from = pages_of(c, table);
+    p.B = B; p.L = L; p.by_l = make_udiv(L); p.by_heads = make_udiv(c->HK);
+    p.k = static_cast<T*>(k); p.v = static_cast<T*>(v);
+    p.starts = starts; p.lengths = lengths;
+    LACT_LAUNCH("k_cache_read", "paged_cache", 0.0, (k_cache_read<T, C, D>), (row_blocks<T, D>(B, c->HK, L)), dim3(256), s, p);
+    LACT_CHECK_LAUNCH();
+    return 0;
+  });
+}
+
+size_t lact_paged_attention_step_workspace_bytes(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d, const int32_t* table) {
+  if (check_step(c, d, table)) return 0;
+  size_t bytes = 0;
+  by_types(d->act_dtype, c->dtype, c->D, [&](auto, auto h, auto e) {
+    bytes = step_workspace<decltype(h), decltype(e)::value>(c, d);
+    return 0;
+  });
+  return bytes;
+}
+
+int lact_paged_attention_step(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d, const void* q, const int32_t* table, const int32_t* lengths, void* out,
+                              void* workspace, void* stream) {
+  if (check_step(c, d, table) || check_ptrs({q, lengths, out, workspace}, "paged attention step tensors")) return -1;
+  if (!aligned16(q)) return fail("paged attention step: queries must be 16-byte aligned");
+  return by_types(d->act_dtype, c->dtype, c->D, [&](auto t, auto h, auto e) {
+    return step_run<decltype(t), decltype(h), decltype(e)::value>(c, d, q, table, lengths, out, workspace, reinterpret_cast<hipStream_t>(stream));
+  });
+}
+
+int lact_axial_rotary(const lact_rotary_desc_t* d, const void* q, const void* k, const void* positions, void* q_out, void* k_out, void* stream) {
+  if (check_rotary(d) || check_ptrs({q, positions, q_out}, "rotary tensors") || (d->HK && check_ptrs({k, k_out}, "rotary tensors"))) return -1;
+  RotaryParams p;
+  memset(&p, 0, sizeof(p));
+  p.op[0] = RotaryOperand{q, q_out, d->q_bs, d->q_ls, d->q_hs, d->H};
+  p.op[1] = RotaryOperand{k, k_out, d->k_bs, d->k_ls, d->k_hs, d->HK};
+  p.B = d->B; p.L = d->L; p.D = d->D; p.pairs = d->pairs; p.axes = d->n_axes;
+  p.by_l = make_udiv(d->L);
+  p.positions = positions; p.position_type = d->position_type; p.pos_bs = d->p_bs; p.pos_ls = d->p_ls;
+  p.sign = d->inverse ? -1.f : 1.f;
+  for (int i = 0; i < d->pairs; ++i) {
+    p.frequency[i] = d->frequencies[i] * 0.63661977236758134308;      // 2 / pi: quarter turns
+    p.axis[i] = (uint8_t)d->axis_of_pair[i];
+  }
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (d->act_dtype == LACT_BF16) launch_rotary<uint16_t>(p, d->interleaved, s);
+  else launch_rotary<float>(p, d->interleaved, s);
+  LACT_CHECK_LAUNCH();
+  return 0;
+}
+
+}  // extern "C"

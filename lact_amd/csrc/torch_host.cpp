@@ -903,6 +903,225 @@ std::vector<Tensor> linear_step(const Tensor& q_, const Tensor& k_, const Tensor
   return {out, next};
 }
 
+// ---- paged cache, rotary positions --------------------------------------------------------------------------------------
+struct CacheCall {
+  lact_paged_cache_t desc{};
+  Tensor table;
+  bool empty = false;      // no page, or no entry of the table
+};
+// The cache's four tensors and the table, checked.  `act`: the type of the tokens, whose pages are of it or of 8 bits.
+CacheCall paged_cache(const Tensor& k, const Tensor& v, const OptTensor& ks, const OptTensor& vs, const Tensor& table, int64_t b, at::ScalarType act) {
+  CacheCall c;
+  auto& D = c.desc;
+  const bool eight = k.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK_TYPE(eight || k.scalar_type() == act, "pages must be ", act, " or Float8_e4m3fn, got ", k.scalar_type());
+  TORCH_CHECK_TYPE(v.scalar_type() == k.scalar_type(), "the cache's values are ", v.scalar_type(), ", its keys ", k.scalar_type());
+  expect(v, k, k.sizes(), "cache.v");
+  if (eight != ks.has_value() || eight != vs.has_value()) throw std::invalid_argument("pages of 8 bits have exponents (k_scale and v_scale), and no others do");
+  for (int i = 0; i < 4; ++i)
+    if (k.size(i) > INT32_MAX) throw std::invalid_argument("the cache is too large");
+  auto dense_inside = [](const Tensor& t) {
+    int64_t n = 1;
+    for (int64_t i = t.dim() - 1; i > 0; n *= t.size(i--))
+      if (t.size(i) != 1 && t.stride(i) != n) return false;
+    return aligned16(t);
+  };
+  auto page = [](const Tensor& t) { return t.size(0) == 1 ? t.numel() : t.stride(0); };
+  if (!dense_inside(k) || !dense_inside(v)) throw std::invalid_argument("pages must be contiguous [heads, page size, head size], on 16-byte boundaries");
+  if (eight) {
+    for (const auto* t : {&*ks, &*vs}) {
+      TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat8_e8m0fnu, "exponents must be Float8_e8m0fnu, got ", t->scalar_type());
+      expect(*t, k, k.sizes().slice(0, 3), "cache.k_scale and cache.v_scale");
+      if (!dense_inside(*t)) throw std::invalid_argument("exponents must be contiguous [heads, page size], on 16-byte boundaries");
+    }
+    D.k_exponents = static_cast<uint8_t*>(ks->data_ptr());
+    D.v_exponents = static_cast<uint8_t*>(vs->data_ptr());
+    D.ke_page = page(*ks); D.ve_page = page(*vs);
+  }
+  if (table.dim() != 2 || table.size(1) > INT32_MAX) throw std::invalid_argument("page_table must have 2 dimensions");
+  c.table = indices(table, k, {b, table.size(1)}, "page_table");
+  D.dtype = eight ? LACT_E4M3 : act == at::kBFloat16 ? LACT_BF16 : LACT_F32;
+  D.pages = (int)k.size(0); D.HK = (int)k.size(1); D.page_size = (int)k.size(2); D.D = (int)k.size(3); D.width = (int)table.size(1);
+  D.k_page = page(k); D.v_page = page(v);
+  D.k = k.data_ptr(); D.v = v.data_ptr();
+  c.empty = D.pages == 0 || D.width == 0;
+  return c;
+}
+
+void cache_write(const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& k_, const Tensor& v_, const Tensor& table, const OptTensor& starts_,
+                 const OptTensor& counts_) {
+  on_gpu(k_);
+  const c10::hip::HIPGuard guard(k_.device().index());
+  const at::AutoGradMode off(false);
+  const int act = act_code(k_);
+  const Tensor k4 = k_.dim() == 3 ? k_.unsqueeze(1) : k_, v4 = v_.dim() == 3 ? v_.unsqueeze(1) : v_;      // one token of every sequence
+  const int64_t b = k4.size(0), l = k4.size(1), hk = ck.size(1), d = ck.size(3);
+  expect_same(v4, k4, "v");
+  expect(k4, k4, {b, l, hk, d}, "k");
+  expect(v4, k4, {b, l, hk, d}, "v");
+  expect(ck, k4, ck.sizes(), "cache.k");
+  const CacheCall c = paged_cache(ck, cv, ks, vs, table, b, k4.scalar_type());
+  const Tensor starts = indices(starts_, k4, {b}, "starts"), counts = indices(counts_, k4, {b}, "counts");
+  std::vector<const Tensor*> written{&ck, &cv};
+  if (ks) written.insert(written.end(), {&*ks, &*vs});
+  if (b == 0 || l == 0 || hk == 0 || c.empty) return;
+  const Tensor k = head_rows(k4.resolve_neg()), v = head_rows(v4.resolve_neg());
+  if (l > INT32_MAX || b > INT32_MAX) throw std::invalid_argument("too many tokens in one call");
+  check(lact_paged_cache_write(&c.desc, act, (int)b, (int)l, ptr(k), k.stride(1), k.stride(0), ptr(v), v.stride(1), v.stride(0), fptr<int32_t>(c.table),
+                               fptr<int32_t>(starts), fptr<int32_t>(counts), stream()));
+  for (const Tensor* t : written)
+    if (!t->is_inference()) torch::autograd::impl::bump_version(*t);
+}
+
+std::vector<Tensor> cache_read(const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& table, const Tensor& lengths_, int64_t l,
+                               const OptTensor& starts_, at::ScalarType dtype) {
+  on_gpu(ck);
+  const c10::hip::HIPGuard guard(ck.device().index());
+  const at::AutoGradMode off(false);
+  TORCH_CHECK_TYPE(dtype == at::kBFloat16 || dtype == at::kFloat, "unsupported dtype ", dtype, ": bf16 or fp32");
+  const int64_t b = lengths_.size(0), hk = ck.size(1), d = ck.size(3);
+  const CacheCall c = paged_cache(ck, cv, ks, vs, table, b, dtype);
+  const Tensor lengths = indices(lengths_, ck, {b}, "lengths"), starts = indices(starts_, ck, {b}, "starts");
+  const auto opt = ck.options().dtype(dtype);
+  if (b == 0 || l == 0 || hk == 0 || d == 0 || c.empty) return {at::zeros({b, l, hk, d}, opt), at::zeros({b, l, hk, d}, opt)};
+  if (l > INT32_MAX || b > INT32_MAX) throw std::invalid_argument("too many tokens in one call");
+  const Tensor k = at::empty({b, l, hk, d}, opt), v = at::empty({b, l, hk, d}, opt);
+  check(lact_paged_cache_read(&c.desc, dtype == at::kBFloat16 ? LACT_BF16 : LACT_F32, (int)b, (int)l, fptr<int32_t>(c.table), fptr<int32_t>(starts), fptr<int32_t>(lengths),
+                              ptr(k), ptr(v), stream()));
+  return {k, v};
+}
+
+Tensor paged_step(const Tensor& q_, const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& table, const Tensor& lengths_, int64_t window,
+                  double scale, double cap, const OptTensor& slopes_) {
+  on_gpu(q_);
+  const c10::hip::HIPGuard guard(q_.device().index());
+  const at::AutoGradMode off(false);
+  lact_paged_step_desc_t D{};
+  D.act_dtype = act_code(q_);
+  const int64_t b = q_.size(0), h = q_.size(1), d = q_.size(2);
+  expect(ck, q_, {ck.size(0), ck.size(1), ck.size(2), d}, "cache.k");
+  const CacheCall c = paged_cache(ck, cv, ks, vs, table, b, q_.scalar_type());
+  const Tensor lengths = indices(lengths_, q_, {b}, "lengths"), q = dense(q_.resolve_neg());
+  Tensor slopes;
+  if (slopes_) {
+    expect(*slopes_, q_, {h}, "distance_slopes");
+    slopes = plain_f32(*slopes_);
+  }
+  const Tensor out = at::empty({b, h, d}, q_.options());
+  if (out.numel() == 0 || c.empty) return out.zero_();
+  D.B = (int)b; D.H = (int)h; D.window = (int)std::min<int64_t>(window, 1 << 30);
+  D.scale = (float)scale; D.score_cap = (float)cap;
+  D.q_bs = h * d;
+  D.slopes = fptr(slopes);
+  const int64_t bytes = (int64_t)lact_paged_attention_step_workspace_bytes(&c.desc, &D, fptr<int32_t>(c.table));
+  if (bytes == 0) check(-1);
+  const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  check(lact_paged_attention_step(&c.desc, &D, ptr(q), fptr<int32_t>(c.table), fptr<int32_t>(lengths), ptr(out), ptr(ws), stream()));
+  return out;
+}
+
+// Pairs of channels: their axes, and how far a unit of position turns them.
+struct RotaryTable {
+  std::vector<double> frequencies;
+  std::vector<int32_t> axes;
+  int64_t n_axes = 0;
+  RotaryTable(const std::vector<int64_t>& sizes, double base, const std::vector<double>& given) : frequencies(given), n_axes((int64_t)sizes.size()) {
+    int64_t pairs = 0;
+    for (const int64_t n : sizes) pairs += n / 2;
+    axes.reserve(pairs);
+    frequencies.reserve(pairs);
+    for (size_t a = 0; a < sizes.size(); ++a) {
+      const long double ratio = std::pow((long double)base, -2.0L / sizes[a]);      // (64 products of long doubles lose nothing that a double has)
+      long double f = 1.0L;
+      for (int64_t i = 0; i < sizes[a] / 2; ++i, f *= ratio) {
+        axes.push_back((int32_t)a);
+        if (given.empty()) frequencies.push_back((double)f);
+      }
+    }
+  }
+};
+struct RotaryCall {
+  lact_rotary_desc_t desc{};
+  Tensor positions;
+};
+// q (and k) turned, forwards or backwards: [b, l, h, d], or [b, h, d] with one position a sequence
+variable_list rotary_run(const Tensor& q_, const Tensor& k_, const Tensor& positions, const RotaryTable& table, bool interleaved, bool inverse) {
+  lact_rotary_desc_t D{};
+  D.act_dtype = act_code(q_);
+  const bool one = q_.dim() == 3;
+  auto rows = [](const Tensor& t) { return !t.defined() || (t.stride(-1) == 1 && !t.is_neg()) ? t : t.clone(at::MemoryFormat::Contiguous).resolve_neg(); };
+  const Tensor q = rows(q_), k = rows(k_);
+  D.B = (int)q.size(0); D.L = one ? 1 : (int)q.size(1); D.H = (int)q.size(-2); D.HK = k.defined() ? (int)k.size(-2) : 0; D.D = (int)q.size(-1);
+  D.pairs = (int)table.axes.size(); D.n_axes = (int)table.n_axes; D.interleaved = interleaved; D.inverse = inverse;
+  D.position_type = positions.scalar_type() == at::kInt ? 0 : positions.scalar_type() == at::kLong ? 1 : 2;
+  D.q_bs = q.stride(0); D.q_ls = one ? 0 : q.stride(1); D.q_hs = q.stride(-2);
+  if (k.defined()) {
+    D.k_bs = k.stride(0); D.k_ls = one ? 0 : k.stride(1); D.k_hs = k.stride(-2);
+  }
+  const bool shared = !one && positions.dim() == 2;
+  D.p_bs = shared ? 0 : positions.stride(0);
+  D.p_ls = one ? 0 : positions.stride(-2);
+  D.frequencies = table.frequencies.data(); D.axis_of_pair = table.axes.data();
+  const Tensor yq = at::empty(q.sizes(), q.options()), yk = k.defined() ? at::empty(k.sizes(), k.options()) : Tensor();
+  check(lact_axial_rotary(&D, ptr(q), ptr(k), ptr(positions), ptr(yq), ptr(yk), stream()));
+  return {yq, yk};
+}
+struct RotaryArgs : torch::CustomClassHolder {
+  RotaryTable table;
+  bool interleaved;
+  RotaryArgs(RotaryTable t, bool i) : table(std::move(t)), interleaved(i) {}
+};
+struct RotaryFn : torch::autograd::Function<RotaryFn> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const OptTensor& k, const Tensor& positions, const c10::intrusive_ptr<RotaryArgs>& args) {
+    ctx->save_for_backward({positions});
+    ctx->saved_data["args"] = c10::IValue::make_capsule(args);
+    ctx->set_materialize_grads(false);
+    auto res = rotary_run(q, value(k), positions, args->table, args->interleaved, false);
+    if (!k) res.pop_back();
+    return res;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool twice = at::GradMode::is_enabled();
+    const at::AutoGradMode off(false);
+    const auto args = c10::static_intrusive_pointer_cast<RotaryArgs>(ctx->saved_data["args"].toCapsule());
+    const Tensor positions = ctx->get_saved_variables()[0], gq = grads[0], gk = grads.size() > 1 ? grads[1] : Tensor();
+    const c10::hip::HIPGuard guard(positions.device().index());
+    variable_list res{Tensor(), Tensor()};
+    if (gq.defined()) res = rotary_run(gq, gk, positions, args->table, args->interleaved, true);
+    else if (gk.defined()) res[1] = rotary_run(gk, Tensor(), positions, args->table, args->interleaved, true)[0];
+    return finish({res[0], res[1], Tensor(), Tensor()}, twice);
+  }
+};
+variable_list rotary(const Tensor& q, const OptTensor& k, const Tensor& positions_, const std::vector<int64_t>& axes, double base, const std::vector<double>& frequencies,
+                     bool interleaved) {
+  on_gpu(q);
+  const c10::hip::HIPGuard guard(q.device().index());
+  act_code(q);
+  std::vector<int64_t> want(q.sizes().begin(), q.sizes().end() - 2);
+  if (k) {
+    expect_same(*k, q, "k");
+    auto sizes = q.sizes().vec();
+    sizes[sizes.size() - 2] = k->size(-2);
+    expect(*k, q, sizes, "k");
+  }
+  TORCH_CHECK_TYPE(positions_.scalar_type() == at::kInt || positions_.scalar_type() == at::kLong || positions_.scalar_type() == at::kFloat,
+                   "positions must be int32, int64 or fp32, got ", positions_.scalar_type());
+  want.push_back((int64_t)axes.size());
+  if (q.dim() == 4 && positions_.dim() == 2) want.erase(want.begin());      // the same for every sequence
+  expect(positions_, q, want, "positions");
+  const Tensor positions = positions_.detach().resolve_neg().contiguous();
+  if (q.size(0) > INT32_MAX || (q.dim() == 4 && q.size(1) > INT32_MAX)) throw std::invalid_argument("too many tokens in one call");
+  RotaryTable table(axes, base, frequencies);
+  if (at::GradMode::is_enabled() && (q.requires_grad() || wants_grad(k))) {
+    refuse_leaves_of_eager_graphs({&q, k ? &*k : nullptr});
+    return RotaryFn::apply(q, k, positions, c10::make_intrusive<RotaryArgs>(std::move(table), interleaved));
+  }
+  const at::AutoGradMode off(false);
+  auto res = rotary_run(q, value(k), positions, table, interleaved, false);
+  if (!k) res.pop_back();
+  return res;
+}
+
 template <class F, class... Args>
 auto apply_released(Args&&... args) {
   const py::gil_scoped_release nogil;
@@ -947,6 +1166,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return return_state ? variable_list{c.out, c.last} : variable_list{c.out};
   });
   m.def("linear_attention_step", &linear_step, py::call_guard<py::gil_scoped_release>());
+  m.def("paged_cache_write", &cache_write, py::call_guard<py::gil_scoped_release>());
+  m.def("paged_cache_read", [](const Tensor& k, const Tensor& v, const OptTensor& ks, const OptTensor& vs, const Tensor& table, const Tensor& lengths, int64_t tokens,
+                               const OptTensor& starts, const py::object& dtype) {
+    const auto type = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
+    const py::gil_scoped_release nogil;
+    return cache_read(k, v, ks, vs, table, lengths, tokens, starts, type);
+  });
+  m.def("paged_attention_step", &paged_step, py::call_guard<py::gil_scoped_release>());
+  m.def("axial_rotary", &rotary, py::call_guard<py::gil_scoped_release>());
   m.def("linear", [](const Tensor& x, const Tensor& weight) { return apply_released<LinearFn>(autocast_bf16(x), weight, autocast_bf16(weight)); });
   m.def("layer_in", [](const Tensor& x, const Tensor& qkv_w, const Tensor& lr_w, const OptTensor& lr_b, const OptTensor& mom_w, const OptTensor& mom_b,
                        const OptTensor& gate_w, const OptTensor& gate_b) { return apply_released<LayerInFn>(x, qkv_w, autocast_bf16(qkv_w), lr_w, lr_b, mom_w, mom_b, gate_w, gate_b); });
