@@ -316,14 +316,14 @@ int lact_paged_cache_read(const lact_paged_cache_t* cache, int32_t act_dtype, in
                           void* k, void* v, void* stream);
 
 /* lact_attention_step over pages: q, out [B, H, D] of act_dtype (q_bs between sequences); the first lengths[b] places are the sequence, the last of them the new token's.
- * A sequence that sees no place has output 0.  workspace: lact_paged_attention_step_workspace_bytes bytes (0: an error). */
+ * A sequence that sees no place has output 0.  workspace: lact_paged_attention_step_workspace_bytes bytes (0 for short sequences, then null). */
 typedef struct lact_paged_step_desc {
   int32_t act_dtype, B, H, window;
   float scale, score_cap;
   int64_t q_bs;
   const float* slopes;
 } lact_paged_step_desc_t;
-size_t lact_paged_attention_step_workspace_bytes(const lact_paged_cache_t* cache, const lact_paged_step_desc_t* desc, const int32_t* table);
+int lact_paged_attention_step_workspace_bytes(const lact_paged_cache_t* cache, const lact_paged_step_desc_t* desc, const int32_t* table, size_t* bytes);
 int lact_paged_attention_step(const lact_paged_cache_t* cache, const lact_paged_step_desc_t* desc, const void* q, const int32_t* table, const int32_t* lengths, void* out,
                               void* workspace, void* stream);
 

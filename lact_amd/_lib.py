@@ -176,11 +176,10 @@ def lib():
     L.lact_linear_attention_step.argtypes = [i32] * 6 + [f32, vp, c_int64, vp, c_int64, vp, c_int64] + [vp] * 5
     L.lact_paged_cache_write.argtypes = [POINTER(PagedCacheDesc)] + [i32] * 3 + [vp, c_int64, c_int64] * 2 + [vp] * 4
     L.lact_paged_cache_read.argtypes = [POINTER(PagedCacheDesc)] + [i32] * 3 + [vp] * 6
-    L.lact_paged_attention_step_workspace_bytes.argtypes = [POINTER(PagedCacheDesc), POINTER(PagedStepDesc), vp]
-    L.lact_paged_attention_step_workspace_bytes.restype = c_size_t
+    L.lact_paged_attention_step_workspace_bytes.argtypes = [POINTER(PagedCacheDesc), POINTER(PagedStepDesc), vp, POINTER(c_size_t)]
     L.lact_paged_attention_step.argtypes = [POINTER(PagedCacheDesc), POINTER(PagedStepDesc)] + [vp] * 6
     L.lact_axial_rotary.argtypes = [POINTER(RotaryDesc)] + [vp] * 6
-    for fn in ("lact_paged_cache_write", "lact_paged_cache_read", "lact_paged_attention_step", "lact_axial_rotary", "lact_masked_attention_forward", "lact_masked_attention_backward", "lact_attention_step", "lact_linear_attention_sizes",
+    for fn in ("lact_paged_cache_write", "lact_paged_cache_read", "lact_paged_attention_step_workspace_bytes", "lact_paged_attention_step", "lact_axial_rotary", "lact_masked_attention_forward", "lact_masked_attention_backward", "lact_attention_step", "lact_linear_attention_sizes",
                "lact_linear_attention_forward", "lact_linear_attention_backward", "lact_linear_attention_step"):
         getattr(L, fn).restype = c_int32
     L.lact_profile_enable.argtypes = [c_int32]

@@ -109,37 +109,51 @@ int check_step(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d, con
   return 0;
 }
 int places(const lact_paged_cache_t* c) { return c->width * c->page_size; }
-template <typename C, int D>
-int step_blocks(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) {
-  // (a window that begins inside a piece of 16 reaches up to 15 places further back)
-  const long long tiles = ceil_div(d->H / c->HK, 32), steps = ceil_div(std::min(places(c), std::min(d->window, places(c)) + 15), PagedShape<C, D>::KEYS);
-  return (int)std::min<long long>(COMPUTE_UNITS, d->B * c->HK * tiles * steps);
+// (a window that begins inside a piece of 16 reaches up to 15 places further back)
+template <typename A>
+int most_steps(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) {
+  return ceil_div(std::min(places(c), std::min(d->window, places(c)) + 15), A::KEYS);
 }
-template <typename C, int D>
+int step_items(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) { return d->B * c->HK * ceil_div(d->H / c->HK, 32); }
+// One block for every item, where the longest has few steps, and no second launch.
+constexpr int WHOLE_STEPS = 4;
+template <typename A>
+bool step_whole(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) { return most_steps<A>(c, d) <= WHOLE_STEPS; }
+template <typename A>
+int step_blocks(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) {
+  const int items = step_items(c, d);
+  return step_whole<A>(c, d) ? items : (int)std::min<long long>(A::BLOCKS * COMPUTE_UNITS, (long long)items * most_steps<A>(c, d));
+}
+template <typename A, int D>
 size_t step_workspace(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) {
-  return (size_t)2 * step_blocks<C, D>(c, d) * std::min(d->H / c->HK, 32) * (D + 2) * sizeof(float);
+  return step_whole<A>(c, d) ? 0 : (size_t)2 * step_blocks<A>(c, d) * std::min(d->H / c->HK, 32) * (D + 2) * sizeof(float);
 }
 template <typename T, typename C, int D>
 int step_run(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d, const void* q, const int32_t* table, const int32_t* lengths, void* out, void* workspace,
              hipStream_t s) {
+  using A = PagedShape<T, C, D>;
   PagedStepParams<T> p;
   memset(&p, 0, sizeof(p));
   p.kv = pages_of(c, table);
   p.B = d->B; p.N = places(c); p.H = d->H; p.HK = c->HK; p.group = d->H / c->HK; p.tiles = ceil_div(p.group, 32);
   p.window = std::min(d->window, p.N);
-  p.blocks = step_blocks<C, D>(c, d);
+  p.whole = step_whole<A>(c, d);
+  p.blocks = step_blocks<A>(c, d);
   p.q = static_cast<const T*>(q); p.bsq = d->q_bs;
   p.lengths = lengths; p.slopes = d->slopes; p.scale = d->scale; p.cap = d->score_cap;
   p.out = static_cast<T*>(out); p.part = static_cast<float*>(workspace);
-  using A = PagedShape<C, D>;
+  if (!p.whole && !workspace) return fail("null pointer: paged attention step workspace");
   auto launch = [&](auto kind) {
     constexpr int BENT = decltype(kind)::value;
     LACT_BIG_LDS((k_paged_step<T, C, D, BENT>), A::LDS);
     LACT_LAUNCH_SMEM("k_paged_step", "paged_step", 0.0, (k_paged_step<T, C, D, BENT>), dim3(p.blocks), dim3(64 * A::NW), A::LDS, s, p);
   };
-  if (sizeof(T) == 2 && p.cap > CAP_QUICK) launch(std::integral_constant<int, sizeof(T) == 2 ? SCORES_FAR_CAP : SCORES_BENT>());
+  constexpr int FAR = sizeof(T) == 2 ? SCORES_FAR_CAP : SCORES_BENT;
+  if (!(p.cap > 0.f || p.slopes)) launch(std::integral_constant<int, SCORES_PLAIN>());
+  else if (p.cap > CAP_QUICK) launch(std::integral_constant<int, FAR>());
   else launch(std::integral_constant<int, SCORES_BENT>());
-  LACT_LAUNCH("k_attn_step_join", "paged_step", 0.0, (k_attn_step_join<T, D, A::KEYS, PagedStepParams<T>>), dim3(p.B * p.H), dim3(512), s, p);
+  if (!p.whole)
+    LACT_LAUNCH("k_attn_step_join", "paged_step", 0.0, (k_attn_step_join<T, D, A::KEYS, PagedStepParams<T>>), dim3(p.B * p.H), dim3(512), s, p);
   LACT_CHECK_LAUNCH();
   return 0;
 }
@@ -232,19 +246,18 @@ int lact_paged_cache_read(const lact_paged_cache_t* c, int32_t act_dtype, int32_
   });
 }
 
-size_t lact_paged_attention_step_workspace_bytes(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d, const int32_t* table) {
-  if (check_step(c, d, table)) return 0;
-  size_t bytes = 0;
-  by_types(d->act_dtype, c->dtype, c->D, [&](auto, auto h, auto e) {
-    bytes = step_workspace<decltype(h), decltype(e)::value>(c, d);
+int lact_paged_attention_step_workspace_bytes(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d, const int32_t* table, size_t* bytes) {
+  if (check_step(c, d, table) || check_ptrs({bytes}, "paged attention step workspace bytes")) return -1;
+  return by_types(d->act_dtype, c->dtype, c->D, [&](auto t, auto h, auto e) {
+    constexpr int D = decltype(e)::value;
+    *bytes = step_workspace<PagedShape<decltype(t), decltype(h), D>, D>(c, d);
     return 0;
   });
-  return bytes;
 }
 
 int lact_paged_attention_step(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d, const void* q, const int32_t* table, const int32_t* lengths, void* out,
                               void* workspace, void* stream) {
-  if (check_step(c, d, table) || check_ptrs({q, lengths, out, workspace}, "paged attention step tensors")) return -1;
+  if (check_step(c, d, table) || check_ptrs({q, lengths, out}, "paged attention step tensors")) return -1;
   if (!aligned16(q)) return fail("paged attention step: queries must be 16-byte aligned");
   return by_types(d->act_dtype, c->dtype, c->D, [&](auto t, auto h, auto e) {
     return step_run<decltype(t), decltype(h), decltype(e)::value>(c, d, q, table, lengths, out, workspace, reinterpret_cast<hipStream_t>(stream));

@@ -5,9 +5,10 @@
 //
 // over the places j that lie on a page; n = lengths[b], read on the device.  A sequence that sees nothing has output 0.
 //
-// Work is split, and parts are joined, as in attention_step.h.  A wave's step is 32 places from a multiple of 16 on: two pieces of 16 rows, each of which
-// lies in one page, as page sizes are multiples of 16.  The wave looks pages up 64 pieces at a time, a lane each, and copies a piece from
-// where its lane says; a piece without a page is copied from zeros and masked.  In a piece that the window or the length ends in, the rows outside repeat one inside.
+// Work is split, and parts are joined, as in attention_step.h, unless a block has a key head of a sequence as a whole (PagedStepParams::whole).  A wave's step is 32
+// places from a multiple of 16 on: two pieces of 16 rows, each of which lies in one page, as page sizes are multiples of 16.  The wave looks up where the
+// keys and the values of 32 pieces lie at once, a lane each, and copies a piece from where its lane says; one without a page is copied from zeros and masked.  In a piece
+// that the window or the length ends in, the rows outside repeat one inside.
 //
 // e4m3: numbers become bf16 exactly as they leave LDS.  A key's exponent is applied in that conversion (a lane has one key's row), a value's to the weight
 // that meets it, both exactly.  fp32 queries and weights meet them in three bf16 parts of 8 bits.
@@ -21,7 +22,7 @@ template <typename T>
 struct PagedStepParams {
   Pages kv;
   int B, N, H, HK, group, tiles, window;     // N: places of a sequence; tiles: of 32 query heads to a key head
-  int blocks;
+  int blocks, whole;                         // of the main kernel; whether each has one item, whose steps are few
   const T* q; long long bsq;
   const int* lengths;
   const float* slopes;
@@ -34,7 +35,7 @@ struct PagedStepParams {
   __device__ __forceinline__ static float mean(float sum, float weights) { return weights == 0.f ? 0.f : sum / weights; }
 };
 
-static __device__ const uint4 paged_zeros[32] = {};      // a row of any type
+static __device__ const uint4 paged_zeros[512] = {};      // a piece of any type
 
 // 32 keys or values as they lie in LDS: the 16-byte granule g of row r at slot g ^ key(r)
 template <typename C, int D>
@@ -45,15 +46,19 @@ struct PagedTile {
     else return MaskTile<C, D>::key(r);
   }
 };
-template <typename C, int D>
+template <typename T, typename C, int D>
 struct PagedShape {
   using S = PagedTile<C, D>;
   static constexpr int NW = sizeof(C) == 4 && D == 128 ? 2 : 4;             // waves, each with a ring of its own
-  static constexpr int EXP = is_e4m3<C>() ? 256 : 0, EXPC = EXP ? 1 : 0;     // exponents of 32 keys and 32 values: 64 bytes of one copy
-  static constexpr int STAGE = 2 * S::BYTES + EXP;
-  static constexpr int RING = 131072 / (NW * 2 * S::BYTES);
+  // To a compute unit.  8 bits take as much work for half the bytes: two waves of a SIMD.  (fp32 queries of 128 in three parts: no registers for that.)
+  static constexpr int BLOCKS = is_e4m3<C>() && !(sizeof(T) == 4 && D == 128) ? 2 : 1;
+  static constexpr int SIMD = sizeof(T) == 2 ? 2 : BLOCKS;                   // waves that registers are kept for: with those of two, sums stay where they are worked on
+  static constexpr int STAGE = 2 * S::BYTES;
+  static constexpr int RING = 131072 / (BLOCKS * NW * STAGE);
+  static constexpr int EXP = is_e4m3<C>() ? 1024 : 0;                        // exponents of 32 pieces of keys and of values, twice
+  static constexpr int WAVE = RING * STAGE + 2 * EXP;
   static constexpr int KEYS = 32 * NW;                                       // of a step
-  static constexpr int LDS = NW * RING * STAGE;
+  static constexpr int LDS = NW * WAVE;
 };
 
 // bf16 parts of an fp32 operand, 24 bits in all; one of bf16
@@ -68,8 +73,8 @@ struct PagedFrag {      // the type of the queries, which the pages have as well
   template <typename T>
   __device__ __forceinline__ void queries(const T* base, int h) {
     mask_own_rows<T, D>(q[0], base, D, h, h + 1);
-    mask_arrived(q[0]);
   }
+  __device__ __forceinline__ void arrived() { mask_arrived(q[0]); }
   __device__ __forceinline__ f32x16 scores(const char* tile, const char*) const {
     f32x16 s;
 #pragma unroll
@@ -118,6 +123,8 @@ struct PagedFrag8 {
         for (int i = 0; i < PARTS; ++i) q[i][ks] = next_part(x);
       }
     }
+  }
+  __device__ __forceinline__ void arrived() {
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) mask_arrived(q[i]);
   }
@@ -157,7 +164,7 @@ struct PagedFrag8 {
   }
   // of the lane's 16 values, in the order of its weights
   __device__ __forceinline__ uint4 value_exponents(const char* exps) const {
-    const uint32_t* e = reinterpret_cast<const uint32_t*>(exps + 32 + 4 * ((threadIdx.x & 63) >> 5));
+    const uint32_t* e = reinterpret_cast<const uint32_t*>(exps + 512 + 4 * ((threadIdx.x & 63) >> 5));
     return make_uint4(e[0], e[2], e[4], e[6]);
   }
   __device__ __forceinline__ void weigh(f32x16& s, const uint4& exps) const {
@@ -192,29 +199,48 @@ struct PagedFrag8 {
 template <typename T, typename C, int D>
 using PagedMath = typename std::conditional<is_e4m3<C>(), PagedFrag8<T, D>, PagedFrag<T, D>>::type;
 
-// 4 bytes per lane to LDS from where each lane says: lane i lands at lds_base + 4 * i
-__device__ __forceinline__ void dma4_from(const void* at, uint32_t lds_base) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\t" ::"s"(lds_base), "v"((uint64_t)at) : "memory", "m0");
+// 16 bytes per lane to LDS from where each lane says: lane i lands at lds_base + 16 * i
+__device__ __forceinline__ void dma16_from(uint64_t at, uint32_t lds_base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\t" ::"s"(lds_base), "v"(at) : "memory", "m0");
 }
 
 template <typename T, typename C, int D, int BENT>
-__global__ __launch_bounds__((64 * PagedShape<C, D>::NW), 1) void k_paged_step(const PagedStepParams<T> p) {
+__global__ __launch_bounds__((64 * PagedShape<T, C, D>::NW), (PagedShape<T, C, D>::SIMD)) void k_paged_step(const PagedStepParams<T> p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  using A = PagedShape<C, D>;
+  using A = PagedShape<T, C, D>;
   using S = PagedTile<C, D>;
-  constexpr int NW = A::NW, RING = A::RING, NC = S::COPIES, HALF = NC / 2, ALL = 2 * NC + A::EXPC;      // copies of a wave for 32 keys and values
-  static_assert(RING <= 32, "one batch of pages holds what is on its way");
+  constexpr int NW = A::NW, RING = A::RING, NC = S::COPIES, HALF = NC / 2, BATCH = 16;      // copies of a wave for 32 keys; tiles that it looks up at once
+  static_assert(RING <= BATCH, "one batch holds what is on its way");
   prefetch_args<sizeof(p)>();
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  StepWork work;
-  work.init<A::KEYS>(p);
-  if ((int)blockIdx.x >= work.blocks) return;
-  long long s0 = work.share(blockIdx.x);
-  const long long s1 = work.share(blockIdx.x + 1);
-  long long begin;
-  int b = work.find<A::KEYS>(p, s0, begin);
-  const uint32_t ring = lds_addr(smem) + wave * RING * A::STAGE;
-  const char* mine = smem + wave * RING * A::STAGE;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, items = p.HK * p.tiles;
+  // the block's steps: from step0 of this item of sequence b on
+  int b, item, step0;
+  long long left;
+  if (p.whole) {
+    b = blockIdx.x / items;
+    item = blockIdx.x - b * items;
+    step0 = 0;
+    left = same(StepWork::steps<A::KEYS>(p, b));
+    if (left == 0) {
+      const int h0 = item / p.tiles * p.group + item % p.tiles * 32, rows = min(32, (item / p.tiles + 1) * p.group - h0);
+      for (int i = threadIdx.x; i < rows * D; i += 64 * NW) Elem<T>::store(p.out + ((size_t)b * p.H + h0) * D + i, 0.f);
+      return;
+    }
+  } else {
+    StepWork work;
+    work.init<A::KEYS>(p);
+    if ((int)blockIdx.x >= work.blocks) return;
+    const long long s0 = work.share(blockIdx.x);
+    long long begin;
+    left = work.share(blockIdx.x + 1) - s0;
+    b = work.find<A::KEYS>(p, s0, begin);
+    if (b >= p.B) return;
+    const int n = same(StepWork::steps<A::KEYS>(p, b));
+    item = (int)((s0 - begin) / n);
+    step0 = (int)(s0 - begin - (long long)item * n);
+  }
+  const uint32_t ring = lds_addr(smem) + wave * A::WAVE;
+  const char* mine = smem + wave * A::WAVE;
   PagedMath<T, C, D> math;
   math.init();
   int crow[NC];
@@ -225,88 +251,87 @@ __global__ __launch_bounds__((64 * PagedShape<C, D>::NW), 1) void k_paged_step(c
     crow[i] = r & 15;
     ccol[i] = (uint32_t)((c % S::G) ^ S::key(r)) * 16;
   }
-  const C* K = static_cast<const C*>(p.kv.k);
-  const C* V = static_cast<const C*>(p.kv.v);
   bool head_of_share = true;
-  while (s0 < s1) {
-    int n = 0;
-    while (b < p.B && (n = same(StepWork::steps<A::KEYS>(p, b))) == 0) ++b;
-    if (b >= p.B) return;                                       // (the shares end with the last sequence)
-    const long long in_b = s0 - begin;
-    const int item = (int)(in_b / n), step0 = (int)(in_b - (long long)item * n);
-    const int step1 = (int)min((long long)n, step0 + (s1 - s0));
+  while (left > 0) {
+    const int n = same(StepWork::steps<A::KEYS>(p, b));
+    if (n == 0) {
+      if (++b >= p.B) return;                                   // (the shares end with the last sequence)
+      continue;
+    }
+    const int step1 = (int)min((long long)n, step0 + left);
     const int hk = item / p.tiles, h0 = hk * p.group + (item - hk * p.tiles) * 32;
     const int rows = min(32, (hk + 1) * p.group - h0), h = h0 + min(lane & 31, rows - 1);
     const int len = same(p.length(b)), lo = same(p.first(b)), lo16 = lo & ~15;
-    math.queries(p.q + b * p.bsq, h);
-    Scores<T, BENT> sc;
-    sc.init(p.scale, p.cap, p.slopes, h);
-    const float c = sc.unit();
-    f32x16 o[D / 32];
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-    float mc = ATTN_LOWEST, sum = 0.f;
     // the wave's tiles: 32 places from place(t) on
     auto place = [&](int t) LACT_INLINE_LAMBDA { return lo16 + ((step0 + t) * NW + wave) * 32; };
     const int tiles = min(step1 - step0, max(0, (len - lo16 - wave * 32 - step0 * A::KEYS + A::KEYS - 1) / A::KEYS));
-    // Pages of the pieces of 32 tiles from a multiple of 32 on, a lane each; which have one, of this batch and the one before it.
-    int page = -1, row = 0;
-    uint64_t there = 0, there_before = 0;
+    // Where the 32 pieces of 16 tiles from a multiple of 16 on lie, keys in the first half of the lanes, values in the second; which have a page, of this batch and the one
+    // before it.
+    uint32_t from_lo = 0, from_hi = 0, there = 0, there_before = 0;
+    int batch = 0;      // the newest
     auto look_up = [&](int t) LACT_INLINE_LAMBDA {
-      const int at = place(t + lane / 2) + (lane & 1) * 16;
-      page = at < len ? p.kv.page(b, at) : -1;
-      row = page >= 0 ? p.kv.rows_before(hk, p.kv.row(at)) : 0;
+      const int at = place(t + (lane & 31) / 2) + (lane & 1) * 16, page = at < len ? p.kv.page(b, at) : -1;
+      const long long row = page >= 0 ? p.kv.rows_before(hk, p.kv.row(at)) : 0;
+      const bool values = lane >= 32;
+      const uint64_t zeros = reinterpret_cast<uint64_t>(paged_zeros);
+      const uint64_t from = page < 0 ? zeros
+                                     : reinterpret_cast<uint64_t>(values ? p.kv.v : p.kv.k) + (page * (values ? p.kv.v_page : p.kv.k_page) + row * D) * (long long)sizeof(C);
+      if constexpr (A::EXP)
+        dma16_from(page < 0 ? zeros : reinterpret_cast<uint64_t>(values ? p.kv.vs : p.kv.ks) + page * (values ? p.kv.vs_page : p.kv.ks_page) + row,
+                   ring + RING * A::STAGE + (t / BATCH & 1) * A::EXP);
+      from_lo = (uint32_t)from;
+      from_hi = (uint32_t)(from >> 32);
       there_before = there;
-      there = __ballot(page >= 0);
+      there = (uint32_t)__ballot(page >= 0);
     };
-    auto copy = [&](const C* base, long long stride, int t, uint32_t to) LACT_INLINE_LAMBDA {
+    auto copy = [&](int t, int half, uint32_t to) LACT_INLINE_LAMBDA {
       const int k0 = place(t);
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const int at = 2 * (t & 31) + x, id = __builtin_amdgcn_readlane(page, at), r = __builtin_amdgcn_readlane(row, at), j0 = k0 + 16 * x;
-        const void* from = uniform(id >= 0 ? static_cast<const void*>(base + id * stride + (long long)r * D) : static_cast<const void*>(paged_zeros));
-        const int first = id >= 0 ? lo - j0 : 0, last = id >= 0 ? len - 1 - j0 : 0;
+        const int at = half + 2 * (t % BATCH) + x, first = lo - (k0 + 16 * x), last = max(0, len - 1 - (k0 + 16 * x));
+        uint64_t address = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(from_lo, at) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(from_hi, at) << 32;
+        asm volatile("s_nop 4" : "+s"(address));      // between a scalar register's write by a vector instruction and its use as an address, which the compiler does not see
+        const void* from = reinterpret_cast<const void*>(address);
 #pragma unroll
         for (int i = x * HALF; i < (x + 1) * HALF; ++i) dma16<false>(from, (uint32_t)min(max(crow[i], first), last) * S::ROWB + ccol[i], to + i * 1024);
       }
     };
-    auto exponents = [&](int t, uint32_t to) LACT_INLINE_LAMBDA {
-      const int at = 2 * (t & 31) + (lane >> 2 & 1), id = __shfl(page, at, 64), r = __shfl(row, at, 64);
-      const bool values = lane & 8;
-      const uint8_t* from = (values ? p.kv.vs : p.kv.ks) + id * (values ? p.kv.vs_page : p.kv.ks_page) + r;
-      dma4_from((id >= 0 ? from : reinterpret_cast<const uint8_t*>(paged_zeros)) + (lane & 3) * 4, to);
-    };
-    auto keys = [&](int t) LACT_INLINE_LAMBDA {
-      const uint32_t to = ring + t % RING * A::STAGE;
-      if constexpr (A::EXPC) exponents(t, to + 2 * S::BYTES);
-      copy(K, p.kv.k_page, t, to);
-    };
-    auto values = [&](int t) LACT_INLINE_LAMBDA { copy(V, p.kv.v_page, t, ring + t % RING * A::STAGE + S::BYTES); };
-    int batch = 0;      // the newest
-    if (tiles > 0) look_up(0);
+    auto keys = [&](int t) LACT_INLINE_LAMBDA { copy(t, 0, ring + t % RING * A::STAGE); };
+    auto values = [&](int t) LACT_INLINE_LAMBDA { copy(t, 32, ring + t % RING * A::STAGE + S::BYTES); };
+    math.queries(p.q + b * p.bsq, h);
+    Scores<T, BENT> sc;
+    sc.init(p.scale, p.cap, p.slopes, h);
+    const float c = sc.unit();
     // no barrier: nobody else uses the wave's ring
+    if (tiles > 0) look_up(0);
 #pragma unroll
     for (int t = 0; t < RING; ++t)
       if (t < tiles) {
         keys(t);
         values(t);
       }
+    math.arrived();
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+    float mc = ATTN_LOWEST, sum = 0.f;
     for (int t = 0; t < tiles; ++t) {
       const bool more = t + RING < tiles, full = t + RING <= tiles;
-      if (full) wait_vmcnt<RING * ALL - NC - A::EXPC>();
+      if (full) wait_vmcnt<(2 * RING - 1) * NC>();
       else wait_vmcnt<0>();
       const char* kt = mine + t % RING * A::STAGE;
       const char* vt = kt + S::BYTES;
+      const char* et = mine + RING * A::STAGE + (t / BATCH & 1) * A::EXP + t % BATCH * 32;
       const int k0 = place(t), at = k0 + 4 * (lane >> 5);
-      const int on_pages = (int)((t / 32 == batch ? there : there_before) >> (2 * (t & 31))) & 3;      // of the two pieces
+      const int on_pages = (t / BATCH == batch ? there : there_before) >> (2 * (t % BATCH)) & 3;      // of the two pieces
       const bool masked = k0 < lo || k0 + 32 > len || on_pages != 3;
-      f32x16 s = math.scores(kt, kt + 2 * S::BYTES);
-      const auto exps = math.value_exponents(kt + 2 * S::BYTES);
+      f32x16 s = math.scores(kt, et);
+      const auto exps = math.value_exponents(et);
       wave_reads_done();
       if (more) {
-        if ((t + RING) % 32 == 0) {
+        if ((t + RING) % BATCH == 0) {
           look_up(t + RING);
           ++batch;
         }
@@ -340,11 +365,11 @@ __global__ __launch_bounds__((64 * PagedShape<C, D>::NW), 1) void k_paged_step(c
         s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], c, -mc));
         sum += s[j];
       }
-      if constexpr (A::EXPC) {
+      if constexpr (A::EXP) {
         math.weigh(s, exps);
         if (masked) mask(0.f);      // (whatever exponent lies beside a row that nobody sees)
       }
-      if (more) wait_vmcnt<RING * ALL - NC>();
+      if (more) wait_vmcnt<(2 * RING - 1) * NC>();
       else wait_vmcnt<0>();
       math.add(o, s, vt);
       wave_reads_done();
@@ -352,14 +377,15 @@ __global__ __launch_bounds__((64 * PagedShape<C, D>::NW), 1) void k_paged_step(c
     }
     const bool whole = step0 == 0 && step1 == n;
     const int stride = min(p.group, 32);
-    attn_step_leave<T, D, NW, RING * A::STAGE>(p, smem, o, mc, sum, rows, whole ? p.out + ((size_t)b * p.H + h0) * D : nullptr,
-                                               p.part + (size_t)(2 * blockIdx.x + (head_of_share ? 0 : 1)) * stride * (D + 2));
+    attn_step_leave<T, D, NW, A::WAVE>(p, smem, o, mc, sum, rows, whole ? p.out + ((size_t)b * p.H + h0) * D : nullptr,
+                                       p.part + (size_t)(2 * blockIdx.x + (head_of_share ? 0 : 1)) * stride * (D + 2));
     __syncthreads();      // the rings are free again
     head_of_share = false;
-    s0 += step1 - step0;
-    if (step1 == n && item + 1 == p.HK * p.tiles) {
-      begin += (long long)n * p.HK * p.tiles;
-      ++b;
+    left -= step1 - step0;
+    step0 = 0;
+    if (++item == items) {
+      item = 0;
+      if (++b >= p.B) return;
     }
   }
 }

@@ -1013,9 +1013,9 @@ Tensor paged_step(const Tensor& q_, const Tensor& ck, const Tensor& cv, const Op
   D.scale = (float)scale; D.score_cap = (float)cap;
   D.q_bs = h * d;
   D.slopes = fptr(slopes);
-  const int64_t bytes = (int64_t)lact_paged_attention_step_workspace_bytes(&c.desc, &D, fptr<int32_t>(c.table));
-  if (bytes == 0) check(-1);
-  const Tensor ws = at::empty({bytes}, q.options().dtype(at::kByte));
+  size_t bytes = 0;
+  check(lact_paged_attention_step_workspace_bytes(&c.desc, &D, fptr<int32_t>(c.table), &bytes));
+  const Tensor ws = bytes ? at::empty({(int64_t)bytes}, q.options().dtype(at::kByte)) : Tensor();
   check(lact_paged_attention_step(&c.desc, &D, ptr(q), fptr<int32_t>(c.table), fptr<int32_t>(lengths), ptr(out), ptr(ws), stream()));
   return out;
 }

@@ -41,7 +41,7 @@ def test_cache_arguments(change, message):
     assert L.lact_paged_cache_write(c, 0, 3, 5, P, 128, 640, P, 128, 640, P, P, P, None) < 0 and message in lib_error()
     assert L.lact_paged_cache_read(c, 0, 3, 5, P, P, P, P, P, None) < 0 and message in lib_error()
     d = ctypes.byref(step_desc())
-    assert L.lact_paged_attention_step_workspace_bytes(c, d, P) == 0 and message in lib_error()
+    assert L.lact_paged_attention_step_workspace_bytes(c, d, P, ctypes.byref(ctypes.c_size_t())) < 0 and message in lib_error()
     assert L.lact_paged_attention_step(c, d, P, P, P, P, P, None) < 0 and message in lib_error()
 
 
@@ -92,24 +92,30 @@ def step_desc(**kw):
     (dict(scale=0.0), "scale"), (dict(scale=math.nan), "scale"), (dict(score_cap=-1.0), "cap"), (dict(score_cap=math.inf), "cap"), (dict(q_bs=510), "aligned"), (dict(q_bs=-512), "aligned")])
 def test_step_arguments(change, message):
     L, c, d = _lib.lib(), ctypes.byref(cache_desc()), ctypes.byref(step_desc(**change))
-    assert L.lact_paged_attention_step_workspace_bytes(c, d, P) == 0 and message in lib_error()
+    assert L.lact_paged_attention_step_workspace_bytes(c, d, P, ctypes.byref(ctypes.c_size_t())) < 0 and message in lib_error()
     assert L.lact_paged_attention_step(c, d, P, P, P, P, P, None) < 0 and message in lib_error()
 
 
 def test_step_pointers_and_workspace():
-    L, c = _lib.lib(), cache_desc()
+    L, c = _lib.lib(), cache_desc(width=40)
     for i in range(5):
         args = [P] * 5
         args[i] = None
-        assert L.lact_paged_attention_step(ctypes.byref(c), ctypes.byref(step_desc()), *args, None) < 0 and "null pointer" in lib_error()
+        assert L.lact_paged_attention_step(ctypes.byref(c), ctypes.byref(step_desc(window=1280)), *args, None) < 0 and "null pointer" in lib_error()
     assert L.lact_paged_attention_step(ctypes.byref(c), ctypes.byref(step_desc()), ctypes.c_void_p((1 << 20) + 2), P, P, P, P, None) < 0 and "aligned" in lib_error()
     assert L.lact_paged_attention_step(ctypes.byref(c), None, P, P, P, P, P, None) < 0 and "descriptor" in lib_error()
-    size = lambda **kw: L.lact_paged_attention_step_workspace_bytes(ctypes.byref(c), ctypes.byref(step_desc(**kw)), P)  # noqa: E731
-    # two parts a block: 3 sequences x 2 heads x 1 step of 128 places (a window of 100 may touch 115), 4 query heads to a key head
-    assert size() == 2 * 6 * 4 * 66 * 4
-    assert size(window=114) == 2 * 12 * 4 * 66 * 4 and size(window=1 << 30) == 2 * 12 * 4 * 66 * 4
+
+    def size(**kw):
+        n = ctypes.c_size_t(7)
+        assert L.lact_paged_attention_step_workspace_bytes(ctypes.byref(c), ctypes.byref(step_desc(**kw)), P, ctypes.byref(n)) == 0
+        return n.value
+    assert L.lact_paged_attention_step_workspace_bytes(ctypes.byref(c), ctypes.byref(step_desc()), P, None) < 0 and "null pointer" in lib_error()
+    # two parts a block, of 4 query heads to a key head: 3 sequences x 2 heads x 10 steps of 128 places; none where every item has a block of its own
+    assert size(window=1 << 30) == 2 * 60 * 4 * 66 * 4 and size() == 0
     c = cache_desc(pages=1 << 20, width=1 << 18)
     assert size(window=1 << 30) == 2 * 256 * 4 * 66 * 4
+    c.dtype = 2
+    assert size(window=1 << 30) == 2 * 512 * 4 * 66 * 4      # two blocks to a compute unit
 
 
 def rotary_desc(**kw):
