@@ -16,6 +16,7 @@ namespace {
 
 constexpr int COMPUTE_UNITS = 256;
 constexpr long long MAX_ROWS = (1LL << 31) - 1;
+constexpr long long MAX_BLOCKS = (1LL << 24) - 1;      // of 256 threads: a launch counts its threads in 32 bits
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 int check_type(int act) { return act == LACT_BF16 || act == LACT_F32 ? 0 : fail("act_dtype must be LACT_BF16 or LACT_F32"); }
@@ -87,13 +88,16 @@ int by_types(int act, int held, int D, F f) {
 
 int check_tokens(const lact_paged_cache_t* c, int B, int L) {
   if (B <= 0 || L <= 0) return fail("paged cache: B and L must be positive");
-  if ((long long)B * c->HK * L > MAX_ROWS) return fail("paged cache: too many tokens in one call");
+  // (tiles of at least 8 tokens, and one more at each end)
+  if ((long long)B * (L / 8 + 2) > MAX_BLOCKS || c->HK > 65535) return fail("paged cache: too many tokens or heads in one call");
   return 0;
 }
 template <typename T, int D>
-dim3 row_blocks(int B, int HK, int L) {
-  const long long per = CACHE_ROWS * (256 / (D * (int)sizeof(T) / 16));
-  return dim3((unsigned)(((long long)B * HK * L + per - 1) / per), 2);
+dim3 cache_grid(const lact_paged_cache_t* c, int B, int L, const int32_t* starts, CacheRows* r) {
+  using A = CacheTile<T, D>;
+  const int tiles = A::tiles(L), groups = ceil_div(c->HK, A::HEADS);
+  *r = CacheRows{B, L, c->HK, make_udiv(tiles), make_udiv(groups), starts};
+  return dim3(B * tiles, 2 * groups);
 }
 
 // ---- one token's attention --------------------------------------------------------------------------
@@ -174,22 +178,25 @@ int check_rotary(const lact_rotary_desc_t* d) {
   return 0;
 }
 template <typename T, int V, bool SIDE>
-void launch_rotary(RotaryParams p, hipStream_t s) {
+int launch_rotary(RotaryParams p, hipStream_t s) {
   p.units = SIDE ? p.D / V : p.pairs / V + (p.D - 2 * p.pairs) / V;
   p.by_units = make_udiv(p.units);
   p.tokens = 256 / p.units;
   const int heads = p.op[0].heads + p.op[1].heads;
   const long long blocks = ((long long)p.B * p.L + p.tokens - 1) / p.tokens;
+  if (blocks > MAX_BLOCKS) return fail("rotary: too many tokens or heads");
   p.per = (int)std::max<long long>(1, std::min<long long>(heads, blocks * heads / (8 * COMPUTE_UNITS)));
   LACT_LAUNCH("k_rotary", "rotary", 0.0, (k_rotary<T, V, SIDE>), dim3((unsigned)blocks, ceil_div(heads, p.per)), dim3(256), s, p);
+  LACT_CHECK_LAUNCH();
+  return 0;
 }
 template <typename T>
-void launch_rotary(const RotaryParams& p, bool side, hipStream_t s) {
+int launch_rotary(const RotaryParams& p, bool side, hipStream_t s) {
   constexpr int E = 16 / (int)sizeof(T);
   bool wide = p.D % E == 0 && (side || p.pairs % E == 0);
   for (const auto& o : p.op) wide = wide && (!o.heads || (aligned16(o.x) && aligned16(o.y) && o.bs % E == 0 && o.ls % E == 0 && o.hs % E == 0));
-  if (side) wide ? launch_rotary<T, E, true>(p, s) : launch_rotary<T, 2, true>(p, s);
-  else wide ? launch_rotary<T, E, false>(p, s) : launch_rotary<T, 1, false>(p, s);
+  if (side) return wide ? launch_rotary<T, E, true>(p, s) : launch_rotary<T, 2, true>(p, s);
+  return wide ? launch_rotary<T, E, false>(p, s) : launch_rotary<T, 1, false>(p, s);
 }
 
 }  // namespace
@@ -215,11 +222,11 @@ int lact_paged_cache_write(const lact_paged_cache_t* c, int32_t act_dtype, int32
     CacheWriteParams<T> p;
     memset(&p, 0, sizeof(p));
     p.to = pages_of(c, table);
-    p.B = B; p.L = L; p.by_l = make_udiv(L); p.by_heads = make_udiv(c->HK);
+    const dim3 grid = cache_grid<T, D>(c, B, L, starts, &p.rows);
     p.k = static_cast<const T*>(k); p.v = static_cast<const T*>(v);
     p.ldk = k_ld; p.bsk = k_bs; p.ldv = v_ld; p.bsv = v_bs;
-    p.starts = starts; p.counts = counts;
-    LACT_LAUNCH("k_cache_write", "paged_cache", 0.0, (k_cache_write<T, C, D>), (row_blocks<T, D>(B, c->HK, L)), dim3(256), s, p);
+    p.counts = counts;
+    LACT_LAUNCH("k_cache_write", "paged_cache", 0.0, (k_cache_write<T, C, D>), grid, dim3(256), s, p);
     LACT_CHECK_LAUNCH();
     return 0;
   });
@@ -237,10 +244,10 @@ int lact_paged_cache_read(const lact_paged_cache_t* c, int32_t act_dtype, int32_
     CacheReadParams<T> p;
     memset(&p, 0, sizeof(p));
     p.from = pages_of(c, table);
-    p.B = B; p.L = L; p.by_l = make_udiv(L); p.by_heads = make_udiv(c->HK);
+    const dim3 grid = cache_grid<T, D>(c, B, L, starts, &p.rows);
     p.k = static_cast<T*>(k); p.v = static_cast<T*>(v);
-    p.starts = starts; p.lengths = lengths;
-    LACT_LAUNCH("k_cache_read", "paged_cache", 0.0, (k_cache_read<T, C, D>), (row_blocks<T, D>(B, c->HK, L)), dim3(256), s, p);
+    p.lengths = lengths;
+    LACT_LAUNCH("k_cache_read", "paged_cache", 0.0, (k_cache_read<T, C, D>), grid, dim3(256), s, p);
     LACT_CHECK_LAUNCH();
     return 0;
   });
@@ -279,10 +286,7 @@ int lact_axial_rotary(const lact_rotary_desc_t* d, const void* q, const void* k,
     p.axis[i] = (uint8_t)d->axis_of_pair[i];
   }
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (d->act_dtype == LACT_BF16) launch_rotary<uint16_t>(p, d->interleaved, s);
-  else launch_rotary<float>(p, d->interleaved, s);
-  LACT_CHECK_LAUNCH();
-  return 0;
+  return d->act_dtype == LACT_BF16 ? launch_rotary<uint16_t>(p, d->interleaved, s) : launch_rotary<float>(p, d->interleaved, s);
 }
 
 }  // extern "C"
