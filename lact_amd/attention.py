@@ -16,13 +16,16 @@ from . import _lib
 _SMALLEST, _LARGEST = 2.0 ** -149, (2.0 - 2.0 ** -23) * 2.0 ** 127      # of fp32
 
 
+_PLAIN = {torch.Tensor, nn.Parameter}
+
+
 def _plain_only(name: str, *ts: Optional[torch.Tensor]) -> None:
     """The kernels read memory: what needs to see tensor operations (function transforms, tracing, forward mode, subclasses) is refused."""
     ts = [t for t in ts if t is not None]
-    if not all(isinstance(t, torch.Tensor) for t in ts):
+    types = set(map(type, ts))
+    if not types <= _PLAIN and not all(isinstance(t, torch.Tensor) for t in ts):
         raise TypeError(f"{name} takes tensors")
-    if torch._C._are_functorch_transforms_active() or torch.jit.is_tracing() or any(
-            type(t) not in (torch.Tensor, nn.Parameter) or torch._C._functorch.is_legacy_batchedtensor(t) for t in ts):
+    if not types <= _PLAIN or torch._C._are_functorch_transforms_active() or torch._C._is_tracing() or any(map(torch._C._functorch.is_legacy_batchedtensor, ts)):
         raise NotImplementedError(f"{name} takes plain tensors: no function transforms, tracing, tensor subclasses or batches of gradients")
     if fwad._current_level >= 0 and any(fwad.unpack_dual(t).tangent is not None for t in ts):
         raise NotImplementedError(f"{name} has no forward-mode derivative (jvp)")

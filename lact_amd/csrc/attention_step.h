@@ -30,9 +30,6 @@ struct AttnStepParams {
   T* out;                                    // [B, H, D]
   float* part;                               // [2 * blocks][rows][D + 2]: sums, then row maximum and row sum; rows = min(group, 32)
   __device__ __forceinline__ int length(int b) const { return min(max(lengths[b], 0), N); }
-  __device__ __forceinline__ int span(int b) const { return min(length(b), window); }      // the keys that steps are counted from
-  // a row's sum over its weights; where nothing weighs anything (scores of -infinity throughout) it has no value
-  __device__ __forceinline__ static float mean(float sum, float weights) { return sum / weights; }
 };
 
 // What the wave has read of LDS is in registers: the next copies may overwrite it.
@@ -59,7 +56,7 @@ struct StepWork {
   int blocks;        // with a share: none is empty
   template <int KEYS, typename P>
   __device__ __forceinline__ static int steps(const P& p, int b) {
-    return b < p.B ? (p.span(b) + KEYS - 1) / KEYS : 0;
+    return b < p.B ? (min(p.length(b), p.window) + KEYS - 1) / KEYS : 0;
   }
   __device__ __forceinline__ static long long scan(long long v) {           // inclusive, over the wave
     const int l = threadIdx.x & 63;
@@ -109,51 +106,6 @@ struct StepWork {
   __device__ __forceinline__ long long share(int block) const { return block * total / blocks; }
   __device__ __forceinline__ int block_of(long long s) const { return (int)(((s + 1) * blocks - 1) / total); }
 };
-
-// The waves' parts of an item together: sums at their place in each one's ring (RINGB bytes apart), [row][D + 4], maximum and row sum behind them.  To `out`, or as they
-// are to `part`, [row][D + 2].
-template <typename T, int D, int NW, int RINGB, typename P>
-__device__ __forceinline__ void attn_step_leave(const P& p, char* smem, const f32x16 (&o)[D / 32], float mc, float sum, int rows, T* out, float* part) {
-  constexpr int LD = D + 4, WSTRIDE = RINGB / 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  sum += __shfl_xor(sum, 32, 64);
-  float* w = reinterpret_cast<float*>(smem + wave * RINGB);
-  if ((lane & 31) < rows) {
-#pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        Elem<float>::store4(w + (lane & 31) * LD + dt * 32 + 8 * g + 4 * (lane >> 5), o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]);
-    if (lane < 32) {
-      w[lane * LD + D] = mc;
-      w[lane * LD + D + 1] = sum;
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * D; i += 64 * NW) {
-    const int r = i / D, d = i % D;
-    const float* src = reinterpret_cast<const float*>(smem) + r * LD;
-    float m = src[D];
-#pragma unroll
-    for (int x = 1; x < NW; ++x) m = fmaxf(m, src[x * WSTRIDE + D]);
-    float acc = 0.f, total = 0.f;
-#pragma unroll
-    for (int x = 0; x < NW; ++x) {
-      const float f = __builtin_amdgcn_exp2f(src[x * WSTRIDE + D] - m);
-      acc += src[x * WSTRIDE + d] * f;
-      total += src[x * WSTRIDE + D + 1] * f;
-    }
-    if (out) {
-      Elem<T>::store(out + (size_t)r * D + d, P::mean(acc, total));
-    } else {
-      part[r * (D + 2) + d] = acc;
-      if (d == 0) {
-        part[r * (D + 2) + D] = m;
-        part[r * (D + 2) + D + 1] = total;
-      }
-    }
-  }
-}
 
 template <typename T, int D, int BENT>
 __global__ __launch_bounds__((64 * AttnStepShape<T, D>::NW), 1) void k_attn_step(const AttnStepParams<T> p) {
@@ -274,10 +226,49 @@ __global__ __launch_bounds__((64 * AttnStepShape<T, D>::NW), 1) void k_attn_step
       wave_reads_done();
       if (more) values(t + RING);
     }
+    // The waves' parts together: sums at their place in each one's ring, [row][D + 4], maximum and row sum behind them.
+    constexpr int LD = D + 4;
+    sum += __shfl_xor(sum, 32, 64);
+    float* w = reinterpret_cast<float*>(mine);
+    if ((lane & 31) < rows) {
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          Elem<float>::store4(w + (lane & 31) * LD + dt * 32 + 8 * g + 4 * (lane >> 5), o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]);
+      if (lane < 32) {
+        w[lane * LD + D] = mc;
+        w[lane * LD + D + 1] = sum;
+      }
+    }
+    __syncthreads();
     const bool whole = step0 == 0 && step1 == n;
     const int stride = min(p.group, 32);
-    attn_step_leave<T, D, NW, RING * 2 * A::TILE>(p, smem, o, mc, sum, rows, whole ? p.out + ((size_t)b * p.H + h0) * D : nullptr,
-                                                  p.part + (size_t)(2 * blockIdx.x + (head_of_share ? 0 : 1)) * stride * (D + 2));
+    float* part = p.part + (size_t)(2 * blockIdx.x + (head_of_share ? 0 : 1)) * stride * (D + 2);
+    constexpr int WSTRIDE = RING * 2 * A::TILE / 4;
+    for (int i = threadIdx.x; i < rows * D; i += 64 * NW) {
+      const int r = i / D, d = i % D;
+      const float* src = reinterpret_cast<const float*>(smem) + r * LD;
+      float m = src[D];
+#pragma unroll
+      for (int x = 1; x < NW; ++x) m = fmaxf(m, src[x * WSTRIDE + D]);
+      float acc = 0.f, total = 0.f;
+#pragma unroll
+      for (int x = 0; x < NW; ++x) {
+        const float f = __builtin_amdgcn_exp2f(src[x * WSTRIDE + D] - m);
+        acc += src[x * WSTRIDE + d] * f;
+        total += src[x * WSTRIDE + D + 1] * f;
+      }
+      if (whole) {
+        Elem<T>::store(p.out + ((size_t)b * p.H + h0 + r) * D + d, acc / total);
+      } else {
+        part[r * (D + 2) + d] = acc;
+        if (d == 0) {
+          part[r * (D + 2) + D] = m;
+          part[r * (D + 2) + D + 1] = total;
+        }
+      }
+    }
     __syncthreads();      // the rings are free again
     head_of_share = false;
     s0 += step1 - step0;
@@ -290,11 +281,12 @@ __global__ __launch_bounds__((64 * AttnStepShape<T, D>::NW), 1) void k_attn_step
 
 // (7 us for 256 parts of one sequence, bound by the launch and the way to them: 512 threads, so that each reads few.)
 // One block of 512 threads per (sequence, query head): the sum of the parts that blocks left of it, and zeros for a sequence without tokens.
-template <typename T, int D, int KEYS, typename P>
-__global__ __launch_bounds__(512) void k_attn_step_join(const P p) {
+template <typename T, int D>
+__global__ __launch_bounds__(512) void k_attn_step_join(const AttnStepParams<T> p) {
   constexpr int GROUPS = 512 / D;
   __shared__ float acc_s[GROUPS][D], sum_s[GROUPS], max_s[8];
   const int b = blockIdx.x / p.H, h = blockIdx.x - b * p.H;
+  constexpr int KEYS = AttnStepShape<T, D>::KEYS;
   const int n = StepWork::steps<KEYS>(p, b);
   T* out = p.out + ((size_t)b * p.H + h) * D;
   if (n == 0) {
@@ -335,7 +327,7 @@ __global__ __launch_bounds__(512) void k_attn_step_join(const P p) {
       acc += acc_s[i][d];
       total += sum_s[i];
     }
-    Elem<T>::store(out + d, P::mean(acc, total));
+    Elem<T>::store(out + d, acc / total);
   }
 }
 

@@ -203,7 +203,7 @@ int step_run(const lact_attention_step_desc_t* d, const void* q, const void* k, 
   };
   if (sizeof(T) == 2 && p.cap > CAP_QUICK) launch(std::integral_constant<int, sizeof(T) == 2 ? SCORES_FAR_CAP : SCORES_BENT>());
   else launch(std::integral_constant<int, SCORES_BENT>());
-  LACT_LAUNCH("k_attn_step_join", "attn_step", 0.0, (k_attn_step_join<T, D, AttnStepShape<T, D>::KEYS, AttnStepParams<T>>), dim3(p.B * p.H), dim3(512), s, p);
+  LACT_LAUNCH("k_attn_step_join", "attn_step", 0.0, (k_attn_step_join<T, D>), dim3(p.B * p.H), dim3(512), s, p);
   LACT_CHECK_LAUNCH();
   return 0;
 }

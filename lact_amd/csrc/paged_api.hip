@@ -118,7 +118,8 @@ template <typename A>
 int most_steps(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) {
   return ceil_div(std::min(places(c), std::min(d->window, places(c)) + 15), A::KEYS);
 }
-int step_items(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) { return d->B * c->HK * ceil_div(d->H / c->HK, 32); }
+int step_columns(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) { return d->H / c->HK <= 16 ? 16 : 32; }
+int step_items(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) { return d->B * c->HK * ceil_div(d->H / c->HK, step_columns(c, d)); }
 // One block for every item, where the longest has few steps, and no second launch.
 constexpr int WHOLE_STEPS = 4;
 template <typename A>
@@ -139,7 +140,8 @@ int step_run(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d, const
   PagedStepParams<T> p;
   memset(&p, 0, sizeof(p));
   p.kv = pages_of(c, table);
-  p.B = d->B; p.N = places(c); p.H = d->H; p.HK = c->HK; p.group = d->H / c->HK; p.tiles = ceil_div(p.group, 32);
+  p.B = d->B; p.N = places(c); p.H = d->H; p.HK = c->HK; p.group = d->H / c->HK;
+  p.columns = step_columns(c, d); p.tiles = ceil_div(p.group, p.columns);
   p.window = std::min(d->window, p.N);
   p.whole = step_whole<A>(c, d);
   p.blocks = step_blocks<A>(c, d);
@@ -147,17 +149,22 @@ int step_run(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d, const
   p.lengths = lengths; p.slopes = d->slopes; p.scale = d->scale; p.cap = d->score_cap;
   p.out = static_cast<T*>(out); p.part = static_cast<float*>(workspace);
   if (!p.whole && !workspace) return fail("null pointer: paged attention step workspace");
-  auto launch = [&](auto kind) {
-    constexpr int BENT = decltype(kind)::value;
-    LACT_BIG_LDS((k_paged_step<T, C, D, BENT>), A::LDS);
-    LACT_LAUNCH_SMEM("k_paged_step", "paged_step", 0.0, (k_paged_step<T, C, D, BENT>), dim3(p.blocks), dim3(64 * A::NW), A::LDS, s, p);
+  auto launch_for = [&](auto kind, auto tiles) {
+    constexpr int BENT = decltype(kind)::value, QT = decltype(tiles)::value;
+    LACT_BIG_LDS((k_paged_step<T, C, D, QT, BENT>), A::LDS);
+    LACT_LAUNCH_SMEM("k_paged_step", "paged_step", 0.0, (k_paged_step<T, C, D, QT, BENT>), dim3(p.blocks), dim3(64 * A::NW), A::LDS, s, p);
   };
+  auto launch = [&](auto kind) { p.columns == 16 ? launch_for(kind, std::integral_constant<int, 1>()) : launch_for(kind, std::integral_constant<int, 2>()); };
   constexpr int FAR = sizeof(T) == 2 ? SCORES_FAR_CAP : SCORES_BENT;
   if (!(p.cap > 0.f || p.slopes)) launch(std::integral_constant<int, SCORES_PLAIN>());
   else if (p.cap > CAP_QUICK) launch(std::integral_constant<int, FAR>());
   else launch(std::integral_constant<int, SCORES_BENT>());
-  if (!p.whole)
-    LACT_LAUNCH("k_attn_step_join", "paged_step", 0.0, (k_attn_step_join<T, D, A::KEYS, PagedStepParams<T>>), dim3(p.B * p.H), dim3(512), s, p);
+  const int items = step_items(c, d);
+  if (!p.whole && p.blocks > 1) {
+    const dim3 grid(p.blocks - 1, std::min(p.group, 32));
+    if (p.blocks > 8 * items) LACT_LAUNCH("k_paged_join", "paged_step", 0.0, (k_paged_join<T, D, A::KEYS, 512>), grid, dim3(512), s, p);
+    else LACT_LAUNCH("k_paged_join", "paged_step", 0.0, (k_paged_join<T, D, A::KEYS, 128>), grid, dim3(128), s, p);
+  }
   LACT_CHECK_LAUNCH();
   return 0;
 }

@@ -904,6 +904,17 @@ std::vector<Tensor> linear_step(const Tensor& q_, const Tensor& k_, const Tensor
 }
 
 // ---- paged cache, rotary positions --------------------------------------------------------------------------------------
+void expect_dims(const OptTensor& t, int64_t n, const char* name) {
+  if (t && t->dim() != n) throw std::invalid_argument(std::string(name) + " must have " + std::to_string(n) + " dimensions, got " + c10::str(t->sizes()));
+}
+// (in front of everything else, so that it is said of tensors anywhere)
+void expect_cache_dims(const Tensor& k, const Tensor& v, const OptTensor& ks, const OptTensor& vs, const Tensor& table) {
+  expect_dims(k, 4, "cache.k");
+  expect_dims(v, 4, "cache.v");
+  expect_dims(ks, 3, "cache.k_scale");
+  expect_dims(vs, 3, "cache.v_scale");
+  expect_dims(table, 2, "page_table");
+}
 struct CacheCall {
   lact_paged_cache_t desc{};
   Tensor table;
@@ -938,7 +949,7 @@ CacheCall paged_cache(const Tensor& k, const Tensor& v, const OptTensor& ks, con
     D.v_exponents = static_cast<uint8_t*>(vs->data_ptr());
     D.ke_page = page(*ks); D.ve_page = page(*vs);
   }
-  if (table.dim() != 2 || table.size(1) > INT32_MAX) throw std::invalid_argument("page_table must have 2 dimensions");
+  if (table.size(1) > INT32_MAX) throw std::invalid_argument("page_table is too wide");
   c.table = indices(table, k, {b, table.size(1)}, "page_table");
   D.dtype = eight ? LACT_E4M3 : act == at::kBFloat16 ? LACT_BF16 : LACT_F32;
   D.pages = (int)k.size(0); D.HK = (int)k.size(1); D.page_size = (int)k.size(2); D.D = (int)k.size(3); D.width = (int)table.size(1);
@@ -950,6 +961,10 @@ CacheCall paged_cache(const Tensor& k, const Tensor& v, const OptTensor& ks, con
 
 void cache_write(const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& k_, const Tensor& v_, const Tensor& table, const OptTensor& starts_,
                  const OptTensor& counts_) {
+  expect_cache_dims(ck, cv, ks, vs, table);
+  if (k_.dim() != v_.dim() || (k_.dim() != 3 && k_.dim() != 4)) throw std::invalid_argument("k and v must both have 4 dimensions, or 3 for one token each");
+  expect_dims(starts_, 1, "starts");
+  expect_dims(counts_, 1, "counts");
   on_gpu(k_);
   const c10::hip::HIPGuard guard(k_.device().index());
   const at::AutoGradMode off(false);
@@ -975,6 +990,9 @@ void cache_write(const Tensor& ck, const Tensor& cv, const OptTensor& ks, const 
 
 std::vector<Tensor> cache_read(const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& table, const Tensor& lengths_, int64_t l,
                                const OptTensor& starts_, at::ScalarType dtype) {
+  expect_cache_dims(ck, cv, ks, vs, table);
+  expect_dims(lengths_, 1, "lengths");
+  expect_dims(starts_, 1, "starts");
   on_gpu(ck);
   const c10::hip::HIPGuard guard(ck.device().index());
   const at::AutoGradMode off(false);
@@ -993,6 +1011,7 @@ std::vector<Tensor> cache_read(const Tensor& ck, const Tensor& cv, const OptTens
 
 Tensor paged_step(const Tensor& q_, const Tensor& ck, const Tensor& cv, const OptTensor& ks, const OptTensor& vs, const Tensor& table, const Tensor& lengths_, int64_t window,
                   double scale, double cap, const OptTensor& slopes_) {
+  expect_cache_dims(ck, cv, ks, vs, table);
   on_gpu(q_);
   const c10::hip::HIPGuard guard(q_.device().index());
   const at::AutoGradMode off(false);

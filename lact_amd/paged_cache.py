@@ -38,8 +38,6 @@ def _tensors(name: str, cache: PagedCache, *more: Optional[torch.Tensor]) -> Non
     if not isinstance(cache, PagedCache):
         raise TypeError(f"{name} takes a PagedCache, got {type(cache).__name__}")
     _plain_only(name, *cache, *more)
-    _dims(name, 4, **{"cache.k": cache.k, "cache.v": cache.v})
-    _dims(name, 3, **{"cache.k_scale": cache.k_scale, "cache.v_scale": cache.v_scale})
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*cache, *more)):
         raise RuntimeError(f"{name} is for inference: call it under torch.no_grad()")
 
@@ -57,10 +55,6 @@ def paged_cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_
     place, for autograd too."""
     name = "paged_cache_write"
     _tensors(name, cache, k, v, page_table, starts, counts)
-    if not (k.dim() == v.dim() and k.dim() in (3, 4)):
-        raise ValueError(f"{name}: k and v must both have 4 dimensions, or 3 for one token each, got {tuple(k.shape)} and {tuple(v.shape)}")
-    _dims(name, 2, page_table=page_table)
-    _dims(name, 1, starts=starts, counts=counts)
     _lib.host().paged_cache_write(*cache, k, v, page_table, starts, counts)
 
 
@@ -73,8 +67,6 @@ def paged_cache_read(cache: PagedCache, page_table: torch.Tensor, lengths: torch
     lengths, starts: [b] int32 (int64 is converted), on the device."""
     name = "paged_cache_read"
     _tensors(name, cache, page_table, lengths, starts)
-    _dims(name, 2, page_table=page_table)
-    _dims(name, 1, lengths=lengths, starts=starts)
     if int(tokens) != tokens or tokens < 0:
         raise ValueError(f"{name}: tokens must be a number of tokens, got {tokens}")
     if dtype is None:
@@ -97,7 +89,6 @@ def paged_attention_step(q: torch.Tensor, cache: PagedCache, page_table: torch.T
     name = "paged_attention_step"
     _tensors(name, cache, q, page_table, lengths, distance_slopes)
     _dims(name, 3, q=q)
-    _dims(name, 2, page_table=page_table)
     q, = _autocast(q)
     window, scale, cap = _options(name, q.shape[2], window, score_cap, scale, distance_slopes)
     return _lib.host().paged_attention_step(q, *cache, page_table, lengths, window, scale, cap, distance_slopes)

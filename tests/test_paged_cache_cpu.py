@@ -113,9 +113,11 @@ def test_step_pointers_and_workspace():
     # two parts a block, of 4 query heads to a key head: 3 sequences x 2 heads x 10 steps of 128 places; none where every item has a block of its own
     assert size(window=1 << 30) == 2 * 60 * 4 * 66 * 4 and size() == 0
     c = cache_desc(pages=1 << 20, width=1 << 18)
-    assert size(window=1 << 30) == 2 * 256 * 4 * 66 * 4
-    c.dtype = 2
     assert size(window=1 << 30) == 2 * 512 * 4 * 66 * 4      # two blocks to a compute unit
+    c.D, c.k_page, c.v_page = 128, 8192, 8192
+    assert size(window=1 << 30, q_bs=1024) == 2 * 256 * 4 * 130 * 4      # one
+    c.dtype = 2
+    assert size(window=1 << 30, q_bs=1024) == 2 * 512 * 4 * 130 * 4
 
 
 def rotary_desc(**kw):
