@@ -188,11 +188,14 @@ template <typename T, int V, bool SIDE>
 int launch_rotary(RotaryParams p, hipStream_t s) {
   p.units = SIDE ? p.D / V : p.pairs / V + (p.D - 2 * p.pairs) / V;
   p.by_units = make_udiv(p.units);
-  p.tokens = 256 / p.units;
   const int heads = p.op[0].heads + p.op[1].heads;
+  p.across = std::min({4, heads, 256 / p.units});
+  p.by_across = make_udiv(p.across);
+  p.tokens = 256 / p.units / p.across;
   const long long blocks = ((long long)p.B * p.L + p.tokens - 1) / p.tokens;
   if (blocks > MAX_BLOCKS) return fail("rotary: too many tokens or heads");
-  p.per = (int)std::max<long long>(1, std::min<long long>(heads, blocks * heads / (8 * COMPUTE_UNITS)));
+  // as many heads to a block, for which it forms a token's angles once, as leave eight blocks to a compute unit
+  p.per = (int)std::max<long long>(p.across, std::min<long long>(heads, blocks * heads / (8 * COMPUTE_UNITS)));
   LACT_LAUNCH("k_rotary", "rotary", 0.0, (k_rotary<T, V, SIDE>), dim3((unsigned)blocks, ceil_div(heads, p.per)), dim3(256), s, p);
   LACT_CHECK_LAUNCH();
   return 0;

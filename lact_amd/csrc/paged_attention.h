@@ -629,8 +629,8 @@ __global__ __launch_bounds__((64 * PagedShape<T, C, D>::NW), (sizeof(T) == 4 && 
 // THREADS: 512 where items have many parts, so that each reads few (256 parts of one sequence: 7 us, bound by the launch and the way to them), else 128.
 template <typename T, int D, int KEYS, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_paged_join(const PagedStepParams<T> p) {
-  constexpr int GROUPS = THREADS / D, WAVES = THREADS / 64;
-  __shared__ float acc_s[GROUPS][D], sum_s[GROUPS], max_s[WAVES];
+  constexpr int GROUPS = THREADS / D;
+  __shared__ float acc_s[GROUPS][D], sum_s[GROUPS], max_s[GROUPS];
   PagedWork<KEYS, PagedStepParams<T>> work(p);
   work.init();
   const int first = blockIdx.x;
@@ -644,34 +644,39 @@ __global__ __launch_bounds__(THREADS) void k_paged_join(const PagedStepParams<T>
   if (h >= (item / p.tiles + 1) * p.group) return;
   const int last = work.block_of(begin + n - 1);
   auto part = [&](int i) { return p.template part_of<D>(i, i != first || work.share(i) == begin) + blockIdx.y * (D + 2); };
-  float m = -INFINITY;
-  for (int i = first + (int)threadIdx.x; i <= last; i += THREADS) m = fmaxf(m, part(i)[D]);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if ((threadIdx.x & 63) == 0) max_s[threadIdx.x >> 6] = m;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < WAVES; ++i) m = fmaxf(m, max_s[i]);
+  // each group of D threads goes through its parts once, with a maximum of its own
   const int grp = threadIdx.x / D, d = threadIdx.x % D;
-  float acc = 0.f, total = 0.f;
+  float m = ATTN_LOWEST, acc = 0.f, total = 0.f;
 #pragma unroll 4
   for (int i = first + grp; i <= last; i += GROUPS) {
     const float* x = part(i);
-    const float w = __builtin_amdgcn_exp2f(x[D] - m);
-    acc += x[d] * w;
-    total += x[D + 1] * w;
+    const float nm = fmaxf(m, x[D]), f = __builtin_amdgcn_exp2f(m - nm), w = __builtin_amdgcn_exp2f(x[D] - nm);
+    acc = fmaf(acc, f, x[d] * w);
+    total = fmaf(total, f, x[D + 1] * w);
+    m = nm;
   }
-  acc_s[grp][d] = acc;
-  if (d == 0) sum_s[grp] = total;
-  __syncthreads();
-  if (grp == 0) {
+  if constexpr (GROUPS > 1) {
+    acc_s[grp][d] = acc;
+    if (d == 0) {
+      max_s[grp] = m;
+      sum_s[grp] = total;
+    }
+    __syncthreads();
+    if (grp != 0) return;
+    float nm = m;
+#pragma unroll
+    for (int i = 1; i < GROUPS; ++i) nm = fmaxf(nm, max_s[i]);
+    const float f = __builtin_amdgcn_exp2f(m - nm);
+    acc *= f;
+    total *= f;
 #pragma unroll
     for (int i = 1; i < GROUPS; ++i) {
-      acc += acc_s[i][d];
-      total += sum_s[i];
+      const float w = __builtin_amdgcn_exp2f(max_s[i] - nm);
+      acc = fmaf(acc_s[i][d], w, acc);
+      total = fmaf(sum_s[i], w, total);
     }
-    Elem<T>::store(p.out + ((size_t)b * p.H + h) * D + d, p.mean(acc, total));
   }
+  Elem<T>::store(p.out + ((size_t)b * p.H + h) * D + d, p.mean(acc, total));
 }
 
 }  // namespace lact

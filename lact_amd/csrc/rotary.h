@@ -6,7 +6,10 @@
 //
 // An angle is formed once for all heads of a token, in quarter turns in fp64 (a far position times a frequency in fp32 would have lost its place in the turn), of
 // which the whole ones are taken off before the rest is rounded to fp32: what is left is at most half a quarter, and its sine and cosine are the first terms of their series.
-// Bound by memory: every channel is read once and written once.
+// Bound by memory: every channel is read once and written once.  24960 tokens of a video, 12 + 12 heads of 128 in bf16, training step (forward and gradients): neighbouring pairs 122 us,
+// in halves 139 (5.0 and 4.4 TB/s; a large copy reaches 5.0).  One head on its way at a time: 136 and 155.  A block has four of a token's heads at once, each of which forms the angles: two
+// at once 127 and 142, eight 152 and 153.  Tried: blocks that walk several tokens, with positions on their way ahead (registers: the forward alone 68 us for 59), 32 bytes a lane for
+// neighbouring pairs.
 #pragma once
 #include "common.h"
 
@@ -23,8 +26,8 @@ struct RotaryParams {
   RotaryOperand op[2];
   int B, L, D, pairs, axes;
   int per;                                    // heads of a block
-  int units, tokens;                          // lanes to a token, tokens of a block
-  UDiv by_units, by_l;
+  int units, across, tokens;                  // lanes to a head, heads of a token at once, tokens of a block
+  UDiv by_units, by_across, by_l;
   const void* positions;
   int position_type;                          // 0: int32, 1: int64, 2: fp32
   long long pos_bs, pos_ls;
@@ -51,31 +54,73 @@ __device__ __forceinline__ double position_of(const RotaryParams& p, int b, int 
   if (p.position_type == 1) return (double)static_cast<const long long*>(p.positions)[at];
   return (double)static_cast<const float*>(p.positions)[at];
 }
-__device__ __forceinline__ Turn turn_of_pair(const RotaryParams& p, int b, int t, int pair) {
-  if (pair >= p.pairs) return Turn{1.f, 0.f};
-  return turn_of(position_of(p, b, t, p.axis[pair]) * p.frequency[pair], p.sign);
+
+// One pair, whose bits stay as they are where nothing is turned (an infinity times a sine of 0 is NaN).
+__device__ __forceinline__ void turn_pair(const Turn& w, float x, float y, float& c, float& d) {
+  c = fmaf(x, w.c, -(y * w.s));
+  d = fmaf(x, w.s, y * w.c);
 }
 
-// One pair, of which what is not turned keeps its bits (an infinity times a sine of 0 is NaN).
+// V elements as they lie in memory: 16 bytes in words, or one or two elements wherever they lie.
+template <typename T, int V>
+struct RotaryFew {
+  T v[V];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = p[i];
+  }
+  __device__ __forceinline__ void store(T* p) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) p[i] = v[i];
+  }
+  __device__ __forceinline__ void unpack(float (&f)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = Elem<T>::load(v + i);
+  }
+  __device__ __forceinline__ void pack(const float (&f)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) Elem<T>::store(v + i, f[i]);
+  }
+  // pair j of neighbours as `from` has it
+  __device__ __forceinline__ void take(const RotaryFew& from, int j) {
+    v[2 * j] = from.v[2 * j];
+    v[2 * j + 1] = from.v[2 * j + 1];
+  }
+};
 template <typename T>
-__device__ __forceinline__ void turn_pair(const Turn& w, T a, T b, T& c, T& d) {
-  const float x = Elem<T>::load(&a), y = Elem<T>::load(&b);
-  Elem<T>::store(&c, fmaf(x, w.c, -(y * w.s)));
-  Elem<T>::store(&d, fmaf(x, w.s, y * w.c));
-}
-
-template <typename T, int N> struct alignas(sizeof(T) * N < 16 ? sizeof(T) : 16) RotaryVec { T v[N]; };
+struct RotaryWide {
+  static constexpr int V = 16 / sizeof(T);
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const T* p) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+  }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]); }
+  __device__ __forceinline__ void unpack(float (&f)[V]) const {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = sizeof(T) == 4 ? __uint_as_float(w[i & 3]) : i & 1 ? bf16_hi(w[i / 2]) : bf16_lo(w[i / 2]);
+  }
+  __device__ __forceinline__ void pack(const float (&f)[V]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = sizeof(T) == 4 ? __float_as_uint(f[i]) : pack_bf16(f[2 * i % V], f[(2 * i + 1) % V]);
+  }
+  __device__ __forceinline__ void take(const RotaryWide& from, int j) {
+    constexpr int WORDS = sizeof(T) / 2;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[WORDS * j + i] = from.w[WORDS * j + i];
+  }
+};
 
 // A lane has V channels of a token's heads, and with halves apart (pairs p and p + pairs) V others.  V = 16 bytes where all sizes, strides and addresses allow
-// it, else 1 (2 where pairs lie side by side).
+// it, else 1 (2 where pairs lie side by side).  Four heads are on their way at once.
 template <typename T, int V, bool SIDE>
 __global__ __launch_bounds__(256) void k_rotary(const RotaryParams p) {
-  using Vec = RotaryVec<T, V>;
-  const int slot = p.by_units.div(threadIdx.x), unit = threadIdx.x - slot * p.units;
-  const long long token = (long long)blockIdx.x * p.tokens + slot;
-  if (slot >= p.tokens || token >= (long long)p.B * p.L) return;
+  using Vec = typename std::conditional<V * sizeof(T) == 16, RotaryWide<T>, RotaryFew<T, V>>::type;
+  const int slot = p.by_units.div(threadIdx.x), unit = threadIdx.x - slot * p.units, place = p.by_across.div(slot);
+  const long long token = (long long)blockIdx.x * p.tokens + place;
+  if (place >= p.tokens || token >= (long long)p.B * p.L) return;
   const int b = p.by_l.div((int)token), t = (int)token - b * p.L;
-  constexpr int N = SIDE ? V / 2 : V;
+  constexpr int N = SIDE ? V / 2 : V, AHEAD = 4;
   const int turning = SIDE ? (2 * p.pairs + V - 1) / V : p.pairs / V;      // units with a pair
   const bool turns = unit < turning;
   const int first = SIDE || turns ? unit * V : 2 * p.pairs + (unit - turning) * V;
@@ -83,29 +128,59 @@ __global__ __launch_bounds__(256) void k_rotary(const RotaryParams p) {
   bool still[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const int pair = SIDE ? unit * N + j : unit * V + j;
+    const int pair = (SIDE ? unit * N : unit * V) + j;
     still[j] = !turns || pair >= p.pairs;
-    w[j] = still[j] ? Turn{1.f, 0.f} : turn_of_pair(p, b, t, pair);
+    w[j] = still[j] ? Turn{1.f, 0.f} : turn_of(position_of(p, b, t, p.axis[pair]) * p.frequency[pair], p.sign);
   }
-  const int h0 = blockIdx.y * p.per, h1 = min(h0 + p.per, p.op[0].heads + p.op[1].heads);
-#pragma unroll 4
-  for (int g = h0; g < h1; ++g) {
-    const RotaryOperand& o = p.op[g >= p.op[0].heads];
-    const int h = g >= p.op[0].heads ? g - p.op[0].heads : g;
-    const T* x = static_cast<const T*>(o.x) + b * o.bs + t * o.ls + h * o.hs;
-    T* y = static_cast<T*>(o.y) + (token * o.heads + h) * p.D;
-    Vec u = *reinterpret_cast<const Vec*>(x + first), r = u;
-    if constexpr (SIDE) {
+  // the lane's heads in turn, first the queries', then the keys'
+  const int g0 = blockIdx.y * p.per + slot - place * p.across;
+  const int end = min((int)(blockIdx.y + 1) * p.per, p.op[0].heads + p.op[1].heads);
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (!still[j]) turn_pair<T>(w[j], u.v[2 * j], u.v[2 * j + 1], r.v[2 * j], r.v[2 * j + 1]);
-    } else if (turns) {
-      Vec u2 = *reinterpret_cast<const Vec*>(x + first + p.pairs), r2;
+  for (int op = 0; op < 2; ++op) {
+    const RotaryOperand& o = p.op[op];
+    const int before = op ? p.op[0].heads : 0, last = min(end, before + o.heads);
+    int g = g0 + p.by_across.div(max(0, before - g0) + p.across - 1) * p.across;      // the first one from there on
+    const T* x = static_cast<const T*>(o.x) + b * o.bs + t * o.ls + (g - before) * o.hs + first;
+    T* y = static_cast<T*>(o.y) + (token * o.heads + g - before) * p.D + first;
+    const long long xs = p.across * o.hs;
+    const int ys = p.across * p.D;
+    for (; g < last; g += AHEAD * p.across, x += AHEAD * xs, y += AHEAD * ys) {
+      Vec u[AHEAD], u2[SIDE ? 1 : AHEAD];
 #pragma unroll
-      for (int j = 0; j < N; ++j) turn_pair<T>(w[j], u.v[j], u2.v[j], r.v[j], r2.v[j]);
-      *reinterpret_cast<Vec*>(y + first + p.pairs) = r2;
+      for (int i = 0; i < AHEAD; ++i)
+        if (g + i * p.across < last) {
+          u[i].load(x + i * xs);
+          if constexpr (!SIDE)
+            if (turns) u2[i].load(x + i * xs + p.pairs);
+        }
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (g + i * p.across < last) {
+          float f[V];
+          u[i].unpack(f);
+          if constexpr (SIDE) {
+            Vec r;
+#pragma unroll
+            for (int j = 0; j < N; ++j) turn_pair(w[j], f[2 * j], f[2 * j + 1], f[2 * j], f[2 * j + 1]);
+            r.pack(f);
+#pragma unroll
+            for (int j = 0; j < N; ++j)
+              if (still[j]) r.take(u[i], j);
+            r.store(y + i * ys);
+          } else if (turns) {
+            float f2[V];
+            u2[i].unpack(f2);
+#pragma unroll
+            for (int j = 0; j < N; ++j) turn_pair(w[j], f[j], f2[j], f[j], f2[j]);
+            u[i].pack(f);
+            u2[i].pack(f2);
+            u[i].store(y + i * ys);
+            u2[i].store(y + i * ys + p.pairs);
+          } else {
+            u[i].store(y + i * ys);
+          }
+        }
     }
-    *reinterpret_cast<Vec*>(y + first) = r;
   }
 }
 
