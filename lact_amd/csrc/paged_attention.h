@@ -56,20 +56,24 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
 }
 
-// The steps of all items in a row: sequence by sequence, each of whose `items` has the same number.  Shares differ by one step at most.  Every wave computes it for itself,
-// 64 sequences at a time, whose lengths stay with its lanes.
+// What a new item costs a block, in steps: the ring runs empty, parts are joined, pages looked up, the ring fills.  32 sequences of up to 8192 places in e4m3 with shares of equal steps / FIGURES
+constexpr int PAGED_START = 2;
+
+// The work of all items in a row: sequence by sequence, each of whose `items` costs the same, its steps and PAGED_START in front of them.  Shares differ by one at most.  Every
+// wave computes it for itself, 64 sequences at a time, whose lengths stay with its lanes.
 template <int KEYS, typename P>
 struct PagedWork {
   const P& p;
-  int items, blocks, more;           // blocks with a share: none is empty; the first `more` have one step more
+  int items, blocks, more;           // blocks with a share: none is empty; the first `more` have one more
   long long total, per;
-  int b0, len, sum;                  // the lanes' sequences from b0 on: lengths, and steps of one item up to and with them
+  int b0, len, sum;                  // the lanes' sequences from b0 on: lengths, and what one item of each up to and with them costs
   __device__ __forceinline__ explicit PagedWork(const P& p_) : p(p_), items(p_.HK * p_.tiles) {}
   __device__ __forceinline__ void load(int from) {
     b0 = from;
     len = p.length(b0 + (int)(threadIdx.x & 63));
-    sum = wave_scan(p.template steps<KEYS>(len));
+    sum = wave_scan(cost(p.template steps<KEYS>(len)));
   }
+  __device__ __forceinline__ static int cost(int steps) { return steps ? steps + PAGED_START : 0; }
   __device__ __forceinline__ int of_all() const { return __builtin_amdgcn_readlane(sum, 63); }
   __device__ __forceinline__ void init() {
     total = 0;
@@ -91,9 +95,9 @@ struct PagedWork {
     if (b < b0 || b >= b0 + 64) load(b & ~63);
     return __builtin_amdgcn_readlane(len, b - b0);
   }
-  // where step s < total lies: sequence, item, step, and how many steps its items have
-  __device__ __forceinline__ void find(long long s, int& b, int& item, int& step, int& n) {
-    const long long x = quotient(s, items);      // in a row of the steps of one item of each
+  // where place s < total of the row lies: sequence, item, place in the item, and how many steps its items have
+  __device__ __forceinline__ void find(long long s, int& b, int& item, int& at, int& n) {
+    const long long x = quotient(s, items);      // in a row of one item of each
     long long before = 0;
     if (p.B > 64) load(0);
     for (;;) {
@@ -102,9 +106,9 @@ struct PagedWork {
         const int i = __ffsll((unsigned long long)past) - 1;
         b = b0 + i;
         n = p.template steps<KEYS>(__builtin_amdgcn_readlane(len, i));
-        const long long in_b = s - (before + __builtin_amdgcn_readlane(sum, i) - n) * items;
-        item = (int)quotient(in_b, n);
-        step = (int)(in_b - (long long)item * n);
+        const long long in_b = s - (before + __builtin_amdgcn_readlane(sum, i) - cost(n)) * items;
+        item = (int)quotient(in_b, cost(n));
+        at = (int)(in_b - (long long)item * cost(n));
         return;
       }
       before += of_all();
@@ -396,15 +400,16 @@ __global__ __launch_bounds__((64 * PagedShape<T, C, D>::NW), (sizeof(T) == 4 && 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   PagedWork<A::KEYS, PagedStepParams<T>> work(p);
   const int items = work.items;
-  // the block's steps: from step0 of this item of sequence b on
-  int b, item, step0, n;
+  // the block's share: from place `at` of this item of sequence b on
+  int b, item, at, n;
   long long left;
   if (p.whole) {
     b = blockIdx.x / items;
     item = blockIdx.x - b * items;
-    step0 = 0;
+    at = 0;
     work.load(b);
-    left = n = p.template steps<A::KEYS>(__builtin_amdgcn_readlane(work.len, 0));
+    n = p.template steps<A::KEYS>(__builtin_amdgcn_readlane(work.len, 0));
+    left = work.cost(n);
     if (n == 0) {
       const int h0 = p.first_head(item), rows = min(16 * QT, (item / p.tiles + 1) * p.group - h0);
       for (int i = threadIdx.x; i < rows * D; i += 64 * NW) Elem<T>::store(p.out + ((size_t)b * p.H + h0) * D + i, 0.f);
@@ -419,7 +424,7 @@ __global__ __launch_bounds__((64 * PagedShape<T, C, D>::NW), (sizeof(T) == 4 && 
     if ((int)blockIdx.x >= work.blocks) return;
     const long long s0 = work.share(blockIdx.x);
     left = work.share(blockIdx.x + 1) - s0;
-    work.find(s0, b, item, step0, n);
+    work.find(s0, b, item, at, n);
   }
   const uint32_t ring = lds_addr(smem) + wave * A::WAVE;
   const char* mine = smem + wave * A::WAVE;
@@ -435,7 +440,8 @@ __global__ __launch_bounds__((64 * PagedShape<T, C, D>::NW), (sizeof(T) == 4 && 
   }
   bool head_of_share = true;
   while (left > 0) {
-    const int step1 = (int)min((long long)n, step0 + left);
+    const int end = (int)min((long long)work.cost(n), at + left), step0 = max(0, at - PAGED_START), step1 = end - PAGED_START;
+    if (step1 <= step0) return;      // (the share ends in front of the item's first step)
     const int hk = item / p.tiles, h0 = p.first_head(item), rows = min(16 * QT, (hk + 1) * p.group - h0);
     const int len = work.length(b), lo = p.first(len), lo16 = lo & ~15;
     // the wave's tiles: 32 places from place(t) on
@@ -507,7 +513,7 @@ __global__ __launch_bounds__((64 * PagedShape<T, C, D>::NW), (sizeof(T) == 4 && 
       const char* kt = mine + t % RING * A::STAGE;
       const char* vt = kt + S::BYTES;
       const char* et = mine + RING * A::STAGE + (t / BATCH & 1) * A::EXP + t % BATCH * 32;
-      const int k0 = place(t), at = k0 + 4 * (lane >> 4);
+      const int k0 = place(t), mine0 = k0 + 4 * (lane >> 4);      // the lane's first key
       const int on_pages = (t / BATCH == batch ? there : there_before) >> (2 * (t % BATCH)) & 3;      // of the two pieces
       const bool masked = k0 < lo || k0 + 32 > len || on_pages != 3;
       PagedScores<QT> s;
@@ -528,14 +534,14 @@ __global__ __launch_bounds__((64 * PagedShape<T, C, D>::NW), (sizeof(T) == 4 && 
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int key = at + 16 * kt + i;
+            const int key = mine0 + 16 * kt + i;
             const bool seen = key >= lo && key < len && (on_pages >> kt & 1);
 #pragma unroll
             for (int x = 0; x < QT; ++x) s.s[x][kt][i] = seen ? s.s[x][kt][i] : nothing;
           }
       };
 #pragma unroll
-      for (int x = 0; x < QT; ++x) bend(sc[x], s.s[x], at - (len - 1));
+      for (int x = 0; x < QT; ++x) bend(sc[x], s.s[x], mine0 - (len - 1));
       if (masked) mask(-__builtin_inff());
 #pragma unroll
       for (int x = 0; x < QT; ++x) {
@@ -614,8 +620,8 @@ __global__ __launch_bounds__((64 * PagedShape<T, C, D>::NW), (sizeof(T) == 4 && 
     }
     __syncthreads();      // the rings are free again
     head_of_share = false;
-    left -= step1 - step0;
-    step0 = 0;
+    left -= end - at;
+    at = 0;
     if (++item == items) {
       item = 0;
       do {
@@ -625,7 +631,7 @@ __global__ __launch_bounds__((64 * PagedShape<T, C, D>::NW), (sizeof(T) == 4 && 
   }
 }
 
-// Joins what blocks left of an item that they share.  A block (x, y): row y of the item that share x + 1 begins inside, if share x does not begin inside it as well.
+// Joins what blocks left of an item that they share.  A block (x, y): row y of the item that share x + 1 begins inside, behind its first step, if share x does not as well.
 // THREADS: 512 where items have many parts, so that each reads few (256 parts of one sequence: 7 us, bound by the launch and the way to them), else 128.
 template <typename T, int D, int KEYS, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_paged_join(const PagedStepParams<T> p) {
@@ -635,15 +641,15 @@ __global__ __launch_bounds__(THREADS) void k_paged_join(const PagedStepParams<T>
   work.init();
   const int first = blockIdx.x;
   if (first + 1 >= work.blocks) return;
-  const long long at = work.share(first + 1);
-  int b, item, step, n;
-  work.find(at, b, item, step, n);
-  const long long begin = at - step;
-  if (step == 0 || work.share(first) > begin) return;
+  const long long next = work.share(first + 1);
+  int b, item, at, n;
+  work.find(next, b, item, at, n);
+  const long long begin = next - at;
+  if (at <= PAGED_START || work.share(first) > begin + PAGED_START) return;
   const int h = p.first_head(item) + (int)blockIdx.y;
   if (h >= (item / p.tiles + 1) * p.group) return;
-  const int last = work.block_of(begin + n - 1);
-  auto part = [&](int i) { return p.template part_of<D>(i, i != first || work.share(i) == begin) + blockIdx.y * (D + 2); };
+  const int last = work.block_of(begin + work.cost(n) - 1);
+  auto part = [&](int i) { return p.template part_of<D>(i, i != first || work.share(i) >= begin) + blockIdx.y * (D + 2); };
   // each group of D threads goes through its parts once, with a maximum of its own
   const int grp = threadIdx.x / D, d = threadIdx.x % D;
   float m = ATTN_LOWEST, acc = 0.f, total = 0.f;
