@@ -120,10 +120,8 @@ int most_steps(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) {
 }
 int step_columns(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) { return d->H / c->HK <= 16 ? 16 : 32; }
 int step_items(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) { return d->B * c->HK * ceil_div(d->H / c->HK, step_columns(c, d)); }
-// One block for every item, where the longest has few steps, and no second launch.
-constexpr int WHOLE_STEPS = 4;
 template <typename A>
-bool step_whole(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) { return most_steps<A>(c, d) <= WHOLE_STEPS; }
+bool step_whole(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) { return most_steps<A>(c, d) <= A::WHOLE; }
 template <typename A>
 int step_blocks(const lact_paged_cache_t* c, const lact_paged_step_desc_t* d) {
   const int items = step_items(c, d);

@@ -56,7 +56,8 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
 }
 
-// What a new item costs a block, in steps: the ring runs empty, parts are joined, pages looked up, the ring fills.  32 sequences of up to 8192 places in e4m3 with shares of equal steps / FIGURES
+// What a new item costs a block, in steps: the ring runs empty, parts are joined, pages looked up, the ring fills.  In the row of all items 0 / 1 / 2 / 3 / 6 for it: 32 sequences of up to
+// 8192 places, 8 heads of 128, e4m3 68 / 61 / 60 / 63 / 65 us, bf16 119 / 100 / 98 / 98 / 102; 64 of up to 16384, e4m3 187 / 174 / 174 / 175 / 180.
 constexpr int PAGED_START = 2;
 
 // The work of all items in a row: sequence by sequence, each of whose `items` costs the same, its steps and PAGED_START in front of them.  Shares differ by one at most.  Every
@@ -141,6 +142,9 @@ struct PagedShape {
   static constexpr int WAVE = RING * STAGE + 2 * EXP;
   static constexpr int KEYS = 32 * NW;                                       // of a step
   static constexpr int LDS = NW * WAVE;
+  // A block has an item as a whole, and no second launch, where the longest has no more steps.  Against shares: 64 sequences of up to 1000 places, 8 heads of 128, e4m3 18.8 us for 22.0; 16 in
+  // bf16 12.3 for 15.2, of 64 9.6 for 12.5; 4 steps of fp32, one sequence of 500, 12 heads of 64 10.5 for 11.9, 8 steps 17.4 for 11.7 (its products take longer).
+  static constexpr int WHOLE = sizeof(C) == 4 ? 4 : 8;
 };
 
 // Products of 16 x 16: a wave's 32 keys in two tiles as rows, QT tiles of 16 query heads as columns.  A lane has the keys 16 kt + 4 h + i (h = lane / 16) of column
