@@ -126,13 +126,14 @@ def test_places_without_a_page(table, lengths, window, d, dtype, held):
 
 
 @KINDS
+@pytest.mark.parametrize("wide", [4, 40])
 @pytest.mark.parametrize("d", [64, 128])
-def test_what_is_not_seen_reaches_nothing(d, dtype, held):
+def test_what_is_not_seen_reaches_nothing(d, wide, dtype, held):
     """Places past the length, in front of the window and on other pages hold NaN and infinities, exponents of NaN beside them."""
     import lact_amd
     print("[gpu-test] paged step, unseen", d, dtype, held, flush=True)
     size, lengths, window = 48, [100, 55, 1, 96], 37
-    table, count = tables(lengths, size, 4)
+    table, count = tables(lengths, size, wide)
     cache = random_cache(count, 2, size, d, held)
     q = torch.randn(len(lengths), 4, d, generator=torch.Generator().manual_seed(3)).to(dtype)
     step = lambda c: lact_amd.paged_attention_step(q.to("cuda"), cuda(c), table.to("cuda"), torch.tensor(lengths, device="cuda"), window)  # noqa: E731
@@ -178,6 +179,66 @@ def test_step_of_many_parts_is_joined(dtype, held):
 def test_step_of_a_long_sequence(dtype, held):
     """More pieces than the waves look up at once, in every block: one head of 70000 places, which a sequence of others splits in odd shares."""
     check_step([70000, 333, 4000], 70016 // 16, 16, 3, 1, 64, dtype, held)
+
+
+@KINDS
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lengths,size,hq,hkv,window,cap,slopes", [
+    ([0, 1500, 1, 0, 700, 16, 1100], 16, 5, 1, None, None, False),               # shares that begin and end anywhere, in front of a first step too
+    ([1300, 20, 1290], 48, 17, 1, None, None, False), ([900, 1500], 16, 33, 1, 1200, None, True),      # more query heads to a key head than 16, and than 32
+    ([1500, 0, 1400], 80, 32, 2, 1111, 20.0, False), ([0, 0, 0], 16, 2, 2, None, None, False), ([1], 16, 1, 1, None, None, False),
+    ([1040, 0, 1030, 16, 17, 1200] * 20, 16, 4, 4, None, None, False),           # more sequences than a wave looks at at once
+    ([i * 37 % 1500 if i % 3 else 0 for i in range(150)], 32, 6, 2, None, None, False)])
+def test_shares_of_long_tables(lengths, size, hq, hkv, window, cap, slopes, d, dtype, held):
+    """Tables wide enough that the work is cut into shares and joined."""
+    check_step(lengths, 4096 // size, size, hq, hkv, d, dtype, held, window, cap, slopes)
+
+
+@KINDS
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq", [15, 16, 17, 31, 32, 33, 48, 49, 65])
+def test_query_heads_of_one_key_head(hq, d, dtype, held):
+    check_step([150, 77], 10, 16, hq, 1, d, dtype, held)
+
+
+@KINDS
+def test_places_without_a_page_in_shares(dtype, held):
+    """Holes of a page and of long runs, in sequences that several blocks share; a sequence of holes alone."""
+    g = torch.Generator().manual_seed(3)
+    wide, size = 140, 16
+    table = torch.randint(0, 60, (3, wide), generator=g, dtype=torch.int32)
+    table[0, ::3] = -1
+    table[1, 20:115] = 60
+    table[2] = -1
+    check_step([2200, 2111, 2240], wide, size, 4, 2, 64, dtype, held, table=table, cache=random_cache(60, 2, size, 64, held))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("wide", [4, 100])
+def test_exponents_of_all_sizes(wide, dtype):
+    """Keys that are small and large against each other, values whose powers of two differ by a hundred."""
+    lengths, size, hkv, d = [60, 33], 16, 2, 64
+    table, count = tables(lengths, size, wide)
+    cache = random_cache(count, hkv, size, d, E4M3)
+    g = torch.Generator().manual_seed(5)
+    cache[2] = torch.randint(90, 122, cache[2].shape, generator=g).to(torch.uint8).view(E8M0)
+    cache[3] = torch.randint(50, 150, cache[3].shape, generator=g).to(torch.uint8).view(E8M0)
+    check_step(lengths, wide, size, 4, hkv, d, dtype, E4M3, table=table, cache=cache)
+
+
+@KINDS
+def test_queries_and_tables_with_strides(dtype, held):
+    import lact_amd
+    lengths, size, hkv, d = [70, 33], 32, 2, 64
+    table, count = tables(lengths, size, 3)
+    cache = cuda(random_cache(count, hkv, size, d, held))
+    q = torch.randn(4, 8, d, device="cuda").to(dtype)
+    n = torch.tensor(lengths, device="cuda")
+    wide = torch.stack((table, table + 1), -1).to("cuda")
+    ref = lact_amd.paged_attention_step(q[::2, 1::2].contiguous(), cache, table.to("cuda"), n.int())
+    assert torch.equal(lact_amd.paged_attention_step(q[::2, 1::2], cache, wide[..., 0], torch.stack((n, n), 1)[:, 1]), ref)
+    odd = torch.cat((torch.zeros(1, device="cuda", dtype=dtype), q[::2, 1::2].flatten()))[1:].view(2, 4, d)
+    assert torch.equal(lact_amd.paged_attention_step(odd, cache, table.long().to("cuda"), n), ref)
 
 
 def test_long_share_of_one_block():
@@ -439,10 +500,11 @@ def test_prompt_and_tokens_agree(d, dtype, held):
 
 
 @KINDS
-def test_captured_tokens(dtype, held):
+@pytest.mark.parametrize("wide", [8, 100])
+def test_captured_tokens(wide, dtype, held):
     """Positions, writing and attention captured once and replayed while the sequences grow and their tables change; eager calls and other work in between."""
     import lact_amd
-    b, hq, hkv, d, size, wide = 3, 4, 2, 64, 16, 8
+    b, hq, hkv, d, size = 3, 4, 2, 64, 16
     q, k, v = (torch.randn(b, n, d, device="cuda").to(dtype) for n in (hq, hkv, hkv))
     caches = [lact_amd.PagedCache(*(None if t is None else t.view(torch.uint8).zero_().view(t.dtype) for t in lact_amd.PagedCache.empty(b * wide, hkv, size, d, dtype=held)))
               for _ in range(2)]
