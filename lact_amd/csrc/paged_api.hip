@@ -285,7 +285,7 @@ int lact_axial_rotary(const lact_rotary_desc_t* d, const void* q, const void* k,
   memset(&p, 0, sizeof(p));
   p.op[0] = RotaryOperand{q, q_out, d->q_bs, d->q_ls, d->q_hs, d->H};
   p.op[1] = RotaryOperand{k, k_out, d->k_bs, d->k_ls, d->k_hs, d->HK};
-  p.B = d->B; p.L = d->L; p.D = d->D; p.pairs = d->pairs; p.axes = d->n_axes;
+  p.B = d->B; p.L = d->L; p.D = d->D; p.pairs = d->pairs;
   p.by_l = make_udiv(d->L);
   p.positions = positions; p.position_type = d->position_type; p.pos_bs = d->p_bs; p.pos_ls = d->p_ls;
   p.sign = d->inverse ? -1.f : 1.f;

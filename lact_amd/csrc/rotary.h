@@ -24,7 +24,7 @@ struct RotaryOperand {
 };
 struct RotaryParams {
   RotaryOperand op[2];
-  int B, L, D, pairs, axes;
+  int B, L, D, pairs;
   int per;                                    // heads of a block
   int units, across, tokens;                  // lanes to a head, heads of a token at once, tokens of a block
   UDiv by_units, by_across, by_l;
