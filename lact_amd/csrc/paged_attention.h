@@ -103,7 +103,8 @@ struct PagedWork {
     if (b < b0 || b >= b0 + 64) load(b & ~63);
     return __builtin_amdgcn_readlane(len, b - b0);
   }
-  // where place s < total of the row lies: sequence, item, place in the item, and how many steps its items have
+  // where place s < total of the row lies: sequence, item, place in the item, and how many steps its items have.  (Lengths that somebody changes meanwhile make no sense, but nothing here
+  // leaves the batch, the heads or the workspace for it.)
   __device__ __forceinline__ void find(long long s, int& b, int& item, int& at, int& n) {
     const long long x = quotient(s, items);      // in a row of one item of each
     long long before = 0;
@@ -111,12 +112,12 @@ struct PagedWork {
     for (;;) {
       const uint64_t past = __ballot(x - before < sum);
       if (past || b0 + 64 >= p.B) {
-        const int i = __ffsll((unsigned long long)past) - 1;
+        const int i = past ? __ffsll((unsigned long long)past) - 1 : p.B - 1 - b0;
         b = b0 + i;
-        n = p.template steps<KEYS>(__builtin_amdgcn_readlane(len, i));
-        const long long in_b = s - (before + __builtin_amdgcn_readlane(sum, i) - cost(n)) * items;
-        item = (int)quotient(in_b, cost(n));
-        at = (int)(in_b - (long long)item * cost(n));
+        n = max(1, p.template steps<KEYS>(__builtin_amdgcn_readlane(len, i)));
+        const long long in_b = max(0LL, s - (before + __builtin_amdgcn_readlane(sum, i) - cost(n)) * items);
+        item = (int)min((long long)items - 1, quotient(in_b, cost(n)));
+        at = (int)min((long long)cost(n) - 1, in_b - (long long)item * cost(n));
         return;
       }
       before += of_all();
@@ -659,7 +660,7 @@ __global__ __launch_bounds__(THREADS) void k_paged_join(const PagedStepParams<T>
   if (at <= PAGED_START || work.share(first) > begin + PAGED_START) return;
   const int h = p.first_head(item) + (int)blockIdx.y;
   if (h >= (item / p.tiles + 1) * p.group) return;
-  const int last = work.block_of(begin + work.cost(n) - 1);
+  const int last = min(work.blocks - 1, work.block_of(begin + work.cost(n) - 1));
   auto part = [&](int i) { return p.template part_of<D>(i, i != first || work.share(i) >= begin) + blockIdx.y * (D + 2); };
   // each group of D threads goes through its parts once, with a maximum of its own
   const int grp = threadIdx.x / D, d = threadIdx.x % D;
