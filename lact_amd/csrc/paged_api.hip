@@ -187,7 +187,8 @@ int launch_rotary(RotaryParams p, hipStream_t s) {
   p.units = SIDE ? p.D / V : p.pairs / V + (p.D - 2 * p.pairs) / V;
   p.by_units = make_udiv(p.units);
   const int heads = p.op[0].heads + p.op[1].heads;
-  p.across = std::min({4, heads, 256 / p.units});
+  // heads side by side, each of which forms the angles: with few heads fewer, so that angles are formed for six at least (rotary.h)
+  p.across = std::min(std::max(1, std::min(4, heads / 6)), 256 / p.units);
   p.by_across = make_udiv(p.across);
   p.tokens = 256 / p.units / p.across;
   const long long blocks = ((long long)p.B * p.L + p.tokens - 1) / p.tokens;

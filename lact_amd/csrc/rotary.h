@@ -8,8 +8,9 @@
 // which the whole ones are taken off before the rest is rounded to fp32: what is left is at most half a quarter, and its sine and cosine are the first terms of their series.
 // Bound by memory: every channel is read once and written once.  24960 tokens of a video, 12 + 12 heads of 128 in bf16, training step (forward and gradients): neighbouring pairs 122 us,
 // in halves 139 (5.0 and 4.4 TB/s; a large copy reaches 5.0).  One head on its way at a time: 136 and 155.  A block has four of a token's heads at once, each of which forms the angles: two
-// at once 127 and 142, eight 152 and 153.  Tried: blocks that walk several tokens, with positions on their way ahead (registers: the forward alone 68 us for 59), 32 bytes a lane for
-// neighbouring pairs.
+// at once 127 and 142, eight 152 and 153.  With few heads fewer: 147285 tokens, 6 + 3 heads of 128, in halves, half of each head turned, forward, one / two / four at once 158 / 198 / 316 us;
+// 24960 tokens, 8 + 8 heads, neighbouring pairs 43 / 39 / 43.  Tried: blocks that walk several tokens, with positions on their way ahead (registers: the forward alone 68 us
+// for 59), 32 bytes a lane for neighbouring pairs.
 #pragma once
 #include "common.h"
 
