@@ -93,9 +93,9 @@ int check_tokens(const lact_paged_cache_t* c, int B, int L) {
   return 0;
 }
 template <typename T, int D>
-dim3 cache_grid(const lact_paged_cache_t* c, int B, int L, const int32_t* starts, CacheRows* r) {
+dim3 cache_grid(const lact_paged_cache_t* c, int B, int L, const int32_t* starts, bool along, CacheRows* r) {
   using A = CacheTile<T, D>;
-  const int tiles = A::tiles(L), groups = ceil_div(c->HK, A::HEADS);
+  const int tiles = along ? ceil_div(A::tiles(L), A::TURNS) : A::tiles(L), groups = ceil_div(c->HK, along ? A::ACROSS : A::HEADS);
   *r = CacheRows{B, L, c->HK, make_udiv(tiles), make_udiv(groups), starts};
   return dim3(B * tiles, 2 * groups);
 }
@@ -231,11 +231,13 @@ int lact_paged_cache_write(const lact_paged_cache_t* c, int32_t act_dtype, int32
     CacheWriteParams<T> p;
     memset(&p, 0, sizeof(p));
     p.to = pages_of(c, table);
-    const dim3 grid = cache_grid<T, D>(c, B, L, starts, &p.rows);
+    const bool along = CacheTile<T, D>::along(c->HK, L);
+    const dim3 grid = cache_grid<T, D>(c, B, L, starts, along, &p.rows);
     p.k = static_cast<const T*>(k); p.v = static_cast<const T*>(v);
     p.ldk = k_ld; p.bsk = k_bs; p.ldv = v_ld; p.bsv = v_bs;
     p.counts = counts;
-    LACT_LAUNCH("k_cache_write", "paged_cache", 0.0, (k_cache_write<T, C, D>), grid, dim3(256), s, p);
+    if (along) LACT_LAUNCH("k_cache_write", "paged_cache", 0.0, (k_cache_write<T, C, D, true>), grid, dim3(256), s, p);
+    else LACT_LAUNCH("k_cache_write", "paged_cache", 0.0, (k_cache_write<T, C, D, false>), grid, dim3(256), s, p);
     LACT_CHECK_LAUNCH();
     return 0;
   });
@@ -253,10 +255,12 @@ int lact_paged_cache_read(const lact_paged_cache_t* c, int32_t act_dtype, int32_
     CacheReadParams<T> p;
     memset(&p, 0, sizeof(p));
     p.from = pages_of(c, table);
-    const dim3 grid = cache_grid<T, D>(c, B, L, starts, &p.rows);
+    const bool along = CacheTile<T, D>::along(c->HK, L);
+    const dim3 grid = cache_grid<T, D>(c, B, L, starts, along, &p.rows);
     p.k = static_cast<T*>(k); p.v = static_cast<T*>(v);
     p.lengths = lengths;
-    LACT_LAUNCH("k_cache_read", "paged_cache", 0.0, (k_cache_read<T, C, D>), grid, dim3(256), s, p);
+    if (along) LACT_LAUNCH("k_cache_read", "paged_cache", 0.0, (k_cache_read<T, C, D, true>), grid, dim3(256), s, p);
+    else LACT_LAUNCH("k_cache_read", "paged_cache", 0.0, (k_cache_read<T, C, D, false>), grid, dim3(256), s, p);
     LACT_CHECK_LAUNCH();
     return 0;
   });

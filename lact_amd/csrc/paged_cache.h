@@ -44,29 +44,36 @@ struct CacheTile {
   static constexpr int TURNS = 4, HEADS = ACROSS * TURNS;                         // of a block
   // tiles that L places from anywhere touch
   static int tiles(int L) { return (L + 2 * PLACES - 2) / PLACES; }
+  // With a quarter of these heads a thread's turns go along the sequence instead, each with a page of its own: 53 sequences of up to 16336 tokens, 2 heads of 64, bf16 into e4m3 and back
+  // 221 us for 319, 8 of 16336, one head of 128 30 for 45; with half of them 8 x 16336, 2 heads of 128 56 for 58, but 53 x 16336, 4 heads of 64 423 for 403.
+  static bool along(int HK, int L) { return 4 * HK <= HEADS && L >= 4 * PLACES; }
 };
 struct CacheRows {
   int B, L, HK;
   UDiv by_tiles, by_groups;      // tiles of a sequence, blocks with some of the heads
   const int* starts;             // [B], null: 0
 };
-// What a thread has: sequence, token (which may lie outside), its place, the first of its heads; keys or values.
-template <typename T, int D>
+// What a thread has in turn i: a head of a token (which may lie outside) and its place; keys or values.
+template <typename T, int D, bool ALONG>
 struct CacheRow {
-  int b, h, t;
-  long long place;
+  using A = CacheTile<T, D>;
+  int b, h;
+  long long start, first;
   bool values;
-  __device__ __forceinline__ explicit CacheRow(const CacheRows& r) {
-    using A = CacheTile<T, D>;
-    const int row = threadIdx.x / A::G, tile = r.by_tiles.div(blockIdx.x);
-    const int half = r.by_groups.div(blockIdx.y);
-    b = tile;
+  const CacheRows& r;
+  __device__ __forceinline__ explicit CacheRow(const CacheRows& r_) : r(r_) {
+    const int row = threadIdx.x / A::G, half = r.by_groups.div(blockIdx.y);
+    b = r.by_tiles.div(blockIdx.x);
     values = half != 0;
-    h = (blockIdx.y - half * (int)r.by_groups.d) * A::HEADS + row / A::PLACES;
-    const long long start = r.starts ? r.starts[b] : 0, first = start - (start & (A::PLACES - 1));
-    place = first + (long long)(blockIdx.x - tile * (int)r.by_tiles.d) * A::PLACES + row % A::PLACES;
-    const long long at = place - start;
-    t = at < 0 || at >= r.L ? -1 : (int)at;
+    h = (blockIdx.y - half * (int)r.by_groups.d) * (ALONG ? A::ACROSS : A::HEADS) + row / A::PLACES;
+    start = r.starts ? r.starts[b] : 0;
+    first = start - (start & (A::PLACES - 1)) + (long long)(blockIdx.x - b * (int)r.by_tiles.d) * (ALONG ? A::TURNS * A::PLACES : A::PLACES) + row % A::PLACES;
+  }
+  __device__ __forceinline__ int head(int i) const { return ALONG ? h : h + i * A::ACROSS; }
+  __device__ __forceinline__ long long place(int i) const { return ALONG ? first + i * A::PLACES : first; }
+  __device__ __forceinline__ int token(int i) const {      // -1: none
+    const long long t = place(i) - start;
+    return t < 0 || t >= r.L || head(i) >= r.HK ? -1 : (int)t;
   }
 };
 
@@ -80,29 +87,37 @@ struct CacheWriteParams {
   const int* counts;          // null: L
 };
 
-template <typename T, typename C, int D>
+template <typename T, typename C, int D, bool ALONG>
 __global__ __launch_bounds__(256) void k_cache_write(const CacheWriteParams<T> p) {
   using A = CacheTile<T, D>;
-  constexpr int E = A::E, G = A::G;
-  const CacheRow<T, D> r(p.rows);
-  const int lane = threadIdx.x % G;
-  const int page = r.t >= 0 && !(p.counts && r.t >= p.counts[r.b]) ? p.to.page(r.b, r.place) : -1;
-  const T* from = (r.values ? p.v : p.k) + r.b * (r.values ? p.bsv : p.bsk) + r.t * (r.values ? p.ldv : p.ldk) + r.h * D + lane * E;
+  constexpr int E = A::E, G = A::G, LOOKUPS = ALONG ? A::TURNS : 1;
+  const CacheRow<T, D, ALONG> r(p.rows);
+  const int lane = threadIdx.x % G, count = p.counts ? p.counts[r.b] : 0x7fffffff;
+  int page[LOOKUPS], row[LOOKUPS];
+#pragma unroll
+  for (int i = 0; i < LOOKUPS; ++i) {
+    const int t = r.token(i);
+    page[i] = t >= 0 && t < count ? p.to.page(r.b, r.place(i)) : -1;
+    row[i] = page[i] >= 0 ? p.to.row(r.place(i)) : 0;
+  }
+  const T* from = (r.values ? p.v : p.k) + r.b * (r.values ? p.bsv : p.bsk) + lane * E;
+  const long long ld = r.values ? p.ldv : p.ldk;
   uint4 u[A::TURNS];
 #pragma unroll
   for (int i = 0; i < A::TURNS; ++i) {
     u[i] = make_uint4(0, 0, 0, 0);
-    if (page >= 0 && r.h + i * A::ACROSS < p.rows.HK) u[i] = *reinterpret_cast<const uint4*>(from + i * A::ACROSS * D);
+    if (page[i % LOOKUPS] >= 0 && r.token(i) >= 0) u[i] = *reinterpret_cast<const uint4*>(from + r.token(i) * ld + r.head(i) * D);
   }
-  const int row = page >= 0 ? p.to.rows_before(r.h, p.to.row(r.place)) : 0;
-  C* to = static_cast<C*>(r.values ? p.to.v : p.to.k) + page * (r.values ? p.to.v_page : p.to.k_page) + (long long)row * D + lane * E;
-  uint8_t* exponent = is_e4m3<C>() ? (r.values ? p.to.vs : p.to.ks) + page * (r.values ? p.to.vs_page : p.to.ks_page) + row : nullptr;
+  C* pages = static_cast<C*>(r.values ? p.to.v : p.to.k);
+  uint8_t* exponents = r.values ? p.to.vs : p.to.ks;
+  const long long stride = r.values ? p.to.v_page : p.to.k_page, estride = r.values ? p.to.vs_page : p.to.ks_page;
 #pragma unroll
   for (int i = 0; i < A::TURNS; ++i) {
-    const bool there = page >= 0 && r.h + i * A::ACROSS < p.rows.HK;
-    const long long rows = (long long)i * A::ACROSS * p.to.size;
+    const bool there = page[i % LOOKUPS] >= 0 && r.token(i) >= 0;
+    const long long rows = p.to.rows_before(r.head(i), row[i % LOOKUPS]);
+    C* to = pages + page[i % LOOKUPS] * stride + rows * D + lane * E;
     if constexpr (!is_e4m3<C>()) {
-      if (there) *reinterpret_cast<uint4*>(to + rows * D) = u[i];
+      if (there) *reinterpret_cast<uint4*>(to) = u[i];
     } else {
       float x[E];
       if constexpr (E == 8) {
@@ -130,9 +145,9 @@ __global__ __launch_bounds__(256) void k_cache_write(const CacheWriteParams<T> p
         c[j] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2] * f, x[4 * j + 3] * f, w, true);
       }
       if (there) {
-        if constexpr (E == 8) *reinterpret_cast<uint2*>(to + rows * D) = make_uint2(c[0], c[1]);
-        else *reinterpret_cast<uint32_t*>(to + rows * D) = c[0];
-        if (lane == 0) exponent[rows] = (uint8_t)e;
+        if constexpr (E == 8) *reinterpret_cast<uint2*>(to) = make_uint2(c[0], c[1]);
+        else *reinterpret_cast<uint32_t*>(to) = c[0];
+        if (lane == 0) exponents[page[i % LOOKUPS] * estride + rows] = (uint8_t)e;
       }
     }
   }
@@ -147,17 +162,22 @@ struct CacheReadParams {
   const int* lengths;
 };
 
-template <typename T, typename C, int D>
+template <typename T, typename C, int D, bool ALONG>
 __global__ __launch_bounds__(256) void k_cache_read(const CacheReadParams<T> p) {
   using A = CacheTile<T, D>;
-  constexpr int E = A::E, G = A::G;
-  const CacheRow<T, D> r(p.rows);
-  if (r.t < 0) return;
-  const int lane = threadIdx.x % G, page = r.place < p.lengths[r.b] ? p.from.page(r.b, r.place) : -1;
-  const int row = page >= 0 ? p.from.rows_before(r.h, p.from.row(r.place)) : 0;
-  const C* from = static_cast<const C*>(r.values ? p.from.v : p.from.k) + page * (r.values ? p.from.v_page : p.from.k_page) + (long long)row * D + lane * E;
-  const uint8_t* exponent = is_e4m3<C>() ? (r.values ? p.from.vs : p.from.ks) + page * (r.values ? p.from.vs_page : p.from.ks_page) + row : nullptr;
-  T* to = (r.values ? p.v : p.k) + (((long long)r.b * p.rows.L + r.t) * p.rows.HK + r.h) * D + lane * E;
+  constexpr int E = A::E, G = A::G, LOOKUPS = ALONG ? A::TURNS : 1;
+  const CacheRow<T, D, ALONG> r(p.rows);
+  const int lane = threadIdx.x % G, length = p.lengths[r.b];
+  int page[LOOKUPS], row[LOOKUPS];
+#pragma unroll
+  for (int i = 0; i < LOOKUPS; ++i) {
+    page[i] = r.token(i) >= 0 && r.place(i) < length ? p.from.page(r.b, r.place(i)) : -1;
+    row[i] = page[i] >= 0 ? p.from.row(r.place(i)) : 0;
+  }
+  const C* pages = static_cast<const C*>(r.values ? p.from.v : p.from.k);
+  const uint8_t* exponents = r.values ? p.from.vs : p.from.ks;
+  const long long stride = r.values ? p.from.v_page : p.from.k_page, estride = r.values ? p.from.vs_page : p.from.ks_page;
+  T* to = (r.values ? p.v : p.k) + (long long)r.b * p.rows.L * p.rows.HK * D + lane * E;
   using Raw = typename std::conditional<!is_e4m3<C>(), uint4, typename std::conditional<E == 8, uint2, uint32_t>::type>::type;
   Raw u[A::TURNS];
   uint32_t e[A::TURNS];
@@ -165,10 +185,10 @@ __global__ __launch_bounds__(256) void k_cache_read(const CacheReadParams<T> p) 
   for (int i = 0; i < A::TURNS; ++i) {
     u[i] = Raw{};
     e[i] = 127;
-    if (page >= 0 && r.h + i * A::ACROSS < p.rows.HK) {
-      const long long rows = (long long)i * A::ACROSS * p.from.size;
-      u[i] = *reinterpret_cast<const Raw*>(from + rows * D);
-      if constexpr (is_e4m3<C>()) e[i] = exponent[rows];
+    if (page[i % LOOKUPS] >= 0 && r.token(i) >= 0) {
+      const long long rows = p.from.rows_before(r.head(i), row[i % LOOKUPS]);
+      u[i] = *reinterpret_cast<const Raw*>(pages + page[i % LOOKUPS] * stride + rows * D + lane * E);
+      if constexpr (is_e4m3<C>()) e[i] = exponents[page[i % LOOKUPS] * estride + rows];
     }
   }
 #pragma unroll
@@ -185,7 +205,7 @@ __global__ __launch_bounds__(256) void k_cache_read(const CacheReadParams<T> p) 
       const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)u[i], false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)u[i], true);
       w = make_uint4(__float_as_uint(a[0] * s), __float_as_uint(a[1] * s), __float_as_uint(b[0] * s), __float_as_uint(b[1] * s));
     }
-    if (r.h + i * A::ACROSS < p.rows.HK) *reinterpret_cast<uint4*>(to + i * A::ACROSS * D) = w;
+    if (r.token(i) >= 0) *reinterpret_cast<uint4*>(to + ((long long)r.token(i) * p.rows.HK + r.head(i)) * D) = w;
   }
 }
 

@@ -325,7 +325,8 @@ def places_written(table, pages, size, starts, counts, l):
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("b,l,hkv,size,starts,counts", [
     (1, 1, 1, 16, None, None), (2, 33, 3, 16, [5, 0], None), (3, 70, 2, 32, [0, 31, 90], [70, 0, 13]), (2, 40, 1, 48, [-7, 130], [40, 2 ** 31 - 1]),
-    (5, 1, 4, 64, [0, 63, 64, 191, 192], [1, 1, 0, 1, 1]), (1, 300, 2, 16, [2 ** 31 - 100], None)])
+    (5, 1, 4, 64, [0, 63, 64, 191, 192], [1, 1, 0, 1, 1]), (1, 300, 2, 16, [2 ** 31 - 100], None), (3, 130, 1, 32, [3, 77, -20], [100, 130, 64]),
+    (2, 64, 2, 48, [15, 0], None)])
 def test_write_puts_tokens_into_their_places(b, l, hkv, size, starts, counts, d, dtype, held):
     """Bit by bit, and nothing else changes."""
     import lact_amd
@@ -409,12 +410,13 @@ def test_reading_every_number_of_8_bits(dtype):
 
 
 @KINDS
+@pytest.mark.parametrize("hkv", [1, 2, 3])
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("starts,lengths,tokens", [(None, [100, 33, 0], 100), ([10, 0, 96], [90, 200, 97], 64), ([-5, 2 ** 31 - 1, 100], [50, 2 ** 31 - 1, 100], 70), ([3, 4, 5], [7, 4, 6], 1)])
-def test_read(starts, lengths, tokens, d, dtype, held):
+def test_read(starts, lengths, tokens, d, hkv, dtype, held):
     import lact_amd
-    print("[gpu-test] paged read", starts, lengths, tokens, d, dtype, held, flush=True)
-    size, wide, hkv = 32, 4, 3
+    print("[gpu-test] paged read", starts, lengths, tokens, d, hkv, dtype, held, flush=True)
+    size = 32
     table = torch.tensor([[0, 5, -1, 2], [7, 7, 1, 9], [3, 4, 10, 6]], dtype=torch.int32)
     cache = random_cache(10, hkv, size, d, held)
     dev = lambda t: None if t is None else torch.tensor(t, device="cuda")  # noqa: E731
