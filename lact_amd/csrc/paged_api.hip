@@ -59,9 +59,13 @@ struct Pieces {
 };
 bool disjoint(const Pieces& a, const Pieces& b) {
   if (a.end() <= b.at || b.end() <= a.at) return true;
-  if (a.n == 1 || b.n == 1 || a.stride != b.stride) return false;      // (one inside the other's gaps: nobody's layout)
-  const long long d = (long long)((b.at - a.at) % (uintptr_t)a.stride);      // parts of the same page, however many pages apart they begin
-  return d >= a.len && a.stride - d >= b.len;
+  if (a.n > 1 && b.n > 1 && a.stride != b.stride) return false;      // (nobody's layout)
+  // one between two of the other's, or parts of the same page, however many pages apart they begin: how far behind one of a's the next one of b's begins
+  const long long stride = a.n > 1 ? a.stride : b.stride;
+  if (stride <= 0) return false;      // (single ones, which share memory)
+  long long d = (long long)(b.at - a.at) % stride;      // (signed: either may begin first)
+  if (d < 0) d += stride;
+  return d >= a.len && stride - d >= b.len;
 }
 // What a write goes to, nothing of which may lie in another part of it or in what is read.
 int check_apart(const lact_paged_cache_t* c, std::initializer_list<Pieces> read) {
@@ -69,12 +73,13 @@ int check_apart(const lact_paged_cache_t* c, std::initializer_list<Pieces> read)
   auto pages = [&](const void* p, long long stride, long long len) { return Pieces{reinterpret_cast<uintptr_t>(p), c->pages, stride, len}; };
   const Pieces to[4] = {pages(c->k, c->k_page * size, rows * c->D * size), pages(c->v, c->v_page * size, rows * c->D * size), pages(c->k_exponents, c->ke_page, rows),
                         pages(c->v_exponents, c->ve_page, rows)};
-  for (int i = 0, n = c->dtype == LACT_E4M3 ? 4 : 2; i < n; ++i) {
+  const int n = c->dtype == LACT_E4M3 ? 4 : 2;
+  for (int i = 0; i < n; ++i)
     for (int j = 0; j < i; ++j)
       if (!disjoint(to[i], to[j])) return fail("paged cache write: keys, values and exponents must not overlap");
+  for (int i = 0; i < n; ++i)
     for (const Pieces& r : read)
       if (r.at && !disjoint(to[i], r)) return fail("paged cache write: what is read must not lie in the cache");
-  }
   return 0;
 }
 

@@ -311,6 +311,52 @@ def test_keys_and_values_in_one_pool(dtype, held):
         assert torch.equal(a, b)
 
 
+@KINDS
+@pytest.mark.parametrize("hkv,size", [(3, 32), (12, 16), (2, 48), (3, 80)])
+def test_pools_of_any_page_length(hkv, size, dtype, held):
+    """One record a page: keys, values, their exponents and room behind them, from which the tokens come; and [pages, 2, ...]."""
+    import lact_amd
+    d, lengths, l = 64, [2 * size + 6, size + 1], 20
+    print("[gpu-test] paged cache, records", hkv, size, dtype, held, flush=True)
+    table, count = tables(lengths, size, 3)
+    plain = random_cache(count, hkv, size, d, held)
+    tail = 2 * 2 * l * hkv * d * dtype.itemsize                                      # of one page's room
+    parts = [t.reshape(count, -1).view(torch.uint8) for t in plain if t is not None]
+    pool = torch.cat((*parts, torch.zeros(count, tail, dtype=torch.uint8)), 1).to("cuda")
+    ends = torch.tensor([p.shape[1] for p in parts]).cumsum(0).tolist()
+    part = lambda i: pool[:, ends[i] - parts[i].shape[1]:ends[i]]  # noqa: E731
+    record = lact_amd.PagedCache(*(None if t is None else part(i).view(t.dtype).unflatten(1, t.shape[1:]) for i, t in enumerate(plain)))
+    codes = torch.stack(parts[:2], 1).to("cuda")
+    exps = torch.stack(parts[2:], 1).to("cuda") if held == E4M3 else None
+    both = lact_amd.PagedCache(*(codes[:, i].view(held).unflatten(1, plain[0].shape[1:]) for i in range(2)),
+                               *(None if exps is None else exps[:, i].view(E8M0).unflatten(1, plain[2].shape[1:]) for i in range(2)))
+    apart = cuda(plain)
+    assert record.k.data_ptr() == pool.data_ptr() and record.v.stride(0) * held.itemsize == pool.stride(0) and both.v.data_ptr() == codes[:, 1].data_ptr()
+    room = pool[1, ends[-1]:].view(dtype).view(2, 2, l, hkv, d)
+    room.copy_(torch.randn(2, 2, l, hkv, d, generator=torch.Generator().manual_seed(5)))
+    new, starts, n = room.clone(), torch.tensor([size - 5, 1], device="cuda"), torch.tensor(lengths, device="cuda")
+    q = torch.randn(2, 2 * hkv, d, generator=torch.Generator().manual_seed(3)).to(dtype).to("cuda")
+    table = table.to("cuda")
+    lact_amd.paged_cache_write(apart, *new, table, starts)
+    ref = lact_amd.paged_attention_step(q, apart, table, n)
+    for cache, tokens in ((record, room), (both, new)):
+        lact_amd.paged_cache_write(cache, *tokens, table, starts)
+        for a, b in zip(cache, apart):
+            assert a is None or torch.equal(a.contiguous().view(torch.uint8), b.view(torch.uint8))
+        assert torch.equal(lact_amd.paged_attention_step(q, cache, table, n), ref)
+        for a, b in zip(lact_amd.paged_cache_read(cache, table, n, 3 * size, dtype=dtype), lact_amd.paged_cache_read(apart, table, n, 3 * size, dtype=dtype)):
+            assert torch.equal(a, b)
+    assert torch.equal(room, new)
+    for name in ("v", "v_scale") if held == E4M3 else ("v",):
+        t = getattr(record, name)
+        off = t.storage_offset() - 16 // t.element_size()
+        bad = record._replace(**{name: t.as_strided(t.shape, t.stride(), off)})
+        with pytest.raises(RuntimeError, match="must not overlap"):
+            lact_amd.paged_cache_write(bad, *new, table, starts)
+    with pytest.raises(RuntimeError, match="must not lie in the cache"):
+        lact_amd.paged_cache_write(record, pool[1, ends[-1] - 16:ends[-1] - 16 + tail // 2].view(dtype).view(2, l, hkv, d)[:1], new[1][:1], table[:1], starts[:1])
+
+
 # ---- writing and reading
 
 def places_written(table, pages, size, starts, counts, l):

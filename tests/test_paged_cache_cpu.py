@@ -2,6 +2,7 @@
 forms."""
 import ctypes
 import math
+import random
 
 import pytest
 import torch
@@ -78,6 +79,52 @@ def test_writes_must_not_overlap():
         for change in (dict(tokens=at(32)), dict(table=at(20 * page)), dict(starts=layout["k_exponents"])):
             assert "must not lie in the cache" in refused(**{**layout, **change}), change
     assert "must not overlap" in refused(**{**record, "v_page": 2 * page + 256})
+
+
+def write_of(c):
+    """What a write of one token says whose table lies in the keys, so that no call gets past the checks: that of the pages among themselves comes first."""
+    far = ctypes.c_void_p(1 << 10)
+    assert _lib.lib().lact_paged_cache_write(ctypes.byref(c), 0, 1, 1, far, c.HK * c.D, c.HK * c.D, far, c.HK * c.D, c.HK * c.D, ctypes.c_void_p(c.k), far, None, None) < 0
+    return "apart" if "must not lie in the cache" in lib_error() else "overlap" if "must not overlap" in lib_error() else lib_error()
+
+
+@pytest.mark.parametrize("heads,size,d", [(2, 32, 64), (3, 32, 64), (12, 64, 128), (6, 64, 128), (8, 48, 64), (8, 80, 128), (5, 16, 64)])
+@pytest.mark.parametrize("values_first", [False, True])
+@pytest.mark.parametrize("dtype", [0, 2])
+def test_pages_of_one_pool(dtype, values_first, heads, size, d):
+    """Keys and values of a page behind one another, their exponents behind them or in a pool of their own: apart, whatever a page's length, also where the values' pages begin some pages further
+    on or back.  16 bytes off and they overlap."""
+    rows = heads * size
+    page, item = rows * d * (1 if dtype == 2 else 2), (1 if dtype == 2 else 2)
+    for record, e_record in ((2 * page, 2 * rows), (2 * page + 2 * rows, 2 * page + 2 * rows)):
+        for shift in (0, 3 * record, -3 * record):
+            parts = [1 << 32, (1 << 32) + page]
+            exps = [1 << 33, (1 << 33) + rows] if record == 2 * page else [(1 << 32) + 2 * page, (1 << 32) + 2 * page + rows]
+            k, v = parts[::-1] if values_first else parts
+            ke, ve = exps[::-1] if values_first else exps
+            kw = dict(dtype=dtype, pages=20, page_size=size, HK=heads, D=d, k_page=record // item, v_page=record // item, ke_page=e_record, ve_page=e_record, k=k, v=v + shift,
+                      k_exponents=ke, v_exponents=ve + shift // record * e_record)
+            assert write_of(cache_desc(**kw)) == "apart", (record, shift)
+            nearer = 16 if values_first else -16
+            assert write_of(cache_desc(**{**kw, "v": v + shift + nearer})) == "overlap", (record, shift)
+            if dtype == 2:
+                assert write_of(cache_desc(**{**kw, "v_exponents": kw["v_exponents"] + nearer})) == "overlap", (record, shift)
+
+
+def test_overlaps_of_pages_are_those_of_their_bytes():
+    """Keys and values the same distance from page to page, at any distance from each other, against all pages one by one."""
+    g, seen = random.Random(1), set()
+    length = 16 * 64 * 2
+    for _ in range(3000):
+        pages, stride = g.randint(1, 5), length + 16 * g.choice((0, 1, g.randint(0, 300)))
+        k = (1 << 24) + 16 * g.randint(0, 999)
+        v = k + g.randint(-6, 6) * stride + g.choice((length, -length, stride - length, 16 * g.randint(0, stride // 16)))
+        at = [range(x, x + pages * stride, stride) for x in (k, v)]
+        overlap = any(abs(x - y) < length for x in at[0] for y in at[1])
+        seen.add(overlap)
+        got = write_of(cache_desc(pages=pages, page_size=16, HK=1, k_page=stride // 2, v_page=stride // 2, k=k, v=v))
+        assert got == ("overlap" if overlap else "apart"), (pages, stride, v - k)
+    assert seen == {True, False}
 
 
 def step_desc(**kw):
