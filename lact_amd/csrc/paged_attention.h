@@ -172,9 +172,17 @@ __device__ __forceinline__ bf16x8 bf16_part(float (&x)[8]) {
   }
   return __builtin_bit_cast(bf16x8, make_uint4(r[0], r[1], r[2], r[3]));
 }
-__device__ __forceinline__ bf16x8 bf16_of(const f32x4& a, const f32x4& b) {
-  return __builtin_bit_cast(bf16x8, make_uint4(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3])));
+// All eight as parts, the leading one first.
+template <int N>
+__device__ __forceinline__ void bf16_parts(const f32x4 (&x)[2], bf16x8 (&p)[N]) {
+  float y[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] = x[j / 4][j % 4];
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = bf16_part(y);
 }
+// bf16 queries: a weight, which may be anything, in two parts of 8 bits, so that what is stored is the only rounding that shows (2^-16 of a weight against 2^-8).
+constexpr int WEIGHT_PARTS = 2;
 
 template <typename T, typename C, int D, int QT> struct PagedMath;
 template <int D, int QT>
@@ -213,16 +221,18 @@ struct PagedMath<uint16_t, uint16_t, D, QT> {
   __device__ __forceinline__ void add(f32x4 (&o)[QT][D / 16], const PagedScores<QT>& x, const char* tile) const {
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     typedef short s16x8 __attribute__((ext_vector_type(8)));
-    bf16x8 p[QT];
+    bf16x8 p[QT][WEIGHT_PARTS];
 #pragma unroll
-    for (int t = 0; t < QT; ++t) p[t] = bf16_of(x.s[t][0], x.s[t][1]);
+    for (int t = 0; t < QT; ++t) bf16_parts(x.s[t], p[t]);
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
       const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + col[dt]));
       const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + col[dt] + 16 * S::ROWB));
       const bf16x8 v = __builtin_bit_cast(bf16x8, (s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]}));
 #pragma unroll
-      for (int t = 0; t < QT; ++t) o[t][dt] = mma16(v, p[t], o[t][dt]);
+      for (int i = WEIGHT_PARTS - 1; i >= 0; --i)
+#pragma unroll
+        for (int t = 0; t < QT; ++t) o[t][dt] = mma16(v, p[t][i], o[t][dt]);
     }
   }
 };
@@ -354,25 +364,16 @@ struct PagedMath<T, uint8_t, D, QT> {
   __device__ __forceinline__ void add(f32x4 (&o)[QT][D / 16], const PagedScores<QT>& x, const char* tile) const {
     typedef int i32x2 __attribute__((ext_vector_type(2)));
     typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-    bf16x8 p[QT][PARTS];
+    constexpr int WEIGHTS = PARTS == 1 ? WEIGHT_PARTS : PARTS;
+    bf16x8 p[QT][WEIGHTS];
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      if constexpr (PARTS == 1) {
-        p[t][0] = bf16_of(x.s[t][0], x.s[t][1]);
-      } else {
-        float y[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = x.s[t][j / 4][j % 4];
-#pragma unroll
-        for (int i = 0; i < PARTS; ++i) p[t][i] = bf16_part(y);
-      }
-    }
+    for (int t = 0; t < QT; ++t) bf16_parts(x.s[t], p[t]);
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
       const i32x2 c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(tile + col[dt]));
       const bf16x8 v = widen((uint32_t)c[0], (uint32_t)c[1], 1.f);
 #pragma unroll
-      for (int i = PARTS - 1; i >= 0; --i)
+      for (int i = WEIGHTS - 1; i >= 0; --i)
 #pragma unroll
         for (int t = 0; t < QT; ++t) o[t][dt] = mma16(v, p[t][i], o[t][dt]);
     }

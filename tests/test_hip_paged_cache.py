@@ -170,6 +170,24 @@ def test_seen_values_that_are_not_finite_are_seen(dtype, held):
         assert bool(bad[1, 2:].all() if which == 0 else bad[1, 2:, 7].all())
 
 
+@pytest.mark.parametrize("held", [BF16, E4M3])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lengths,size,hq,hkv,cap,slopes", [([700, 33, 1], 16, 4, 2, None, False), ([3000, 2600], 48, 5, 1, None, False), ([1500, 900], 16, 20, 1, 20.0, False), ([800], 16, 2, 1, None, True)])
+def test_weights_keep_their_bits(lengths, size, hq, hkv, cap, slopes, d, held):
+    """bf16 queries: what is stored is rounded to bf16, nothing in front of it.  A weight in two parts of bf16 is off by 2^-8 of 2^-8 of itself; the rest is fp32's, with three times as many
+    terms as one part has, and twice the exponent's error where a distance adds to the score."""
+    import lact_amd
+    print("[gpu-test] paged step, weights", lengths, size, hq, hkv, d, held, cap, slopes, flush=True)
+    table, count = tables(lengths, size, 4096 // size)
+    cache = random_cache(count, hkv, size, d, held)
+    q = torch.randn(len(lengths), hq, d, generator=torch.Generator().manual_seed(3)).to(BF16)
+    sl = 2.0 ** -torch.arange(4, hq + 4).float() if slopes else None
+    out = lact_amd.paged_attention_step(q.to("cuda"), cuda(cache), table.to("cuda"), torch.tensor(lengths, device="cuda"), score_cap=cap, distance_slopes=None if sl is None else sl.to("cuda"))
+    p_err, _ = errors(F32, E4M3, max(lengths), d, 8.0 + (max(lengths) if slopes else 0))
+    ref, bound = PO.step(q, *numbers(cache), table, lengths, None, cap, sl, None, 2.0 ** -16 + p_err, HALF[BF16])
+    near(out, ref, bound, "out")
+
+
 @KINDS
 def test_step_of_many_parts_is_joined(dtype, held):
     check_step([i * 7 % 190 for i in range(600)], 12, 16, 4, 4, 64, dtype, held)
