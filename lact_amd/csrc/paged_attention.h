@@ -355,7 +355,7 @@ struct PagedMath<T, uint8_t, D, QT> {
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {      // an exponent of 255 is infinity here
+      for (int i = 0; i < 4; ++i) {      // an exponent of 255, which stands for NaN, is infinity here: what the weight's leading part leaves of it is NaN
         const uint32_t w = kt ? exps.y : exps.x, f = (i == 3 ? w >> 1 : w << (23 - 8 * i)) & 0x7f800000u;
 #pragma unroll
         for (int t = 0; t < QT; ++t) x.s[t][kt][i] *= __uint_as_float(max(f, 0x400000u));

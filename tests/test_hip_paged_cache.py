@@ -244,6 +244,31 @@ def test_exponents_of_all_sizes(wide, dtype):
     check_step(lengths, wide, size, 4, hkv, d, dtype, E4M3, table=table, cache=cache)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("wide", [4, 100])
+def test_a_seen_exponent_of_255_is_nan(wide, d, dtype):
+    """The exponent that stands for NaN, beside numbers that are large, small and 0: of a key all its head's outputs are NaN, of a value as well; everybody else's stay."""
+    import lact_amd
+    print("[gpu-test] paged step, exponents of NaN", wide, d, dtype, flush=True)
+    lengths, size = [60, 33], 16
+    table, count = tables(lengths, size, wide)
+    cache = random_cache(count, 2, size, d, E4M3)
+    for t in cache[:2]:
+        t.view(torch.uint8)[:, :, 5] = torch.tensor([0, 1, 0x80, 0x7e], dtype=torch.uint8).repeat(d // 4)
+    q = torch.randn(2, 4, d, generator=torch.Generator().manual_seed(3)).to(dtype)
+    step = lambda c: lact_amd.paged_attention_step(q.to("cuda"), cuda(c), table.to("cuda"), torch.tensor(lengths, device="cuda")).cpu()  # noqa: E731
+    ref = step(cache)
+    for which in (2, 3):
+        for place in (5, 31, 59):
+            c = [t.clone() for t in cache]
+            c[which].view(torch.uint8)[table[0, place // size], 1, place % size] = 255
+            out = step(c)
+            want, _ = PO.step(q, *numbers(c), table, lengths)
+            assert torch.equal(torch.isnan(out), torch.isnan(want)) and bool(torch.isnan(out[0, 2:]).all()), (which, place)
+            assert torch.equal(out[1], ref[1]) and torch.equal(out[0, :2], ref[0, :2])
+
+
 @KINDS
 def test_queries_and_tables_with_strides(dtype, held):
     import lact_amd
