@@ -181,8 +181,21 @@ __device__ __forceinline__ void bf16_parts(const f32x4 (&x)[2], bf16x8 (&p)[N]) 
 #pragma unroll
   for (int i = 0; i < N; ++i) p[i] = bf16_part(y);
 }
-// bf16 queries: a weight, which may be anything, in two parts of 8 bits, so that what is stored is the only rounding that shows (2^-16 of a weight against 2^-8).
+// bf16 queries: a weight, which may be anything, in two parts of 8 bits, so that what is stored is the only rounding that shows (2^-15 of a weight against 2^-8).
 constexpr int WEIGHT_PARTS = 2;
+// The two for values that may be infinite: the leading part is cut below the weight, so that both are positive, and none of a weight that is not 0 is 0.
+__device__ __forceinline__ void positive_parts(const f32x4 (&x)[2], bf16x8 (&p)[WEIGHT_PARTS]) {
+  uint32_t lead[4], rest[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float a = x[i / 2][2 * i % 4], b = x[i / 2][2 * i % 4 + 1];
+    const uint32_t c = __builtin_elementwise_sub_sat(__float_as_uint(a), 1u), d = __builtin_elementwise_sub_sat(__float_as_uint(b), 1u);
+    lead[i] = __builtin_amdgcn_perm(d, c, 0x07060302u);      // their upper halves
+    rest[i] = pack_bf16(a - __uint_as_float(c & 0xffff0000u), b - __uint_as_float(d & 0xffff0000u));
+  }
+  p[0] = __builtin_bit_cast(bf16x8, make_uint4(lead[0], lead[1], lead[2], lead[3]));
+  p[1] = __builtin_bit_cast(bf16x8, make_uint4(rest[0], rest[1], rest[2], rest[3]));
+}
 
 template <typename T, typename C, int D, int QT> struct PagedMath;
 template <int D, int QT>
@@ -223,7 +236,7 @@ struct PagedMath<uint16_t, uint16_t, D, QT> {
     typedef short s16x8 __attribute__((ext_vector_type(8)));
     bf16x8 p[QT][WEIGHT_PARTS];
 #pragma unroll
-    for (int t = 0; t < QT; ++t) bf16_parts(x.s[t], p[t]);
+    for (int t = 0; t < QT; ++t) positive_parts(x.s[t], p[t]);
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
       const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + col[dt]));
@@ -487,8 +500,14 @@ __global__ __launch_bounds__((64 * PagedShape<T, C, D>::NW), (sizeof(T) == 4 && 
         uint64_t address = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(from_lo, at) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane(from_hi, at) << 32;
         asm volatile("s_nop 4" : "+s"(address));      // between a scalar register's write by a vector instruction and its use as an address, which the compiler does not see
         const void* from = reinterpret_cast<const void*>(address);
+        if (!A::EXP && half && (first > 0 || last < 15)) {      // values: zeros, as 0 times an infinity that is seen is NaN (8 bits have none)
 #pragma unroll
-        for (int i = x * HALF; i < (x + 1) * HALF; ++i) dma16<false>(from, (uint32_t)min(max(crow[i], first), last) * S::ROWB + ccol[i], to + i * 1024);
+          for (int i = x * HALF; i < (x + 1) * HALF; ++i)
+            dma16_from((crow[i] < first || crow[i] > last ? reinterpret_cast<uint64_t>(paged_zeros) : address + (uint32_t)crow[i] * S::ROWB) + ccol[i], to + i * 1024);
+        } else {
+#pragma unroll
+          for (int i = x * HALF; i < (x + 1) * HALF; ++i) dma16<false>(from, (uint32_t)min(max(crow[i], first), last) * S::ROWB + ccol[i], to + i * 1024);
+        }
       }
     };
     auto keys = [&](int t) LACT_INLINE_LAMBDA { copy(t, 0, ring + t % RING * A::STAGE); };

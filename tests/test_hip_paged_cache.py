@@ -174,7 +174,7 @@ def test_seen_values_that_are_not_finite_are_seen(dtype, held):
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("lengths,size,hq,hkv,cap,slopes", [([700, 33, 1], 16, 4, 2, None, False), ([3000, 2600], 48, 5, 1, None, False), ([1500, 900], 16, 20, 1, 20.0, False), ([800], 16, 2, 1, None, True)])
 def test_weights_keep_their_bits(lengths, size, hq, hkv, cap, slopes, d, held):
-    """bf16 queries: what is stored is rounded to bf16, nothing in front of it.  A weight in two parts of bf16 is off by 2^-8 of 2^-8 of itself; the rest is fp32's, with three times as many
+    """bf16 queries: what is stored is rounded to bf16, nothing in front of it.  The second part of a weight is at most 2^-7 of it, and off by 2^-8 of itself; the rest is fp32's, with three times as many
     terms as one part has, and twice the exponent's error where a distance adds to the score."""
     import lact_amd
     print("[gpu-test] paged step, weights", lengths, size, hq, hkv, d, held, cap, slopes, flush=True)
@@ -184,7 +184,7 @@ def test_weights_keep_their_bits(lengths, size, hq, hkv, cap, slopes, d, held):
     sl = 2.0 ** -torch.arange(4, hq + 4).float() if slopes else None
     out = lact_amd.paged_attention_step(q.to("cuda"), cuda(cache), table.to("cuda"), torch.tensor(lengths, device="cuda"), score_cap=cap, distance_slopes=None if sl is None else sl.to("cuda"))
     p_err, _ = errors(F32, E4M3, max(lengths), d, 8.0 + (max(lengths) if slopes else 0))
-    ref, bound = PO.step(q, *numbers(cache), table, lengths, None, cap, sl, None, 2.0 ** -16 + p_err, HALF[BF16])
+    ref, bound = PO.step(q, *numbers(cache), table, lengths, None, cap, sl, None, 2.0 ** -15 + p_err, HALF[BF16])
     near(out, ref, bound, "out")
 
 
@@ -267,6 +267,28 @@ def test_a_seen_exponent_of_255_is_nan(wide, d, dtype):
             want, _ = PO.step(q, *numbers(c), table, lengths)
             assert torch.equal(torch.isnan(out), torch.isnan(want)) and bool(torch.isnan(out[0, 2:]).all()), (which, place)
             assert torch.equal(out[1], ref[1]) and torch.equal(out[0, :2], ref[0, :2])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("wide,window", [(4, None), (4, 20), (100, None)])
+def test_seen_values_that_are_infinite(wide, window, d, dtype):
+    """Infinities of one sign among the values that are seen make that infinity, of both signs NaN, in the first and last places that are seen as anywhere else, beside places that are not."""
+    import lact_amd
+    lengths, size = [60, 33], 16
+    print("[gpu-test] paged step, infinities", wide, window, d, dtype, flush=True)
+    table, count = tables(lengths, size, wide)
+    cache = random_cache(count, 2, size, d, dtype)
+    q = torch.randn(2, 4, d, generator=torch.Generator().manual_seed(3)).to(dtype)
+    for seq, places in ((0, (59,)), (0, (44,)), (0, (40, 47)), (1, (32,)), (1, (13,)), (1, (31, 32, 14))):
+        c = [t if t is None else t.clone() for t in cache]
+        for i, place in enumerate(places):
+            c[1][table[seq, place // size], 1, place % size, 3 + i:9] = math.inf if i < 2 else -math.inf
+        out = lact_amd.paged_attention_step(q.to("cuda"), cuda(c), table.to("cuda"), torch.tensor(lengths, device="cuda"), window).cpu().double()
+        ref, bound = PO.step(q, *numbers(c), table, lengths, window, None, None, None, *errors(dtype, dtype, 60, d))
+        assert torch.equal(torch.isnan(out), torch.isnan(ref)) and torch.equal(torch.isinf(out), torch.isinf(ref)) and bool((out[torch.isinf(ref)] == ref[torch.isinf(ref)]).all()), (seq, places)
+        finite = torch.isfinite(ref)
+        near(out[finite], ref[finite], bound[finite], f"{seq} {places}")
 
 
 @KINDS
