@@ -42,11 +42,19 @@ def _tensors(name: str, cache: PagedCache, *more: Optional[torch.Tensor]) -> Non
         raise RuntimeError(f"{name} is for inference: call it under torch.no_grad()")
 
 
+def _as_pages(cache: PagedCache, *ts: torch.Tensor):
+    """Under autocast, which cannot change the pages' type: tokens of theirs.  (8 bits take tokens of either type.)"""
+    if cache.k.dtype == torch.float8_e4m3fn or not (ts[0].is_cuda and torch.is_autocast_enabled("cuda")):
+        return ts
+    return tuple(t.to(cache.k.dtype) if t.is_floating_point() else t for t in ts)
+
+
 @torch.compiler.disable
 def paged_cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, starts: Optional[torch.Tensor] = None,
                       counts: Optional[torch.Tensor] = None) -> None:
     """k, v: [b, l, hkv, d], or [b, hkv, d] for one token each, of the pages' type, or bf16 or fp32 for pages of 8 bits.  Token i of sequence s goes to its place
-    starts[s] + i (starts None: i) if i < counts[s] (counts None: all do); what else lies in the pages stays.
+    starts[s] + i (starts None: i) if i < counts[s] (counts None: all do); what else lies in the pages stays.  Under autocast they are cast to the pages' type,
+    and for pages of 8 bits taken as they are.
 
     In 8 bits a row (one head of one token) is multiplied by the power of two with which its largest magnitude just fits in e4m3 (448), and rounded to nearest; NaN and
     infinities become NaN, beside the others' own scale.
@@ -55,6 +63,7 @@ def paged_cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_
     place, for autograd too."""
     name = "paged_cache_write"
     _tensors(name, cache, k, v, page_table, starts, counts)
+    k, v = _as_pages(cache, k, v)
     _lib.host().paged_cache_write(*cache, k, v, page_table, starts, counts)
 
 
@@ -84,11 +93,11 @@ def paged_attention_step(q: torch.Tensor, cache: PagedCache, page_table: torch.T
 
     lengths: [b] int32 (int64 is converted), on the device: the first lengths[i] places of sequence i are its tokens, the last of them the one that q belongs to (its key
     and value are in the cache already).  Lengths are cut to what the table holds; a sequence that sees nothing (length 0, no page) has output 0.  Places past
-    the length and further back than the window are not seen, whatever they hold, and need no page.  For inference: under torch.no_grad(), or with operands that need no
-    gradient."""
+    the length and further back than the window are not seen, whatever they hold, and need no page.  Under autocast q is cast to the pages' type, for pages of 8 bits
+    to autocast's.  For inference: under torch.no_grad(), or with operands that need no gradient."""
     name = "paged_attention_step"
     _tensors(name, cache, q, page_table, lengths, distance_slopes)
     _dims(name, 3, q=q)
-    q, = _autocast(q)
+    q, = _autocast(q) if cache.k.dtype == torch.float8_e4m3fn else _as_pages(cache, q)
     window, scale, cap = _options(name, q.shape[2], window, score_cap, scale, distance_slopes)
     return _lib.host().paged_attention_step(q, *cache, page_table, lengths, window, scale, cap, distance_slopes)

@@ -734,3 +734,36 @@ def test_refusals_on_the_gpu():
         leaf = of(c, k=c.k.float().requires_grad_(True))
         with pytest.raises(RuntimeError, match="inference"):
             lact_amd.paged_attention_step(q.float(), leaf, table, n)
+
+
+@pytest.mark.parametrize("given", [BF16, F32])
+@pytest.mark.parametrize("held", [BF16, F32, E4M3])
+def test_autocast_takes_what_the_pages_hold(held, given):
+    """Under autocast tokens and queries of either type go with pages of any: cast to the pages' type; 8 bits take tokens as they are, and queries of autocast's type."""
+    import lact_amd
+    size, hkv, d = 16, 2, 64
+    table, starts = torch.tensor([[0, 1], [2, 3]], device="cuda"), torch.tensor([0, 9], device="cuda")
+    k, v, q = (torch.randn(2, *n, d, device="cuda").to(given) for n in ((20, hkv), (20, hkv), (4,)))
+    n = torch.tensor([20, 29], device="cuda")
+    empty = lambda: lact_amd.PagedCache(*(None if t is None else t.view(torch.uint8).zero_().view(t.dtype) for t in lact_amd.PagedCache.empty(4, hkv, size, d, dtype=held)))  # noqa: E731
+    write = given if held == E4M3 else held
+    ask = BF16 if held == E4M3 else held
+    with torch.autocast("cuda", BF16):
+        one = empty()
+        lact_amd.paged_cache_write(one, k, v, table, starts)
+        lact_amd.paged_cache_write(one, k[:, 0], v[:, 0], table, n)
+        out = lact_amd.paged_attention_step(q, one, table, n + 1)
+        back = lact_amd.paged_cache_read(one, table, n, 30)
+    two = empty()
+    lact_amd.paged_cache_write(two, k.to(write), v.to(write), table, starts)
+    lact_amd.paged_cache_write(two, k[:, 0].to(write), v[:, 0].to(write), table, n)
+    ref = lact_amd.paged_attention_step(q.to(ask), two, table, n + 1)
+    for a, b in ((out, ref), *zip(back, lact_amd.paged_cache_read(two, table, n, 30)), *zip(one, two)):
+        assert a is None or (a.dtype == b.dtype and torch.equal(a.view(torch.uint8), b.view(torch.uint8)))
+    if held != E4M3:
+        assert out.dtype == held
+        other = F32 if held == BF16 else BF16
+        with pytest.raises(TypeError):      # and nothing is cast without it
+            lact_amd.paged_attention_step(q.to(other), two, table, n)
+        with pytest.raises(TypeError):
+            lact_amd.paged_cache_write(two, k.to(other), v.to(other), table, starts)
