@@ -13,7 +13,7 @@
 // the keys and the values of 32 pieces lie at once, a lane each, and copies a piece from where its lane says; one without a page is copied from zeros and masked.  In a
 // piece that the window or the length ends in, the rows outside repeat one inside.
 //
-// e4m3: numbers become bf16 exactly as they leave LDS.  A key's exponent is applied in that conversion (a lane has one key's row), a value's to the weight that meets
+// e4m3: numbers become bf16 as they leave LDS, exactly down to multiples of 2^-133.  A key's exponent is applied in that conversion (a lane has one key's row), a value's to the weight that meets
 // it.  fp32 queries and weights meet them in three bf16 parts of 8 bits.  (Products below 2^-126 count as 0: values under 2^-118.)
 //
 // What bounds it is the one read of the keys and values.  131072 places of 8 heads of 128 with 4 queries each in bf16: 93 us and 6 for the join, 5.8 and 5.4 TB/s (a large copy

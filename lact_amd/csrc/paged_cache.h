@@ -1,6 +1,7 @@
 // A cache of keys and values in pages: [pages, HK, page size, D] each, bf16, fp32 or e4m3.  A sequence's place n lies in page table[b][n / size] at row n % size; what
 // points outside the pages is no page.  A row of e4m3 has an exponent beside it (e8m0, [pages, HK, page size]): the smallest e with which the row's largest finite
-// magnitude is at most 448 2^(e - 127).  The scale is a power of two, so that a number loses nothing but what lies under e4m3's three bits, and what is read back is exact in bf16.
+// magnitude is at most 448 2^(e - 127).  The scale is a power of two, so that a number loses nothing but what lies under e4m3's three bits, and what is read back is exact in bf16
+// where it is a multiple of bf16's smallest number, 2^-133, and below 2^128; with an exponent under 3 smaller ones are rounded.
 //
 // A head's rows of one page follow each other: what attention reads of a page is one piece, in 8 bits of 16 tokens 2 KB.
 #pragma once

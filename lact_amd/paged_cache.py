@@ -70,7 +70,8 @@ def paged_cache_write(cache: PagedCache, k: torch.Tensor, v: torch.Tensor, page_
 @torch.compiler.disable
 def paged_cache_read(cache: PagedCache, page_table: torch.Tensor, lengths: torch.Tensor, tokens: int, starts: Optional[torch.Tensor] = None, *,
                      dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(k, v): [b, tokens, hkv, d], of the pages' type, or for pages of 8 bits bf16 (which holds their numbers exactly) or with `dtype` fp32: entry i of sequence s is
+    """(k, v): [b, tokens, hkv, d], of the pages' type, or for pages of 8 bits bf16 (which holds their numbers exactly but for what is not a
+    multiple of 2^-133 or reaches 2^128) or with `dtype` fp32: entry i of sequence s is
     its place starts[s] + i (starts None: i), zeros from place lengths[s] on and where there is no page.
 
     lengths, starts: [b] int32 (int64 is converted), on the device."""

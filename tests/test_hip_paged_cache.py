@@ -520,6 +520,25 @@ def test_reading_every_number_of_8_bits(dtype):
         assert torch.equal(torch.isnan(t), torch.isnan(want)) and torch.equal(t[~torch.isnan(t)], want[~torch.isnan(want)])
 
 
+def test_the_smallest_numbers_of_8_bits():
+    """Under exponents of 0 to 3 the codes 0 to 8 are multiples of 2^-136 to 2^-133: fp32 has them all, bf16 those of 2^-133, and others to nearest, ties to even."""
+    import lact_amd
+    d, size = 64, 16
+    codes = (torch.arange(d, dtype=torch.uint8) % 9).expand(1, 1, size, d).contiguous().view(E4M3)
+    exps = (torch.arange(size, dtype=torch.uint8) % 4).expand(1, 1, size).contiguous().view(E8M0)
+    table, n = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([size], device="cuda")
+    want = (torch.arange(d) % 9)[None] * 2 ** (torch.arange(size) % 4)[:, None]                # in 2^-136
+    for dtype, w in ((F32, want.double() * 2.0 ** -136), (BF16, torch.round(want.double() / 8) * 2.0 ** -133)):
+        for t in lact_amd.paged_cache_read(cuda((codes, codes, exps, exps)), table, n, size, dtype=dtype):
+            assert torch.equal(t[0, :, 0].double().cpu(), w), dtype
+    small = torch.full((1, 1, d), 5 * 2.0 ** -133)                                             # written, its row's exponent is 0
+    cache = lact_amd.PagedCache.empty(1, 1, size, d, dtype=E4M3)
+    lact_amd.paged_cache_write(cache, small.to("cuda"), small.to("cuda"), table)
+    assert int(cache.k_scale.view(torch.uint8)[0, 0, 0]) == 0
+    for dtype in (F32, BF16):
+        assert bool((lact_amd.paged_cache_read(cache, table, n, 1, dtype=dtype)[1].double() == 5 * 2.0 ** -133).all())
+
+
 @KINDS
 @pytest.mark.parametrize("hkv", [1, 2, 3])
 @pytest.mark.parametrize("d", [64, 128])
