@@ -110,6 +110,25 @@ def test_lengths_outside_the_table(dtype, held):
 
 
 @KINDS
+@pytest.mark.parametrize("wide", [3, 50])
+def test_lengths_past_the_table_are_its_end(wide, dtype, held):
+    """The same query of every sequence, over the same pages: longer lengths, in 32 bits and past them, are the table's places bit by bit, and negative ones none."""
+    import lact_amd
+    size, ends = 32, wide * 32
+    lengths = torch.tensor([ends, ends + 1, 10 ** 9, 2 ** 31 - 1, 2 ** 31, 2 ** 40, 2 ** 32 + 7, -1, -2 ** 31, -2 ** 40, -2 ** 32 + 7], device="cuda")
+    cache = cuda(random_cache(wide, 1, size, 64, held))
+    table = torch.randperm(wide, generator=torch.Generator().manual_seed(2)).expand(len(lengths), wide).to("cuda")
+    q = torch.randn(1, 2, 64, generator=torch.Generator().manual_seed(3)).to(dtype).to("cuda")
+    for window in (None, 50):
+        for n, t in ((lengths, table), (lengths.clamp(-2 ** 31, 2 ** 31 - 1).int(), table.int())):
+            one = lambda i: lact_amd.paged_attention_step(q, cache, t[i:i + 1], n[i:i + 1], window)  # noqa: E731
+            ref = one(0)
+            assert bool(ref.any())
+            for i in range(1, len(lengths)):
+                assert torch.equal(one(i), ref if i < 7 else torch.zeros_like(ref)), (window, i)
+
+
+@KINDS
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("table,lengths,window", [
     ([[0, -1, 2, -1, 4, -1]], [96], None),                                # every other page
