@@ -1130,6 +1130,11 @@ variable_list rotary(const Tensor& q, const OptTensor& k, const Tensor& position
   expect(positions_, q, want, "positions");
   const Tensor positions = positions_.detach().resolve_neg().contiguous();
   if (q.size(0) > INT32_MAX || (q.dim() == 4 && q.size(1) > INT32_MAX)) throw std::invalid_argument("too many tokens in one call");
+  if (q.size(0) == 0 || q.size(q.dim() - 3) == 0) {      // no token: copies, which have gradients
+    variable_list none{q.clone()};
+    if (k) none.push_back(k->clone());
+    return none;
+  }
   RotaryTable table(axes, base, frequencies);
   if (at::GradMode::is_enabled() && (q.requires_grad() || wants_grad(k))) {
     refuse_leaves_of_eager_graphs({&q, k ? &*k : nullptr});

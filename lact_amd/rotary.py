@@ -43,7 +43,5 @@ def axial_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     if torch.is_grad_enabled() and positions.requires_grad:
         raise RuntimeError(f"{name}: positions have no gradient; detach them")
     q, k = (_autocast(q) + (None,)) if k is None else _autocast(q, k)
-    if 0 in q.shape[:-2]:
-        return q.clone(), None if k is None else k.clone()
     res = _lib.host().axial_rotary(q, k, positions, axes, float(base), frequencies, bool(interleaved))
     return (res[0], None) if k is None else (res[0], res[1])

@@ -283,3 +283,21 @@ def test_autocast_empty_calls_and_refusals():
     first, = torch.autograd.grad(y, x, y, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(first.sum(), x)
+
+
+@pytest.mark.parametrize("shape", [(0, 6), (2, 0), (0, 0), (0,)])
+def test_calls_without_tokens_are_checked(shape):
+    """What other calls refuse is refused where there is nothing to turn as well; keys of another batch among it, which would come back as they are."""
+    import lact_amd
+    f = lact_amd.axial_rotary
+    q, k = (torch.zeros(*shape, h, 64, device="cuda", dtype=BF16, requires_grad=True) for h in (4, 2))
+    p = torch.zeros(*shape, 2, dtype=torch.int32, device="cuda")
+    a, b = f(q, k, p, (32, 32))
+    assert a.shape == q.shape and b.shape == k.shape and a.dtype == b.dtype == BF16
+    assert all(g.shape == t.shape for g, t in zip(torch.autograd.grad([a, b], [q, k], [a, b]), (q, k)))
+    assert f(q, None, p, (32, 32))[1] is None
+    more = torch.ones(*(n + 3 for n in shape), 2, 64, device="cuda", dtype=BF16)
+    for bad, error in ((dict(k=more), ValueError), (dict(k=k.float()), TypeError), (dict(q=q.half(), k=k.half()), TypeError), (dict(k=k.cpu()), RuntimeError),
+                       (dict(positions=p[..., :1]), ValueError), (dict(positions=p.double()), TypeError), (dict(positions=p.cpu()), RuntimeError), (dict(q=q.cpu(), k=k.cpu(), positions=p.cpu()), RuntimeError)):
+        with pytest.raises(error):
+            f(**{**dict(q=q, k=k, positions=p, axes=(32, 32)), **bad})
