@@ -32,9 +32,10 @@ def axial_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     _plain_only(name, q, k, positions)
     if q.dim() not in (3, 4) or (k is not None and k.dim() != q.dim()):
         raise ValueError(f"{name}: q and k must both have 4 dimensions, or 3 for one token each")
-    axes = [int(n) for n in axes]
-    if not axes or min(axes) <= 0 or any(n % 2 for n in axes) or sum(axes) > q.shape[-1]:
-        raise ValueError(f"{name}: axes must be positive even numbers of channels that fit a head of {q.shape[-1]}, got {axes}")
+    given = list(axes)
+    axes = [int(n) for n in given]
+    if not axes or axes != given or min(axes) <= 0 or any(n % 2 for n in axes) or sum(axes) > q.shape[-1]:
+        raise ValueError(f"{name}: axes must be positive even numbers of channels that fit a head of {q.shape[-1]}, got {given}")
     if not (0.0 < base < math.inf):
         raise ValueError(f"{name}: base must be positive and finite, got {base}")
     given, frequencies = frequencies is not None, [] if frequencies is None else [float(f) for f in frequencies]

@@ -237,6 +237,15 @@ def test_python_refusals():
         f(torch.autograd.forward_ad.make_dual(x, x), None, p, (32, 32))
 
 
+@pytest.mark.parametrize("axes", [(32.5, 32), (32, 31.999), (2.25,), (32, -2.5)])
+def test_axes_are_whole_numbers(axes):
+    x, p = torch.zeros(1, 6, 2, 64), torch.zeros(6, len(axes), dtype=torch.int32)
+    with pytest.raises(ValueError, match="even numbers"):
+        lact_amd.axial_rotary(x, x, p, axes)
+    with pytest.raises(RuntimeError, match="MI355X"):
+        lact_amd.axial_rotary(x, x, p, (float(2 * int(n / 2) if n > 0 else 2) for n in axes))      # (what is whole may come in any type)
+
+
 def test_oracle_of_8_bits_is_torchs():
     """The codes' values, and rounding, against torch's own type where a row's scale is 1."""
     codes = torch.arange(256, dtype=torch.uint8)
