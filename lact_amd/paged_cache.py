@@ -37,6 +37,8 @@ class PagedCache(NamedTuple):
 def _tensors(name: str, cache: PagedCache, *more: Optional[torch.Tensor]) -> None:
     if not isinstance(cache, PagedCache):
         raise TypeError(f"{name} takes a PagedCache, got {type(cache).__name__}")
+    if cache.k is None or cache.v is None:
+        raise TypeError(f"{name} takes a PagedCache with keys and values")
     _plain_only(name, *cache, *more)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*cache, *more)):
         raise RuntimeError(f"{name} is for inference: call it under torch.no_grad()")

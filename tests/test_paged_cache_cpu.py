@@ -237,6 +237,15 @@ def test_python_refusals():
         f(torch.autograd.forward_ad.make_dual(x, x), None, p, (32, 32))
 
 
+@pytest.mark.parametrize("part", ["k", "v"])
+def test_caches_without_keys_or_values(part):
+    cache = lact_amd.PagedCache.empty(4, 2, 16, 64, device="cpu")._replace(**{part: None})
+    table, n, q = torch.zeros(1, 2, dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    for call in (lambda: lact_amd.paged_attention_step(q, cache, table, n), lambda: lact_amd.paged_cache_write(cache, q, q, table), lambda: lact_amd.paged_cache_read(cache, table, n, 3)):
+        with pytest.raises(TypeError, match="keys and values"):
+            call()
+
+
 @pytest.mark.parametrize("axes", [(32.5, 32), (32, 31.999), (2.25,), (32, -2.5)])
 def test_axes_are_whole_numbers(axes):
     x, p = torch.zeros(1, 6, 2, 64), torch.zeros(6, len(axes), dtype=torch.int32)
