@@ -96,8 +96,9 @@ def paged_attention_step(q: torch.Tensor, cache: PagedCache, page_table: torch.T
 
     lengths: [b] int32 (int64 is converted), on the device: the first lengths[i] places of sequence i are its tokens, the last of them the one that q belongs to (its key
     and value are in the cache already).  Lengths are cut to what the table holds; a sequence that sees nothing (length 0, no page) has output 0.  Places past
-    the length and further back than the window are not seen, whatever they hold, and need no page.  Under autocast q is cast to the pages' type, for pages of 8 bits
-    to autocast's.  For inference: under torch.no_grad(), or with operands that need no gradient."""
+    the length and further back than the window are not seen, whatever they hold, and need no page.  Values are weighed and summed in fp32, and divided
+    by their weights' sum last: the places seen times the largest magnitude (in 8 bits 448 times the largest power of two) have to stay below 2^119.  Under autocast q is
+    cast to the pages' type, for pages of 8 bits to autocast's.  For inference: under torch.no_grad(), or with operands that need no gradient."""
     name = "paged_attention_step"
     _tensors(name, cache, q, page_table, lengths, distance_slopes)
     _dims(name, 3, q=q)

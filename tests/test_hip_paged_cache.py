@@ -311,6 +311,27 @@ def test_seen_values_that_are_infinite(wide, window, d, dtype):
 
 
 @KINDS
+@pytest.mark.parametrize("wide", [32, 200])
+def test_large_values_within_the_bound(wide, dtype, held):
+    """500 places of values up to 2^109, in 8 bits of rows that hold as much, whose scores rise slowly: the running maximum lags behind them by up to 2^8."""
+    import lact_amd
+    size, d, n = 16, 64, 500
+    table, count = tables([n], size, wide)
+    cache = random_cache(count, 1, size, d, held)
+    q = torch.full((1, 2, d), 0.25, dtype=dtype)
+    for j in range(n):
+        cache[0][table[0, j // size], 0, j % size] = 0.01 * j if held != E4M3 else torch.ones(d).to(held)
+    if held == E4M3:
+        for x, e in ((2, 0), (3, 100)):
+            cache[x] = torch.full(cache[x].shape, 127 + e, dtype=torch.uint8).view(E8M0)
+    else:
+        cache[1] = ((torch.rand(cache[1].shape, generator=torch.Generator().manual_seed(8)) * 2 - 1) * 2.0 ** 109).to(held)
+    out = lact_amd.paged_attention_step(q.to("cuda"), cuda(cache), table.to("cuda"), torch.tensor([n], device="cuda"))
+    ref, bound = PO.step(q, *numbers(cache), table, [n], None, None, None, None, *errors(dtype, held, n, d, 16.0))
+    near(out, ref, bound, "out")
+
+
+@KINDS
 def test_queries_and_tables_with_strides(dtype, held):
     import lact_amd
     lengths, size, hkv, d = [70, 33], 32, 2, 64
