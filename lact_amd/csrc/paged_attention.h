@@ -11,15 +11,18 @@
 //
 // A wave's step is 32 places from a multiple of 16 on: two pieces of 16 rows, each of which lies in one page, as page sizes are multiples of 16.  The wave looks up where
 // the keys and the values of 32 pieces lie at once, a lane each, and copies a piece from where its lane says; one without a page is copied from zeros and masked.  In a
-// piece that the window or the length ends in, the rows outside repeat one inside.
+// piece that the window or the length ends in, the keys outside repeat one inside and the values outside are zeros (of 8 bits, which have no infinities, they repeat one too).
 //
-// e4m3: numbers become bf16 as they leave LDS, exactly down to multiples of 2^-133.  A key's exponent is applied in that conversion (a lane has one key's row), a value's to the weight that meets
-// it.  fp32 queries and weights meet them in three bf16 parts of 8 bits.  (Products below 2^-126 count as 0: values under 2^-118.)
+// e4m3: numbers become bf16 as they leave LDS, exactly down to multiples of 2^-133.  A key's exponent is applied in that conversion (a lane has one key's row), a value's to
+// the weight that meets it.  fp32 queries and weights meet them in three bf16 parts of 8 bits.  (Products below 2^-126 count as 0: values under 2^-118.)
 //
-// What bounds it is the one read of the keys and values.  131072 places of 8 heads of 128 with 4 queries each in bf16: 93 us and 6 for the join, 5.8 and 5.4 TB/s (a large copy
-// reaches 5.0); 64 sequences of up to 16384 in e4m3, 5 queries each: 170 + 6 us, 5.4 TB/s; 32 of up to 8192 with a cap and a distance: 54 + 5 us, 4.6 TB/s: what lies between two
-// items.  The pages' size and order make no difference (16 to 256 places: 2 %).  Products of 32 x 32 with as many columns for any group: 71 us instead of 66 in the last of these,
-// 191 instead of 185 in the one before; one block to a compute unit in 8 bits: 117 and 282.
+// Nothing is rounded to fewer bits in front of the output but the weights of bf16 queries, which meet the values in two bf16 parts: 2^-15 of each.  In one part (2^-8) outputs of 131072 places
+// were off by 2.3e-3 of their norm where rounding them alone costs 1.7e-3; the second costs 1 % of a long case and 0.4-1.2 us of short ones (16 sequences of up to 1000: 12.4 -> 13.6).
+//
+// What bounds it is the one read of the keys and values.  131072 places of 8 heads of 128 with 4 queries each in bf16: 95 us and 6.5 for the join, 5.6 and 5.3 TB/s (a large copy
+// reaches 5.0); 64 sequences of up to 16384 in e4m3, 5 queries each: 172 + 7 us, 5.3 TB/s; 32 of up to 8192 with a cap and a distance: 55 + 5 us, 4.6 TB/s: what lies between two
+// items.  The pages' size and order make no difference (16 to 256 places: 2 %).  One block to a compute unit in 8 bits, with a ring twice as deep: 68 us instead of 61 in the last of
+// these, 184 instead of 178 in the one before, with heads of 64 44 instead of 36.
 #pragma once
 #include "attention_step.h"
 #include "paged_cache.h"
@@ -64,7 +67,7 @@ __device__ __forceinline__ int wave_scan(int v) {
 }
 
 // What a new item costs a block, in steps: the ring runs empty, parts are joined, pages looked up, the ring fills.  In the row of all items 0 / 1 / 2 / 3 / 6 for it: 32 sequences of up to
-// 8192 places, 8 heads of 128, e4m3 68 / 61 / 60 / 63 / 65 us, bf16 119 / 100 / 98 / 98 / 102; 64 of up to 16384, e4m3 187 / 174 / 174 / 175 / 180.
+// 8192 places, 8 heads of 128, e4m3 69 / 61 / 61 / 62 / 64 us, bf16 113 / 99 / 96 / 97 / 98; 64 of up to 16384, e4m3 178 / 178 / 179 / 177 / 182.
 constexpr int PAGED_START = 2;
 
 // The work of all items in a row: sequence by sequence, each of whose `items` costs the same, its steps and PAGED_START in front of them.  Shares differ by one at most.  Every
@@ -150,8 +153,9 @@ struct PagedShape {
   static constexpr int WAVE = RING * STAGE + 2 * EXP;
   static constexpr int KEYS = 32 * NW;                                       // of a step
   static constexpr int LDS = NW * WAVE;
-  // A block has an item as a whole, and no second launch, where the longest has no more steps.  Against shares: 64 sequences of up to 1000 places, 8 heads of 128, e4m3 18.8 us for 22.0; 16 in
-  // bf16 12.3 for 15.2, of 64 9.6 for 12.5; 4 steps of fp32, one sequence of 500, 12 heads of 64 10.5 for 11.9, 8 steps 17.4 for 11.7 (its products take longer).
+  // A block has an item as a whole, and no second launch, where the longest has no more steps.  Against shares: 64 sequences of up to 1000 places, 8 heads of 128, e4m3 19.9 us for 22.6, bf16 32.8
+  // for 32.7; 16 of up to 1000 in bf16 13.6 for 16.1, of up to 500 9.6 for 13.7; 4 steps of fp32, one sequence of 500, 12 heads of 64 10.8 for 13.0, 64 of up to 500 of 8 heads of 128 40.0 for
+  // 41.4, but 8 steps 17.6 for 12.9 (its products take longer).
   static constexpr int WHOLE = sizeof(C) == 4 ? 4 : 8;
 };
 

@@ -45,8 +45,8 @@ struct CacheTile {
   static constexpr int TURNS = 4, HEADS = ACROSS * TURNS;                         // of a block
   // tiles that L places from anywhere touch
   static int tiles(int L) { return (L + 2 * PLACES - 2) / PLACES; }
-  // With a quarter of these heads a thread's turns go along the sequence instead, each with a page of its own: 53 sequences of up to 16336 tokens, 2 heads of 64, bf16 into e4m3 and back
-  // 221 us for 319, 8 of 16336, one head of 128 30 for 45; with half of them 8 x 16336, 2 heads of 128 56 for 58, but 53 x 16336, 4 heads of 64 423 for 403.
+  // With a quarter of these heads a thread's turns go along the sequence instead, each with a page of its own.  bf16 into e4m3 and back, pages of 64: 53 sequences of 16336 tokens, 2 heads of 64
+  // 286 us for 348, 8 of 16336, one head of 128 40 for 53; with half of them it is worse: 8 x 16336, 2 heads of 128 92 for 84, 53 x 16336, 4 heads of 64 572 for 521.
   static bool along(int HK, int L) { return 4 * HK <= HEADS && L >= 4 * PLACES; }
 };
 struct CacheRows {
